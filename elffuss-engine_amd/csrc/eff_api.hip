@@ -6,6 +6,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <chrono>
 #include <deque>
 #include <memory>
@@ -16,6 +17,7 @@
 #include "../../include/elffuss_amd.h"
 #include "eff_formats.h"
 #include "eff_kernels.h"
+#include "eff_kv.h"
 
 using namespace eff;
 
@@ -1471,3 +1473,232 @@ int eff_topk_noalloc(eff_ctx *ctx, eff_buf *logits, uint32_t base, uint32_t voca
 }
 
 }  // extern "C"
+
+// ---- paged key/value cache -------------------------------------------------
+
+namespace {
+
+// The view of a cache and the batch of a call, checked. `who` names the call.
+int kv_views(eff_ctx *ctx, const eff_kv_cache *c, const eff_kv_batch *b, KvView &kv, KvBatchView &bv, const char *who) {
+  if (!c || !b) return fail(ctx, EFF_E_INVALID, "%s: null cache or batch", who);
+  if (!kv_type_known(c->type)) return fail(ctx, EFF_E_TYPE, "%s: unsupported cache type %d", who, c->type);
+  const size_t page = eff_kv_page_bytes(c->type, c->heads, c->head_dim, c->page_tokens);
+  if (!page)
+    return fail(ctx, EFF_E_SHAPE, "%s: no cache of %u heads of %u values in pages of %u tokens", who, c->heads,
+                c->head_dim, c->page_tokens);
+  if (c->pages == 0) return fail(ctx, EFF_E_INVALID, "%s: a cache without pages", who);
+  int rc = check_out(ctx, c->buf, (uint64_t)c->pages * page, who);
+  if (rc) return rc;
+  if (b->seqs == 0 || b->table_pages == 0 || b->max_new == 0 || b->max_len == 0)
+    return fail(ctx, EFF_E_INVALID, "%s: empty batch seqs=%u table_pages=%u max_new=%u max_len=%u", who, b->seqs,
+                b->table_pages, b->max_new, b->max_len);
+  if (b->max_len > (uint64_t)b->table_pages * c->page_tokens)
+    return fail(ctx, EFF_E_BOUNDS, "%s: max_len=%u and the table has %u pages of %u tokens", who, b->max_len,
+                b->table_pages, c->page_tokens);
+  if (b->max_len > 0x7FFFFFFFu || b->tokens > 0x7FFFFFFFu || b->seqs > 0x7FFFFFFFu)
+    return fail(ctx, EFF_E_SHAPE, "%s: max_len=%u tokens=%u seqs=%u: below 2^31", who, b->max_len, b->tokens, b->seqs);
+  if ((rc = check_out(ctx, b->table, 4ull * b->seqs * b->table_pages, who)) ||
+      (rc = check_out(ctx, b->starts, 4ull * (b->seqs + 1ull), who)) ||
+      (rc = check_out(ctx, b->lens, 4ull * b->seqs, who)))
+    return rc;
+  kv.base = (uint8_t *)c->buf->ptr;
+  kv.type = c->type;
+  kv.heads = c->heads;
+  kv.dim = c->head_dim;
+  kv.page_log2 = (uint32_t)__builtin_ctz(c->page_tokens);
+  kv.pages = c->pages;
+  kv.block_bytes = kv_block_bytes(c->type, c->head_dim, c->page_tokens);
+  kv.page_bytes = page;
+  bv = {(const uint32_t *)b->table->ptr, (const uint32_t *)b->starts->ptr, (const uint32_t *)b->lens->ptr,
+        b->seqs, b->tokens, b->table_pages, b->max_new, b->max_len};
+  return EFF_OK;
+}
+
+// Rows of `n` floats, `stride` (0: n) floats from token to token from `offset`.
+int kv_row_view(eff_ctx *ctx, eff_buf *buf, uint64_t offset, uint32_t &stride, uint64_t n, uint32_t tokens,
+                const float **p, const char *who) {
+  if (!buf) return fail(ctx, EFF_E_INVALID, "%s: null buffer", who);
+  if (n > 0x7FFFFFFFull) return fail(ctx, EFF_E_SHAPE, "%s: rows of %llu floats", who, (unsigned long long)n);
+  if (stride == 0u) stride = (uint32_t)n;
+  if ((offset | stride) & 3u)
+    return fail(ctx, EFF_E_INVALID, "%s: offset=%llu and stride=%u must be multiples of 4 floats", who,
+                (unsigned long long)offset, stride);
+  if (stride < n) return fail(ctx, EFF_E_INVALID, "%s: stride=%u below the row's %llu floats", who, stride, (unsigned long long)n);
+  if (offset > buf->size) return fail(ctx, EFF_E_BOUNDS, "%s: offset=%llu in a buffer of %zu bytes", who, (unsigned long long)offset, buf->size);
+  const uint64_t floats = tokens ? offset + (uint64_t)(tokens - 1u) * stride + n : 0ull;
+  const int rc = check_out(ctx, buf, floats * 4u, who);
+  if (rc) return rc;
+  *p = (const float *)buf->ptr + offset;
+  return EFF_OK;
+}
+
+bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return an && bn && x < y + bn && y < x + an;
+}
+
+// Bytes from a row view's first float to its last.
+uint64_t row_span(uint32_t stride, uint64_t n, uint32_t tokens) {
+  return tokens ? ((uint64_t)(tokens - 1u) * stride + n) * 4u : 0u;
+}
+
+}  // namespace
+
+size_t eff_kv_page_bytes(int type, uint32_t heads, uint32_t dim, uint32_t page) {
+  if (!kv_type_known(type) || !kv_dim_known(dim) || heads == 0 || heads > 4096u || page < kKvPageMin ||
+      page > kKvPageMax || (page & (page - 1u)))
+    return 0;
+  return 2ull * heads * kv_block_bytes(type, dim, page);
+}
+
+int eff_rope_table(eff_ctx *ctx, const double *freqs, uint32_t n, uint32_t positions, float scale, eff_buf *out) {
+  if (!ctx) return EFF_E_INVALID;
+  if (!freqs) return fail(ctx, EFF_E_INVALID, "rope table: null frequencies");
+  if (n == 0 || n > kRopeMaxPairs || positions == 0 || positions > 0x7FFFFFFFu)
+    return fail(ctx, EFF_E_SHAPE, "rope table: n=%u (1..%u) positions=%u", n, kRopeMaxPairs, positions);
+  int rc = check_out(ctx, out, (uint64_t)positions * n * 8u, "rope table");
+  if (rc || (rc = use_device(ctx))) return rc;
+  RopeFreqs f{};
+  memcpy(f.f, freqs, n * sizeof(double));
+  hipError_t e = launch_rope_table(f, n, positions, scale, (float *)out->ptr, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "rope table launch");
+  return EFF_OK;
+}
+
+int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *r) {
+  if (!ctx) return EFF_E_INVALID;
+  KvView kv;
+  KvBatchView b;
+  int rc = kv_views(ctx, cache, batch, kv, b, "kv append");
+  if (rc) return rc;
+  if (!r) return fail(ctx, EFF_E_INVALID, "kv append: null rows");
+  if (!r->q != (r->q_heads == 0)) return fail(ctx, EFF_E_INVALID, "kv append: q and q_heads=%u", r->q_heads);
+  if (r->q_heads > 65536u) return fail(ctx, EFF_E_SHAPE, "kv append: q_heads=%u", r->q_heads);
+  KvAppendArgs a{};
+  const uint64_t nk = (uint64_t)kv.heads * kv.dim, nq = (uint64_t)r->q_heads * kv.dim;
+  a.q_stride = r->q_stride, a.k_stride = r->k_stride, a.v_stride = r->v_stride;
+  if ((rc = kv_row_view(ctx, r->k, r->k_offset, a.k_stride, nk, b.tokens, &a.k, "kv append k")) ||
+      (rc = kv_row_view(ctx, r->v, r->v_offset, a.v_stride, nk, b.tokens, &a.v, "kv append v")))
+    return rc;
+  if (r->q) {
+    if ((rc = kv_row_view(ctx, r->q, r->q_offset, a.q_stride, nq, b.tokens, &a.q, "kv append q")) ||
+        (rc = check_out(ctx, r->q_out, (uint64_t)b.tokens * nq * 4u, "kv append q_out")))
+      return rc;
+    a.q_out = (float *)r->q_out->ptr;
+    a.q_heads = r->q_heads;
+    // in place a row is read by the lanes that write it, if it is where it was
+    const uint64_t out = (uint64_t)b.tokens * nq * 4u;
+    const bool same = a.q == a.q_out && a.q_stride == nq;
+    if ((!same && overlap(a.q, row_span(a.q_stride, nq, b.tokens), a.q_out, out)) ||
+        overlap(a.k, row_span(a.k_stride, nk, b.tokens), a.q_out, out) ||
+        overlap(a.v, row_span(a.v_stride, nk, b.tokens), a.q_out, out))
+      return fail(ctx, EFF_E_INVALID, "kv append: q_out overlaps the rows");
+  }
+  if (r->rope_dim) {
+    if ((r->rope_dim & 3u) || r->rope_dim > kv.dim)
+      return fail(ctx, EFF_E_SHAPE, "kv append: rope_dim=%u must be a multiple of 4 up to %u", r->rope_dim, kv.dim);
+    if (r->rope_mode > EFF_ROPE_HALVES) return fail(ctx, EFF_E_INVALID, "kv append: rope_mode=%u", r->rope_mode);
+    if ((rc = check_out(ctx, r->rope, 4ull * r->rope_positions * r->rope_dim, "kv append rope"))) return rc;
+    if (r->rope_positions < b.max_len)
+      return fail(ctx, EFF_E_BOUNDS, "kv append: the rope table has %u positions and max_len=%u", r->rope_positions,
+                  b.max_len);
+    a.rope = (const float *)r->rope->ptr;
+    a.rope_dim = r->rope_dim;
+    a.halves = r->rope_mode == EFF_ROPE_HALVES;
+  }
+  if (r->q_norm && (rc = check_out(ctx, r->q_norm, 4ull * kv.dim, "kv append q_norm"))) return rc;
+  if (r->k_norm && (rc = check_out(ctx, r->k_norm, 4ull * kv.dim, "kv append k_norm"))) return rc;
+  a.q_norm = r->q_norm ? (const float *)r->q_norm->ptr : nullptr;
+  a.k_norm = r->k_norm ? (const float *)r->k_norm->ptr : nullptr;
+  a.eps = r->norm_eps;
+  if (b.tokens == 0) return EFF_OK;
+  if ((uint64_t)b.tokens * (r->q_heads + 2ull * kv.heads) > 0x7FFFFFFFull)
+    return fail(ctx, EFF_E_SHAPE, "kv append: %u tokens of %u + 2 x %u heads", b.tokens, r->q_heads, kv.heads);
+  if ((rc = use_device(ctx))) return rc;
+  hipError_t e = launch_kv_append(kv, b, a, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "kv append launch");
+  ++ctx->stats.kv_append;
+  return EFF_OK;
+}
+
+int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
+                uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window) {
+  if (!ctx) return EFF_E_INVALID;
+  KvView kv;
+  KvBatchView b;
+  int rc = kv_views(ctx, cache, batch, kv, b, "kv attn");
+  if (rc) return rc;
+  if (q_heads == 0 || q_heads > 65536u || q_heads % kv.heads)
+    return fail(ctx, EFF_E_SHAPE, "kv attn: q_heads=%u over %u key/value heads", q_heads, kv.heads);
+  if (!(scale - scale == 0.f)) return fail(ctx, EFF_E_INVALID, "kv attn: the scale is not finite");
+  KvAttnArgs a{};
+  const uint64_t n = (uint64_t)q_heads * kv.dim;
+  a.q_stride = q_stride;
+  if ((rc = kv_row_view(ctx, q, q_offset, a.q_stride, n, b.tokens, &a.q, "kv attn q")) ||
+      (rc = check_out(ctx, out, (uint64_t)b.tokens * n * 4u, "kv attn out")))
+    return rc;
+  a.out = (float *)out->ptr;
+  if (overlap(a.q, row_span(a.q_stride, n, b.tokens), a.out, (uint64_t)b.tokens * n * 4u))
+    return fail(ctx, EFF_E_INVALID, "kv attn: q and out overlap");
+  a.q_heads = q_heads;
+  a.scale = scale;
+  a.window = window;
+  if (b.tokens == 0) return EFF_OK;
+  if ((uint64_t)b.tokens * q_heads > 0x7FFFFFFFull)
+    return fail(ctx, EFF_E_SHAPE, "kv attn: %u tokens of %u heads", b.tokens, q_heads);
+  if ((rc = use_device(ctx))) return rc;
+  hipError_t e = launch_kv_attn(kv, b, a, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "kv attn launch");
+  ++ctx->stats.kv_attn;
+  return EFF_OK;
+}
+
+int eff_logits_apply(eff_ctx *ctx, eff_buf *in, eff_buf *out, uint32_t rows, uint32_t vocab, uint32_t stride,
+                     const eff_logits_rules *r) {
+  if (!ctx) return EFF_E_INVALID;
+  if (!r) return fail(ctx, EFF_E_INVALID, "logits: null rules");
+  if (vocab == 0 || vocab > 0x7FFFFFFFu) return fail(ctx, EFF_E_SHAPE, "logits: vocab=%u", vocab);
+  if (stride == 0u) stride = vocab;
+  if (stride < vocab) return fail(ctx, EFF_E_INVALID, "logits: stride=%u below vocab=%u", stride, vocab);
+  const uint64_t bytes = rows ? ((uint64_t)(rows - 1u) * stride + vocab) * 4u : 0u;
+  int rc;
+  if ((rc = check_out(ctx, in, bytes, "logits in")) || (rc = check_out(ctx, out, bytes, "logits out"))) return rc;
+  if (in->ptr != out->ptr && overlap(in->ptr, bytes, out->ptr, bytes))
+    return fail(ctx, EFF_E_INVALID, "logits: in and out overlap and are not the same");
+  LogitsArgs a{};
+  a.in = (const float *)in->ptr, a.out = (float *)out->ptr;
+  a.rows = rows, a.vocab = vocab, a.stride = stride;
+  if (r->history || r->history_starts || r->penalties) {
+    if ((rc = check_out(ctx, r->history, 0, "logits history")) ||
+        (rc = check_out(ctx, r->history_starts, 4ull * (rows + 1ull), "logits history_starts")) ||
+        (rc = check_out(ctx, r->penalties, 24ull * rows, "logits penalties")))
+      return rc;
+    a.history = (const uint32_t *)r->history->ptr, a.history_starts = (const uint32_t *)r->history_starts->ptr;
+    a.history_count = (uint32_t)std::min<uint64_t>(r->history->size / 4u, 0x7FFFFFFFu);
+    a.penalties = (const double *)r->penalties->ptr;
+  }
+  if (r->bias_ids || r->bias_values || r->bias_starts) {
+    if ((rc = check_out(ctx, r->bias_ids, 0, "logits bias_ids")) ||
+        (rc = check_out(ctx, r->bias_values, 0, "logits bias_values")) ||
+        (rc = check_out(ctx, r->bias_starts, 4ull * (rows + 1ull), "logits bias_starts")))
+      return rc;
+    a.bias_ids = (const uint32_t *)r->bias_ids->ptr, a.bias_values = (const float *)r->bias_values->ptr;
+    a.bias_starts = (const uint32_t *)r->bias_starts->ptr;
+    a.bias_count = (uint32_t)std::min<uint64_t>(std::min(r->bias_ids->size, r->bias_values->size) / 4u, 0x7FFFFFFFu);
+  }
+  if (r->mask || r->mask_of) {
+    if ((rc = check_out(ctx, r->mask, (uint64_t)r->mask_count * ((vocab + 31ull) / 32u) * 4u, "logits mask")) ||
+        (rc = check_out(ctx, r->mask_of, 4ull * rows, "logits mask_of")))
+      return rc;
+    a.mask = (const uint32_t *)r->mask->ptr, a.mask_of = (const uint32_t *)r->mask_of->ptr;
+    a.mask_count = r->mask_count;
+  }
+  if (rows == 0) return EFF_OK;
+  if ((uint64_t)rows * (vocab / 1024u + 1ull) > 0x7FFFFFFFull)
+    return fail(ctx, EFF_E_SHAPE, "logits: %u rows of %u", rows, vocab);
+  if ((rc = use_device(ctx))) return rc;
+  hipError_t e = launch_logits(a, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "logits launch");
+  ++ctx->stats.logits;
+  return EFF_OK;
+}

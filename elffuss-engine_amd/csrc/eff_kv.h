@@ -1,0 +1,107 @@
+// The paged key/value cache: its layout, and the views that the entry points
+// give the append and attention kernels.
+//
+// Page p of a cache is [K, V][head][block]; a block holds the `page_tokens` rows
+// of one head: fp16 rows of head_dim values (EFF_KV_F16), or int8 rows followed
+// by the rows' f32 scales (EFF_KV_I8: value = int8 * scale). A head's rows lie
+// side by side, so that a wave reads 16 rows of a page as one run.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/elffuss_amd.h"
+
+namespace eff {
+
+constexpr uint32_t kKvPageMin = 16, kKvPageMax = 1024;   // tokens of a page, a power of two
+
+inline bool kv_type_known(int t) { return t == EFF_KV_F16 || t == EFF_KV_I8; }
+inline bool kv_dim_known(uint32_t d) { return d == 64u || d == 96u || d == 128u || d == 256u; }
+
+// Bytes of one head's rows of a page, K or V.
+constexpr uint32_t kv_block_bytes(int type, uint32_t dim, uint32_t page) {
+  return page * (type == EFF_KV_F16 ? 2u * dim : dim + 4u);
+}
+
+struct KvView {
+  uint8_t *base;
+  int type;
+  uint32_t heads, dim, page_log2, pages;
+  uint32_t block_bytes;   // kv_block_bytes
+  uint64_t page_bytes;    // 2 * heads * block_bytes
+};
+
+struct KvBatchView {
+  const uint32_t *table;    // [seqs][table_pages]
+  const uint32_t *starts;   // [seqs + 1]
+  const uint32_t *lens;     // [seqs]
+  uint32_t seqs, tokens, table_pages, max_new, max_len;
+};
+
+// The rows of one append: f32, `stride` floats from token to token.
+struct KvAppendArgs {
+  const float *q, *k, *v;            // q null: none
+  uint32_t q_stride, k_stride, v_stride;
+  float *q_out;                      // [tokens][q_heads * dim]
+  uint32_t q_heads;
+  const float *rope;                 // [positions][2][rope_dim / 2]
+  uint32_t rope_dim;                 // 0: no rotation
+  int halves;                        // pairs (i, i + rope_dim / 2), else (2 i, 2 i + 1)
+  const float *q_norm, *k_norm;      // null: none
+  float eps;
+};
+
+struct KvAttnArgs {
+  const float *q;
+  uint32_t q_stride;
+  float *out;                        // [tokens][q_heads * dim]
+  uint32_t q_heads;
+  float scale;
+  uint32_t window;                   // 0: none
+};
+
+constexpr uint32_t kRopeMaxPairs = 256;
+struct RopeFreqs {
+  double f[kRopeMaxPairs];
+};
+hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positions, float scale, float *out,
+                             hipStream_t stream);
+hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t stream);
+hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, hipStream_t stream);
+
+struct LogitsArgs {
+  const float *in;
+  float *out;
+  uint32_t rows, vocab, stride;
+  const uint32_t *history, *history_starts;   // null: none
+  uint32_t history_count;
+  const double *penalties;                    // [rows][3]: repeat, frequency, presence
+  const uint32_t *bias_ids, *bias_starts;     // null: none
+  const float *bias_values;
+  uint32_t bias_count;
+  const uint32_t *mask, *mask_of;             // null: none
+  uint32_t mask_count;
+};
+hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream);
+
+#ifdef __HIP__
+// The sequence of new token t: the last whose first token is at most t (the
+// whole wave asks for one t). Returns `seqs` for a token of no sequence.
+__device__ __forceinline__ uint32_t kv_seq_of(const KvBatchView &b, uint32_t t) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t n = 0;
+  for (uint32_t at = 0; at <= b.seqs; at += 64u) {
+    const uint32_t i = at + lane;
+    const uint32_t c = __popcll(__ballot(i <= b.seqs && b.starts[i <= b.seqs ? i : b.seqs] <= t));
+    n += c;
+    if (c < 64u) break;
+  }
+  return n ? min(n - 1u, b.seqs) : b.seqs;
+}
+
+// Tokens of sequence s, the new ones included, as far as the call reaches.
+__device__ __forceinline__ uint32_t kv_len(const KvBatchView &b, uint32_t s) { return min(b.lens[s], b.max_len); }
+#endif
+
+}  // namespace eff

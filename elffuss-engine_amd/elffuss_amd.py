@@ -23,6 +23,8 @@ TYPES = {"Q8_0": Q8_0, "Q2_K": Q2_K, "Q4_K": Q4_K, "Q6_K": Q6_K, "IQ2_XXS": IQ2_
 OPT_GEMV_MAX_TOKENS, OPT_GEMM_MIN_TOKENS, OPT_GEMV_KERNEL, OPT_SPLIT_CONFIG, OPT_SPLIT_MIN_TOKENS = 1, 2, 3, 4, 5
 OPT_GEMM_CONFIG, OPT_GEMM_SPLIT, OPT_SPLIT_SLICES = 6, 7, 8
 GEMV_SECTIONS, GEMV_SWIGLU = 1, 2
+KV_F16, KV_I8, KV_NO_PAGE = 1, 24, 0xFFFFFFFF
+ROPE_PAIRS, ROPE_HALVES = 0, 1
 TOPK_HEADER, TOPK_P_MAX, TOPK_CAP, TOPK_M_MAX = 8, 128, 256, 192
 TOPK_NOALLOC_SCRATCH_BYTES = 18432
 
@@ -44,7 +46,8 @@ class Stats(ctypes.Structure):
     _fields_ = [("gemv", ctypes.c_uint64), ("gemm", ctypes.c_uint64), ("skinny", ctypes.c_uint64),
                 ("dequant", ctypes.c_uint64), ("topk", ctypes.c_uint64), ("not_applicable", ctypes.c_uint64),
                 ("split", ctypes.c_uint64), ("fused", ctypes.c_uint64), ("gather", ctypes.c_uint64),
-                ("gemm_x", ctypes.c_uint64), ("split_x", ctypes.c_uint64), ("cpu_path", ctypes.c_uint64)]
+                ("gemm_x", ctypes.c_uint64), ("split_x", ctypes.c_uint64), ("cpu_path", ctypes.c_uint64),
+                ("kv_append", ctypes.c_uint64), ("kv_attn", ctypes.c_uint64), ("logits", ctypes.c_uint64)]
 
 
 class SplitPlan(ctypes.Structure):
@@ -129,6 +132,11 @@ def lib():
         "eff_read_floor": ([p, p, ctypes.c_size_t, u32, u32, p], i32),
         "eff_qgemv_topk": ([p, i32, p, p, p, u32, u32, u32, p, u32, u32, p], i32),
         "eff_topk_out_bytes": ([], sz),
+        "eff_kv_page_bytes": ([i32, u32, u32, u32], sz),
+        "eff_rope_table": ([p, p, u32, u32, ctypes.c_float, p], i32),
+        "eff_kv_append": ([p, p, p, p], i32),
+        "eff_kv_attn": ([p, p, p, p, u64, u32, p, u32, ctypes.c_float, u32], i32),
+        "eff_logits_apply": ([p, p, p, u32, u32, u32, p], i32),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -145,7 +153,8 @@ EXPORTED = ("eff_type_from_name eff_type_name eff_type_geometry eff_init eff_shu
             "eff_read_begin eff_read_end eff_read_poll eff_read_error eff_read_release "
             "eff_bytes_reordered eff_bytes_buffer_r eff_blocks_from_buffer eff_scales_from eff_buf_mark_r "
             "eff_buf_blocks_r eff_buf_write_r eff_repack eff_unrepack eff_quantize eff_fill_normal eff_qmatmul eff_qgemv "
-            "eff_qgemm eff_qgemm_planned eff_gemm_x_layout eff_gemm_prepare_x eff_qgemm_prepared eff_qmatmul_x_layout eff_qmatmul_prepare_x eff_qmatmul_prepared eff_split_plan eff_qmatmul_cpu_path eff_qgemv_multi eff_dequant eff_gather eff_gather_norm eff_topk eff_topk_noalloc eff_qgemv_topk eff_topk_out_bytes eff_read_floor").split()
+            "eff_qgemm eff_qgemm_planned eff_gemm_x_layout eff_gemm_prepare_x eff_qgemm_prepared eff_qmatmul_x_layout eff_qmatmul_prepare_x eff_qmatmul_prepared eff_split_plan eff_qmatmul_cpu_path eff_qgemv_multi eff_dequant eff_gather eff_gather_norm eff_topk eff_topk_noalloc eff_qgemv_topk eff_topk_out_bytes eff_read_floor "
+            "eff_kv_page_bytes eff_rope_table eff_kv_append eff_kv_attn eff_logits_apply").split()
 
 
 def type_code(t):
@@ -277,6 +286,84 @@ class Buffer:
         if self.handle:
             self.ctx._check(lib().eff_buf_retire(self.ctx.h, self.handle))
             self.handle = None
+
+
+class _Described:
+    """A C description of a call's buffers and sizes, made once and given to many calls.
+
+    The buffers stay referenced here; `ref` is what the library takes."""
+
+    def _describe(self, struct, **values):
+        self.buffers = [v for v in values.values() if isinstance(v, Buffer)]
+        self.c = struct(**{k: v.handle if isinstance(v, Buffer) else v for k, v in values.items()})
+        self.ref = ctypes.addressof(self.c)
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int32), ("heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("page_tokens", ctypes.c_uint32), ("pages", ctypes.c_uint32), ("buf", ctypes.c_void_p)]
+
+
+class _KvBatch(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+                ("seqs", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("table_pages", ctypes.c_uint32),
+                ("max_new", ctypes.c_uint32), ("max_len", ctypes.c_uint32)]
+
+
+class _KvRows(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_offset", ctypes.c_uint64), ("k_offset", ctypes.c_uint64), ("v_offset", ctypes.c_uint64),
+                ("q_stride", ctypes.c_uint32), ("k_stride", ctypes.c_uint32), ("v_stride", ctypes.c_uint32),
+                ("q_heads", ctypes.c_uint32), ("q_out", ctypes.c_void_p), ("rope", ctypes.c_void_p),
+                ("rope_positions", ctypes.c_uint32), ("rope_dim", ctypes.c_uint32), ("rope_mode", ctypes.c_uint32),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("norm_eps", ctypes.c_float)]
+
+
+class _LogitsRules(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("history", "history_starts", "penalties", "bias_ids", "bias_values",
+                                               "bias_starts", "mask", "mask_of")] + [("mask_count", ctypes.c_uint32)]
+
+
+def kv_page_bytes(t, heads, head_dim, page_tokens):
+    """Bytes of a cache page, K and V of every head (0: no such cache)."""
+    return lib().eff_kv_page_bytes(t, heads, head_dim, page_tokens)
+
+
+class KvCache(_Described):
+    """One layer's paged key/value cache in `buf` (eff_kv_cache)."""
+
+    def __init__(self, t, heads, head_dim, page_tokens, pages, buf):
+        self._describe(_KvCache, type=t, heads=heads, head_dim=head_dim, page_tokens=page_tokens, pages=pages, buf=buf)
+
+
+class KvBatch(_Described):
+    """The sequences of a call and their new tokens (eff_kv_batch); u32 buffers."""
+
+    def __init__(self, table, starts, lens, *, seqs, tokens, table_pages, max_new, max_len):
+        self._describe(_KvBatch, table=table, starts=starts, lens=lens, seqs=seqs, tokens=tokens,
+                       table_pages=table_pages, max_new=max_new, max_len=max_len)
+
+
+class KvRows(_Described):
+    """The f32 rows of an append (eff_kv_rows); k, v (and q) are a buffer or (buffer, offset in floats)."""
+
+    def __init__(self, *, k, v, q=None, q_stride=0, k_stride=0, v_stride=0, q_heads=0, q_out=None, rope=None,
+                 rope_positions=0, rope_dim=0, rope_mode=ROPE_PAIRS, q_norm=None, k_norm=None, eps=1e-6):
+        at = [x if isinstance(x, tuple) else (x, 0) for x in (q, k, v)]
+        self._describe(_KvRows, q=at[0][0], k=at[1][0], v=at[2][0], q_offset=at[0][1], k_offset=at[1][1],
+                       v_offset=at[2][1], q_stride=q_stride, k_stride=k_stride, v_stride=v_stride, q_heads=q_heads,
+                       q_out=q_out, rope=rope, rope_positions=rope_positions, rope_dim=rope_dim, rope_mode=rope_mode,
+                       q_norm=q_norm, k_norm=k_norm, norm_eps=eps)
+
+
+class LogitsRules(_Described):
+    """Penalties, biases and masks of a batch's logits (eff_logits_rules)."""
+
+    def __init__(self, *, history=None, history_starts=None, penalties=None, bias_ids=None, bias_values=None,
+                 bias_starts=None, mask=None, mask_of=None, mask_count=0):
+        self._describe(_LogitsRules, history=history, history_starts=history_starts, penalties=penalties,
+                       bias_ids=bias_ids, bias_values=bias_values, bias_starts=bias_starts, mask=mask,
+                       mask_of=mask_of, mask_count=mask_count)
 
 
 class Graph:
@@ -477,6 +564,27 @@ class Context:
         self._check(lib().eff_topk_noalloc(self.h, logits.handle, base, vocab, m,
                                            ids.ctypes.data if ids.size else None, ids.size, serial, out.handle))
         return out
+
+    def rope_table(self, freqs, positions, scale=1.0, out=None):
+        """cos and sin of position * freqs (64-bit), [positions][2][len(freqs)] f32 (eff_rope_table)."""
+        f = np.ascontiguousarray(freqs, dtype=np.float64)
+        if out is None:
+            out = self.alloc(8 * f.size * positions)
+        self._check(lib().eff_rope_table(self.h, f.ctypes.data, f.size, positions, scale, out.handle))
+        return out
+
+    def kv_append(self, cache, batch, rows):
+        """The new tokens' k and v into the cache, q and k normed and rotated (eff_kv_append)."""
+        self._check(lib().eff_kv_append(self.h, cache.ref, batch.ref, rows.ref))
+
+    def kv_attn(self, cache, batch, q, out, q_heads, scale, window=0, q_offset=0, q_stride=0):
+        """Attention of the new tokens over the cache (eff_kv_attn)."""
+        self._check(lib().eff_kv_attn(self.h, cache.ref, batch.ref, q.handle, q_offset, q_stride, out.handle, q_heads,
+                                      scale, window))
+
+    def logits_apply(self, logits, out, rows, vocab, rules, stride=0):
+        """Penalties, biases and masks on a batch's logits (eff_logits_apply)."""
+        self._check(lib().eff_logits_apply(self.h, logits.handle, out.handle, rows, vocab, stride, rules.ref))
 
     def read_floor(self, src, nbytes, workgroups, unroll, sink):
         """eff_read_floor: a streaming read of nbytes of src (measurement only)."""

@@ -77,6 +77,13 @@ extern "C" {
 #define EFF_GEMV_SECTIONS  1  /* 'secciones': ys[i] = W_i x for 2..4 matrices */
 #define EFF_GEMV_SWIGLU    2  /* 'swiglu': ys[0] = silu(W_gate x) * (W_up x) */
 
+/* ---- paged key/value cache ------------------------------------------------ */
+#define EFF_KV_F16    1    /* rows of fp16 (ggml code of F16) */
+#define EFF_KV_I8     24   /* rows of int8 with one f32 scale a row (ggml code of I8) */
+#define EFF_KV_NO_PAGE  0xFFFFFFFFu  /* a table entry without a page (so is any number past the cache) */
+#define EFF_ROPE_PAIRS  0  /* rotation of the pairs (2 i, 2 i + 1) */
+#define EFF_ROPE_HALVES 1  /* rotation of the pairs (i, i + rope_dim / 2) */
+
 /* ---- top-k output layout (kernels.topk.wgsl.js:40-60) ------------------- */
 #define EFF_TOPK_M_MAX     192   /* largest M = K' + |S| accepted (TOPK_M_MAX) */
 #define EFF_TOPK_P_MAX     128   /* penalised ids (TOPK_P_MAX) */
@@ -109,6 +116,9 @@ typedef struct eff_stats {
                            split-x router call but those of up to 8 tokens that prepare x inside the
                            product: eff_split_plan's prepares_x; one per eff_qmatmul_prepare_x for it) */
   uint64_t cpu_path;    /* products with the reference CPU path's arithmetic (eff_qmatmul_cpu_path) */
+  uint64_t kv_append;   /* eff_kv_append launches */
+  uint64_t kv_attn;     /* eff_kv_attn launches */
+  uint64_t logits;      /* eff_logits_apply launches */
 } eff_stats;
 
 /* ---- types and geometry -------------------------------------------------- */
@@ -482,6 +492,114 @@ int eff_topk_noalloc(eff_ctx *ctx, eff_buf *logits, uint32_t base, uint32_t voca
 
 /* Size in bytes of the top-k output record (topkBytesSalida). */
 size_t eff_topk_out_bytes(void);
+
+/* ---- paged key/value cache: append, attention ---------------------------- */
+
+/* A cache of one layer: `pages` pages of `page_tokens` tokens (a power of two,
+ * 16..1024) for `heads` key/value heads of `head_dim` (64, 96, 128 or 256)
+ * values, in `buf`. Page p starts at p * eff_kv_page_bytes: its K, then its V,
+ * each [head][token][head_dim] in fp16 (EFF_KV_F16), or per head the int8 rows
+ * and after them the rows' f32 scales (EFF_KV_I8; a value is int8 * scale).
+ * The reference's cache is one fp16 buffer per layer (README.md:101); pages let
+ * requests of different lengths share the memory, and give it back. */
+typedef struct eff_kv_cache {
+  int32_t type;
+  uint32_t heads, head_dim, page_tokens, pages;
+  eff_buf *buf;
+} eff_kv_cache;
+
+/* Bytes of one page (K and V of every head); 0 for a type, size or head count
+ * that the cache does not have. */
+size_t eff_kv_page_bytes(int type, uint32_t heads, uint32_t head_dim, uint32_t page_tokens);
+
+/* The new tokens of one call, of `seqs` sequences; u32 device buffers.
+ *   starts [seqs + 1]: sequence s has the new tokens starts[s] .. starts[s + 1),
+ *          at most max_new of them; starts[0] = 0, starts[seqs] = tokens
+ *   lens   [seqs]: tokens of the sequence, the new ones included, at most
+ *          max_len: its last new token is at position lens[s] - 1
+ *   table  [seqs][table_pages]: the pages of the sequence, in order
+ * A table entry >= pages (EFF_KV_NO_PAGE) has no page: what would be appended
+ * there is not, and attention sees nothing there. A new token without a
+ * position (more new tokens than lens[s]) is not cached and its rows are
+ * zeros. The buffers are read on the device when the call runs, so a recorded
+ * call (eff_graph_begin) takes the next step's values; max_new and max_len
+ * are what it was planned for. */
+typedef struct eff_kv_batch {
+  eff_buf *table, *starts, *lens;
+  uint32_t seqs, tokens, table_pages, max_new, max_len;
+} eff_kv_batch;
+
+/* The f32 rows of an append, one per new token. An offset is in floats from
+ * the buffer's start, a stride in floats from token to token (0: the row's
+ * own size); both multiples of 4. One buffer may hold q, k and v (the output
+ * of one projection). q may be NULL with q_heads = 0. q_out is [tokens][q_heads * head_dim]; it
+ * may be q's own buffer only where q has that layout.
+ *   q_norm, k_norm  f32 [head_dim] or NULL: RMS norm weights, with norm_eps
+ *   rope            f32 [rope_positions][2][rope_dim / 2], cos then sin
+ *                   (eff_rope_table); NULL with rope_dim = 0: no rotation.
+ *                   rope_dim: a multiple of 4, at most head_dim; the values
+ *                   past it are not rotated. rope_positions >= max_len */
+typedef struct eff_kv_rows {
+  eff_buf *q, *k, *v;
+  uint64_t q_offset, k_offset, v_offset;
+  uint32_t q_stride, k_stride, v_stride;
+  uint32_t q_heads;
+  eff_buf *q_out;
+  eff_buf *rope;
+  uint32_t rope_positions, rope_dim, rope_mode;
+  eff_buf *q_norm, *k_norm;
+  float norm_eps;
+} eff_kv_rows;
+
+/* cos and sin of position * freqs[i] (host, 64-bit, n <= 256 of them) times
+ * `scale`, for the positions 0 .. positions - 1: out [positions][2][n] f32. The
+ * angles are computed in 64 bits. The reference computes them in its RoPE
+ * kernel, in f32 (ops.js:1158-1456). */
+int eff_rope_table(eff_ctx *ctx, const double *freqs, uint32_t n, uint32_t positions, float scale, eff_buf *out);
+
+/* Norm (optional) and rotation of the new tokens' q and k, q to q_out, k and v
+ * into the cache. An int8 row: scale = max|x| * (1 / 127), n = round(x * (127 /
+ * max|x|)), ties to even; a row with a NaN or an infinity has no finite value. */
+int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *rows);
+
+/* out [tokens][q_heads * head_dim] = attention of q (rows as in eff_kv_rows,
+ * rotated: eff_kv_append's q_out) over the cache: q head h reads key/value head
+ * h / (q_heads / heads). A new token at position p sees the cached tokens of
+ * its sequence at positions <= p, and of these the last `window` if window > 0
+ * (the append comes first). softmax(scale * q . k) in f32; a token that sees
+ * nothing gives zeros. What lies in the cache at positions it does not see does
+ * not reach its output, whatever bits it has; a NaN or an infinity among what
+ * it sees does. q and out may not overlap. f32-accurate. */
+int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
+                uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window);
+
+/* ---- rules on the logits of a batch --------------------------------------- */
+
+/* Device buffers; a NULL group is not applied.
+ *   history [history_starts[rows]] u32: the token ids of each row's history,
+ *           row r's from history_starts[r] (u32 [rows + 1]); an id may repeat,
+ *           one past the vocabulary counts for nothing
+ *   penalties f64 [rows][3]: repeat, frequency, presence (1, 0, 0: none)
+ *   bias_ids u32, bias_values f32, bias_starts u32 [rows + 1]: as history; of
+ *           several values of one id in a row the last counts
+ *   mask    u32 [mask_count][(vocab + 31) / 32]: bit v % 32 of word v / 32 set:
+ *           token v is allowed; mask_of u32 [rows]: the row's mask, none if
+ *           >= mask_count */
+typedef struct eff_logits_rules {
+  eff_buf *history, *history_starts, *penalties;
+  eff_buf *bias_ids, *bias_values, *bias_starts;
+  eff_buf *mask, *mask_of;
+  uint32_t mask_count;
+} eff_logits_rules;
+
+/* out[r][v] from in[r][v], f32 rows `stride` floats apart (0: vocab): for a token c > 0 times
+ * in the history z = z > 0 ? z / repeat : z * repeat, then z -= frequency * c +
+ * presence (each in 64 bits, rounded to f32); then z += bias; then -inf where the
+ * mask does not allow it. out may be in (the same buffer). With frequency = 0
+ * the penalties are sample()'s (sample.js:78-153), bit for bit, over a window
+ * that the caller cuts; eff_topk reads a row (base = r * stride). */
+int eff_logits_apply(eff_ctx *ctx, eff_buf *in, eff_buf *out, uint32_t rows, uint32_t vocab, uint32_t stride,
+                     const eff_logits_rules *rules);
 
 /* ---- measurement --------------------------------------------------------- */
 
