@@ -89,6 +89,8 @@ struct eff_ctx {
   int64_t sx_min_tokens = 0;        // 0: the measured default (sx_routes)
   void *act_scratch = nullptr;      // x in the CPU path's 8-bit blocks (eff_qmatmul_cpu_path)
   size_t act_scratch_bytes = 0;
+  void *attn_scratch = nullptr;     // counters and sums of eff_kv_attn's chunks
+  size_t attn_scratch_bytes = 0;
   // Pinned staging ring of eff_buf_write: the source bytes are copied here on
   // the calling thread and the device copy is enqueued from here, so a write
   // returns without waiting for the device. `pend` holds the ring ranges whose
@@ -555,6 +557,7 @@ int eff_shutdown(eff_ctx *ctx) {
   if (ctx->xh_scratch) (void)hipFree(ctx->xh_scratch);
   if (ctx->sx_scratch) (void)hipFree(ctx->sx_scratch);
   if (ctx->act_scratch) (void)hipFree(ctx->act_scratch);
+  if (ctx->attn_scratch) (void)hipFree(ctx->attn_scratch);
   if (ctx->sk_scratch) (void)hipFree(ctx->sk_scratch);
   if (ctx->sxt_scratch) (void)hipFree(ctx->sxt_scratch);
   for (void *p : ctx->kept) (void)hipFree(p);
@@ -1495,8 +1498,8 @@ int kv_views(eff_ctx *ctx, const eff_kv_cache *c, const eff_kv_batch *b, KvView 
   if (b->max_len > (uint64_t)b->table_pages * c->page_tokens)
     return fail(ctx, EFF_E_BOUNDS, "%s: max_len=%u and the table has %u pages of %u tokens", who, b->max_len,
                 b->table_pages, c->page_tokens);
-  if (b->max_len > 0x7FFFFFFFu || b->tokens > 0x7FFFFFFFu || b->seqs > 0x7FFFFFFFu)
-    return fail(ctx, EFF_E_SHAPE, "%s: max_len=%u tokens=%u seqs=%u: below 2^31", who, b->max_len, b->tokens, b->seqs);
+  if (b->max_len > 1u << 30 || b->tokens > 1u << 30 || b->seqs > 1u << 30)
+    return fail(ctx, EFF_E_SHAPE, "%s: max_len=%u tokens=%u seqs=%u: at most 2^30", who, b->max_len, b->tokens, b->seqs);
   if ((rc = check_out(ctx, b->table, 4ull * b->seqs * b->table_pages, who)) ||
       (rc = check_out(ctx, b->starts, 4ull * (b->seqs + 1ull), who)) ||
       (rc = check_out(ctx, b->lens, 4ull * b->seqs, who)))
@@ -1647,7 +1650,12 @@ int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *bat
   if ((uint64_t)b.tokens * q_heads > 0x7FFFFFFFull)
     return fail(ctx, EFF_E_SHAPE, "kv attn: %u tokens of %u heads", b.tokens, q_heads);
   if ((rc = use_device(ctx))) return rc;
-  hipError_t e = launch_kv_attn(kv, b, a, ctx->stream);
+  // the joined chunks' scratch: its counters are zeroed when it is made
+  const size_t need = kv_attn_scratch(kv, b, a), before = ctx->attn_scratch_bytes;
+  if ((rc = grow(ctx, &ctx->attn_scratch, &ctx->attn_scratch_bytes, need, "attention"))) return rc;
+  if (ctx->attn_scratch_bytes != before)
+    EFF_HIP(ctx, hipMemsetAsync(ctx->attn_scratch, 0, kAttnCounters * 4u, ctx->stream));
+  hipError_t e = launch_kv_attn(kv, b, a, ctx->attn_scratch, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "kv attn launch");
   ++ctx->stats.kv_attn;
   return EFF_OK;

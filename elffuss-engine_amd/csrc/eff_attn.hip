@@ -3,92 +3,610 @@
 //   s_t = scale * q . k_t  for the tokens t the row sees: those up to its own
 //         position, the last `window` of them if there is one
 //   out = sum_t softmax(s)_t v_t;  a row that sees nothing is zeros
-// The softmax is taken in one pass with the running maximum and sum.
+//
+// Rows are (new token, query head of the group): the query heads that share a
+// key/value head are rows of one tile, so a cached row is read once for all of
+// them. A wave takes 32 cached tokens a step, in registers from end to end:
+//   S' = K q'   16 tokens x 16 rows per v_mfma_f32_16x16x32_f16: lane (n, g) =
+//               (lane % 16, lane / 16) gets row n's scores of tokens 4 g .. 4 g + 3
+//   P           the running maximum and sum of row n live in its 4 lanes
+//   O' += V' P' the same lanes hold what the second operand needs: 8 of the 32
+//               tokens of row n, and V's operand is 8 rows of V, 2 E bytes each,
+//               turned in the lane with v_perm (E = D / 16 columns of a lane)
+// so neither scores nor weights ever leave the lane.
+//
+// Precision. q (scaled by a power of two to a row maximum of 2^13) and p (scaled
+// by 2^14) are split in two fp16 parts, 22 bits, each its own matrix step; the
+// cached fp16 or int8 values are exact operands; sums are f32. An int8 row's scale
+// multiplies its scores, and its weight relative to the largest value scale
+// the row has seen (so that the weight's fp16 parts stay in range).
+#include <algorithm>
+
 #include "eff_device.h"
 #include "eff_kv.h"
 
 namespace eff {
 
-// One workgroup per row (new token and query head): a wave per cached token,
-// the lanes over the head's values.
-template <int TYPE, int D>
-__global__ __launch_bounds__(256) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a) {
-  constexpr int N = (D + 63) / 64;
-  __shared__ float sm[4], sl[4], so[4][D];
-  const uint32_t t = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t kvh = h / (a.q_heads / kv.heads);
-  const uint32_t s = kv_seq_of(b, t);
-  if (s >= b.seqs) return;
-  const uint32_t n = b.starts[s + 1] - b.starts[s], len = kv_len(b, s), back = n - (t - b.starts[s]);
-  const uint32_t end = back <= len ? len - back + 1u : 0u;   // the row sees [first, end)
-  const uint32_t first = a.window && end > a.window ? end - a.window : 0u;
-  float q[N], o[N], m = -INFINITY, l = 0.f;
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// int8 quants (with the sign bit flipped: 0 .. 255) in the low bytes of fp16
+// 1024 + u, less 1152: exact.
+__device__ __forceinline__ uint32_t i8_half2(uint32_t bits) {
+  const half2v c = {(_Float16)1152.f, (_Float16)1152.f};
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, bits) - c);
+}
+
+__device__ __forceinline__ half8 i8_half8(uint32_t a, uint32_t b) {
+  a ^= 0x80808080u, b ^= 0x80808080u;
+  const uint32_t k = 0x64646464u;
+  const u32x4 v = {i8_half2(__builtin_amdgcn_perm(k, a, 0x04010400u)), i8_half2(__builtin_amdgcn_perm(k, a, 0x04030402u)),
+                   i8_half2(__builtin_amdgcn_perm(k, b, 0x04010400u)), i8_half2(__builtin_amdgcn_perm(k, b, 0x04030402u))};
+  return __builtin_bit_cast(half8, v);
+}
+
+template <int N>
+__device__ __forceinline__ void ld_words(uint32_t *o, const uint8_t *p) {
+  if constexpr (N == 1) {
+    *o = *(const uint32_t *)p;
+  } else if constexpr (N == 2) {
+    const uint2 v = *(const uint2 *)p;
+    o[0] = v.x, o[1] = v.y;
+  } else {
+    const u32x4 v = *(const u32x4 *)p;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint32_t d = lane + 64u * i;
-    q[i] = d < (uint32_t)D ? a.q[(uint64_t)t * a.q_stride + h * D + d] * a.scale : 0.f;
-    o[i] = 0.f;
-  }
-  for (uint32_t p = first + wave; p < end; p += 4u) {
-    const uint32_t page = b.table[(uint64_t)s * b.table_pages + (p >> kv.page_log2)];
-    if (page >= kv.pages) continue;
-    const uint32_t slot = p & ((1u << kv.page_log2) - 1u);
-    const uint8_t *kb = kv.base + (uint64_t)page * kv.page_bytes + (uint64_t)kvh * kv.block_bytes;
-    const uint8_t *vb = kb + (uint64_t)kv.heads * kv.block_bytes;
-    float k[N], v[N], dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t d = lane + 64u * i, at = slot * D + (d < (uint32_t)D ? d : 0u);
-      if constexpr (TYPE == EFF_KV_F16) {
-        k[i] = (float)((const _Float16 *)kb)[at];
-        v[i] = (float)((const _Float16 *)vb)[at];
-      } else {
-        const uint64_t so = (uint64_t)D << kv.page_log2;
-        k[i] = (float)((const int8_t *)kb)[at] * ((const float *)(kb + so))[slot];
-        v[i] = (float)((const int8_t *)vb)[at] * ((const float *)(vb + so))[slot];
-      }
-      if (d < (uint32_t)D) dot += q[i] * k[i];
-    }
-    dot = wave_sum(dot);
-    const float mn = fmaxf(m, dot), al = m == mn ? 1.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(dot - mn);
-    l = l * al + w;
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * al + w * v[i];
-    m = mn;
-  }
-  if (lane == 0u) sm[wave] = m, sl[wave] = l;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (lane + 64u * i < (uint32_t)D) so[wave][lane + 64u * i] = o[i];
-  __syncthreads();
-  float mm = -INFINITY;
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w]);
-  for (uint32_t d = threadIdx.x; d < (uint32_t)D; d += 256u) {
-    float sum = 0.f, tot = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      const float f = sm[w] == -INFINITY ? 0.f : expf(sm[w] - mm);
-      tot += f * sl[w];
-      sum += f * so[w][d];
-    }
-    a.out[((uint64_t)t * a.q_heads + h) * D + d] = tot == 0.f ? 0.f : sum / tot;
+    for (int i = 0; i < 4; ++i) o[i] = v[i];
   }
 }
 
-template <int TYPE>
-static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, hipStream_t s) {
-  const dim3 grid(a.q_heads, b.tokens);
-  switch (kv.dim) {
-    case 64: hipLaunchKernelGGL((k_attn<TYPE, 64>), grid, dim3(256), 0, s, kv, b, a); break;
-    case 96: hipLaunchKernelGGL((k_attn<TYPE, 96>), grid, dim3(256), 0, s, kv, b, a); break;
-    case 128: hipLaunchKernelGGL((k_attn<TYPE, 128>), grid, dim3(256), 0, s, kv, b, a); break;
-    case 256: hipLaunchKernelGGL((k_attn<TYPE, 256>), grid, dim3(256), 0, s, kv, b, a); break;
-    default: return hipErrorInvalidValue;
+// Maximum over the 4 lanes that hold a row.
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+
+__device__ __forceinline__ float row_add(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// The rows of a tile, their tokens and what they see.
+struct AttnTile {
+  uint32_t seq, token0;   // the sequence's first new token
+  uint32_t r0, rows;      // rows r0 .. r0 + rows - 1 of the sequence's n * group
+  int first, last;        // positions of the first and last row
+  int begin, end;         // the cached tokens that any row sees
+};
+
+// The tile of a workgroup: `per_seq` tiles of each sequence, or (per_seq = 0)
+// the tiles of the sequences one after the other.
+template <uint32_t R>
+__device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, uint32_t window, uint32_t tile,
+                                          uint32_t per_seq, AttnTile &t) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t sub;
+  if (per_seq) {
+    t.seq = tile / per_seq, sub = tile % per_seq;
+  } else {
+    uint32_t base = 0;
+    t.seq = b.seqs;
+    sub = 0;
+    for (uint32_t at = 0; at < b.seqs; at += 64u) {
+      const uint32_t i = at + lane;
+      uint32_t n = 0;
+      if (i < b.seqs) {
+        const uint32_t s0 = b.starts[i], s1 = b.starts[i + 1];
+        n = s1 > s0 ? (min(s1 - s0, b.max_new) * group + R - 1u) / R : 0u;
+      }
+      uint32_t sum = n;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(sum, o);
+        if ((int)lane >= o) sum += u;
+      }
+      const uint64_t past = __ballot(base + sum > tile);
+      if (past) {
+        const int l = __ffsll((unsigned long long)past) - 1;
+        t.seq = at + l;
+        sub = tile - (base + __shfl(sum - n, l));
+        break;
+      }
+      base += __shfl(sum, 63);
+    }
   }
+  if (t.seq >= b.seqs) return false;
+  t.seq = __builtin_amdgcn_readfirstlane(t.seq);
+  sub = __builtin_amdgcn_readfirstlane(sub);
+  const uint32_t s0 = __builtin_amdgcn_readfirstlane(b.starts[t.seq]);
+  const uint32_t s1 = min((uint32_t)__builtin_amdgcn_readfirstlane(b.starts[t.seq + 1]), b.tokens);
+  const uint32_t n = s1 > s0 ? min(s1 - s0, b.max_new) : 0u;
+  t.token0 = s0;
+  t.r0 = sub * R;
+  if (t.r0 >= n * group) return false;
+  t.rows = min(R, n * group - t.r0);
+  const int len = __builtin_amdgcn_readfirstlane((int)kv_len(b, t.seq));
+  t.first = len - (int)n + (int)(t.r0 / group);
+  t.last = len - (int)n + (int)((t.r0 + t.rows - 1u) / group);
+  t.end = max(t.last + 1, 0);
+  t.begin = window ? max(0, t.first - (int)min(window, 0x40000000u) + 1) : 0;
+  return true;
+}
+
+// One wave's share of a tile of 16 MT rows.
+template <int TYPE, int D, int MT>
+struct AttnWave {
+  static constexpr bool I8 = TYPE == EFF_KV_I8;
+  static constexpr int E = D / 16;                     // columns of a lane
+  static constexpr int KS = D / 32;                    // matrix steps of a score
+  static constexpr int KW = I8 ? 2 : 4;                // words of a lane's part of a step of K
+  static constexpr int VW = I8 ? (E + 3) / 4 : E / 2;  // words of a lane's part of a row of V
+  static constexpr int ROW = I8 ? D : 2 * D;           // bytes of a cached row
+
+  half8 qh[MT][KS], ql[MT][KS];
+  float sc[MT];            // what a raw score of row n is multiplied by (log2 e included)
+  int pos[MT];             // the row's position, -1 for none
+  float m[MT], l[MT];      // running maximum (log2), and this lane's share of the sum
+  float vref[MT], vinv[MT];   // I8: the largest value scale so far, and its reciprocal
+  float4v acc[MT][E];
+
+  uint32_t kw[2][KS * KW];
+  uint32_t ks[2][4];     // I8: the scales of the lane's tokens (f32 bits)
+  uint32_t vw[8][VW];
+  uint32_t vs[2][4];
+
+  // column of acc[.][i][j] of lane group g: lanes hold 4 columns of the first
+  // 64, and at D = 96 2 of the last 32; else E side by side
+  static __device__ __forceinline__ uint32_t column(uint32_t g, int i, int j) {
+    if constexpr (D == 96) return i < 4 ? 4u * (4u * g + j) + i : 64u + 2u * (4u * g + j) + (i - 4);
+    return (uint32_t)E * (4u * g + j) + i;
+  }
+
+  __device__ __forceinline__ void init(const KvBatchView &b, const KvAttnArgs &a, const AttnTile &t, uint32_t group, uint32_t kvh,
+                                       uint32_t row0, uint32_t n, uint32_t g) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const uint32_t r = row0 + 16u * mt + n;
+      const bool on = r < t.rows;
+      const uint32_t tok = (t.r0 + (on ? r : 0u)) / group, h = (t.r0 + (on ? r : 0u)) % group;
+      const float *src = a.q + (uint64_t)(t.token0 + tok) * a.q_stride + (kvh * group + h) * D;
+      float q[KS][8], top = 0.f;
+#pragma unroll
+      for (int c = 0; c < KS; ++c) {
+        uint32_t d;
+        if constexpr (I8) d = 2 * (c / 2) + 1 < KS ? 64u * (c / 2) + 16u * g + 8u * (c & 1) : 32u * c + 8u * g;
+        else d = 32u * c + 8u * g;
+        const float4 u = *(const float4 *)(src + d), w = *(const float4 *)(src + d + 4);
+        const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          q[c][i] = on ? x[i] : 0.f;
+          top = fmaxf(top, fabsf(q[c][i]));
+        }
+      }
+      top = row_max(top);
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
+      const float up = ldexpf(1.f, 13 - e);
+      sc[mt] = a.scale * 1.44269504088896341f * ldexpf(1.f, e - 13);
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = q[c][i] * up;
+          qh[mt][c][i] = (_Float16)x;
+          ql[mt][c][i] = (_Float16)(x - (float)qh[mt][c][i]);
+        }
+      pos[mt] = on ? t.first + (int)(tok - t.r0 / group) : -1;
+      m[mt] = -INFINITY, l[mt] = 0.f, vref[mt] = 0.f, vinv[mt] = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[mt][i] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // K of the 16 tokens from `blk`'s slot `slot` on, into half u of the step.
+  __device__ __forceinline__ void load_k(int u, const uint8_t *blk, uint32_t slot, uint32_t page_log2, uint32_t n, uint32_t g) {
+    const uint8_t *p = blk + slot * ROW;
+    if constexpr (!I8) {
+#pragma unroll
+      for (int c = 0; c < KS; ++c) ld_words<4>(kw[u] + 4 * c, p + (n * ROW + 16u * g) + 64u * c);
+    } else {
+#pragma unroll
+      for (int c = 0; c + 1 < KS; c += 2) ld_words<4>(kw[u] + 2 * c, p + (n * ROW + 16u * g) + 32u * c);
+      if constexpr (KS & 1) ld_words<2>(kw[u] + 2 * (KS - 1), p + (n * ROW + 8u * g) + 32u * (KS - 1));
+      ld_words<4>(ks[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
+    }
+  }
+
+  __device__ __forceinline__ void load_v(int u, const uint8_t *blk, uint32_t slot, uint32_t page_log2, uint32_t n, uint32_t g) {
+    const uint8_t *p = blk + slot * ROW;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint8_t *r = p + 4u * g * ROW + j * ROW;
+      uint32_t *o = vw[4 * u + j];
+      if constexpr (D == 96 && I8) {
+        o[0] = *(const uint32_t *)(r + 4u * n);
+        o[1] = *(const uint16_t *)(r + 64 + 2u * n);
+      } else if constexpr (D == 96) {
+        ld_words<2>(o, r + 8u * n);
+        o[2] = *(const uint32_t *)(r + 128 + 4u * n);
+      } else if constexpr (VW == 8) {
+        ld_words<4>(o, r + 32u * n);
+        ld_words<4>(o + 4, r + 32u * n + 16);
+      } else {
+        ld_words<VW>(o, r + 4u * VW * n);
+      }
+    }
+    if constexpr (I8) ld_words<4>(vs[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
+  }
+
+  // Column i of the 8 tokens of the lane as the first operand; with PART only of
+  // the tokens whose bit is set in `on`.
+  template <bool PART = false>
+  __device__ __forceinline__ half8 v_operand(int i, uint32_t on = 0) const {
+    u32x4 o;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if constexpr (I8) {
+        const uint32_t w = i / 4, k = i % 4;
+        const uint32_t sel = 0x0C000C00u | k | ((4u + k) << 16);
+        o[x] = i8_half2(__builtin_amdgcn_perm(vw[2 * x + 1][w] ^ 0x80808080u, vw[2 * x][w] ^ 0x80808080u, sel) | 0x64006400u);
+      } else {
+        o[x] = __builtin_amdgcn_perm(vw[2 * x + 1][i / 2], vw[2 * x][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+        if constexpr (PART) o[x] &= (on >> (2 * x) & 1u ? 0xFFFFu : 0u) | (on >> (2 * x + 1) & 1u ? 0xFFFF0000u : 0u);
+      }
+    }
+    return __builtin_bit_cast(half8, o);
+  }
+
+  // The step at token t0: scores, weights and the weighted sum. `masked`: some
+  // row does not see every one of its 32 tokens (wave-uniform); a half without
+  // a page is `gone`.
+  __device__ __forceinline__ void scores(float s[MT][2][4]) const {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float4v c[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) c[mt] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        half8 a;
+        if constexpr (I8) a = i8_half8(kw[u][2 * k], kw[u][2 * k + 1]);
+        else a = __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          c[mt] = mfma(a, qh[mt][k], c[mt]);
+          c[mt] = mfma(a, ql[mt][k], c[mt]);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[mt][u][j] = c[mt][j] * (I8 ? sc[mt] * __uint_as_float(ks[u][j]) : sc[mt]);
+    }
+  }
+
+  // Whether the row of tile mt sees token t0 + 16 u + 4 g + j.
+  static __device__ __forceinline__ bool sees(int pos, int window, int t) { return t <= pos && (window == 0 || t > pos - window); }
+
+  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[MT][2][4]) {
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = t0 + 16 * u + 4 * (int)g + j;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            if (gone[u] || !sees(pos[mt], window, at)) s[mt][u][j] = -INFINITY;
+          // what no row sees may be any bits
+          if (gone[u] || at < t.begin || at >= t.end) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vw[4 * u + j][w] = 0u;
+            if constexpr (I8) vs[u][j] = 0u;
+          }
+        }
+    }
+    half8 ph[MT], pl[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
+                       fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3])));
+      mx = row_max(mx);
+      float vx = 0.f;
+      if constexpr (I8) {
+        // of the tokens that the row sees only: another row's may not be finite
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vx = fmaxf(vx, !masked || s[mt][u][j] != -INFINITY ? __uint_as_float(vs[u][j]) : 0.f);
+        vx = row_max(vx);
+      }
+      if (__any(mx > m[mt] || (I8 && vx > vref[mt]))) {
+        const float mn = fmaxf(m[mt], mx);
+        const float al = m[mt] == mn ? 1.f : __builtin_amdgcn_exp2f(m[mt] - mn);
+        m[mt] = mn;
+        l[mt] *= al;
+        float f = al;
+        if constexpr (I8) {
+          if (vx > vref[mt]) {
+            const float vn = fmaxf(vx, 1e-30f);
+            f = al * (vref[mt] / vn);
+            vref[mt] = vn;
+            vinv[mt] = 1.f / vn;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[mt][i] *= f;
+      }
+      const float mm = m[mt] == -INFINITY ? 0.f : m[mt] - 14.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float p = __builtin_amdgcn_exp2f(s[mt][u][j] - mm);
+          sum += p;
+          // a weight of nothing takes nothing of a scale that is not finite
+          if constexpr (I8) p = masked && s[mt][u][j] == -INFINITY ? 0.f : p * (__uint_as_float(vs[u][j]) * vinv[mt]);
+          const _Float16 h = (_Float16)p;
+          ph[mt][4 * u + j] = h;
+          pl[mt][4 * u + j] = (_Float16)(p - (float)h);
+        }
+      l[mt] += sum;
+    }
+    if constexpr (!I8) {
+      // A value that only some rows see and that is not finite: 0 * inf would
+      // reach the others. One position's rows at a time, with what they do not
+      // see cleared.
+      if (masked && t.first != t.last) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            const uint32_t x = vw[k][w] & 0x7FFF7FFFu;
+            top = max(top, max(x & 0xFFFFu, x >> 16));
+          }
+        if (__any(top >= 0x7C00u)) {
+          apart(t0, t, window, g, ph, pl);
+          return;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const half8 a = v_operand(i);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        acc[mt][i] = mfma(a, ph[mt], acc[mt][i]);
+        acc[mt][i] = mfma(a, pl[mt], acc[mt][i]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void apart(int t0, const AttnTile &t, int window, uint32_t g, const half8 *ph, const half8 *pl) {
+#pragma unroll 1
+    for (int p = t.first; p <= t.last; ++p) {
+      uint32_t on = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (sees(p, window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4)) on |= 1u << k;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const half8 a = v_operand<true>(i, on);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float4v c = {0.f, 0.f, 0.f, 0.f};
+          c = mfma(a, ph[mt], c);
+          c = mfma(a, pl[mt], c);
+          if (pos[mt] == p) acc[mt][i] += c;
+        }
+      }
+    }
+  }
+
+  // The steps of the tokens lo + 32 k of every `stride`, up to hi. Page numbers
+  // are read 32 steps ahead, one in each lane.
+  __device__ __forceinline__ void run(const KvView &kv, const KvBatchView &b, const AttnTile &t, uint32_t kvh, int window, int lo,
+                                      int hi, int stride, uint32_t n, uint32_t g) {
+    const uint32_t *table = b.table + (uint64_t)t.seq * b.table_pages;
+    const uint32_t lane = threadIdx.x & 63u, mask = (1u << kv.page_log2) - 1u;
+    const uint64_t head = (uint64_t)kvh * kv.block_bytes, to_v = (uint64_t)kv.heads * kv.block_bytes;
+    if (lo >= hi) return;
+    uint32_t ids = 0;
+    const uint8_t *blk[2];
+    bool gone[2];
+    auto find = [&](int i, int t0) {   // the pages of step i's two halves
+      if ((i & 31) == 0) {
+        const int at = t0 + (int)(lane >> 1) * stride + 16 * (int)(lane & 1u);
+        ids = at < hi ? table[(uint32_t)at >> kv.page_log2] : ~0u;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t p = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + u);
+        gone[u] = p >= kv.pages;
+        blk[u] = kv.base + (gone[u] ? 0ull : (uint64_t)p * kv.page_bytes) + head;
+      }
+    };
+    find(0, lo);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_k(u, blk[u], (uint32_t)(lo + 16 * u) & mask, kv.page_log2, n, g);
+    int i = 0;
+#pragma unroll 1
+    for (int t0 = lo; t0 < hi; t0 += stride, ++i) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) load_v(u, blk[u] + to_v, (uint32_t)(t0 + 16 * u) & mask, kv.page_log2, n, g);
+      float s[MT][2][4];
+      scores(s);
+      const bool was[2] = {gone[0], gone[1]};
+      const bool masked = was[0] || was[1] || t0 + 31 > t.first || t0 + 32 > hi || t0 < t.begin || (window && t0 <= t.last - window);
+      if (t0 + stride < hi) {
+        find(i + 1, t0 + stride);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) load_k(u, blk[u], (uint32_t)(t0 + stride + 16 * u) & mask, kv.page_log2, n, g);
+      }
+      step(t0, masked, was, t, window, g, s);
+    }
+  }
+};
+
+struct AttnPlan {
+  uint32_t tiles, per_seq;    // row tiles; tiles of each sequence (0: packed)
+  uint32_t chunk, chunks;     // cached tokens of a workgroup, chunks of a tile at most
+  uint32_t rows;              // rows of a tile at most
+};
+
+// The joined sums of chunks: per (tile, head) the chunks' weighted sums, then
+// their maxima and sums.
+__host__ __device__ constexpr uint64_t attn_part_floats(const AttnPlan &p, uint32_t dim) {
+  return (uint64_t)p.chunks * p.rows * (dim + 2u);
+}
+
+constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
+
+// Four waves take the 32-token steps of a chunk in turn; their sums meet in
+// LDS. Where a tile has several chunks, the last workgroup of the tile to arrive
+// joins them, in chunk order; stores and loads of the chunks' sums go past the
+// XCD's L2 (sc1), every wave waits for its stores before the barrier ahead of the
+// counter's increment, and the counter is left at zero for the next launch.
+template <int TYPE, int D, int MT>
+__global__ __launch_bounds__(256) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
+  using W = AttnWave<TYPE, D, MT>;
+  constexpr uint32_t R = 16u * MT, LD = D + 4u;
+  __shared__ float so[4][R][LD];
+  __shared__ float sm[4][R], sl[4][R], sv[4][R];
+  __shared__ uint32_t arrived;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
+  const uint32_t group = a.q_heads / kv.heads;
+  const uint32_t kvh = blockIdx.x % kv.heads, w0 = blockIdx.x / kv.heads, chunk = w0 % p.chunks, tile = w0 / p.chunks;
+  AttnTile t;
+  if (!attn_tile<R>(b, group, a.window, tile, p.per_seq, t)) return;
+  const int window = (int)min(a.window, 0x40000000u), base = t.begin & ~31;
+  const uint32_t chunks = t.end > base ? ((uint32_t)(t.end - base) + p.chunk - 1u) / p.chunk : 1u;
+  if (chunk >= chunks) return;
+  const int lo = base + (int)(chunk * p.chunk), hi = min(lo + (int)p.chunk, t.end);
+  W w;
+  w.init(b, a, t, group, kvh, 0, n, g);
+  w.run(kv, b, t, kvh, window, lo + 32 * (int)wave, hi, 128, n, g);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const float l = row_add(w.l[mt]);
+    if (g == 0u) sm[wave][16 * mt + n] = w.m[mt], sl[wave][16 * mt + n] = l, sv[wave][16 * mt + n] = w.vref[mt];
+#pragma unroll
+    for (int i = 0; i < W::E; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) so[wave][16 * mt + n][W::column(g, i, j)] = w.acc[mt][i][j];
+  }
+  __syncthreads();
+  const uint64_t at = ((uint64_t)tile * kv.heads + kvh) * attn_part_floats(p, D);
+  const rsrc_t prs = make_rsrc(part + at, attn_part_floats(p, D) * 4u);
+  const uint32_t ml = p.chunks * p.rows * D;   // where the maxima and sums begin
+  for (uint32_t i = tid; i < t.rows * (D / 4u); i += 256u) {
+    const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u));
+    float mx = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) mx = fmaxf(mx, sm[v][r]);
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float f = sm[v][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[v][r] - mx);
+      l += f * sl[v][r];
+      const float4v x = *(const float4v *)&so[v][r][d];
+      o += x * (W::I8 ? f * sv[v][r] : f);
+    }
+    if (chunks == 1u) {
+      const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+      float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+      *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+    } else {
+      const uint32_t row = chunk * p.rows + r;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((row * D + d) * 4u), 0, kSc1);
+      if (d == 0u) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((ml + 2u * row) * 4u), 0, kSc1);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((ml + 2u * row + 1u) * 4u), 0, kSc1);
+      }
+    }
+  }
+  if (chunks == 1u) return;
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint32_t *c = cnt + (uint64_t)tile * kv.heads + kvh;
+  if (tid == 0u) arrived = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived != chunks - 1u) return;
+  if (tid == 0u) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (uint32_t i = tid; i < t.rows * (D / 4u); i += 256u) {
+    const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u));
+    float mx = -INFINITY, l = 0.f;
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t z = 0; z < chunks; ++z)
+      mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * (z * p.rows + r)) * 4u), 0, kSc1)));
+    for (uint32_t z = 0; z < chunks; ++z) {
+      const uint32_t row = z * p.rows + r;
+      const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * row) * 4u), 0, kSc1));
+      const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * row + 1u) * 4u), 0, kSc1));
+      const float4v x = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)((row * D + d) * 4u), 0, kSc1));
+      const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
+      l += f * lz;
+      o += x * f;
+    }
+    const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+    float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+    *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+  }
+}
+
+static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a) {
+  const uint32_t group = a.q_heads / kv.heads;
+  constexpr uint32_t R = 16u;
+  AttnPlan p{};
+  const uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group;
+  const uint64_t each = (most + R - 1u) / R, direct = each * b.seqs, packed = (uint64_t)b.tokens * group / R + b.seqs;
+  p.per_seq = direct <= packed ? (uint32_t)each : 0u;
+  p.tiles = (uint32_t)std::min(direct, packed);
+  p.rows = (uint32_t)std::min<uint64_t>(most, R);
+  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
+  const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
+  uint64_t chunk = (span * wgs / 4096u + 127u) / 128u * 128u;
+  chunk = std::min<uint64_t>(std::max<uint64_t>(chunk, 256u), std::max<uint64_t>((span + 127u) / 128u * 128u, 128u));
+  if (wgs > kAttnCounters) chunk = (span + 127u) / 128u * 128u;
+  p.chunk = (uint32_t)chunk;
+  p.chunks = (uint32_t)((span + chunk - 1u) / chunk);
+  return p;
+}
+
+size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a) {
+  const AttnPlan p = attn_plan(kv, b, a);
+  return p.chunks > 1u ? kAttnCounters * 4u + (uint64_t)p.tiles * kv.heads * attn_part_floats(p, kv.dim) * 4u : 0u;
+}
+
+template <int TYPE, int D>
+static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t s) {
+  const AttnPlan p = attn_plan(kv, b, a);
+  const uint64_t grid = (uint64_t)p.tiles * p.chunks * kv.heads;
+  if (grid > 0x7FFFFFFFull || (p.chunks > 1u && !scratch)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((k_attn<TYPE, D, 1>), dim3((uint32_t)grid), dim3(256), 0, s, kv, b, a, p, (uint32_t *)scratch,
+                     (float *)((uint8_t *)scratch + kAttnCounters * 4u));
   return hipGetLastError();
 }
 
-hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, hipStream_t stream) {
-  return kv.type == EFF_KV_F16 ? attn_go<EFF_KV_F16>(kv, b, a, stream) : attn_go<EFF_KV_I8>(kv, b, a, stream);
+template <int TYPE>
+static hipError_t attn_dim(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t s) {
+  switch (kv.dim) {
+    case 64: return attn_go<TYPE, 64>(kv, b, a, scratch, s);
+    case 96: return attn_go<TYPE, 96>(kv, b, a, scratch, s);
+    case 128: return attn_go<TYPE, 128>(kv, b, a, scratch, s);
+    case 256: return attn_go<TYPE, 256>(kv, b, a, scratch, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t stream) {
+  return kv.type == EFF_KV_F16 ? attn_dim<EFF_KV_F16>(kv, b, a, scratch, stream) : attn_dim<EFF_KV_I8>(kv, b, a, scratch, stream);
 }
 
 }  // namespace eff

@@ -68,7 +68,12 @@ struct RopeFreqs {
 hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positions, float scale, float *out,
                              hipStream_t stream);
 hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t stream);
-hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, hipStream_t stream);
+// The scratch of the joined chunks (0: none): counters, zero before the first
+// launch and left zero by each, then the chunks' sums.
+constexpr uint32_t kAttnCounters = 65536;
+size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a);
+hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch,
+                          hipStream_t stream);
 
 struct LogitsArgs {
   const float *in;
