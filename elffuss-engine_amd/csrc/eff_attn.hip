@@ -166,15 +166,15 @@ struct AttnWave {
     return (uint32_t)E * (4u * g + j) + i;
   }
 
-  __device__ __forceinline__ void init(const KvBatchView &b, const KvAttnArgs &a, const AttnTile &t, uint32_t group, uint32_t kvh,
-                                       uint32_t row0, uint32_t n, uint32_t g) {
+  // The rows' q as it is in memory; invalid rows read the tile's first.
+  __device__ __forceinline__ void load_q(float q[MT][KS][8], const KvAttnArgs &a, const AttnTile &t, uint32_t group, uint32_t kvh,
+                                         uint32_t row0, uint32_t n, uint32_t g) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const uint32_t r = row0 + 16u * mt + n;
       const bool on = r < t.rows;
       const uint32_t tok = (t.r0 + (on ? r : 0u)) / group, h = (t.r0 + (on ? r : 0u)) % group;
       const float *src = a.q + (uint64_t)(t.token0 + tok) * a.q_stride + (kvh * group + h) * D;
-      float q[KS][8], top = 0.f;
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
         uint32_t d;
@@ -183,24 +183,34 @@ struct AttnWave {
         const float4 u = *(const float4 *)(src + d), w = *(const float4 *)(src + d + 4);
         const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          q[c][i] = on ? x[i] : 0.f;
-          top = fmaxf(top, fabsf(q[c][i]));
-        }
+        for (int i = 0; i < 8; ++i) q[mt][c][i] = x[i];
       }
+      pos[mt] = on ? t.first + (int)(tok - t.r0 / group) : -1;
+    }
+  }
+
+  // q in its two fp16 parts, and empty sums. Rows that are none see nothing
+  // (pos -1), so what q they have does not matter.
+  __device__ __forceinline__ void init(const float q[MT][KS][8], float scale) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float top = 0.f;
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[mt][c][i]));
       top = row_max(top);
       const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
       const float up = ldexpf(1.f, 13 - e);
-      sc[mt] = a.scale * 1.44269504088896341f * ldexpf(1.f, e - 13);
+      sc[mt] = scale * 1.44269504088896341f * ldexpf(1.f, e - 13);
 #pragma unroll
       for (int c = 0; c < KS; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float x = q[c][i] * up;
+          const float x = q[mt][c][i] * up;
           qh[mt][c][i] = (_Float16)x;
           ql[mt][c][i] = (_Float16)(x - (float)qh[mt][c][i]);
         }
-      pos[mt] = on ? t.first + (int)(tok - t.r0 / group) : -1;
       m[mt] = -INFINITY, l[mt] = 0.f, vref[mt] = 0.f, vinv[mt] = 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) acc[mt][i] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -409,47 +419,51 @@ struct AttnWave {
     }
   }
 
-  // The steps of the tokens lo + 32 k of every `stride`, up to hi. Page numbers
-  // are read 32 steps ahead, one in each lane.
-  __device__ __forceinline__ void run(const KvView &kv, const KvBatchView &b, const AttnTile &t, uint32_t kvh, int window, int lo,
-                                      int hi, int stride, uint32_t n, uint32_t g) {
-    const uint32_t *table = b.table + (uint64_t)t.seq * b.table_pages;
-    const uint32_t lane = threadIdx.x & 63u, mask = (1u << kv.page_log2) - 1u;
-    const uint64_t head = (uint64_t)kvh * kv.block_bytes, to_v = (uint64_t)kv.heads * kv.block_bytes;
-    if (lo >= hi) return;
-    uint32_t ids = 0;
-    const uint8_t *blk[2];
+  // The walk over a tile's cached tokens: the steps lo, lo + stride, ... up to hi.
+  // Page numbers are read 32 steps ahead, two in each pair of lanes.
+  struct Walk {
+    const uint32_t *table;
+    const uint8_t *blk[2];   // the pages of the step's two halves
     bool gone[2];
-    auto find = [&](int i, int t0) {   // the pages of step i's two halves
-      if ((i & 31) == 0) {
-        const int at = t0 + (int)(lane >> 1) * stride + 16 * (int)(lane & 1u);
-        ids = at < hi ? table[(uint32_t)at >> kv.page_log2] : ~0u;
-      }
+    uint32_t ids;
+    int lo, hi, stride;
+  };
+
+  static __device__ __forceinline__ void read_ids(Walk &k, const KvView &kv, int t0) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const int at = t0 + (int)(lane >> 1) * k.stride + 16 * (int)(lane & 1u);
+    k.ids = at < k.hi ? k.table[(uint32_t)at >> kv.page_log2] : ~0u;
+  }
+
+  __device__ __forceinline__ void fetch_k(Walk &k, const KvView &kv, uint32_t kvh, int i, int t0, uint32_t n, uint32_t g) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t p = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + u);
-        gone[u] = p >= kv.pages;
-        blk[u] = kv.base + (gone[u] ? 0ull : (uint64_t)p * kv.page_bytes) + head;
-      }
-    };
-    find(0, lo);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) load_k(u, blk[u], (uint32_t)(lo + 16 * u) & mask, kv.page_log2, n, g);
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t p = __builtin_amdgcn_readlane(k.ids, 2 * (i & 31) + u);
+      k.gone[u] = p >= kv.pages;
+      k.blk[u] = kv.base + (k.gone[u] ? 0ull : (uint64_t)p * kv.page_bytes) + (uint64_t)kvh * kv.block_bytes;
+      load_k(u, k.blk[u], (uint32_t)(t0 + 16 * u) & ((1u << kv.page_log2) - 1u), kv.page_log2, n, g);
+    }
+  }
+
+  // The first step's keys are on their way (read_ids, fetch_k).
+  __device__ __forceinline__ void run(Walk &k, const KvView &kv, const AttnTile &t, uint32_t kvh, int window, uint32_t n, uint32_t g) {
+    const uint64_t to_v = (uint64_t)kv.heads * kv.block_bytes;
     int i = 0;
 #pragma unroll 1
-    for (int t0 = lo; t0 < hi; t0 += stride, ++i) {
+    for (int t0 = k.lo; t0 < k.hi; t0 += k.stride, ++i) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) load_v(u, blk[u] + to_v, (uint32_t)(t0 + 16 * u) & mask, kv.page_log2, n, g);
+      for (int u = 0; u < 2; ++u)
+        load_v(u, k.blk[u] + to_v, (uint32_t)(t0 + 16 * u) & ((1u << kv.page_log2) - 1u), kv.page_log2, n, g);
       float s[MT][2][4];
       scores(s);
-      const bool was[2] = {gone[0], gone[1]};
-      const bool masked = was[0] || was[1] || t0 + 31 > t.first || t0 + 32 > hi || t0 < t.begin || (window && t0 <= t.last - window);
-      if (t0 + stride < hi) {
-        find(i + 1, t0 + stride);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) load_k(u, blk[u], (uint32_t)(t0 + stride + 16 * u) & mask, kv.page_log2, n, g);
+      const bool gone[2] = {k.gone[0], k.gone[1]};
+      const bool masked = gone[0] || gone[1] || t0 + 31 > t.first || t0 < t.begin || (window && t0 <= t.last - window);
+      const int next = t0 + k.stride;
+      if (next < k.hi) {
+        if (((i + 1) & 31) == 0) read_ids(k, kv, next);
+        fetch_k(k, kv, kvh, i + 1, next, n, g);
       }
-      step(t0, masked, was, t, window, g, s);
+      step(t0, masked, gone, t, window, g, s);
     }
   }
 };
@@ -474,7 +488,7 @@ constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 // XCD's L2 (sc1), every wave waits for its stores before the barrier ahead of the
 // counter's increment, and the counter is left at zero for the next launch.
 template <int TYPE, int D, int MT>
-__global__ __launch_bounds__(256) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
   using W = AttnWave<TYPE, D, MT>;
   constexpr uint32_t R = 16u * MT, LD = D + 4u;
   __shared__ float so[4][R][LD];
@@ -490,8 +504,17 @@ __global__ __launch_bounds__(256) void k_attn(KvView kv, KvBatchView b, KvAttnAr
   if (chunk >= chunks) return;
   const int lo = base + (int)(chunk * p.chunk), hi = min(lo + (int)p.chunk, t.end);
   W w;
-  w.init(b, a, t, group, kvh, 0, n, g);
-  w.run(kv, b, t, kvh, window, lo + 32 * (int)wave, hi, 128, n, g);
+  {
+    typename W::Walk k;
+    k.table = b.table + (uint64_t)t.seq * b.table_pages;
+    k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 128;
+    W::read_ids(k, kv, k.lo);
+    float q[MT][W::KS][8];
+    w.load_q(q, a, t, group, kvh, 0, n, g);
+    w.fetch_k(k, kv, kvh, 0, k.lo, n, g);   // of the first page, where the wave has no step
+    w.init(q, a.scale);
+    w.run(k, kv, t, kvh, window, n, g);
+  }
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const float l = row_add(w.l[mt]);
@@ -539,24 +562,60 @@ __global__ __launch_bounds__(256) void k_attn(KvView kv, KvBatchView b, KvAttnAr
   __syncthreads();
   if (arrived != chunks - 1u) return;
   if (tid == 0u) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (uint32_t i = tid; i < t.rows * (D / 4u); i += 256u) {
-    const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u));
+  // the chunks' weights relative to the largest maximum, [chunk][row], and the
+  // rows' sums: a wave per row, its lanes over the chunks
+  float *wt = &so[0][0][0], *half = wt + 4u * R * LD - 1024u;
+  for (uint32_t r = wave; r < t.rows; r += 4u) {
     float mx = -INFINITY, l = 0.f;
-    float4v o = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t z = 0; z < chunks; ++z)
+    for (uint32_t z = lane; z < chunks; z += 64u)
       mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * (z * p.rows + r)) * 4u), 0, kSc1)));
-    for (uint32_t z = 0; z < chunks; ++z) {
-      const uint32_t row = z * p.rows + r;
-      const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * row) * 4u), 0, kSc1));
-      const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * row + 1u) * 4u), 0, kSc1));
-      const float4v x = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)((row * D + d) * 4u), 0, kSc1));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    for (uint32_t z = lane; z < chunks; z += 64u) {
+      const int at = (int)((ml + 2u * (z * p.rows + r)) * 4u);
+      const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
+      const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
       const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
+      wt[z * p.rows + r] = f;
       l += f * lz;
-      o += x * f;
     }
-    const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
-    float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
-    *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+    l = wave_sum(l);
+    if (lane == 0u) sl[0][r] = l;
+  }
+  __syncthreads();
+  // each thread a part of the chunks of 4 columns of a row
+  const uint32_t items = t.rows * (D / 4u), parts = max(1u, 256u / items);
+  for (uint32_t i0 = 0; i0 < items; i0 += 256u) {
+    const uint32_t part_i = parts > 1u ? tid / items : 0u, i = parts > 1u ? tid % items : i0 + tid;
+    const bool on = i < items && part_i < parts;
+    const uint32_t r = on ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    if (on) {
+      constexpr uint32_t U = 8;
+      for (uint32_t z = part_i; z < chunks; z += U * parts) {
+        float4v x[U];
+#pragma unroll
+        for (uint32_t k = 0; k < U; ++k) {
+          const uint32_t row = min(z + k * parts, chunks - 1u) * p.rows + r;
+          x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)((row * D + d) * 4u), 0, kSc1));
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < U; ++k)
+          if (z + k * parts < chunks) o += x[k] * wt[(z + k * parts) * p.rows + r];
+      }
+    }
+    if (parts > 1u) {
+      *(float4v *)(half + 4u * tid) = o;
+      __syncthreads();
+      if (on && part_i == 0u)
+        for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * items));
+    }
+    if (on && part_i == 0u) {
+      const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+      const float l = sl[0][r];
+      float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+      *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+    }
   }
 }
 
@@ -571,9 +630,15 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
-  uint64_t chunk = (span * wgs / 4096u + 127u) / 128u * 128u;
-  chunk = std::min<uint64_t>(std::max<uint64_t>(chunk, 256u), std::max<uint64_t>((span + 127u) / 128u * 128u, 128u));
-  if (wgs > kAttnCounters) chunk = (span + 127u) / 128u * 128u;
+  // Chunks of at least 1024 tokens, and then about 4096 workgroups, so that long
+  // and short sequences even out; shorter chunks only while there are below 512
+  // workgroups. The join keeps a weight for each chunk and row in LDS.
+  const uint64_t whole = (span + 127u) / 128u * 128u;
+  auto per = [&](uint64_t n) { return (span * wgs / n + 127u) / 128u * 128u; };
+  uint64_t chunk = std::max(per(4096u), std::min<uint64_t>(1024u, std::max<uint64_t>(per(512u), 256u)));
+  const uint64_t most_chunks = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;
+  chunk = std::min(std::max(chunk, (span / most_chunks + 128u) / 128u * 128u), whole);
+  if (wgs > kAttnCounters) chunk = whole;
   p.chunk = (uint32_t)chunk;
   p.chunks = (uint32_t)((span + chunk - 1u) / chunk);
   return p;
