@@ -137,8 +137,9 @@ __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, 
   return true;
 }
 
-// One wave's share of a tile of 16 MT rows.
-template <int TYPE, int D, int MT>
+// One wave's share of a tile of 16 MT rows. QL: the parts of q are in LDS, shared
+// by the waves of the tile, and read for each step.
+template <int TYPE, int D, int MT, bool QL>
 struct AttnWave {
   static constexpr bool I8 = TYPE == EFF_KV_I8;
   static constexpr int E = D / 16;                     // columns of a lane
@@ -147,7 +148,8 @@ struct AttnWave {
   static constexpr int VW = I8 ? (E + 3) / 4 : E / 2;  // words of a lane's part of a row of V
   static constexpr int ROW = I8 ? D : 2 * D;           // bytes of a cached row
 
-  half8 qh[MT][KS], ql[MT][KS];
+  half8 qh[QL ? 1 : MT][QL ? 1 : KS], ql[QL ? 1 : MT][QL ? 1 : KS];
+  const uint8_t *qs;       // QL: [mt][step][part][lane] of 16 bytes
   float sc[MT];            // what a raw score of row n is multiplied by (log2 e included)
   int pos[MT];             // the row's position, -1 for none
   float m[MT], l[MT];      // running maximum (log2), and this lane's share of the sum
@@ -191,7 +193,8 @@ struct AttnWave {
 
   // q in its two fp16 parts, and empty sums. Rows that are none see nothing
   // (pos -1), so what q they have does not matter.
-  __device__ __forceinline__ void init(const float q[MT][KS][8], float scale) {
+  __device__ __forceinline__ void init(const float q[MT][KS][8], float scale, uint8_t *lds, uint32_t wave, uint32_t waves) {
+    qs = lds + 16u * (threadIdx.x & 63u);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float top = 0.f;
@@ -205,12 +208,21 @@ struct AttnWave {
       sc[mt] = scale * 1.44269504088896341f * ldexpf(1.f, e - 13);
 #pragma unroll
       for (int c = 0; c < KS; ++c)
+      {
+        half8 h, r;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float x = q[mt][c][i] * up;
-          qh[mt][c][i] = (_Float16)x;
-          ql[mt][c][i] = (_Float16)(x - (float)qh[mt][c][i]);
+          h[i] = (_Float16)x;
+          r[i] = (_Float16)(x - (float)h[i]);
         }
+        if constexpr (!QL) {
+          qh[mt][c] = h, ql[mt][c] = r;
+        } else if ((mt * KS + c) % waves == wave) {
+          *(half8 *)(const_cast<uint8_t *>(qs) + (mt * KS + c) * 2048) = h;
+          *(half8 *)(const_cast<uint8_t *>(qs) + (mt * KS + c) * 2048 + 1024) = r;
+        }
+      }
       m[mt] = -INFINITY, l[mt] = 0.f, vref[mt] = 0.f, vinv[mt] = 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) acc[mt][i] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -253,10 +265,8 @@ struct AttnWave {
     if constexpr (I8) ld_words<4>(vs[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
   }
 
-  // Column i of the 8 tokens of the lane as the first operand; with PART only of
-  // the tokens whose bit is set in `on`.
-  template <bool PART = false>
-  __device__ __forceinline__ half8 v_operand(int i, uint32_t on = 0) const {
+  // Column i of the 8 tokens of the lane as the first operand.
+  __device__ __forceinline__ u32x4 v_operand(int i) const {
     u32x4 o;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -266,10 +276,9 @@ struct AttnWave {
         o[x] = i8_half2(__builtin_amdgcn_perm(vw[2 * x + 1][w] ^ 0x80808080u, vw[2 * x][w] ^ 0x80808080u, sel) | 0x64006400u);
       } else {
         o[x] = __builtin_amdgcn_perm(vw[2 * x + 1][i / 2], vw[2 * x][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-        if constexpr (PART) o[x] &= (on >> (2 * x) & 1u ? 0xFFFFu : 0u) | (on >> (2 * x + 1) & 1u ? 0xFFFF0000u : 0u);
       }
     }
-    return __builtin_bit_cast(half8, o);
+    return o;
   }
 
   // The step at token t0: scores, weights and the weighted sum. `masked`: some
@@ -288,8 +297,13 @@ struct AttnWave {
         else a = __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          c[mt] = mfma(a, qh[mt][k], c[mt]);
-          c[mt] = mfma(a, ql[mt][k], c[mt]);
+          if constexpr (QL) {
+            c[mt] = mfma(a, *(const half8 *)(qs + (mt * KS + k) * 2048), c[mt]);
+            c[mt] = mfma(a, *(const half8 *)(qs + (mt * KS + k) * 2048 + 1024), c[mt]);
+          } else {
+            c[mt] = mfma(a, qh[mt][k], c[mt]);
+            c[mt] = mfma(a, ql[mt][k], c[mt]);
+          }
         }
       }
 #pragma unroll
@@ -370,8 +384,7 @@ struct AttnWave {
     }
     if constexpr (!I8) {
       // A value that only some rows see and that is not finite: 0 * inf would
-      // reach the others. One position's rows at a time, with what they do not
-      // see cleared.
+      // reach the others.
       if (masked && t.first != t.last) {
         uint32_t top = 0;
 #pragma unroll
@@ -381,15 +394,12 @@ struct AttnWave {
             const uint32_t x = vw[k][w] & 0x7FFF7FFFu;
             top = max(top, max(x & 0xFFFFu, x >> 16));
           }
-        if (__any(top >= 0x7C00u)) {
-          apart(t0, t, window, g, ph, pl);
-          return;
-        }
+        if (__any(top >= 0x7C00u)) poison(t0, gone, window, g);
       }
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const half8 a = v_operand(i);
+      const half8 a = __builtin_bit_cast(half8, v_operand(i));
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         acc[mt][i] = mfma(a, ph[mt], acc[mt][i]);
@@ -398,25 +408,33 @@ struct AttnWave {
     }
   }
 
-  __device__ __forceinline__ void apart(int t0, const AttnTile &t, int window, uint32_t g, const half8 *ph, const half8 *pl) {
-#pragma unroll 1
-    for (int p = t.first; p <= t.last; ++p) {
-      uint32_t on = 0;
+  // fp16 1 where a half is not finite, else 0; and the halves that are.
+  static __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & 0x7C00u) == 0x7C00u ? 0x3C00u : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0x3C000000u : 0u);
+  }
+
+  // The columns of the rows that see a value that is not finite become NaN (the
+  // product of the two indicators says which), and such values are taken out of
+  // the step.
+  __device__ __forceinline__ void poison(int t0, const bool gone[2], int window, uint32_t g) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (sees(p, window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4)) on |= 1u << k;
+    for (int mt = 0; mt < MT; ++mt) {
+      half8 seen;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) seen[k] = (_Float16)(!gone[k / 4] && sees(pos[mt], window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4) ? 1.f : 0.f);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const half8 a = v_operand<true>(i, on);
+        const u32x4 v = v_operand(i);
+        const u32x4 bad = {not_finite(v[0]), not_finite(v[1]), not_finite(v[2]), not_finite(v[3])};
+        const float4v c = mfma(__builtin_bit_cast(half8, bad), seen, float4v{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float4v c = {0.f, 0.f, 0.f, 0.f};
-          c = mfma(a, ph[mt], c);
-          c = mfma(a, pl[mt], c);
-          if (pos[mt] == p) acc[mt][i] += c;
-        }
+        for (int j = 0; j < 4; ++j) acc[mt][i][j] = c[j] > 0.f ? NAN : acc[mt][i][j];
       }
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) vw[k][w] &= ~(not_finite(vw[k][w]) / 0x3C00u * 0xFFFFu);
   }
 
   // The walk over a tile's cached tokens: the steps lo, lo + stride, ... up to hi.
@@ -472,6 +490,7 @@ struct AttnPlan {
   uint32_t tiles, per_seq;    // row tiles; tiles of each sequence (0: packed)
   uint32_t chunk, chunks;     // cached tokens of a workgroup, chunks of a tile at most
   uint32_t rows;              // rows of a tile at most
+  uint32_t waves;             // of a workgroup
 };
 
 // The joined sums of chunks: per (tile, head) the chunks' weighted sums, then
@@ -482,17 +501,18 @@ __host__ __device__ constexpr uint64_t attn_part_floats(const AttnPlan &p, uint3
 
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
-// Four waves take the 32-token steps of a chunk in turn; their sums meet in
+// NW waves take the 32-token steps of a chunk in turn; their sums meet in
 // LDS. Where a tile has several chunks, the last workgroup of the tile to arrive
 // joins them, in chunk order; stores and loads of the chunks' sums go past the
 // XCD's L2 (sc1), every wave waits for its stores before the barrier ahead of the
 // counter's increment, and the counter is left at zero for the next launch.
-template <int TYPE, int D, int MT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
-  using W = AttnWave<TYPE, D, MT>;
-  constexpr uint32_t R = 16u * MT, LD = D + 4u;
-  __shared__ float so[4][R][LD];
-  __shared__ float sm[4][R], sl[4][R], sv[4][R];
+template <int TYPE, int D, int MT, int NW, bool QL>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
+  using W = AttnWave<TYPE, D, MT, QL>;
+  constexpr uint32_t R = 16u * MT, LD = D + 4u, T = 64u * NW;
+  static_assert(!QL || MT * W::KS * 2048u <= NW * R * LD * 4u, "q's parts share the sums' space");
+  __shared__ float so[NW][R][LD];
+  __shared__ float sm[NW][R], sl[NW][R], sv[NW][R];
   __shared__ uint32_t arrived;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
@@ -507,13 +527,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn(KvView kv, KvBat
   {
     typename W::Walk k;
     k.table = b.table + (uint64_t)t.seq * b.table_pages;
-    k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 128;
+    k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 32 * NW;
     W::read_ids(k, kv, k.lo);
     float q[MT][W::KS][8];
     w.load_q(q, a, t, group, kvh, 0, n, g);
     w.fetch_k(k, kv, kvh, 0, k.lo, n, g);   // of the first page, where the wave has no step
-    w.init(q, a.scale);
+    w.init(q, a.scale, (uint8_t *)so, wave, NW);
+    if constexpr (QL) __syncthreads();
     w.run(k, kv, t, kvh, window, n, g);
+    if constexpr (QL) __syncthreads();   // the sums take q's place
   }
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -528,14 +550,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn(KvView kv, KvBat
   const uint64_t at = ((uint64_t)tile * kv.heads + kvh) * attn_part_floats(p, D);
   const rsrc_t prs = make_rsrc(part + at, attn_part_floats(p, D) * 4u);
   const uint32_t ml = p.chunks * p.rows * D;   // where the maxima and sums begin
-  for (uint32_t i = tid; i < t.rows * (D / 4u); i += 256u) {
+  for (uint32_t i = tid; i < t.rows * (D / 4u); i += T) {
     const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u));
     float mx = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) mx = fmaxf(mx, sm[v][r]);
+    for (int v = 0; v < NW; ++v) mx = fmaxf(mx, sm[v][r]);
     float4v o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
+    for (int v = 0; v < NW; ++v) {
       const float f = sm[v][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[v][r] - mx);
       l += f * sl[v][r];
       const float4v x = *(const float4v *)&so[v][r][d];
@@ -564,8 +586,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn(KvView kv, KvBat
   if (tid == 0u) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // the chunks' weights relative to the largest maximum, [chunk][row], and the
   // rows' sums: a wave per row, its lanes over the chunks
-  float *wt = &so[0][0][0], *half = wt + 4u * R * LD - 1024u;
-  for (uint32_t r = wave; r < t.rows; r += 4u) {
+  float *wt = &so[0][0][0], *half = wt + NW * R * LD - 4u * T;
+  for (uint32_t r = wave; r < t.rows; r += NW) {
     float mx = -INFINITY, l = 0.f;
     for (uint32_t z = lane; z < chunks; z += 64u)
       mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * (z * p.rows + r)) * 4u), 0, kSc1)));
@@ -584,8 +606,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn(KvView kv, KvBat
   }
   __syncthreads();
   // each thread a part of the chunks of 4 columns of a row
-  const uint32_t items = t.rows * (D / 4u), parts = max(1u, 256u / items);
-  for (uint32_t i0 = 0; i0 < items; i0 += 256u) {
+  const uint32_t items = t.rows * (D / 4u), parts = max(1u, T / items);
+  for (uint32_t i0 = 0; i0 < items; i0 += T) {
     const uint32_t part_i = parts > 1u ? tid / items : 0u, i = parts > 1u ? tid % items : i0 + tid;
     const bool on = i < items && part_i < parts;
     const uint32_t r = on ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
@@ -630,17 +652,25 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
-  // Chunks of at least 1024 tokens, and then about 4096 workgroups, so that long
-  // and short sequences even out; shorter chunks only while there are below 512
-  // workgroups. The join keeps a weight for each chunk and row in LDS.
+  // About 256 workgroups, one for each CU, in chunks of 256 tokens at least: below,
+  // a wave has one step, and the join costs more than the steps it takes over
+  // (1 x 8 heads of 128 over 2000 tokens: 256 10.0 us, 512 11.8, one chunk 23). At
+  // most 1024 for several sequences, whose lengths differ by what the host does not
+  // know (64 up to 16384: 384 us, one chunk each 453; 40 of int8 up to 9001 52.9,
+  // 2048 76.2), and 4096 for one (130001: 94.3, 1024 104.4). Where the tiles alone
+  // fill half of the CUs and are short, no chunks: a join takes 5 us (24 x 8 heads
+  // of drafts that see 1024: 17.8 us, chunks of 512 22.5).
   const uint64_t whole = (span + 127u) / 128u * 128u;
-  auto per = [&](uint64_t n) { return (span * wgs / n + 127u) / 128u * 128u; };
-  uint64_t chunk = std::max(per(4096u), std::min<uint64_t>(1024u, std::max<uint64_t>(per(512u), 256u)));
+  uint64_t chunk = std::min<uint64_t>(std::max<uint64_t>((span * wgs / 256u + 127u) / 128u * 128u, 256u), b.seqs > 1u ? 1024u : 4096u);
+  if (wgs >= 128u && whole <= 2176u) chunk = whole;
   const uint64_t most_chunks = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;
   chunk = std::min(std::max(chunk, (span / most_chunks + 128u) / 128u * 128u), whole);
   if (wgs > kAttnCounters) chunk = whole;
   p.chunk = (uint32_t)chunk;
   p.chunks = (uint32_t)((span + chunk - 1u) / chunk);
+  // 8 waves where a CU has one workgroup and the steps to share (the drafts above:
+  // 15.8 us, 4 waves 17.8; 1024 workgroups of 300 tokens 30, 4 waves 21)
+  p.waves = p.chunks == 1u && wgs <= 256u && span >= 512u && kv.dim < 256u ? 8u : 4u;
   return p;
 }
 
@@ -654,8 +684,15 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   const AttnPlan p = attn_plan(kv, b, a);
   const uint64_t grid = (uint64_t)p.tiles * p.chunks * kv.heads;
   if (grid > 0x7FFFFFFFull || (p.chunks > 1u && !scratch)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_attn<TYPE, D, 1>), dim3((uint32_t)grid), dim3(256), 0, s, kv, b, a, p, (uint32_t *)scratch,
-                     (float *)((uint8_t *)scratch + kAttnCounters * 4u));
+  uint32_t *cnt = (uint32_t *)scratch;
+  float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
+  if constexpr (D < 256) {
+    if (p.waves == 8u) {
+      hipLaunchKernelGGL((k_attn<TYPE, D, 1, 8, false>), dim3((uint32_t)grid), dim3(512), 0, s, kv, b, a, p, cnt, part);
+      return hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((k_attn<TYPE, D, 1, 4, (D == 256)>), dim3((uint32_t)grid), dim3(256), 0, s, kv, b, a, p, cnt, part);
   return hipGetLastError();
 }
 
