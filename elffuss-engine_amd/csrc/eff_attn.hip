@@ -50,6 +50,10 @@ __device__ __forceinline__ half8 i8_half8(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(half8, v);
 }
 
+__device__ __forceinline__ half8 join8(const half2v v[4]) {
+  return half8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+}
+
 template <int N>
 __device__ __forceinline__ void ld_words(uint32_t *o, const uint8_t *p) {
   if constexpr (N == 1) {
@@ -64,15 +68,41 @@ __device__ __forceinline__ void ld_words(uint32_t *o, const uint8_t *p) {
   }
 }
 
-// Maximum over the 4 lanes that hold a row.
+// A constant that the compiler does not see, so that it keeps the instruction
+// around it.
+__device__ __forceinline__ float unseen(float v) {
+  __asm__("" : "=s"(v) : "0"(v));
+  return v;
+}
+
+// The larger of two numbers. (fmaxf first quiets each operand that may be a
+// signalling NaN, an instruction each; a NaN here makes the row's sum NaN anyway.)
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, unseen(INFINITY)); }
+
+// Maximum and sum over the 4 lanes that hold a row (lane % 16). The swaps leave
+// the two halves (two 16-lane rows) of v side by side in two registers.
 __device__ __forceinline__ float row_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = max2(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max2(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 __device__ __forceinline__ float row_add(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Two values in two fp16 parts: v = hi + lo to 22 bits. (hi * -1 + v in one
+// instruction each, with the conversions.)
+__device__ __forceinline__ void split2(float a, float b, half2v &hi, half2v &lo) {
+  uint32_t h = __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b});
+  __asm__("" : "+v"(h));   // one packed conversion, not two more for the halves
+  hi = __builtin_bit_cast(half2v, h);
+  const float m = unseen(-1.f);
+  lo = half2v{(_Float16)fmaf((float)hi[0], m, a), (_Float16)fmaf((float)hi[1], m, b)};
 }
 
 // The rows of a tile, their tokens and what they see.
@@ -83,11 +113,11 @@ struct AttnTile {
   int begin, end;         // the cached tokens that any row sees
 };
 
-// The tile of a workgroup: `per_seq` tiles of each sequence, or (per_seq = 0)
-// the tiles of the sequences one after the other.
+// The tile of a workgroup, of the sequences that have min_rows .. max_rows rows:
+// `per_seq` tiles of each sequence, or (per_seq = 0) their tiles one after the other.
 template <uint32_t R>
 __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, uint32_t window, uint32_t tile,
-                                          uint32_t per_seq, AttnTile &t) {
+                                          uint32_t per_seq, uint32_t min_rows, uint32_t max_rows, AttnTile &t) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t sub;
   if (per_seq) {
@@ -101,7 +131,8 @@ __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, 
       uint32_t n = 0;
       if (i < b.seqs) {
         const uint32_t s0 = b.starts[i], s1 = b.starts[i + 1];
-        n = s1 > s0 ? (min(s1 - s0, b.max_new) * group + R - 1u) / R : 0u;
+        n = s1 > s0 ? min(s1 - s0, b.max_new) * group : 0u;
+        n = n >= min_rows && n <= max_rows ? (n + R - 1u) / R : 0u;
       }
       uint32_t sum = n;
 #pragma unroll
@@ -127,7 +158,7 @@ __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, 
   const uint32_t n = s1 > s0 ? min(s1 - s0, b.max_new) : 0u;
   t.token0 = s0;
   t.r0 = sub * R;
-  if (t.r0 >= n * group) return false;
+  if (t.r0 >= n * group || n * group < min_rows || n * group > max_rows) return false;
   t.rows = min(R, n * group - t.r0);
   const int len = __builtin_amdgcn_readfirstlane((int)kv_len(b, t.seq));
   t.first = len - (int)n + (int)(t.r0 / group);
@@ -150,9 +181,9 @@ struct AttnWave {
 
   half8 qh[QL ? 1 : MT][QL ? 1 : KS], ql[QL ? 1 : MT][QL ? 1 : KS];
   const uint8_t *qs;       // QL: [mt][step][part][lane] of 16 bytes
-  float sc[MT];            // what a raw score of row n is multiplied by (log2 e included)
+  float sc[MT];            // > 0: what a raw score of row n is multiplied by (log2 e included)
   int pos[MT];             // the row's position, -1 for none
-  float m[MT], l[MT];      // running maximum (log2), and this lane's share of the sum
+  float m[MT], l[MT];      // running maximum (of raw scores), and this lane's share of the sum
   float vref[MT], vinv[MT];   // I8: the largest value scale so far, and its reciprocal
   float4v acc[MT][E];
 
@@ -204,18 +235,16 @@ struct AttnWave {
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[mt][c][i]));
       top = row_max(top);
       const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
-      const float up = ldexpf(1.f, 13 - e);
-      sc[mt] = scale * 1.44269504088896341f * ldexpf(1.f, e - 13);
+      // the scale's sign goes to q; a scale of zero makes every score zero
+      const float up = scale == 0.f ? 0.f : copysignf(ldexpf(1.f, 13 - e), scale);
+      sc[mt] = fmaxf(fabsf(scale) * 1.44269504088896341f * ldexpf(1.f, e - 13), 1e-37f);
 #pragma unroll
       for (int c = 0; c < KS; ++c)
       {
-        half8 h, r;
+        half2v hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = q[mt][c][i] * up;
-          h[i] = (_Float16)x;
-          r[i] = (_Float16)(x - (float)h[i]);
-        }
+        for (int i = 0; i < 4; ++i) split2(q[mt][c][2 * i] * up, q[mt][c][2 * i + 1] * up, hi[i], lo[i]);
+        const half8 h = join8(hi), r = join8(lo);
         if constexpr (!QL) {
           qh[mt][c] = h, ql[mt][c] = r;
         } else if ((mt * KS + c) % waves == wave) {
@@ -244,7 +273,11 @@ struct AttnWave {
   }
 
   __device__ __forceinline__ void load_v(int u, const uint8_t *blk, uint32_t slot, uint32_t page_log2, uint32_t n, uint32_t g) {
-    const uint8_t *p = blk + slot * ROW;
+    load_rows(u, blk + slot * ROW, blk + ((uint32_t)D << page_log2) + slot * 4u, n, g);
+  }
+
+  // The lane's parts of the rows 4 g .. 4 g + 3 of half u, in memory or in LDS.
+  __device__ __forceinline__ void load_rows(int u, const uint8_t *p, const uint8_t *scales, uint32_t n, uint32_t g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint8_t *r = p + 4u * g * ROW + j * ROW;
@@ -262,7 +295,7 @@ struct AttnWave {
         ld_words<VW>(o, r + 4u * VW * n);
       }
     }
-    if constexpr (I8) ld_words<4>(vs[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
+    if constexpr (I8) ld_words<4>(vs[u], scales + 16u * g);
   }
 
   // Column i of the 8 tokens of the lane as the first operand.
@@ -309,7 +342,7 @@ struct AttnWave {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[mt][u][j] = c[mt][j] * (I8 ? sc[mt] * __uint_as_float(ks[u][j]) : sc[mt]);
+        for (int j = 0; j < 4; ++j) s[mt][u][j] = I8 ? c[mt][j] * __uint_as_float(ks[u][j]) : c[mt][j];
     }
   }
 
@@ -337,8 +370,8 @@ struct AttnWave {
     half8 ph[MT], pl[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float mx = fmaxf(fmaxf(fmaxf(s[mt][0][0], s[mt][0][1]), fmaxf(s[mt][0][2], s[mt][0][3])),
-                       fmaxf(fmaxf(s[mt][1][0], s[mt][1][1]), fmaxf(s[mt][1][2], s[mt][1][3])));
+      float mx = max2(max2(max2(s[mt][0][0], s[mt][0][1]), max2(s[mt][0][2], s[mt][0][3])),
+                      max2(max2(s[mt][1][0], s[mt][1][1]), max2(s[mt][1][2], s[mt][1][3])));
       mx = row_max(mx);
       float vx = 0.f;
       if constexpr (I8) {
@@ -351,7 +384,7 @@ struct AttnWave {
       }
       if (__any(mx > m[mt] || (I8 && vx > vref[mt]))) {
         const float mn = fmaxf(m[mt], mx);
-        const float al = m[mt] == mn ? 1.f : __builtin_amdgcn_exp2f(m[mt] - mn);
+        const float al = m[mt] == mn ? 1.f : __builtin_amdgcn_exp2f((m[mt] - mn) * sc[mt]);
         m[mt] = mn;
         l[mt] *= al;
         float f = al;
@@ -366,20 +399,25 @@ struct AttnWave {
 #pragma unroll
         for (int i = 0; i < E; ++i) acc[mt][i] *= f;
       }
-      const float mm = m[mt] == -INFINITY ? 0.f : m[mt] - 14.f;
+      const float up = m[mt] == -INFINITY ? 0.f : 14.f - m[mt] * sc[mt];
       float sum = 0.f;
+      half2v hi[4], lo[4];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float p = __builtin_amdgcn_exp2f(s[mt][u][j] - mm);
-          sum += p;
-          // a weight of nothing takes nothing of a scale that is not finite
-          if constexpr (I8) p = masked && s[mt][u][j] == -INFINITY ? 0.f : p * (__uint_as_float(vs[u][j]) * vinv[mt]);
-          const _Float16 h = (_Float16)p;
-          ph[mt][4 * u + j] = h;
-          pl[mt][4 * u + j] = (_Float16)(p - (float)h);
+        for (int j = 0; j < 4; j += 2) {
+          float p[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x = s[mt][u][j + k];
+            p[k] = __builtin_amdgcn_exp2f(fmaf(x, sc[mt], up));
+            sum += p[k];
+            // a weight of nothing takes nothing of a scale that is not finite
+            if constexpr (I8) p[k] = masked && x == -INFINITY ? 0.f : p[k] * (__uint_as_float(vs[u][j + k]) * vinv[mt]);
+          }
+          split2(p[0], p[1], hi[2 * u + j / 2], lo[2 * u + j / 2]);
         }
+      ph[mt] = join8(hi), pl[mt] = join8(lo);
       l[mt] += sum;
     }
     if constexpr (!I8) {
@@ -491,6 +529,9 @@ struct AttnPlan {
   uint32_t chunk, chunks;     // cached tokens of a workgroup, chunks of a tile at most
   uint32_t rows;              // rows of a tile at most
   uint32_t waves;             // of a workgroup
+  uint32_t max_rows;          // of the sequences taken; those with more go to k_attn_rows:
+  uint32_t many;              // 16-row tiles of one of its waves (0: none go)
+  uint32_t many_tiles, many_per_seq;
 };
 
 // The joined sums of chunks: per (tile, head) the chunks' weighted sums, then
@@ -499,6 +540,7 @@ __host__ __device__ constexpr uint64_t attn_part_floats(const AttnPlan &p, uint3
   return (uint64_t)p.chunks * p.rows * (dim + 2u);
 }
 
+constexpr uint32_t kFewRows = 64;
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
 // NW waves take the 32-token steps of a chunk in turn; their sums meet in
@@ -518,7 +560,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   const uint32_t group = a.q_heads / kv.heads;
   const uint32_t kvh = blockIdx.x % kv.heads, w0 = blockIdx.x / kv.heads, chunk = w0 % p.chunks, tile = w0 / p.chunks;
   AttnTile t;
-  if (!attn_tile<R>(b, group, a.window, tile, p.per_seq, t)) return;
+  if (!attn_tile<R>(b, group, a.window, tile, p.per_seq, 1u, p.max_rows, t)) return;
   const int window = (int)min(a.window, 0x40000000u), base = t.begin & ~31;
   const uint32_t chunks = t.end > base ? ((uint32_t)(t.end - base) + p.chunk - 1u) / p.chunk : 1u;
   if (chunk >= chunks) return;
@@ -540,7 +582,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const float l = row_add(w.l[mt]);
-    if (g == 0u) sm[wave][16 * mt + n] = w.m[mt], sl[wave][16 * mt + n] = l, sv[wave][16 * mt + n] = w.vref[mt];
+    if (g == 0u) sm[wave][16 * mt + n] = w.m[mt] * w.sc[mt], sl[wave][16 * mt + n] = l, sv[wave][16 * mt + n] = w.vref[mt];
 #pragma unroll
     for (int i = 0; i < W::E; ++i)
 #pragma unroll
@@ -641,14 +683,204 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   }
 }
 
+// Many rows: four waves of 16 MT rows each walk the same cached tokens, 32 a
+// step, which come through LDS: three buffers, filled two steps ahead past the
+// registers (the wave that waits for a step's loads and passes the barrier knows
+// that every wave is done with the buffer it fills next). K's 16-byte pieces are
+// turned within their row, so that the 16 rows of an operand lie in different banks.
+template <int TYPE, int D>
+struct AttnStage {
+  static constexpr uint32_t ROW = TYPE == EFF_KV_I8 ? D : 2 * D, PIECES = ROW / 16u;
+  static constexpr uint32_t V = 32u * ROW, SCALES = 2u * V, BYTES = 2u * V + (TYPE == EFF_KV_I8 ? 256u : 0u);
+  static constexpr uint32_t LOADS = 2u * V / 1024u;   // of 64 lanes, 16 bytes each
+  static constexpr uint32_t MINE = (LOADS + 3u) / 4u;
+
+  // where piece c of row r lies in the row, and back
+  static __device__ __forceinline__ uint32_t place(uint32_t r, uint32_t c) {
+    if constexpr (PIECES % 8u == 0u) return c ^ (r & 7u);
+    else if constexpr (PIECES == 4u) return c ^ (r >> 1 & 3u);
+    else if constexpr (PIECES == 12u) return (c + (r >> 1 & 3u)) % 12u;
+    else return (c + (r >> 2 & 1u)) % PIECES;
+  }
+  static __device__ __forceinline__ uint32_t piece(uint32_t r, uint32_t at) {
+    if constexpr (PIECES % 8u == 0u) return at ^ (r & 7u);
+    else if constexpr (PIECES == 4u) return at ^ (r >> 1 & 3u);
+    else if constexpr (PIECES == 12u) return (at + 12u - (r >> 1 & 3u)) % 12u;
+    else return (at + PIECES - (r >> 2 & 1u)) % PIECES;
+  }
+};
+
+// 16 (4) bytes a lane from its own address into LDS at lds + 16 (4) * lane.
+__device__ __forceinline__ void fill16(const uint8_t *p, const uint8_t *lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+  __asm__ volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+}
+
+__device__ __forceinline__ void fill4(const uint8_t *p, const uint8_t *lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+  __asm__ volatile("global_load_lds_dword %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+}
+
+// Waits for all but the N youngest loads of the wave and for its LDS reads, then
+// for the other waves.
+template <uint32_t N>
+__device__ __forceinline__ void wait_step() {
+  __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+template <int TYPE, int D, int MT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles,
+                                                                      uint32_t per_seq, uint32_t min_rows) {
+  using W = AttnWave<TYPE, D, MT, false>;
+  using S = AttnStage<TYPE, D>;
+  constexpr uint32_t R = 64u * MT;
+  __shared__ __align__(1024) uint8_t buf[3][S::BYTES];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
+  const uint32_t group = a.q_heads / kv.heads;
+  // the last tiles of a sequence see the most: first
+  const uint32_t kvh = blockIdx.x % kv.heads, tile = tiles - 1u - blockIdx.x / kv.heads;
+  AttnTile t;
+  if (!attn_tile<R>(b, group, a.window, tile, per_seq, min_rows, ~0u, t)) return;
+  const int window = (int)min(a.window, 0x40000000u), base = t.begin & ~31;
+  // the wave's own rows
+  AttnTile m = t;
+  const uint32_t row0 = 16u * MT * wave;
+  m.rows = t.rows > row0 ? min(t.rows - row0, 16u * MT) : 0u;
+  if (m.rows) {
+    m.r0 = t.r0 + row0;
+    m.first = t.first + (int)(m.r0 / group - t.r0 / group);
+    m.last = t.first + (int)((m.r0 + m.rows - 1u) / group - t.r0 / group);
+    m.end = max(m.last + 1, 0);
+    m.begin = window ? max(0, m.first - window + 1) : 0;
+  } else {
+    m.r0 = t.r0, m.end = 0;
+  }
+  W w;
+  float q[MT][W::KS][8];
+  w.load_q(q, a, m, group, kvh, 0, n, g);
+  w.init(q, a.scale, nullptr, wave, 4);
+
+  const uint32_t *table = b.table + (uint64_t)t.seq * b.table_pages;
+  const uint64_t to_v = (uint64_t)kv.heads * kv.block_bytes;
+  const uint32_t mask = (1u << kv.page_log2) - 1u;
+  uint32_t off[S::MINE];   // of the lane's pieces: its place in the half's rows
+#pragma unroll
+  for (uint32_t k = 0; k < S::MINE; ++k) {
+    const uint32_t at = ((4u * k + wave) * 64u + lane) % (S::V / 16u), r = at / S::PIECES;
+    // V lies as it is
+    off[k] = (r & 15u) * S::ROW + 16u * ((4u * k + wave) * 64u < S::V / 16u ? S::piece(r, at % S::PIECES) : at % S::PIECES);
+  }
+  uint32_t ids = 0;
+  const int steps = t.end > base ? (t.end - base + 31) / 32 : 0;
+  uint32_t gone = 0;       // two bits a step, of the last three
+  auto issue = [&](int i) {
+    const int t0 = base + 32 * i;
+    if ((i & 31) == 0) {
+      const int at = t0 + 16 * (int)lane;
+      ids = at < t.end ? table[(uint32_t)at >> kv.page_log2] : ~0u;
+    }
+    const uint8_t *blk[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t p = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + u);
+      gone = gone << 1 | (p >= kv.pages);
+      blk[u] = kv.base + (p >= kv.pages ? 0ull : (uint64_t)p * kv.page_bytes) + (uint64_t)kvh * kv.block_bytes;
+    }
+    const uint32_t slot[2] = {(uint32_t)t0 & mask, (uint32_t)(t0 + 16) & mask};
+    const uint8_t *lds = buf[i % 3];
+#pragma unroll
+    for (uint32_t k = 0; k < S::MINE; ++k) {
+      const uint32_t l = 4u * k + wave;   // load l of K's and V's
+      if (S::LOADS % 4u && l >= S::LOADS) break;
+      const uint32_t r = (l * 64u + lane) % (S::V / 16u) / S::PIECES;
+      const uint8_t *p = (r < 16u ? blk[0] + slot[0] * S::ROW : blk[1] + slot[1] * S::ROW) + off[k] + (l * 64u < S::V / 16u ? 0ull : to_v);
+      fill16(p, lds + 1024u * l);
+    }
+    if constexpr (W::I8) {
+      if (wave == 3u) {
+        const uint32_t u = lane >> 4 & 1u;
+        fill4((u ? blk[1] + slot[1] * 4u : blk[0] + slot[0] * 4u) + ((uint32_t)D << kv.page_log2) + 4u * (lane & 15u) + (lane < 32u ? 0ull : to_v),
+              lds + S::SCALES);
+      }
+    }
+  };
+  // loads of the next step that the wave may leave under way
+  constexpr uint32_t NEXT = S::LOADS / 4u;
+  if (steps) issue(0);
+  if (steps > 1) issue(1);
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    if (i + 1 < steps) wait_step<NEXT>();
+    else wait_step<0>();
+    const bool was[2] = {i + 1 < steps ? (gone & 8u) != 0u : (gone & 2u) != 0u, i + 1 < steps ? (gone & 4u) != 0u : (gone & 1u) != 0u};
+    if (i + 2 < steps) issue(i + 2);
+    const int t0 = base + 32 * i;
+    if (t0 >= m.end || t0 + 32 <= m.begin) continue;
+    const uint8_t *lds = buf[i % 3];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t r = 16u * u + n;
+      const uint8_t *p = lds + r * S::ROW;
+      if constexpr (!W::I8) {
+#pragma unroll
+        for (int c = 0; c < W::KS; ++c) ld_words<4>(w.kw[u] + 4 * c, p + 16u * S::place(r, 4u * c + g));
+      } else {
+#pragma unroll
+        for (int c = 0; c + 1 < W::KS; c += 2) ld_words<4>(w.kw[u] + 2 * c, p + 16u * S::place(r, 2u * c + g));
+        if constexpr (W::KS & 1) ld_words<2>(w.kw[u] + 2 * (W::KS - 1), p + 16u * S::place(r, 2u * (W::KS - 1) + g / 2u) + 8u * (g & 1u));
+        ld_words<4>(w.ks[u], lds + S::SCALES + 64u * u + 16u * g);
+      }
+    }
+    float s[MT][2][4];
+    w.scores(s);
+    __builtin_amdgcn_sched_barrier(0);   // V's registers are K's
+#pragma unroll
+    for (int u = 0; u < 2; ++u) w.load_rows(u, lds + S::V + 16u * u * S::ROW, lds + S::SCALES + 128u + 64u * u, n, g);
+    const bool masked = was[0] || was[1] || t0 + 31 > m.first || t0 < m.begin || (window && t0 <= m.last - window);
+    w.step(t0, masked, was, m, window, g, s);
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const float l = row_add(w.l[mt]);
+    const uint32_t r = 16u * mt + n;
+    if (r >= m.rows) continue;
+    const float f = l == 0.f ? 0.f : (W::I8 ? w.vref[mt] : 1.f) / l;
+    const uint32_t tok = (m.r0 + r) / group, h = (m.r0 + r) % group;
+    float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int i = 0; i + 3 < W::E; i += 4)
+        *(float4v *)(dst + W::column(g, i, j)) = float4v{w.acc[mt][i][j], w.acc[mt][i + 1][j], w.acc[mt][i + 2][j], w.acc[mt][i + 3][j]} * f;
+      if constexpr (W::E & 2) *(float2v *)(dst + W::column(g, W::E - 2, j)) = float2v{w.acc[mt][W::E - 2][j], w.acc[mt][W::E - 1][j]} * f;
+    }
+  }
+}
+
+// Tiles of R rows for sequences of at most `most` rows, `rows` of them in all.
+static void attn_tiles(uint64_t most, uint64_t rows, uint32_t seqs, uint32_t r, uint32_t *tiles, uint32_t *per_seq) {
+  const uint64_t each = (most + r - 1u) / r, direct = each * seqs, packed = rows / r + seqs;
+  *per_seq = direct <= packed ? (uint32_t)each : 0u;
+  *tiles = (uint32_t)std::min(direct, packed);
+}
+
 static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a) {
   const uint32_t group = a.q_heads / kv.heads;
   constexpr uint32_t R = 16u;
   AttnPlan p{};
-  const uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group;
-  const uint64_t each = (most + R - 1u) / R, direct = each * b.seqs, packed = (uint64_t)b.tokens * group / R + b.seqs;
-  p.per_seq = direct <= packed ? (uint32_t)each : 0u;
-  p.tiles = (uint32_t)std::min(direct, packed);
+  uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group;
+  const uint64_t rows = (uint64_t)b.tokens * group;
+  p.max_rows = ~0u;
+  // Sequences with more than 64 rows go to k_attn_rows where their tiles fill half
+  // of the CUs without chunks
+  if (most > kFewRows && rows / 64u * kv.heads >= 128u) {
+    p.many = kv.dim < 256u && rows / 128u * kv.heads >= 512u ? 2u : 1u;
+    attn_tiles(most, rows, b.seqs, 64u * p.many, &p.many_tiles, &p.many_per_seq);
+    p.max_rows = kFewRows;
+    most = kFewRows;
+    if (b.seqs == 1u) return p;
+  }
+  attn_tiles(most, rows, b.seqs, R, &p.tiles, &p.per_seq);
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
@@ -663,6 +895,7 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   const uint64_t whole = (span + 127u) / 128u * 128u;
   uint64_t chunk = std::min<uint64_t>(std::max<uint64_t>((span * wgs / 256u + 127u) / 128u * 128u, 256u), b.seqs > 1u ? 1024u : 4096u);
   if (wgs >= 128u && whole <= 2176u) chunk = whole;
+  if (wgs >= 4096u) chunk = whole;
   const uint64_t most_chunks = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;
   chunk = std::min(std::max(chunk, (span / most_chunks + 128u) / 128u * 128u), whole);
   if (wgs > kAttnCounters) chunk = whole;
@@ -682,6 +915,19 @@ size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs 
 template <int TYPE, int D>
 static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t s) {
   const AttnPlan p = attn_plan(kv, b, a);
+  if (p.many) {
+    const uint64_t g = (uint64_t)p.many_tiles * kv.heads;
+    const uint32_t min_rows = b.seqs == 1u ? 1u : kFewRows + 1u;
+    if (g > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    if constexpr (D < 256) {
+      if (p.many == 2u)
+        hipLaunchKernelGGL((k_attn_rows<TYPE, D, 2>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
+    }
+    if (p.many == 1u)
+      hipLaunchKernelGGL((k_attn_rows<TYPE, D, 1>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !p.tiles) return e;
+  }
   const uint64_t grid = (uint64_t)p.tiles * p.chunks * kv.heads;
   if (grid > 0x7FFFFFFFull || (p.chunks > 1u && !scratch)) return hipErrorInvalidValue;
   uint32_t *cnt = (uint32_t *)scratch;

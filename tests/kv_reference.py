@@ -39,18 +39,25 @@ def attend(values, table, starts, lens, q, q_heads, scale, window, page):
     out = np.zeros(q.shape)
     group = q_heads // heads
     for s, length in enumerate(lens):
-        for t in range(starts[s], starts[s + 1]):
-            end = int(length) - (starts[s + 1] - t) + 1
-            at = np.arange(max(0, end - window) if window else 0, max(end, 0))
-            p = table[s][at // page] if len(at) else np.zeros(0, np.int64)
-            at, p = at[p < pages], p[p < pages].astype(np.int64)
-            if not len(at):
-                continue
-            for h in range(q_heads):
-                k, v = values[p, 0, h // group, at % page], values[p, 1, h // group, at % page]
-                x = k @ q[t, h].astype(np.float64) * scale
-                w = np.exp(x - x.max())
-                out[t, h] = w @ v / w.sum()
+        new = slice(starts[s], starts[s + 1])
+        pos = int(length) - int(starts[s + 1] - starts[s]) + np.arange(starts[s + 1] - starts[s])
+        at = np.arange(int(length))
+        p = table[s][at // page] if len(at) else np.zeros(0, np.uint32)
+        at, p = at[p < pages], p[p < pages].astype(np.int64)
+        seen = at[None] <= pos[:, None]
+        if window:
+            seen &= at[None] > pos[:, None] - window
+        some = seen.any(1)
+        if not some.any():
+            continue
+        # what is not seen may be any bits
+        used = seen.any(0)
+        at, p, seen = at[used], p[used], seen[:, used]
+        for h in range(q_heads):
+            k, v = values[p, 0, h // group, at % page], values[p, 1, h // group, at % page]
+            x = np.where(seen, q[new, h].astype(np.float64) @ k.T * scale, -np.inf)[some]
+            w = np.exp(x - x.max(1, keepdims=True))
+            out[np.arange(starts[s], starts[s + 1])[some], h] = w @ v / w.sum(1, keepdims=True)
     return out
 
 

@@ -98,6 +98,24 @@ def test_prompt_heads(ctx, eff, t, heads, group, new):
 
 
 @pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads,group,new,lens,window", [
+    (4, 4, [700], [700], 0), (8, 3, [400, 129], [403, 1000], 0), (2, 8, [333, 1, 300], [2000, 50, 300], 0),
+    (4, 5, [600], [900], 100), (16, 1, [2100, 2100], [2100, 2222], 0)])
+def test_long_prompts(ctx, eff, t, dim, heads, group, new, lens, window):
+    """Enough rows for the kernel of many rows, with one and two row tiles to a wave."""
+    run(eff, ctx, dim, t, heads, group, dim, 32, new, lens, window)
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+def test_long_prompt_in_a_batch(ctx, eff, t):
+    """Prompts and decoding requests together: each goes to its kernel."""
+    new, lens = [1, 900, 0, 5, 1, 16, 17, 300, 1], [3000, 900, 10, 77, 0, 16, 2000, 5000, 1]
+    run(eff, ctx, 21, t, 4, 4, 64, 16, new, lens)
+    run(eff, ctx, 22, t, 4, 4, 128, 64, new, lens, 500, max_new=4000, max_len=5001)
+
+
+@pytest.mark.parametrize("t", [F16, I8])
 @pytest.mark.parametrize("window", [1, 7, 16, 33, 100, 5000])
 @pytest.mark.parametrize("new,lens", [([1, 1, 1], [1, 50, 900]), ([6, 40], [500, 40])])
 def test_window(ctx, eff, t, window, new, lens):
@@ -112,11 +130,11 @@ def test_mixed_batch(ctx, eff):
 
 
 @pytest.mark.parametrize("t", [F16, I8])
-@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("new", [1, 20, 600])
 def test_what_is_not_seen(ctx, eff, t, new):
     """NaN, infinities or zeros at the places that no token sees: the same bits."""
     rng = np.random.default_rng(new)
-    b = Batch(rng, [new, new], [new + 5, 333], 64, spare=3)
+    b = Batch(rng, [new, new], [new + 5, new + 333], 64, spare=3)
     q = rng.standard_normal((b.tokens, 8, 128)).astype(np.float32)
     got = []
     for dirty in (np.nan, np.inf, -np.inf, 0.0):
@@ -130,13 +148,14 @@ def test_what_is_not_seen(ctx, eff, t, new):
 @pytest.mark.parametrize("t", [F16, I8])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", [0, 1])
-def test_later_tokens_do_not_reach_earlier_rows(ctx, eff, t, bad, where):
+@pytest.mark.parametrize("new,group", [(40, 4), (700, 16)])
+def test_later_tokens_do_not_reach_earlier_rows(ctx, eff, t, bad, where, new, group):
     """A key (where = 0) or value (1) that is not finite: rows before it are not changed, rows that see it are not finite."""
     rng = np.random.default_rng(3)
-    new, length, at = 40, 50, 31
+    length, at = new + 10, new - 9
     b = Batch(rng, [new], [length], 16)
     rows = rng.standard_normal((b.pages, 2, 1, 16, 64)).astype(np.float32)
-    q = rng.standard_normal((new, 4, 64)).astype(np.float32)
+    q = rng.standard_normal((new, group, 64)).astype(np.float32)
     clean, _ = encode(t, rows)
     data = clean.copy().reshape(b.pages, 2, -1)
     page, slot = b.table[0, at // 16], at % 16
@@ -144,8 +163,8 @@ def test_later_tokens_do_not_reach_earlier_rows(ctx, eff, t, bad, where):
         data[page, where, slot * 128 + 6:slot * 128 + 8] = np.frombuffer(np.float16(bad).tobytes(), np.uint8)
     else:
         data[page, where, 16 * 64 + 4 * slot:16 * 64 + 4 * slot + 4] = np.frombuffer(np.float32(bad).tobytes(), np.uint8)
-    a = launch(eff, ctx, t, 1, 64, b, clean, q, 4, 0.1)
-    g = launch(eff, ctx, t, 1, 64, b, data.reshape(b.pages, -1), q, 4, 0.1)
+    a = launch(eff, ctx, t, 1, 64, b, clean, q, group, 0.1)
+    g = launch(eff, ctx, t, 1, 64, b, data.reshape(b.pages, -1), q, group, 0.1)
     before = at - (length - new)          # new tokens before position `at`
     assert np.array_equal(a[:before].view(np.uint32), g[:before].view(np.uint32))
     if where == 1 or not np.isinf(bad):
