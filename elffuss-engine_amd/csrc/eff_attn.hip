@@ -439,10 +439,9 @@ struct AttnWave {
     for (int i = 0; i < E; ++i) {
       const half8 a = __builtin_bit_cast(half8, v_operand(i));
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        acc[mt][i] = mfma(a, ph[mt], acc[mt][i]);
-        acc[mt][i] = mfma(a, pl[mt], acc[mt][i]);
-      }
+      for (int mt = 0; mt < MT; ++mt) acc[mt][i] = mfma(a, ph[mt], acc[mt][i]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) acc[mt][i] = mfma(a, pl[mt], acc[mt][i]);
     }
   }
 
@@ -530,8 +529,7 @@ struct AttnPlan {
   uint32_t rows;              // rows of a tile at most
   uint32_t waves;             // of a workgroup
   uint32_t max_rows;          // of the sequences taken; those with more go to k_attn_rows:
-  uint32_t many;              // 16-row tiles of one of its waves (0: none go)
-  uint32_t many_tiles, many_per_seq;
+  uint32_t many_tiles, many_per_seq;   // its tiles (0: none go)
 };
 
 // The joined sums of chunks: per (tile, head) the chunks' weighted sums, then
@@ -683,17 +681,18 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   }
 }
 
-// Many rows: four waves of 16 MT rows each walk the same cached tokens, 32 a
-// step, which come through LDS: three buffers, filled two steps ahead past the
-// registers (the wave that waits for a step's loads and passes the barrier knows
-// that every wave is done with the buffer it fills next). K's 16-byte pieces are
-// turned within their row, so that the 16 rows of an operand lie in different banks.
+// Many rows: NW waves of 16 MT rows each walk the same cached tokens, 32 a step,
+// which come through LDS: two buffers, one filled while the other is read (a wave
+// that has waited for its loads and passed the barrier knows that the step's
+// tokens are there, and that every wave is done with the buffer it fills next).
+// K's 16-byte pieces are turned within their row, so that the 16 rows of an operand
+// lie in different banks.
 template <int TYPE, int D>
 struct AttnStage {
   static constexpr uint32_t ROW = TYPE == EFF_KV_I8 ? D : 2 * D, PIECES = ROW / 16u;
-  static constexpr uint32_t V = 32u * ROW, SCALES = 2u * V, BYTES = 2u * V + (TYPE == EFF_KV_I8 ? 256u : 0u);
-  static constexpr uint32_t LOADS = 2u * V / 1024u;   // of 64 lanes, 16 bytes each
-  static constexpr uint32_t MINE = (LOADS + 3u) / 4u;
+  static constexpr uint32_t FILLS = (ROW + 63u) / 64u;        // loads of 64 x 16 bytes for 16 rows
+  static constexpr uint32_t HALF = 1024u * FILLS;             // and the LDS they take
+  static constexpr uint32_t V = 2u * HALF, SCALES = 2u * V, BYTES = 2u * V + (TYPE == EFF_KV_I8 ? 256u : 0u);
 
   // where piece c of row r lies in the row, and back
   static __device__ __forceinline__ uint32_t place(uint32_t r, uint32_t c) {
@@ -710,31 +709,22 @@ struct AttnStage {
   }
 };
 
-// 16 (4) bytes a lane from its own address into LDS at lds + 16 (4) * lane.
-__device__ __forceinline__ void fill16(const uint8_t *p, const uint8_t *lds) {
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  __asm__ volatile("global_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
-}
-
+// 4 bytes a lane from its own address into LDS at lds + 4 * lane.
 __device__ __forceinline__ void fill4(const uint8_t *p, const uint8_t *lds) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
   __asm__ volatile("global_load_lds_dword %0, off" : : "v"(p), "{m0}"(m0) : "memory");
 }
 
-// Waits for all but the N youngest loads of the wave and for its LDS reads, then
-// for the other waves.
-template <uint32_t N>
-__device__ __forceinline__ void wait_step() {
-  __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
-}
+// Waits for the wave's loads and LDS reads, then for the other waves.
+__device__ __forceinline__ void wait_step() { __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-template <int TYPE, int D, int MT>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles,
-                                                                      uint32_t per_seq, uint32_t min_rows) {
+template <int TYPE, int D, int MT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles, uint32_t per_seq,
+                                                          uint32_t min_rows) {
   using W = AttnWave<TYPE, D, MT, false>;
   using S = AttnStage<TYPE, D>;
-  constexpr uint32_t R = 64u * MT;
-  __shared__ __align__(1024) uint8_t buf[3][S::BYTES];
+  constexpr uint32_t R = 16u * NW * MT;
+  __shared__ __align__(1024) uint8_t buf[2][S::BYTES];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
   // the last tiles of a sequence see the most: first
@@ -758,21 +748,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(KvView kv, 
   W w;
   float q[MT][W::KS][8];
   w.load_q(q, a, m, group, kvh, 0, n, g);
-  w.init(q, a.scale, nullptr, wave, 4);
+  w.init(q, a.scale, nullptr, wave, NW);
 
   const uint32_t *table = b.table + (uint64_t)t.seq * b.table_pages;
   const uint64_t to_v = (uint64_t)kv.heads * kv.block_bytes;
   const uint32_t mask = (1u << kv.page_log2) - 1u;
-  uint32_t off[S::MINE];   // of the lane's pieces: its place in the half's rows
+  // a step's fills: K's 16 rows of each half, then V's; the wave's are NW apart
+  constexpr uint32_t MINE = 4u * S::FILLS / NW;
+  uint32_t off[MINE];   // of a lane's piece within the 16 rows
 #pragma unroll
-  for (uint32_t k = 0; k < S::MINE; ++k) {
-    const uint32_t at = ((4u * k + wave) * 64u + lane) % (S::V / 16u), r = at / S::PIECES;
-    // V lies as it is
-    off[k] = (r & 15u) * S::ROW + 16u * ((4u * k + wave) * 64u < S::V / 16u ? S::piece(r, at % S::PIECES) : at % S::PIECES);
+  for (uint32_t k = 0; k < MINE; ++k) {
+    const uint32_t l = NW * k + wave, at = l % S::FILLS * 64u + lane, r = at / S::PIECES;
+    off[k] = l / S::FILLS < 2u ? r * S::ROW + 16u * S::piece(r, at % S::PIECES) : 16u * at;
   }
   uint32_t ids = 0;
   const int steps = t.end > base ? (t.end - base + 31) / 32 : 0;
-  uint32_t gone = 0;       // two bits a step, of the last three
+  bool gone[2] = {};
   auto issue = [&](int i) {
     const int t0 = base + 32 * i;
     if ((i & 31) == 0) {
@@ -780,54 +771,51 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(KvView kv, 
       ids = at < t.end ? table[(uint32_t)at >> kv.page_log2] : ~0u;
     }
     const uint8_t *blk[2];
+    uint32_t slot[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t p = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + u);
-      gone = gone << 1 | (p >= kv.pages);
-      blk[u] = kv.base + (p >= kv.pages ? 0ull : (uint64_t)p * kv.page_bytes) + (uint64_t)kvh * kv.block_bytes;
+      gone[u] = p >= kv.pages;
+      blk[u] = kv.base + (gone[u] ? 0ull : (uint64_t)p * kv.page_bytes) + (uint64_t)kvh * kv.block_bytes;
+      slot[u] = (uint32_t)(t0 + 16 * u) & mask;
     }
-    const uint32_t slot[2] = {(uint32_t)t0 & mask, (uint32_t)(t0 + 16) & mask};
-    const uint8_t *lds = buf[i % 3];
+    const uint8_t *lds = buf[i & 1];
 #pragma unroll
-    for (uint32_t k = 0; k < S::MINE; ++k) {
-      const uint32_t l = 4u * k + wave;   // load l of K's and V's
-      if (S::LOADS % 4u && l >= S::LOADS) break;
-      const uint32_t r = (l * 64u + lane) % (S::V / 16u) / S::PIECES;
-      const uint8_t *p = (r < 16u ? blk[0] + slot[0] * S::ROW : blk[1] + slot[1] * S::ROW) + off[k] + (l * 64u < S::V / 16u ? 0ull : to_v);
-      fill16(p, lds + 1024u * l);
+    for (uint32_t k = 0; k < MINE; ++k) {
+      const uint32_t l = NW * k + wave, which = l / S::FILLS, sub = l % S::FILLS, u = which & 1u;
+      const rsrc_t r = make_rsrc((u ? blk[1] : blk[0]) + (which >> 1 ? to_v : 0ull), kv.block_bytes);
+      const uint32_t row = (u ? slot[1] : slot[0]) * S::ROW;
+      // 16 rows that are no whole number of fills: the last one's upper lanes have none
+      if (S::ROW % 64u == 0u || sub * 64u + lane < S::ROW)
+        dma16(r, lds + which * S::HALF + sub * 1024u, off[k], row);
     }
     if constexpr (W::I8) {
-      if (wave == 3u) {
+      if (wave == NW - 1u) {
         const uint32_t u = lane >> 4 & 1u;
         fill4((u ? blk[1] + slot[1] * 4u : blk[0] + slot[0] * 4u) + ((uint32_t)D << kv.page_log2) + 4u * (lane & 15u) + (lane < 32u ? 0ull : to_v),
               lds + S::SCALES);
       }
     }
   };
-  // loads of the next step that the wave may leave under way
-  constexpr uint32_t NEXT = S::LOADS / 4u;
   if (steps) issue(0);
-  if (steps > 1) issue(1);
 #pragma unroll 1
   for (int i = 0; i < steps; ++i) {
-    if (i + 1 < steps) wait_step<NEXT>();
-    else wait_step<0>();
-    const bool was[2] = {i + 1 < steps ? (gone & 8u) != 0u : (gone & 2u) != 0u, i + 1 < steps ? (gone & 4u) != 0u : (gone & 1u) != 0u};
-    if (i + 2 < steps) issue(i + 2);
+    const bool was[2] = {gone[0], gone[1]};
+    wait_step();
+    if (i + 1 < steps) issue(i + 1);
     const int t0 = base + 32 * i;
     if (t0 >= m.end || t0 + 32 <= m.begin) continue;
-    const uint8_t *lds = buf[i % 3];
+    const uint8_t *lds = buf[i & 1];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint32_t r = 16u * u + n;
-      const uint8_t *p = lds + r * S::ROW;
+      const uint8_t *p = lds + u * S::HALF + n * S::ROW;
       if constexpr (!W::I8) {
 #pragma unroll
-        for (int c = 0; c < W::KS; ++c) ld_words<4>(w.kw[u] + 4 * c, p + 16u * S::place(r, 4u * c + g));
+        for (int c = 0; c < W::KS; ++c) ld_words<4>(w.kw[u] + 4 * c, p + 16u * S::place(n, 4u * c + g));
       } else {
 #pragma unroll
-        for (int c = 0; c + 1 < W::KS; c += 2) ld_words<4>(w.kw[u] + 2 * c, p + 16u * S::place(r, 2u * c + g));
-        if constexpr (W::KS & 1) ld_words<2>(w.kw[u] + 2 * (W::KS - 1), p + 16u * S::place(r, 2u * (W::KS - 1) + g / 2u) + 8u * (g & 1u));
+        for (int c = 0; c + 1 < W::KS; c += 2) ld_words<4>(w.kw[u] + 2 * c, p + 16u * S::place(n, 2u * c + g));
+        if constexpr (W::KS & 1) ld_words<2>(w.kw[u] + 2 * (W::KS - 1), p + 16u * S::place(n, 2u * (W::KS - 1) + g / 2u) + 8u * (g & 1u));
         ld_words<4>(w.ks[u], lds + S::SCALES + 64u * u + 16u * g);
       }
     }
@@ -835,7 +823,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_rows(KvView kv, 
     w.scores(s);
     __builtin_amdgcn_sched_barrier(0);   // V's registers are K's
 #pragma unroll
-    for (int u = 0; u < 2; ++u) w.load_rows(u, lds + S::V + 16u * u * S::ROW, lds + S::SCALES + 128u + 64u * u, n, g);
+    for (int u = 0; u < 2; ++u) w.load_rows(u, lds + S::V + u * S::HALF, lds + S::SCALES + 128u + 64u * u, n, g);
     const bool masked = was[0] || was[1] || t0 + 31 > m.first || t0 < m.begin || (window && t0 <= m.last - window);
     w.step(t0, masked, was, m, window, g, s);
   }
@@ -874,8 +862,7 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // Sequences with more than 64 rows go to k_attn_rows where their tiles fill half
   // of the CUs without chunks
   if (most > kFewRows && rows / 64u * kv.heads >= 128u) {
-    p.many = kv.dim < 256u && rows / 128u * kv.heads >= 512u ? 2u : 1u;
-    attn_tiles(most, rows, b.seqs, 64u * p.many, &p.many_tiles, &p.many_per_seq);
+    attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
     p.max_rows = kFewRows;
     most = kFewRows;
     if (b.seqs == 1u) return p;
@@ -915,16 +902,11 @@ size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs 
 template <int TYPE, int D>
 static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t s) {
   const AttnPlan p = attn_plan(kv, b, a);
-  if (p.many) {
+  if (p.many_tiles) {
     const uint64_t g = (uint64_t)p.many_tiles * kv.heads;
     const uint32_t min_rows = b.seqs == 1u ? 1u : kFewRows + 1u;
     if (g > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    if constexpr (D < 256) {
-      if (p.many == 2u)
-        hipLaunchKernelGGL((k_attn_rows<TYPE, D, 2>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
-    }
-    if (p.many == 1u)
-      hipLaunchKernelGGL((k_attn_rows<TYPE, D, 1>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
+    hipLaunchKernelGGL((k_attn_rows<TYPE, D, 1, 4>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.tiles) return e;
   }
