@@ -91,18 +91,27 @@ struct LogitsArgs {
 hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream);
 
 #ifdef __HIP__
-// The sequence of new token t: the last whose first token is at most t (the
-// whole wave asks for one t). Returns `seqs` for a token of no sequence.
-__device__ __forceinline__ uint32_t kv_seq_of(const KvBatchView &b, uint32_t t) {
+// The sequence of new token t (the whole wave asks for one t): the last whose
+// first token is at most t, its first token, the next one's, and its length; one
+// round trip up to 63 sequences. False for a token of no sequence.
+struct KvSeq {
+  uint32_t seq, first, next, len;
+};
+__device__ __forceinline__ bool kv_seq_of(const KvBatchView &b, uint32_t t, KvSeq &s) {
   const uint32_t lane = threadIdx.x & 63u;
-  uint32_t n = 0;
-  for (uint32_t at = 0; at <= b.seqs; at += 64u) {
+  for (uint32_t at = 0;; at += 63u) {   // a block's last start is the next one's first
     const uint32_t i = at + lane;
-    const uint32_t c = __popcll(__ballot(i <= b.seqs && b.starts[i <= b.seqs ? i : b.seqs] <= t));
-    n += c;
-    if (c < 64u) break;
+    const uint32_t start = i <= b.seqs ? b.starts[i] : ~0u, len = i < b.seqs ? b.lens[i] : 0u;
+    const uint64_t past = __ballot(start > t);
+    const uint32_t n = past ? (uint32_t)__ffsll((unsigned long long)past) - 1u : 64u;   // starts[at .. at + n) <= t
+    if (n == 64u && at + 64u <= b.seqs) continue;
+    if (n == 0u || at + n > b.seqs) return false;
+    s.seq = at + n - 1u;
+    s.first = __builtin_amdgcn_readlane(start, n - 1u);
+    s.next = n < 64u ? __builtin_amdgcn_readlane(start, n) : ~0u;
+    s.len = min((uint32_t)__builtin_amdgcn_readlane(len, n - 1u), b.max_len);
+    return true;
   }
-  return n ? min(n - 1u, b.seqs) : b.seqs;
 }
 
 // Tokens of sequence s, the new ones included, as far as the call reaches.

@@ -41,101 +41,122 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
 }
 
 // A workgroup takes rows of one token; L lanes take a row, 4 values each: the
-// pairs 2 l and 2 l + 1 of the row's D / 2 pairs.
-template <int TYPE, int D>
+// pairs 2 l and 2 l + 1 of the row's D / 2 pairs. The token's sequence and page are
+// two dependent round trips; a thread's U rows are requested before them, so that
+// many tokens keep enough bytes under way (7 prompts of up to 1021 tokens of 24
+// heads of 256: U = 1 77 us, 4 WAIT_FOR_MEASUREMENT).
+template <int TYPE, int D, int U>
 __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t wgs) {
 #pragma clang fp contract(off)
   constexpr uint32_t L = D == 96 ? 32u : D / 4u, ROWS = 256u / L;
-  const uint32_t t = blockIdx.x / wgs, lane = threadIdx.x & 63u, l = lane % L;
-  const uint32_t heads = a.q_heads + 2u * kv.heads;
-  const uint32_t r = (blockIdx.x % wgs) * ROWS + threadIdx.x / L;
-  const uint32_t s = kv_seq_of(b, t);
-  if (s >= b.seqs) return;
-  const uint32_t n = b.starts[s + 1] - b.starts[s], len = kv_len(b, s), back = n - (t - b.starts[s]);
-  const bool on = r < heads && l < D / 4u, placed = back <= len;
-  const uint32_t pos = placed ? len - back : 0u;
-  const bool is_q = r < a.q_heads, is_v = r >= a.q_heads + kv.heads;
-  const uint32_t h = is_q ? r : is_v ? r - a.q_heads - kv.heads : r - a.q_heads;
-  const float *src = is_q ? a.q + (uint64_t)t * a.q_stride : is_v ? a.v + (uint64_t)t * a.v_stride
-                                                                  : a.k + (uint64_t)t * a.k_stride;
-  // the places of the lane's pairs: (i0, j0) and (i0 + step, j0 + step)
+  const uint32_t t = blockIdx.x / wgs, l = (threadIdx.x & 63u) % L;
+  const uint32_t heads = a.q_heads + 2u * kv.heads, r0 = (blockIdx.x % wgs) * ROWS * U + threadIdx.x / L;
   const uint32_t half = a.rope_dim / 2u;
-  const bool split = !is_v && a.halves && 2u * l < half;
-  const uint32_t i0 = split ? 2u * l : 4u * l, j0 = split ? half + 2u * l : 4u * l + 1u;
-  float x[4] = {};   // pair 0, pair 1
-  if (on) {
-    if (split) {
-      const float2 u = *(const float2 *)(src + h * D + i0), w = *(const float2 *)(src + h * D + j0);
-      x[0] = u.x, x[1] = w.x, x[2] = u.y, x[3] = w.y;
-    } else {
-      const float4 u = *(const float4 *)(src + h * D + i0);
-      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-    }
-  }
-  const uint32_t step = split ? 1u : 2u;
-  const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-  if (w != nullptr) {
-    float sum = 0.f;
+  // the places of the lane's pairs: (i0, j0) and (i0 + step, j0 + step); v rows
+  // take the unsplit ones
+  const bool turns = 2u * l < half, apart = turns && a.halves;
+  float x[U][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += x[i] * x[i];
-    sum = group_sum<L>(sum);
-    const float inv = 1.f / sqrtf(sum / (float)D + a.eps);
-    if (on) {
-      x[0] = x[0] * inv * w[i0], x[1] = x[1] * inv * w[j0];
-      x[2] = x[2] * inv * w[i0 + step], x[3] = x[3] * inv * w[j0 + step];
+  for (uint32_t u = 0; u < U; ++u) {
+    const uint32_t r = r0 + ROWS * u;
+    const bool is_q = r < a.q_heads, is_v = r >= a.q_heads + kv.heads;
+    const uint32_t h = is_q ? r : is_v ? r - a.q_heads - kv.heads : r - a.q_heads;
+    const float *src = (is_q ? a.q + (uint64_t)t * a.q_stride : is_v ? a.v + (uint64_t)t * a.v_stride : a.k + (uint64_t)t * a.k_stride) + h * D;
+    x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
+    if (r < heads && l < D / 4u) {
+      if (apart && !is_v) {
+        const float2 c = *(const float2 *)(src + 2u * l), d = *(const float2 *)(src + half + 2u * l);
+        x[u][0] = c.x, x[u][1] = d.x, x[u][2] = c.y, x[u][3] = d.y;
+      } else {
+        const float4 c = *(const float4 *)(src + 4u * l);
+        x[u][0] = c.x, x[u][1] = c.y, x[u][2] = c.z, x[u][3] = c.w;
+      }
     }
   }
-  if (!is_v && on && 2u * l < half) {
-    const float *cs = a.rope + (uint64_t)pos * a.rope_dim + 2u * l;
-    const float2 c = *(const float2 *)cs, sn = *(const float2 *)(cs + half);
-    const float y0 = x[0] * c.x - x[1] * sn.x, y1 = x[0] * sn.x + x[1] * c.x;
-    const float y2 = x[2] * c.y - x[3] * sn.y, y3 = x[2] * sn.y + x[3] * c.y;
-    x[0] = y0, x[1] = y1, x[2] = y2, x[3] = y3;
-  }
-  if (is_q) {
-    if (!on) return;
-    float *o = a.q_out + ((uint64_t)t * a.q_heads + h) * D;
-    if (!placed) x[0] = x[1] = x[2] = x[3] = 0.f;
-    if (split) {
-      *(float2 *)(o + i0) = make_float2(x[0], x[2]);
-      *(float2 *)(o + j0) = make_float2(x[1], x[3]);
-    } else {
-      *(float4 *)(o + i0) = make_float4(x[0], x[1], x[2], x[3]);
-    }
-    return;
-  }
+  KvSeq s;
+  if (!kv_seq_of(b, t, s)) return;
+  const uint32_t back = s.next - t;   // positions from the sequence's end
+  const bool placed = back <= s.len;
+  const uint32_t pos = placed ? s.len - back : 0u;
   // a page number past the cache holds nothing
-  const uint32_t page = placed ? b.table[(uint64_t)s * b.table_pages + (pos >> kv.page_log2)] : ~0u;
+  const uint32_t page = placed ? b.table[(uint64_t)s.seq * b.table_pages + (pos >> kv.page_log2)] : ~0u;
   const uint32_t slot = pos & ((1u << kv.page_log2) - 1u);
-  const bool store = on && page < kv.pages;
-  uint8_t *blk = kv.base + (store ? (uint64_t)page * kv.page_bytes + (uint64_t)((is_v ? kv.heads : 0u) + h) * kv.block_bytes : 0u);
-  if constexpr (TYPE == EFF_KV_F16) {
-    if (!store) return;
-    _Float16 *o = (_Float16 *)blk + slot * D;
-    if (split) {
-      o[i0] = (_Float16)x[0], o[i0 + 1] = (_Float16)x[2], o[j0] = (_Float16)x[1], o[j0 + 1] = (_Float16)x[3];
+  float2 cs = make_float2(1.f, 1.f), sn = make_float2(0.f, 0.f);
+  if (turns) {
+    const float *p = a.rope + (uint64_t)pos * a.rope_dim + 2u * l;
+    cs = *(const float2 *)p, sn = *(const float2 *)(p + half);
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < U; ++u) {
+    const uint32_t r = r0 + ROWS * u;
+    const bool on = r < heads && l < D / 4u, is_q = r < a.q_heads, is_v = r >= a.q_heads + kv.heads;
+    const uint32_t h = is_q ? r : is_v ? r - a.q_heads - kv.heads : r - a.q_heads;
+    const bool split = apart && !is_v;
+    const uint32_t i0 = split ? 2u * l : 4u * l, j0 = split ? half + 2u * l : 4u * l + 1u, step = split ? 1u : 2u;
+    const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    if (w != nullptr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += x[u][i] * x[u][i];
+      sum = group_sum<L>(sum);
+      const float inv = 1.f / sqrtf(sum / (float)D + a.eps);
+      if (on) {
+        x[u][0] = x[u][0] * inv * w[i0], x[u][1] = x[u][1] * inv * w[j0];
+        x[u][2] = x[u][2] * inv * w[i0 + step], x[u][3] = x[u][3] * inv * w[j0 + step];
+      }
+    }
+    if (!is_v && turns) {
+      const float y0 = x[u][0] * cs.x - x[u][1] * sn.x, y1 = x[u][0] * sn.x + x[u][1] * cs.x;
+      const float y2 = x[u][2] * cs.y - x[u][3] * sn.y, y3 = x[u][2] * sn.y + x[u][3] * cs.y;
+      x[u][0] = y0, x[u][1] = y1, x[u][2] = y2, x[u][3] = y3;
+    }
+    if (is_q) {
+      if (!on) continue;
+      float *o = a.q_out + ((uint64_t)t * a.q_heads + h) * D;
+      if (!placed) x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
+      if (split) {
+        *(float2 *)(o + i0) = make_float2(x[u][0], x[u][2]);
+        *(float2 *)(o + j0) = make_float2(x[u][1], x[u][3]);
+      } else {
+        *(float4 *)(o + i0) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+      }
+      continue;
+    }
+    const bool store = on && page < kv.pages;
+    uint8_t *blk = kv.base + (store ? (uint64_t)page * kv.page_bytes + (uint64_t)((is_v ? kv.heads : 0u) + h) * kv.block_bytes : 0u);
+    if constexpr (TYPE == EFF_KV_F16) {
+      if (!store) continue;
+      typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+      _Float16 *o = (_Float16 *)blk + slot * D;
+      if (split) {
+        *(half2v *)(o + i0) = half2v{(_Float16)x[u][0], (_Float16)x[u][2]};
+        *(half2v *)(o + j0) = half2v{(_Float16)x[u][1], (_Float16)x[u][3]};
+      } else {
+        *(half4 *)(o + i0) = half4{(_Float16)x[u][0], (_Float16)x[u][1], (_Float16)x[u][2], (_Float16)x[u][3]};
+      }
     } else {
+      // the largest magnitude by its bits: a NaN is larger than any number, and
+      // makes the row's scale, and so every value of the row, NaN
+      uint32_t top = 0;
 #pragma unroll
-      for (uint32_t i = 0; i < 4u; ++i) o[i0 + i] = (_Float16)x[i];
+      for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[u][i]) & 0x7FFFFFFFu);
+      const float m = __uint_as_float(group_max<L>(top));
+      if (!store) continue;
+      const float inv = m > 0.f ? 127.f / m : 0.f;
+      int8_t *o = (int8_t *)blk + slot * D;
+      uint32_t q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = rintf(x[u][i] * inv);
+        q[i] = (uint32_t)(int)(y >= -127.f && y <= 127.f ? y : 0.f) & 0xFFu;
+      }
+      if (split) {
+        *(uint16_t *)(o + i0) = (uint16_t)(q[0] | q[2] << 8), *(uint16_t *)(o + j0) = (uint16_t)(q[1] | q[3] << 8);
+      } else {
+        *(uint32_t *)(o + i0) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+      }
+      if (l == 0u) ((float *)(blk + ((uint64_t)D << kv.page_log2)))[slot] = m * (1.f / 127.f);
     }
-  } else {
-    // the largest magnitude by its bits: a NaN is larger than any number, and
-    // makes the row's scale, and so every value of the row, NaN
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    const float m = __uint_as_float(group_max<L>(top));
-    if (!store) return;
-    const float inv = m > 0.f ? 127.f / m : 0.f;
-    int8_t *o = (int8_t *)blk + slot * D;
-    int8_t q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float y = rintf(x[i] * inv);
-      q[i] = (int8_t)(int)(y >= -127.f && y <= 127.f ? y : 0.f);
-    }
-    o[i0] = q[0], o[j0] = q[1], o[i0 + step] = q[2], o[j0 + step] = q[3];
-    if (l == 0u) ((float *)(blk + ((uint64_t)D << kv.page_log2)))[slot] = m * (1.f / 127.f);
   }
 }
 
@@ -147,19 +168,28 @@ hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positi
   return hipGetLastError();
 }
 
+template <int TYPE, int D>
+static hipError_t append_dim(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
+  constexpr uint32_t rows = D == 96 ? 8u : 1024u / D;   // of a workgroup, U = 1
+  const uint32_t heads = a.q_heads + 2u * kv.heads;
+  // 4 rows a thread where that still gives a CU 8 workgroups
+  const uint32_t one = (heads + rows - 1u) / rows, four = (heads + 4u * rows - 1u) / (4u * rows);
+  if ((uint64_t)b.tokens * four >= 2048u)
+    hipLaunchKernelGGL((k_kv_append<TYPE, D, 4>), dim3(b.tokens * four), dim3(256), 0, s, kv, b, a, four);
+  else
+    hipLaunchKernelGGL((k_kv_append<TYPE, D, 1>), dim3(b.tokens * one), dim3(256), 0, s, kv, b, a, one);
+  return hipGetLastError();
+}
+
 template <int TYPE>
 static hipError_t append_go(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
-  const uint32_t rows = kv.dim == 96u ? 8u : 1024u / kv.dim;   // of a workgroup
-  const uint32_t wgs = (a.q_heads + 2u * kv.heads + rows - 1u) / rows;
-  const dim3 grid(b.tokens * wgs);
   switch (kv.dim) {
-    case 64: hipLaunchKernelGGL((k_kv_append<TYPE, 64>), grid, dim3(256), 0, s, kv, b, a, wgs); break;
-    case 96: hipLaunchKernelGGL((k_kv_append<TYPE, 96>), grid, dim3(256), 0, s, kv, b, a, wgs); break;
-    case 128: hipLaunchKernelGGL((k_kv_append<TYPE, 128>), grid, dim3(256), 0, s, kv, b, a, wgs); break;
-    case 256: hipLaunchKernelGGL((k_kv_append<TYPE, 256>), grid, dim3(256), 0, s, kv, b, a, wgs); break;
+    case 64: return append_dim<TYPE, 64>(kv, b, a, s);
+    case 96: return append_dim<TYPE, 96>(kv, b, a, s);
+    case 128: return append_dim<TYPE, 128>(kv, b, a, s);
+    case 256: return append_dim<TYPE, 256>(kv, b, a, s);
     default: return hipErrorInvalidValue;
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t stream) {
