@@ -26,134 +26,151 @@ __global__ __launch_bounds__(256) void k_rope_table(RopeFreqs f, uint32_t pairs,
   out[(uint64_t)p * 2u * pairs + pairs + j] = (float)(s * (double)scale);
 }
 
+// Sum and maximum over groups of L lanes: DPP within 16, then swaps of 16-lane
+// rows and of the wave's halves.
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o);
+  v = dpp_row_sum(v);
+  if constexpr (L >= 32) {
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (L == 64) {
+    auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
   return v;
 }
 
 template <int L>
 __device__ __forceinline__ uint32_t group_max(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+  if constexpr (L >= 32) {
+    auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)p[0], (uint32_t)p[1]);
+  }
+  if constexpr (L == 64) {
+    auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max((uint32_t)p[0], (uint32_t)p[1]);
+  }
   return v;
 }
 
-// A workgroup takes rows of one token; L lanes take a row, 4 values each: the
-// pairs 2 l and 2 l + 1 of the row's D / 2 pairs. The token's sequence and page are
-// two dependent round trips; a thread's U rows are requested before them, so that
-// many tokens keep enough bytes under way (7 prompts of up to 1021 tokens of 24
-// heads of 256: U = 1 77 us, 4 WAIT_FOR_MEASUREMENT).
+// The lane's 4 values of a row, as its pairs: (0, 1) and (2, 3). `apart`: 2 l and
+// 2 l + 1 of each half of the rotated part, else 4 side by side.
+__device__ __forceinline__ void load4(float x[4], const float *p, bool apart, uint32_t half, uint32_t l) {
+  if (apart) {
+    const float2 c = *(const float2 *)(p + 2u * l), d = *(const float2 *)(p + half + 2u * l);
+    x[0] = c.x, x[1] = d.x, x[2] = c.y, x[3] = d.y;
+  } else {
+    const float4 c = *(const float4 *)(p + 4u * l);
+    x[0] = c.x, x[1] = c.y, x[2] = c.z, x[3] = c.w;
+  }
+}
+
+// A workgroup takes rows of one token and of one kind (q, k or v: what differs
+// between them is then scalar); L lanes take a row, 4 values each: the pairs 2 l
+// and 2 l + 1 of the row's D / 2 pairs. Its bytes bound a long append, round trips a
+// short one: the token's sequence and then its page are two dependent ones, and a
+// thread's U rows are requested before them, so that many tokens keep enough bytes
+// under way (us, U = 1 / 4: 4780 tokens of 24 heads of 256 with norms 72.2 / 56.9, 3.9
+// TB/s; 4780 of 48 heads of 128 54.4 / 48.8, 4.6 TB/s; 1340 tokens 14.9 / 16.1, 270
+// 6.8 / 7.1).
 template <int TYPE, int D, int U>
-__global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t wgs) {
+__global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t q_wgs, uint32_t k_wgs) {
 #pragma clang fp contract(off)
   constexpr uint32_t L = D == 96 ? 32u : D / 4u, ROWS = 256u / L;
-  const uint32_t t = blockIdx.x / wgs, l = (threadIdx.x & 63u) % L;
-  const uint32_t heads = a.q_heads + 2u * kv.heads, r0 = (blockIdx.x % wgs) * ROWS * U + threadIdx.x / L;
-  const uint32_t half = a.rope_dim / 2u;
-  // the places of the lane's pairs: (i0, j0) and (i0 + step, j0 + step); v rows
-  // take the unsplit ones
-  const bool turns = 2u * l < half, apart = turns && a.halves;
+  const uint32_t wgs = q_wgs + 2u * k_wgs, t = blockIdx.x / wgs, w = blockIdx.x % wgs, l = (threadIdx.x & 63u) % L;
+  const bool is_q = w < q_wgs, is_v = w >= q_wgs + k_wgs;
+  const uint32_t heads = is_q ? a.q_heads : kv.heads, h0 = (is_q ? w : is_v ? w - q_wgs - k_wgs : w - q_wgs) * ROWS * U + threadIdx.x / L;
+  const float *src = is_q ? a.q + (uint64_t)t * a.q_stride : is_v ? a.v + (uint64_t)t * a.v_stride : a.k + (uint64_t)t * a.k_stride;
+  const float *norm = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+  const uint32_t half = is_v ? 0u : a.rope_dim / 2u;
+  const bool in = D != 96 || l < D / 4u, turns = 2u * l < half, apart = turns && a.halves;
   float x[U][4];
 #pragma unroll
   for (uint32_t u = 0; u < U; ++u) {
-    const uint32_t r = r0 + ROWS * u;
-    const bool is_q = r < a.q_heads, is_v = r >= a.q_heads + kv.heads;
-    const uint32_t h = is_q ? r : is_v ? r - a.q_heads - kv.heads : r - a.q_heads;
-    const float *src = (is_q ? a.q + (uint64_t)t * a.q_stride : is_v ? a.v + (uint64_t)t * a.v_stride : a.k + (uint64_t)t * a.k_stride) + h * D;
     x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
-    if (r < heads && l < D / 4u) {
-      if (apart && !is_v) {
-        const float2 c = *(const float2 *)(src + 2u * l), d = *(const float2 *)(src + half + 2u * l);
-        x[u][0] = c.x, x[u][1] = d.x, x[u][2] = c.y, x[u][3] = d.y;
-      } else {
-        const float4 c = *(const float4 *)(src + 4u * l);
-        x[u][0] = c.x, x[u][1] = c.y, x[u][2] = c.z, x[u][3] = c.w;
-      }
-    }
+    if (in && h0 + ROWS * u < heads) load4(x[u], src + (h0 + ROWS * u) * D, apart, half, l);
   }
+  float weight[4] = {};
+  if (norm && in) load4(weight, norm, apart, half, l);
   KvSeq s;
   if (!kv_seq_of(b, t, s)) return;
   const uint32_t back = s.next - t;   // positions from the sequence's end
   const bool placed = back <= s.len;
   const uint32_t pos = placed ? s.len - back : 0u;
   // a page number past the cache holds nothing
-  const uint32_t page = placed ? b.table[(uint64_t)s.seq * b.table_pages + (pos >> kv.page_log2)] : ~0u;
-  const uint32_t slot = pos & ((1u << kv.page_log2) - 1u);
-  float2 cs = make_float2(1.f, 1.f), sn = make_float2(0.f, 0.f);
+  uint32_t page = ~0u;
+  if (placed && !is_q) page = b.table[(uint64_t)s.seq * b.table_pages + (pos >> kv.page_log2)];
+  float2 c = make_float2(1.f, 1.f), d = make_float2(0.f, 0.f);
   if (turns) {
     const float *p = a.rope + (uint64_t)pos * a.rope_dim + 2u * l;
-    cs = *(const float2 *)p, sn = *(const float2 *)(p + half);
+    c = *(const float2 *)p, d = *(const float2 *)(p + half);
   }
+  const bool store = is_q || page < kv.pages;
+  uint8_t *block = kv.base + (is_q || !store ? 0u : (uint64_t)page * kv.page_bytes + (is_v ? (uint64_t)kv.heads * kv.block_bytes : 0u));
+  const uint32_t slot = pos & ((1u << kv.page_log2) - 1u);
 #pragma unroll
   for (uint32_t u = 0; u < U; ++u) {
-    const uint32_t r = r0 + ROWS * u;
-    const bool on = r < heads && l < D / 4u, is_q = r < a.q_heads, is_v = r >= a.q_heads + kv.heads;
-    const uint32_t h = is_q ? r : is_v ? r - a.q_heads - kv.heads : r - a.q_heads;
-    const bool split = apart && !is_v;
-    const uint32_t i0 = split ? 2u * l : 4u * l, j0 = split ? half + 2u * l : 4u * l + 1u, step = split ? 1u : 2u;
-    const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-    if (w != nullptr) {
+    const uint32_t h = h0 + ROWS * u;
+    float *y = x[u];
+    if (norm) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += x[u][i] * x[u][i];
-      sum = group_sum<L>(sum);
-      const float inv = 1.f / sqrtf(sum / (float)D + a.eps);
-      if (on) {
-        x[u][0] = x[u][0] * inv * w[i0], x[u][1] = x[u][1] * inv * w[j0];
-        x[u][2] = x[u][2] * inv * w[i0 + step], x[u][3] = x[u][3] * inv * w[j0 + step];
-      }
+      for (int i = 0; i < 4; ++i) sum += y[i] * y[i];
+      const float inv = __builtin_amdgcn_rsqf(group_sum<L>(sum) * (1.f / D) + a.eps);   // to one unit in the last place
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = y[i] * inv * weight[i];
     }
-    if (!is_v && turns) {
-      const float y0 = x[u][0] * cs.x - x[u][1] * sn.x, y1 = x[u][0] * sn.x + x[u][1] * cs.x;
-      const float y2 = x[u][2] * cs.y - x[u][3] * sn.y, y3 = x[u][2] * sn.y + x[u][3] * cs.y;
-      x[u][0] = y0, x[u][1] = y1, x[u][2] = y2, x[u][3] = y3;
+    if (turns) {
+      const float y0 = y[0] * c.x - y[1] * d.x, y1 = y[0] * d.x + y[1] * c.x;
+      const float y2 = y[2] * c.y - y[3] * d.y, y3 = y[2] * d.y + y[3] * c.y;
+      y[0] = y0, y[1] = y1, y[2] = y2, y[3] = y3;
     }
+    const bool on = in && h < heads;
     if (is_q) {
       if (!on) continue;
       float *o = a.q_out + ((uint64_t)t * a.q_heads + h) * D;
-      if (!placed) x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.f;
-      if (split) {
-        *(float2 *)(o + i0) = make_float2(x[u][0], x[u][2]);
-        *(float2 *)(o + j0) = make_float2(x[u][1], x[u][3]);
+      if (!placed) y[0] = y[1] = y[2] = y[3] = 0.f;
+      if (apart) {
+        *(float2 *)(o + 2u * l) = make_float2(y[0], y[2]), *(float2 *)(o + half + 2u * l) = make_float2(y[1], y[3]);
       } else {
-        *(float4 *)(o + i0) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+        *(float4 *)(o + 4u * l) = make_float4(y[0], y[1], y[2], y[3]);
       }
       continue;
     }
-    const bool store = on && page < kv.pages;
-    uint8_t *blk = kv.base + (store ? (uint64_t)page * kv.page_bytes + (uint64_t)((is_v ? kv.heads : 0u) + h) * kv.block_bytes : 0u);
+    uint8_t *blk = block + (uint64_t)h * kv.block_bytes;
     if constexpr (TYPE == EFF_KV_F16) {
-      if (!store) continue;
+      if (!on || !store) continue;
       typedef _Float16 half2v __attribute__((ext_vector_type(2)));
       _Float16 *o = (_Float16 *)blk + slot * D;
-      if (split) {
-        *(half2v *)(o + i0) = half2v{(_Float16)x[u][0], (_Float16)x[u][2]};
-        *(half2v *)(o + j0) = half2v{(_Float16)x[u][1], (_Float16)x[u][3]};
+      if (apart) {
+        *(half2v *)(o + 2u * l) = half2v{(_Float16)y[0], (_Float16)y[2]};
+        *(half2v *)(o + half + 2u * l) = half2v{(_Float16)y[1], (_Float16)y[3]};
       } else {
-        *(half4 *)(o + i0) = half4{(_Float16)x[u][0], (_Float16)x[u][1], (_Float16)x[u][2], (_Float16)x[u][3]};
+        *(half4 *)(o + 4u * l) = half4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
       }
     } else {
       // the largest magnitude by its bits: a NaN is larger than any number, and
       // makes the row's scale, and so every value of the row, NaN
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[u][i]) & 0x7FFFFFFFu);
+      for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(y[i]) & 0x7FFFFFFFu);
       const float m = __uint_as_float(group_max<L>(top));
-      if (!store) continue;
+      if (!on || !store) continue;
       const float inv = m > 0.f ? 127.f / m : 0.f;
       int8_t *o = (int8_t *)blk + slot * D;
       uint32_t q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = rintf(x[u][i] * inv);
-        q[i] = (uint32_t)(int)(y >= -127.f && y <= 127.f ? y : 0.f) & 0xFFu;
-      }
-      if (split) {
-        *(uint16_t *)(o + i0) = (uint16_t)(q[0] | q[2] << 8), *(uint16_t *)(o + j0) = (uint16_t)(q[1] | q[3] << 8);
+      for (int i = 0; i < 4; ++i) q[i] = (uint32_t)(int)__builtin_amdgcn_fmed3f(rintf(y[i] * inv), -127.f, 127.f) & 0xFFu;   // a NaN too
+      if (apart) {
+        *(uint16_t *)(o + 2u * l) = (uint16_t)(q[0] | q[2] << 8), *(uint16_t *)(o + half + 2u * l) = (uint16_t)(q[1] | q[3] << 8);
       } else {
-        *(uint32_t *)(o + i0) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+        *(uint32_t *)(o + 4u * l) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
       }
       if (l == 0u) ((float *)(blk + ((uint64_t)D << kv.page_log2)))[slot] = m * (1.f / 127.f);
     }
@@ -168,16 +185,18 @@ hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positi
   return hipGetLastError();
 }
 
+template <int TYPE, int D, int U>
+static void append_launch(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
+  constexpr uint32_t rows = (D == 96 ? 8u : 1024u / D) * U;   // of a workgroup
+  const uint32_t q = (a.q_heads + rows - 1u) / rows, k = (kv.heads + rows - 1u) / rows;
+  hipLaunchKernelGGL((k_kv_append<TYPE, D, U>), dim3(b.tokens * (q + 2u * k)), dim3(256), 0, s, kv, b, a, q, k);
+}
+
 template <int TYPE, int D>
 static hipError_t append_dim(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
-  constexpr uint32_t rows = D == 96 ? 8u : 1024u / D;   // of a workgroup, U = 1
-  const uint32_t heads = a.q_heads + 2u * kv.heads;
-  // 4 rows a thread where that still gives a CU 8 workgroups
-  const uint32_t one = (heads + rows - 1u) / rows, four = (heads + 4u * rows - 1u) / (4u * rows);
-  if ((uint64_t)b.tokens * four >= 2048u)
-    hipLaunchKernelGGL((k_kv_append<TYPE, D, 4>), dim3(b.tokens * four), dim3(256), 0, s, kv, b, a, four);
-  else
-    hipLaunchKernelGGL((k_kv_append<TYPE, D, 1>), dim3(b.tokens * one), dim3(256), 0, s, kv, b, a, one);
+  // 4 rows a thread where a CU still has 8 workgroups to take
+  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= 2048ull * 4096u) append_launch<TYPE, D, 4>(kv, b, a, s);
+  else append_launch<TYPE, D, 1>(kv, b, a, s);
   return hipGetLastError();
 }
 
