@@ -275,6 +275,9 @@ napi_value Stats(napi_env env, napi_callback_info info) {
   napi_set_named_property(env, o, "gemmX", make_int(env, (int64_t)s.gemm_x));
   napi_set_named_property(env, o, "splitX", make_int(env, (int64_t)s.split_x));
   napi_set_named_property(env, o, "cpuPath", make_int(env, (int64_t)s.cpu_path));
+  napi_set_named_property(env, o, "kvAppend", make_int(env, (int64_t)s.kv_append));
+  napi_set_named_property(env, o, "kvAttn", make_int(env, (int64_t)s.kv_attn));
+  napi_set_named_property(env, o, "logits", make_int(env, (int64_t)s.logits));
   return o;
 }
 
@@ -680,6 +683,103 @@ napi_value QGemvTopK(napi_env env, napi_callback_info info) {
 
 napi_value TopKOutBytes(napi_env env, napi_callback_info) { return make_int(env, (int64_t)eff_topk_out_bytes()); }
 
+// ---- paged key/value cache, logits rules -----------------------------------
+
+napi_value prop(napi_env env, napi_value o, const char *name) {
+  napi_valuetype t;
+  napi_value v = undefined(env);
+  if (napi_typeof(env, o, &t) == napi_ok && t == napi_object) napi_get_named_property(env, o, name, &v);
+  return v;
+}
+
+// A buffer of a description: null where it has none.
+eff_buf *buf_prop(napi_env env, napi_value o, const char *name) {
+  napi_value v = prop(env, o, name);
+  napi_valuetype t;
+  return napi_typeof(env, v, &t) == napi_ok && t == napi_external ? external<eff_buf>(env, v) : nullptr;
+}
+
+uint32_t u32_prop(napi_env env, napi_value o, const char *name) { return (uint32_t)i64(env, prop(env, o, name)); }
+
+eff_kv_cache kv_cache(napi_env env, napi_value o) {
+  return {(int32_t)i64(env, prop(env, o, "type")), u32_prop(env, o, "heads"), u32_prop(env, o, "headDim"),
+          u32_prop(env, o, "pageTokens"), u32_prop(env, o, "pages"), buf_prop(env, o, "buf")};
+}
+
+eff_kv_batch kv_batch(napi_env env, napi_value o) {
+  return {buf_prop(env, o, "table"), buf_prop(env, o, "starts"), buf_prop(env, o, "lens"), u32_prop(env, o, "seqs"),
+          u32_prop(env, o, "tokens"), u32_prop(env, o, "tablePages"), u32_prop(env, o, "maxNew"),
+          u32_prop(env, o, "maxLen")};
+}
+
+// kvPageBytes(type, heads, headDim, pageTokens)
+napi_value KvPageBytes(napi_env env, napi_callback_info info) {
+  napi_value a[4];
+  get_args(env, info, 4, a);
+  return make_int(env, (int64_t)eff_kv_page_bytes((int)i64(env, a[0]), (uint32_t)i64(env, a[1]), (uint32_t)i64(env, a[2]),
+                                                  (uint32_t)i64(env, a[3])));
+}
+
+// ropeTable(ctx, freqs (Float64Array), positions, scale, out)
+napi_value RopeTable(napi_env env, napi_callback_info info) {
+  napi_value a[5];
+  get_args(env, info, 5, a);
+  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
+  void *f = nullptr;
+  size_t len = 0;
+  if (!bytes_of(env, a[1], &f, &len) || len % 8 || ((uintptr_t)f & 7))
+    return throw_msg(env, "ropeTable: the frequencies must be a Float64Array");
+  return status(env, ctx, eff_rope_table(ctx, (const double *)f, (uint32_t)(len / 8), (uint32_t)i64(env, a[2]),
+                                         (float)f64(env, a[3], 1.0), external<eff_buf>(env, a[4])));
+}
+
+// kvAppend(ctx, cache, batch, rows)
+napi_value KvAppend(napi_env env, napi_callback_info info) {
+  napi_value a[4];
+  get_args(env, info, 4, a);
+  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
+  const eff_kv_cache c = kv_cache(env, a[1]);
+  const eff_kv_batch b = kv_batch(env, a[2]);
+  eff_kv_rows r{};
+  r.q = buf_prop(env, a[3], "q"), r.k = buf_prop(env, a[3], "k"), r.v = buf_prop(env, a[3], "v");
+  r.q_offset = (uint64_t)i64(env, prop(env, a[3], "qOffset"));
+  r.k_offset = (uint64_t)i64(env, prop(env, a[3], "kOffset"));
+  r.v_offset = (uint64_t)i64(env, prop(env, a[3], "vOffset"));
+  r.q_stride = u32_prop(env, a[3], "qStride"), r.k_stride = u32_prop(env, a[3], "kStride");
+  r.v_stride = u32_prop(env, a[3], "vStride"), r.q_heads = u32_prop(env, a[3], "qHeads");
+  r.q_out = buf_prop(env, a[3], "qOut"), r.rope = buf_prop(env, a[3], "rope");
+  r.rope_positions = u32_prop(env, a[3], "ropePositions"), r.rope_dim = u32_prop(env, a[3], "ropeDim");
+  r.rope_mode = u32_prop(env, a[3], "ropeMode");
+  r.q_norm = buf_prop(env, a[3], "qNorm"), r.k_norm = buf_prop(env, a[3], "kNorm");
+  r.norm_eps = (float)f64(env, prop(env, a[3], "normEps"), 1e-6);
+  return status(env, ctx, eff_kv_append(ctx, &c, &b, &r));
+}
+
+// kvAttn(ctx, cache, batch, q, qOffset, qStride, out, qHeads, scale, window)
+napi_value KvAttn(napi_env env, napi_callback_info info) {
+  napi_value a[10];
+  get_args(env, info, 10, a);
+  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
+  const eff_kv_cache c = kv_cache(env, a[1]);
+  const eff_kv_batch b = kv_batch(env, a[2]);
+  return status(env, ctx, eff_kv_attn(ctx, &c, &b, external<eff_buf>(env, a[3]), (uint64_t)i64(env, a[4]),
+                                      (uint32_t)i64(env, a[5]), external<eff_buf>(env, a[6]), (uint32_t)i64(env, a[7]),
+                                      (float)f64(env, a[8]), (uint32_t)i64(env, a[9])));
+}
+
+// logitsApply(ctx, in, out, rows, vocab, stride, rules)
+napi_value LogitsApply(napi_env env, napi_callback_info info) {
+  napi_value a[7];
+  get_args(env, info, 7, a);
+  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
+  const eff_logits_rules r = {buf_prop(env, a[6], "history"), buf_prop(env, a[6], "historyStarts"),
+                              buf_prop(env, a[6], "penalties"), buf_prop(env, a[6], "biasIds"),
+                              buf_prop(env, a[6], "biasValues"), buf_prop(env, a[6], "biasStarts"),
+                              buf_prop(env, a[6], "mask"), buf_prop(env, a[6], "maskOf"), u32_prop(env, a[6], "maskCount")};
+  return status(env, ctx, eff_logits_apply(ctx, external<eff_buf>(env, a[1]), external<eff_buf>(env, a[2]),
+                                           (uint32_t)i64(env, a[3]), (uint32_t)i64(env, a[4]), (uint32_t)i64(env, a[5]), &r));
+}
+
 napi_value Register(napi_env env, napi_value exports) {
   struct { const char *name; napi_callback fn; } fns[] = {
       {"typeFromName", TypeFromName}, {"geometry", Geometry}, {"bufferMath", BufferMath},
@@ -693,7 +793,8 @@ napi_value Register(napi_env env, napi_value exports) {
       {"graphDestroy", GraphDestroy}, {"gemmXLayout", GemmXLayout}, {"gemmPrepareX", GemmPrepareX},
       {"qgemmPrepared", QGemmPrepared}, {"qmatmulXLayout", QMatmulXLayout},
       {"qmatmulPrepareX", QMatmulPrepareX}, {"qmatmulPrepared", QMatmulPrepared},
-      {"qmatmulCpuPath", QMatmulCpuPath},
+      {"qmatmulCpuPath", QMatmulCpuPath}, {"kvPageBytes", KvPageBytes}, {"ropeTable", RopeTable},
+      {"kvAppend", KvAppend}, {"kvAttn", KvAttn}, {"logitsApply", LogitsApply},
   };
   for (auto &f : fns) {
     napi_value v;

@@ -890,8 +890,101 @@ function createTopKGPU(device, ctx) {
   };
 }
 
+// ---- paged key/value cache and logits rules ---------------------------------
+//
+// The reference keeps one fp16 cache per layer and applies the penalties on the
+// host (README.md:101, sample.js:78-153). Here the cache is pages shared by
+// requests, and the rules on the logits of a batch run on the device; the
+// descriptions are those of include/elffuss_amd.h (eff_kv_cache, eff_kv_batch,
+// eff_kv_rows, eff_logits_rules). No counterpart in the reference's operators.
+const KV_TIPOS = { F16: 1, I8: 24 };
+const ROPE = { PARES: 0, MITADES: 1 };
+const SIN_PAGINA = 0xFFFFFFFF;
+
+const manejador = (buf) => (buf ? buf._h : undefined);
+
+// A cache as the addon takes it.
+function descCache(c) {
+  const type = KV_TIPOS[c.tipo];
+  if (type === undefined) {
+    const e = new Error(`tipo de caché no soportado: «${c.tipo}»`);
+    e.code = STATUS.E_TYPE;
+    throw e;
+  }
+  return { type, heads: c.cabezas, headDim: c.dim, pageTokens: c.tokensPagina, pages: c.paginas, buf: manejador(c.buf) };
+}
+
+// A batch: { tabla, inicios, largos (u32 buffers), secuencias, tokens, paginasTabla, maxNuevos, maxLargo }.
+function descLote(l) {
+  return { table: manejador(l.tabla), starts: manejador(l.inicios), lens: manejador(l.largos), seqs: l.secuencias,
+    tokens: l.tokens, tablePages: l.paginasTabla, maxNew: l.maxNuevos, maxLen: l.maxLargo };
+}
+
+function createKvOps(device, deps) {
+  const ctx = deps.ctx;
+  return {
+    // Pages of one layer, zeroed: { tipo: 'F16' | 'I8', cabezas, dim, tokensPagina, paginas }.
+    creaCache(o) {
+      const d = descCache(o);
+      const bytes = native.kvPageBytes(d.type, d.heads, d.headDim, d.pageTokens);
+      if (!bytes) {
+        const e = new Error(`caché: no hay páginas de ${o.tokensPagina} tokens, ${o.cabezas} cabezas de ${o.dim}`);
+        e.code = STATUS.E_SHAPE;
+        throw e;
+      }
+      return Object.assign({}, o, { buf: device.createBuffer({ size: bytes * o.paginas, label: 'kv' }) });
+    },
+    // cos and sin of position * freqs[i], once per model.
+    tablaRope(freqs, posiciones, escala) {
+      const out = device.createBuffer({ size: posiciones * freqs.length * 8, label: 'rope' });
+      native.ropeTable(device._ctx, freqs, posiciones, escala === undefined ? 1 : escala, out._h);
+      return out;
+    },
+    // New k, v rows into the cache; q rotated into a pooled buffer, which it resolves to (null without q).
+    // filas: { q, k, v, desdeQ, desdeK, desdeV, pasoQ, pasoK, pasoV, cabezasQ, rope, posicionesRope, dimRope,
+    // modoRope, normaQ, normaK, eps }.
+    anade(cache, lote, filas) {
+      const f = filas;
+      const q = f.q ? ctx.alloc(lote.tokens * f.cabezasQ * cache.dim * 4, 'kv.q') : null;
+      native.kvAppend(device._ctx, descCache(cache), descLote(lote), { q: manejador(f.q), k: manejador(f.k), v: manejador(f.v),
+        qOffset: f.desdeQ, kOffset: f.desdeK, vOffset: f.desdeV, qStride: f.pasoQ, kStride: f.pasoK, vStride: f.pasoV,
+        qHeads: f.q ? f.cabezasQ : 0, qOut: manejador(q), rope: manejador(f.rope), ropePositions: f.posicionesRope,
+        ropeDim: f.dimRope, ropeMode: f.modoRope, qNorm: manejador(f.normaQ), kNorm: manejador(f.normaK), normEps: f.eps });
+      return Promise.resolve(q);
+    },
+    // Attention of the new tokens over the cache, into a pooled buffer. opts: { ventana, desdeQ, pasoQ }.
+    atiende(cache, lote, q, cabezasQ, escala, opts) {
+      const o = opts || {};
+      const out = ctx.alloc(lote.tokens * cabezasQ * cache.dim * 4, 'kv.atencion');
+      native.kvAttn(device._ctx, descCache(cache), descLote(lote), q._h, o.desdeQ || 0, o.pasoQ || 0, out._h, cabezasQ, escala,
+        o.ventana || 0);
+      return Promise.resolve(out);
+    },
+  };
+}
+
+// Penalties, biases and masks on logits [filas][vocab], into a pooled buffer or `opts.salida` (which may be the
+// logits). reglas: { historia, iniciosHistoria, castigos (f64 [filas][3]), idsSesgo, valoresSesgo, iniciosSesgo,
+// mascara, mascaraDe, mascaras }; opts: { paso, salida }.
+function createLogitsOps(device, deps) {
+  const ctx = deps.ctx;
+  return {
+    aplica(logits, filas, vocab, reglas, opts) {
+      const o = opts || {};
+      const r = reglas;
+      const paso = o.paso || vocab;
+      const out = o.salida || ctx.alloc(Math.max(1, filas) * paso * 4, 'logits');
+      native.logitsApply(device._ctx, logits._h, out._h, filas, vocab, paso, { history: manejador(r.historia),
+        historyStarts: manejador(r.iniciosHistoria), penalties: manejador(r.castigos), biasIds: manejador(r.idsSesgo),
+        biasValues: manejador(r.valoresSesgo), biasStarts: manejador(r.iniciosSesgo), mask: manejador(r.mascara),
+        maskOf: manejador(r.mascaraDe), maskCount: r.mascaras });
+      return Promise.resolve(out);
+    },
+  };
+}
+
 module.exports = {
-  native, STATUS, OPT, GEMV_MODE, TOPK, QUANT_TYPES, quantInfo,
+  native, STATUS, OPT, GEMV_MODE, TOPK, QUANT_TYPES, quantInfo, createKvOps, createLogitsOps, KV_TIPOS, ROPE, SIN_PAGINA,
   requestDevice, readback, createContext,
   createQuantOps, createGemvOps, GEMV2_TIPOS, GEMV2_MAX_TOKENS, createGemm2Ops, GEMM2_TIPOS, createFusionOps, createTopKGPU, estadisticasTopK, TIPOS_GATHER_NORMA,
   TIPOS_R, TIPO_R, TIPO_GGUF, bytesReordenado, bytesBufferR, bloquesDeBuffer, escalasDesde,
