@@ -1551,7 +1551,8 @@ size_t eff_kv_page_bytes(int type, uint32_t heads, uint32_t dim, uint32_t page) 
   if (!kv_type_known(type) || !kv_dim_known(dim) || heads == 0 || heads > 4096u || page < kKvPageMin ||
       page > kKvPageMax || (page & (page - 1u)))
     return 0;
-  return 2ull * heads * kv_block_bytes(type, dim, page);
+  const uint64_t bytes = 2ull * heads * kv_block_bytes(type, dim, page);
+  return bytes < 1ull << 31 ? bytes : 0;   // a page is read through one buffer resource
 }
 
 int eff_rope_table(eff_ctx *ctx, const double *freqs, uint32_t n, uint32_t positions, float scale, eff_buf *out) {

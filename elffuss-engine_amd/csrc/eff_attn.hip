@@ -168,94 +168,89 @@ __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, 
   return true;
 }
 
-// One wave's share of a tile of 16 MT rows. QL: the parts of q are in LDS, shared
-// by the waves of the tile, and read for each step.
-template <int TYPE, int D, int MT, bool QL>
+// One wave's share of a tile of 16 rows.
+//   SCALED  rows of the cache have scales
+//   I8      K and V arrive as int8 (else fp16, also where int8 was converted on the way)
+//   QL      the parts of q are in LDS, shared by the waves of the tile, and read for
+//           each step
+//   TR      V arrives as the operand it is (turned by the LDS read)
+template <int D, bool SCALED, bool I8, bool QL, bool TR>
 struct AttnWave {
-  static constexpr bool I8 = TYPE == EFF_KV_I8;
   static constexpr int E = D / 16;                     // columns of a lane
   static constexpr int KS = D / 32;                    // matrix steps of a score
   static constexpr int KW = I8 ? 2 : 4;                // words of a lane's part of a step of K
   static constexpr int VW = I8 ? (E + 3) / 4 : E / 2;  // words of a lane's part of a row of V
-  static constexpr int ROW = I8 ? D : 2 * D;           // bytes of a cached row
+  static constexpr int ROW = I8 ? D : 2 * D;           // bytes of a row as it arrives
 
-  half8 qh[QL ? 1 : MT][QL ? 1 : KS], ql[QL ? 1 : MT][QL ? 1 : KS];
-  const uint8_t *qs;       // QL: [mt][step][part][lane] of 16 bytes
-  float sc[MT];            // > 0: what a raw score of row n is multiplied by (log2 e included)
-  int pos[MT];             // the row's position, -1 for none
-  float m[MT], l[MT];      // running maximum (of raw scores), and this lane's share of the sum
-  float vref[MT], vinv[MT];   // I8: the largest value scale so far, and its reciprocal
-  float4v acc[MT][E];
+  half8 qh[QL ? 1 : KS], ql[QL ? 1 : KS];
+  const uint8_t *qs;    // QL: [step][part][lane] of 16 bytes
+  float sc;             // > 0: what a raw score of row n is multiplied by (log2 e included)
+  int pos;              // the row's position, -1 for none
+  float m, l;           // running maximum (of raw scores), and this lane's share of the sum
+  float vref, vinv;     // SCALED: the largest value scale so far, and its reciprocal
+  float4v acc[E];
 
   uint32_t kw[2][KS * KW];
-  uint32_t ks[2][4];     // I8: the scales of the lane's tokens (f32 bits)
-  uint32_t vw[8][VW];
+  uint32_t ks[2][4];                          // SCALED: the scales of the lane's tokens (f32 bits)
+  uint32_t vw[TR ? E : 8][TR ? 4 : VW];       // V: 8 rows, or the operands of E columns
   uint32_t vs[2][4];
 
-  // column of acc[.][i][j] of lane group g: lanes hold 4 columns of the first
-  // 64, and at D = 96 2 of the last 32; else E side by side
+  // column of acc[i][j] of lane group g: TR, and at D = 96, side by side with the
+  // group's 4 rows; else E side by side
   static __device__ __forceinline__ uint32_t column(uint32_t g, int i, int j) {
+    if constexpr (TR) return 16u * i + 4u * g + j;
     if constexpr (D == 96) return i < 4 ? 4u * (4u * g + j) + i : 64u + 2u * (4u * g + j) + (i - 4);
     return (uint32_t)E * (4u * g + j) + i;
   }
 
-  // The rows' q as it is in memory; invalid rows read the tile's first.
-  __device__ __forceinline__ void load_q(float q[MT][KS][8], const KvAttnArgs &a, const AttnTile &t, uint32_t group, uint32_t kvh,
-                                         uint32_t row0, uint32_t n, uint32_t g) {
+  // The rows' q as it is in memory; rows that are none read the tile's first.
+  __device__ __forceinline__ void load_q(float q[KS][8], const KvAttnArgs &a, const AttnTile &t, uint32_t group, uint32_t kvh,
+                                         uint32_t n, uint32_t g) {
+    const bool on = n < t.rows;
+    const uint32_t r = t.r0 + (on ? n : 0u), tok = r / group, h = r % group;
+    const float *src = a.q + (uint64_t)(t.token0 + tok) * a.q_stride + (kvh * group + h) * D;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const uint32_t r = row0 + 16u * mt + n;
-      const bool on = r < t.rows;
-      const uint32_t tok = (t.r0 + (on ? r : 0u)) / group, h = (t.r0 + (on ? r : 0u)) % group;
-      const float *src = a.q + (uint64_t)(t.token0 + tok) * a.q_stride + (kvh * group + h) * D;
-#pragma unroll
-      for (int c = 0; c < KS; ++c) {
-        uint32_t d;
-        if constexpr (I8) d = 2 * (c / 2) + 1 < KS ? 64u * (c / 2) + 16u * g + 8u * (c & 1) : 32u * c + 8u * g;
-        else d = 32u * c + 8u * g;
-        const float4 u = *(const float4 *)(src + d), w = *(const float4 *)(src + d + 4);
-        const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[mt][c][i] = x[i];
-      }
-      pos[mt] = on ? t.first + (int)(tok - t.r0 / group) : -1;
+    for (int c = 0; c < KS; ++c) {
+      uint32_t d;
+      if constexpr (I8) d = 2 * (c / 2) + 1 < KS ? 64u * (c / 2) + 16u * g + 8u * (c & 1) : 32u * c + 8u * g;
+      else d = 32u * c + 8u * g;
+      const float4 u = *(const float4 *)(src + d), w = *(const float4 *)(src + d + 4);
+      q[c][0] = u.x, q[c][1] = u.y, q[c][2] = u.z, q[c][3] = u.w;
+      q[c][4] = w.x, q[c][5] = w.y, q[c][6] = w.z, q[c][7] = w.w;
     }
+    pos = on ? t.first + (int)(tok - t.r0 / group) : -1;
   }
 
   // q in its two fp16 parts, and empty sums. Rows that are none see nothing
   // (pos -1), so what q they have does not matter.
-  __device__ __forceinline__ void init(const float q[MT][KS][8], float scale, uint8_t *lds, uint32_t wave, uint32_t waves) {
+  __device__ __forceinline__ void init(const float q[KS][8], float scale, uint8_t *lds, uint32_t wave, uint32_t waves) {
     qs = lds + 16u * (threadIdx.x & 63u);
+    float top = 0.f;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float top = 0.f;
+    for (int c = 0; c < KS; ++c)
 #pragma unroll
-      for (int c = 0; c < KS; ++c)
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[c][i]));
+    top = row_max(top);
+    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
+    // the scale's sign goes to q; a scale of zero makes every score zero
+    const float up = scale == 0.f ? 0.f : copysignf(ldexpf(1.f, 13 - e), scale);
+    sc = fmaxf(fabsf(scale) * 1.44269504088896341f * ldexpf(1.f, e - 13), 1e-37f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[mt][c][i]));
-      top = row_max(top);
-      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
-      // the scale's sign goes to q; a scale of zero makes every score zero
-      const float up = scale == 0.f ? 0.f : copysignf(ldexpf(1.f, 13 - e), scale);
-      sc[mt] = fmaxf(fabsf(scale) * 1.44269504088896341f * ldexpf(1.f, e - 13), 1e-37f);
+    for (int c = 0; c < KS; ++c) {
+      half2v hi[4], lo[4];
 #pragma unroll
-      for (int c = 0; c < KS; ++c)
-      {
-        half2v hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split2(q[mt][c][2 * i] * up, q[mt][c][2 * i + 1] * up, hi[i], lo[i]);
-        const half8 h = join8(hi), r = join8(lo);
-        if constexpr (!QL) {
-          qh[mt][c] = h, ql[mt][c] = r;
-        } else if ((mt * KS + c) % waves == wave) {
-          *(half8 *)(const_cast<uint8_t *>(qs) + (mt * KS + c) * 2048) = h;
-          *(half8 *)(const_cast<uint8_t *>(qs) + (mt * KS + c) * 2048 + 1024) = r;
-        }
+      for (int i = 0; i < 4; ++i) split2(q[c][2 * i] * up, q[c][2 * i + 1] * up, hi[i], lo[i]);
+      const half8 h = join8(hi), r = join8(lo);
+      if constexpr (!QL) {
+        qh[c] = h, ql[c] = r;
+      } else if (c % waves == wave) {
+        *(half8 *)(const_cast<uint8_t *>(qs) + c * 2048) = h;
+        *(half8 *)(const_cast<uint8_t *>(qs) + c * 2048 + 1024) = r;
       }
-      m[mt] = -INFINITY, l[mt] = 0.f, vref[mt] = 0.f, vinv[mt] = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) acc[mt][i] = float4v{0.f, 0.f, 0.f, 0.f};
     }
+    m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
   }
 
   // K of the 16 tokens from `blk`'s slot `slot` on, into half u of the step.
@@ -272,12 +267,9 @@ struct AttnWave {
     }
   }
 
+  // V of the same tokens: the lane's columns of the rows 4 g .. 4 g + 3.
   __device__ __forceinline__ void load_v(int u, const uint8_t *blk, uint32_t slot, uint32_t page_log2, uint32_t n, uint32_t g) {
-    load_rows(u, blk + slot * ROW, blk + ((uint32_t)D << page_log2) + slot * 4u, n, g);
-  }
-
-  // The lane's parts of the rows 4 g .. 4 g + 3 of half u, in memory or in LDS.
-  __device__ __forceinline__ void load_rows(int u, const uint8_t *p, const uint8_t *scales, uint32_t n, uint32_t g) {
+    const uint8_t *p = blk + slot * ROW;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint8_t *r = p + 4u * g * ROW + j * ROW;
@@ -295,7 +287,7 @@ struct AttnWave {
         ld_words<VW>(o, r + 4u * VW * n);
       }
     }
-    if constexpr (I8) ld_words<4>(vs[u], scales + 16u * g);
+    if constexpr (I8) ld_words<4>(vs[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
   }
 
   // Column i of the 8 tokens of the lane as the first operand.
@@ -303,7 +295,9 @@ struct AttnWave {
     u32x4 o;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      if constexpr (I8) {
+      if constexpr (TR) {
+        o[x] = vw[i][x];
+      } else if constexpr (I8) {
         const uint32_t w = i / 4, k = i % 4;
         const uint32_t sel = 0x0C000C00u | k | ((4u + k) << 16);
         o[x] = i8_half2(__builtin_amdgcn_perm(vw[2 * x + 1][w] ^ 0x80808080u, vw[2 * x][w] ^ 0x80808080u, sel) | 0x64006400u);
@@ -314,138 +308,138 @@ struct AttnWave {
     return o;
   }
 
-  // The step at token t0: scores, weights and the weighted sum. `masked`: some
-  // row does not see every one of its 32 tokens (wave-uniform); a half without
-  // a page is `gone`.
-  __device__ __forceinline__ void scores(float s[MT][2][4]) const {
+  // Takes the tokens whose bit is set out of V.
+  __device__ __forceinline__ void clear_v(uint32_t gone) {
+    if constexpr (TR) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float4v c[MT];
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t keep = (gone >> (2 * x) & 1u ? 0u : 0xFFFFu) | (gone >> (2 * x + 1) & 1u ? 0u : 0xFFFF0000u);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) c[mt] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        half8 a;
-        if constexpr (I8) a = i8_half8(kw[u][2 * k], kw[u][2 * k + 1]);
-        else a = __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          if constexpr (QL) {
-            c[mt] = mfma(a, *(const half8 *)(qs + (mt * KS + k) * 2048), c[mt]);
-            c[mt] = mfma(a, *(const half8 *)(qs + (mt * KS + k) * 2048 + 1024), c[mt]);
-          } else {
-            c[mt] = mfma(a, qh[mt][k], c[mt]);
-            c[mt] = mfma(a, ql[mt][k], c[mt]);
-          }
-        }
+        for (int i = 0; i < E; ++i) vw[i][x] &= keep;
       }
+    } else {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[mt][u][j] = I8 ? c[mt][j] * __uint_as_float(ks[u][j]) : c[mt][j];
+        for (int w = 0; w < VW; ++w) vw[k][w] = gone >> k & 1u ? 0u : vw[k][w];
+    }
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) vs[k / 4][k % 4] = gone >> k & 1u ? 0u : vs[k / 4][k % 4];
     }
   }
 
-  // Whether the row of tile mt sees token t0 + 16 u + 4 g + j.
+  // The step's raw scores: s[u][j] of token 16 u + 4 g + j. The two halves in turn,
+  // so that a matrix step does not wait for the one before it.
+  __device__ __forceinline__ void scores(float s[2][4]) const {
+    float4v c[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      half8 a[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (I8) a[u] = i8_half8(kw[u][2 * k], kw[u][2 * k + 1]);
+        else a[u] = __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
+      }
+      half8 h, r;
+      if constexpr (QL) h = *(const half8 *)(qs + k * 2048), r = *(const half8 *)(qs + k * 2048 + 1024);
+      else h = qh[k], r = ql[k];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) c[u] = mfma(a[u], h, c[u]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) c[u] = mfma(a[u], r, c[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[u][j] = SCALED ? c[u][j] * __uint_as_float(ks[u][j]) : c[u][j];
+  }
+
   static __device__ __forceinline__ bool sees(int pos, int window, int t) { return t <= pos && (window == 0 || t > pos - window); }
 
-  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[MT][2][4]) {
+  // The weights of the step at token t0, and the weighted sum. `masked`: some row
+  // does not see every one of its 32 tokens (wave-uniform); a half without a page is
+  // `gone`.
+  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[2][4]) {
     if (masked) {
+      uint32_t none = 0;   // tokens that no row sees: may be any bits
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = t0 + 16 * (k / 4) + 4 * (int)g + k % 4;
+        if (gone[k / 4] || !sees(pos, window, at)) s[k / 4][k % 4] = -INFINITY;
+        if (gone[k / 4] || at < t.begin || at >= t.end) none |= 1u << k;
+      }
+      clear_v(none);
+    }
+    float mx = max2(max2(max2(s[0][0], s[0][1]), max2(s[0][2], s[0][3])), max2(max2(s[1][0], s[1][1]), max2(s[1][2], s[1][3])));
+    mx = row_max(mx);
+    float vx = 0.f;
+    if constexpr (SCALED) {
+      // of the tokens that the row sees only: another row's may not be finite
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = t0 + 16 * u + 4 * (int)g + j;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            if (gone[u] || !sees(pos[mt], window, at)) s[mt][u][j] = -INFINITY;
-          // what no row sees may be any bits
-          if (gone[u] || at < t.begin || at >= t.end) {
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vw[4 * u + j][w] = 0u;
-            if constexpr (I8) vs[u][j] = 0u;
-          }
-        }
+        for (int j = 0; j < 4; ++j) vx = fmaxf(vx, !masked || s[u][j] != -INFINITY ? __uint_as_float(vs[u][j]) : 0.f);
+      vx = row_max(vx);
     }
-    half8 ph[MT], pl[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float mx = max2(max2(max2(s[mt][0][0], s[mt][0][1]), max2(s[mt][0][2], s[mt][0][3])),
-                      max2(max2(s[mt][1][0], s[mt][1][1]), max2(s[mt][1][2], s[mt][1][3])));
-      mx = row_max(mx);
-      float vx = 0.f;
-      if constexpr (I8) {
-        // of the tokens that the row sees only: another row's may not be finite
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vx = fmaxf(vx, !masked || s[mt][u][j] != -INFINITY ? __uint_as_float(vs[u][j]) : 0.f);
-        vx = row_max(vx);
-      }
-      if (__any(mx > m[mt] || (I8 && vx > vref[mt]))) {
-        const float mn = fmaxf(m[mt], mx);
-        const float al = m[mt] == mn ? 1.f : __builtin_amdgcn_exp2f((m[mt] - mn) * sc[mt]);
-        m[mt] = mn;
-        l[mt] *= al;
-        float f = al;
-        if constexpr (I8) {
-          if (vx > vref[mt]) {
-            const float vn = fmaxf(vx, 1e-30f);
-            f = al * (vref[mt] / vn);
-            vref[mt] = vn;
-            vinv[mt] = 1.f / vn;
-          }
+    if (__any(mx > m || (SCALED && vx > vref))) {
+      const float mn = fmaxf(m, mx);
+      float f = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * sc);
+      m = mn;
+      l *= f;
+      if constexpr (SCALED) {
+        if (vx > vref) {
+          const float vn = fmaxf(vx, 1e-30f);
+          f *= vref / vn;
+          vref = vn;
+          vinv = 1.f / vn;
         }
-#pragma unroll
-        for (int i = 0; i < E; ++i) acc[mt][i] *= f;
       }
-      const float up = m[mt] == -INFINITY ? 0.f : 14.f - m[mt] * sc[mt];
-      float sum = 0.f;
-      half2v hi[4], lo[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          float p[2];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float x = s[mt][u][j + k];
-            p[k] = __builtin_amdgcn_exp2f(fmaf(x, sc[mt], up));
-            sum += p[k];
-            // a weight of nothing takes nothing of a scale that is not finite
-            if constexpr (I8) p[k] = masked && x == -INFINITY ? 0.f : p[k] * (__uint_as_float(vs[u][j + k]) * vinv[mt]);
-          }
-          split2(p[0], p[1], hi[2 * u + j / 2], lo[2 * u + j / 2]);
-        }
-      ph[mt] = join8(hi), pl[mt] = join8(lo);
-      l[mt] += sum;
+      for (int i = 0; i < E; ++i) acc[i] *= f;
     }
-    if constexpr (!I8) {
+    const float up = m == -INFINITY ? 0.f : 14.f - m * sc;
+    float sum = 0.f;
+    half2v hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      float p[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float y = s[k / 4][k % 4 + x];
+        p[x] = __builtin_amdgcn_exp2f(fmaf(y, sc, up));
+        sum += p[x];
+        // a weight of nothing takes nothing of a scale that is not finite
+        if constexpr (SCALED) p[x] = masked && y == -INFINITY ? 0.f : p[x] * (__uint_as_float(vs[k / 4][k % 4 + x]) * vinv);
+      }
+      split2(p[0], p[1], hi[k / 2], lo[k / 2]);
+    }
+    l += sum;
+    if constexpr (!SCALED) {
       // A value that only some rows see and that is not finite: 0 * inf would
       // reach the others.
       if (masked && t.first != t.last) {
         uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < (TR ? E : 8); ++k)
 #pragma unroll
-          for (int w = 0; w < VW; ++w) {
+          for (int w = 0; w < (TR ? 4 : VW); ++w) {
             const uint32_t x = vw[k][w] & 0x7FFF7FFFu;
             top = max(top, max(x & 0xFFFFu, x >> 16));
           }
         if (__any(top >= 0x7C00u)) poison(t0, gone, window, g);
       }
     }
+    const half8 ph = join8(hi), pl = join8(lo);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const half8 a = __builtin_bit_cast(half8, v_operand(i));
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) acc[mt][i] = mfma(a, ph[mt], acc[mt][i]);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) acc[mt][i] = mfma(a, pl[mt], acc[mt][i]);
+      const half8 v = __builtin_bit_cast(half8, v_operand(i));
+      acc[i] = mfma(v, ph, acc[i]);
+      acc[i] = mfma(v, pl, acc[i]);
     }
   }
 
-  // fp16 1 where a half is not finite, else 0; and the halves that are.
+  // fp16 1 where a half is not finite, else 0.
   static __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     return ((w & 0x7C00u) == 0x7C00u ? 0x3C00u : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0x3C000000u : 0u);
   }
@@ -454,24 +448,21 @@ struct AttnWave {
   // product of the two indicators says which), and such values are taken out of
   // the step.
   __device__ __forceinline__ void poison(int t0, const bool gone[2], int window, uint32_t g) {
+    half8 seen;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      half8 seen;
+    for (int k = 0; k < 8; ++k) seen[k] = (_Float16)(!gone[k / 4] && sees(pos, window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4) ? 1.f : 0.f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) seen[k] = (_Float16)(!gone[k / 4] && sees(pos[mt], window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4) ? 1.f : 0.f);
+    for (int i = 0; i < E; ++i) {
+      const u32x4 v = v_operand(i);
+      const u32x4 bad = {not_finite(v[0]), not_finite(v[1]), not_finite(v[2]), not_finite(v[3])};
+      const float4v c = mfma(__builtin_bit_cast(half8, bad), seen, float4v{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const u32x4 v = v_operand(i);
-        const u32x4 bad = {not_finite(v[0]), not_finite(v[1]), not_finite(v[2]), not_finite(v[3])};
-        const float4v c = mfma(__builtin_bit_cast(half8, bad), seen, float4v{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[mt][i][j] = c[j] > 0.f ? NAN : acc[mt][i][j];
-      }
+      for (int j = 0; j < 4; ++j) acc[i][j] = c[j] > 0.f ? NAN : acc[i][j];
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < (TR ? E : 8); ++k)
 #pragma unroll
-      for (int w = 0; w < VW; ++w) vw[k][w] &= ~(not_finite(vw[k][w]) / 0x3C00u * 0xFFFFu);
+      for (int w = 0; w < (TR ? 4 : VW); ++w) vw[k][w] &= ~(not_finite(vw[k][w]) / 0x3C00u * 0xFFFFu);
   }
 
   // The walk over a tile's cached tokens: the steps lo, lo + stride, ... up to hi.
@@ -509,7 +500,7 @@ struct AttnWave {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         load_v(u, k.blk[u] + to_v, (uint32_t)(t0 + 16 * u) & ((1u << kv.page_log2) - 1u), kv.page_log2, n, g);
-      float s[MT][2][4];
+      float s[2][4];
       scores(s);
       const bool gone[2] = {k.gone[0], k.gone[1]};
       const bool masked = gone[0] || gone[1] || t0 + 31 > t.first || t0 < t.begin || (window && t0 <= t.last - window);
@@ -546,11 +537,12 @@ constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 // joins them, in chunk order; stores and loads of the chunks' sums go past the
 // XCD's L2 (sc1), every wave waits for its stores before the barrier ahead of the
 // counter's increment, and the counter is left at zero for the next launch.
-template <int TYPE, int D, int MT, int NW, bool QL>
+template <int TYPE, int D, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
-  using W = AttnWave<TYPE, D, MT, QL>;
-  constexpr uint32_t R = 16u * MT, LD = D + 4u, T = 64u * NW;
-  static_assert(!QL || MT * W::KS * 2048u <= NW * R * LD * 4u, "q's parts share the sums' space");
+  constexpr bool I8 = TYPE == EFF_KV_I8, QL = D == 256;   // 256 wide, q's parts would take a quarter of the registers
+  using W = AttnWave<D, I8, I8, QL, false>;
+  constexpr uint32_t R = 16u, LD = D + 4u, T = 64u * NW;
+  static_assert(!QL || W::KS * 2048u <= NW * R * LD * 4u, "q's parts share the sums' space");
   __shared__ float so[NW][R][LD];
   __shared__ float sm[NW][R], sl[NW][R], sv[NW][R];
   __shared__ uint32_t arrived;
@@ -569,23 +561,20 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
     k.table = b.table + (uint64_t)t.seq * b.table_pages;
     k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 32 * NW;
     W::read_ids(k, kv, k.lo);
-    float q[MT][W::KS][8];
-    w.load_q(q, a, t, group, kvh, 0, n, g);
+    float q[W::KS][8];
+    w.load_q(q, a, t, group, kvh, n, g);
     w.fetch_k(k, kv, kvh, 0, k.lo, n, g);   // of the first page, where the wave has no step
     w.init(q, a.scale, (uint8_t *)so, wave, NW);
     if constexpr (QL) __syncthreads();
     w.run(k, kv, t, kvh, window, n, g);
     if constexpr (QL) __syncthreads();   // the sums take q's place
   }
+  const float wl = row_add(w.l);
+  if (g == 0u) sm[wave][n] = w.m * w.sc, sl[wave][n] = wl, sv[wave][n] = w.vref;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const float l = row_add(w.l[mt]);
-    if (g == 0u) sm[wave][16 * mt + n] = w.m[mt] * w.sc[mt], sl[wave][16 * mt + n] = l, sv[wave][16 * mt + n] = w.vref[mt];
+  for (int i = 0; i < W::E; ++i)
 #pragma unroll
-    for (int i = 0; i < W::E; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) so[wave][16 * mt + n][W::column(g, i, j)] = w.acc[mt][i][j];
-  }
+    for (int j = 0; j < 4; ++j) so[wave][n][W::column(g, i, j)] = w.acc[i][j];
   __syncthreads();
   const uint64_t at = ((uint64_t)tile * kv.heads + kvh) * attn_part_floats(p, D);
   const rsrc_t prs = make_rsrc(part + at, attn_part_floats(p, D) * 4u);
@@ -601,7 +590,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
       const float f = sm[v][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[v][r] - mx);
       l += f * sl[v][r];
       const float4v x = *(const float4v *)&so[v][r][d];
-      o += x * (W::I8 ? f * sv[v][r] : f);
+      o += x * (I8 ? f * sv[v][r] : f);
     }
     if (chunks == 1u) {
       const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
@@ -681,49 +670,56 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   }
 }
 
-// Many rows: NW waves of 16 MT rows each walk the same cached tokens, 32 a step,
-// which come through LDS: two buffers, one filled while the other is read (a wave
-// that has waited for its loads and passed the barrier knows that the step's
-// tokens are there, and that every wave is done with the buffer it fills next).
-// K's 16-byte pieces are turned within their row, so that the 16 rows of an operand
-// lie in different banks.
-template <int TYPE, int D>
+// Many rows: four waves of 16 rows each walk the same cached tokens, 32 a step,
+// which come through LDS as fp16: two buffers, one filled while the other is read. A
+// wave that has waited for its loads (or LDS writes) and passed the barrier knows that
+// the step's tokens are there, and that every wave is done with the buffer it fills
+// next. fp16 pages go straight to LDS; int8 ones are requested before the step and
+// converted after it, once for the four waves.
+// K's 16-byte pieces are turned within their row, and V's 32-byte ones, so that the
+// 16 rows of an operand lie in different banks; V's operand comes out of LDS turned
+// (ds_read_b64_tr_b16: of 16 lanes, lane 4 j + q reads 4 values of row j, and lane c
+// gets column c of the 4 rows).
+template <int D>
 struct AttnStage {
-  static constexpr uint32_t ROW = TYPE == EFF_KV_I8 ? D : 2 * D, PIECES = ROW / 16u;
-  static constexpr uint32_t FILLS = (ROW + 63u) / 64u;        // loads of 64 x 16 bytes for 16 rows
-  static constexpr uint32_t HALF = 1024u * FILLS;             // and the LDS they take
-  static constexpr uint32_t V = 2u * HALF, SCALES = 2u * V, BYTES = 2u * V + (TYPE == EFF_KV_I8 ? 256u : 0u);
+  static constexpr uint32_t ROW = 2 * D, PIECES = ROW / 16u;
+  static constexpr uint32_t FILLS = ROW / 64u;                // loads of 64 x 16 bytes for 16 rows
+  static constexpr uint32_t HALF = 16u * ROW;
+  static constexpr uint32_t V = 2u * HALF, SCALES = 2u * V, BYTES = 2u * V + 256u;
 
-  // where piece c of row r lies in the row, and back
+  // where piece c of K's row r lies in the row, and what lies there
   static __device__ __forceinline__ uint32_t place(uint32_t r, uint32_t c) {
-    if constexpr (PIECES % 8u == 0u) return c ^ (r & 7u);
-    else if constexpr (PIECES == 4u) return c ^ (r >> 1 & 3u);
-    else if constexpr (PIECES == 12u) return (c + (r >> 1 & 3u)) % 12u;
-    else return (c + (r >> 2 & 1u)) % PIECES;
+    return PIECES % 8u == 0u ? c ^ (r & 7u) : (c + (r >> 1 & 3u)) % PIECES;
   }
   static __device__ __forceinline__ uint32_t piece(uint32_t r, uint32_t at) {
-    if constexpr (PIECES % 8u == 0u) return at ^ (r & 7u);
-    else if constexpr (PIECES == 4u) return at ^ (r >> 1 & 3u);
-    else if constexpr (PIECES == 12u) return (at + 12u - (r >> 1 & 3u)) % 12u;
-    else return (at + PIECES - (r >> 2 & 1u)) % PIECES;
+    return PIECES % 8u == 0u ? at ^ (r & 7u) : (at + PIECES - (r >> 1 & 3u)) % PIECES;
+  }
+  // the same of the 16 columns c of V's row r
+  static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) {
+    return PIECES >= 16u ? c ^ (r & 7u) : PIECES == 8u ? c ^ (r >> 1 & 3u) : (c + (r >> 2 & 3u)) % (PIECES / 2u);
+  }
+  static __device__ __forceinline__ uint32_t v_piece(uint32_t r, uint32_t at) {
+    const uint32_t c = at / 2u;
+    return (PIECES >= 16u ? c ^ (r & 7u) : PIECES == 8u ? c ^ (r >> 1 & 3u) : (c + PIECES / 2u - (r >> 2 & 3u)) % (PIECES / 2u)) * 2u + (at & 1u);
   }
 };
 
-// 4 bytes a lane from its own address into LDS at lds + 4 * lane.
-__device__ __forceinline__ void fill4(const uint8_t *p, const uint8_t *lds) {
-  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  __asm__ volatile("global_load_lds_dword %0, off" : : "v"(p), "{m0}"(m0) : "memory");
-}
-
-// Waits for the wave's loads and LDS reads, then for the other waves.
+// Waits for the wave's loads and LDS operations, then for the other waves.
 __device__ __forceinline__ void wait_step() { __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-template <int TYPE, int D, int MT, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles, uint32_t per_seq,
-                                                          uint32_t min_rows) {
-  using W = AttnWave<TYPE, D, MT, false>;
-  using S = AttnStage<TYPE, D>;
-  constexpr uint32_t R = 16u * NW * MT;
+typedef short short4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 ld_turned(const uint8_t *p) {
+  typedef __attribute__((address_space(3))) short4v *lds_ptr;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(__attribute__((address_space(3))) void *)p));
+}
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles,
+                                                                      uint32_t per_seq, uint32_t min_rows) {
+  constexpr bool I8 = TYPE == EFF_KV_I8;
+  using W = AttnWave<D, I8, false, false, true>;
+  using S = AttnStage<D>;
+  constexpr uint32_t NW = 4u, R = 16u * NW;
   __shared__ __align__(1024) uint8_t buf[2][S::BYTES];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
@@ -734,8 +730,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_rows(KvView kv, KvBatchView
   const int window = (int)min(a.window, 0x40000000u), base = t.begin & ~31;
   // the wave's own rows
   AttnTile m = t;
-  const uint32_t row0 = 16u * MT * wave;
-  m.rows = t.rows > row0 ? min(t.rows - row0, 16u * MT) : 0u;
+  const uint32_t row0 = 16u * wave;
+  m.rows = t.rows > row0 ? min(t.rows - row0, 16u) : 0u;
   if (m.rows) {
     m.r0 = t.r0 + row0;
     m.first = t.first + (int)(m.r0 / group - t.r0 / group);
@@ -746,103 +742,150 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_rows(KvView kv, KvBatchView
     m.r0 = t.r0, m.end = 0;
   }
   W w;
-  float q[MT][W::KS][8];
-  w.load_q(q, a, m, group, kvh, 0, n, g);
+  float q[W::KS][8];
+  w.load_q(q, a, m, group, kvh, n, g);
   w.init(q, a.scale, nullptr, wave, NW);
 
   const uint32_t *table = b.table + (uint64_t)t.seq * b.table_pages;
-  const uint64_t to_v = (uint64_t)kv.heads * kv.block_bytes;
-  const uint32_t mask = (1u << kv.page_log2) - 1u;
-  // a step's fills: K's 16 rows of each half, then V's; the wave's are NW apart
-  constexpr uint32_t MINE = 4u * S::FILLS / NW;
-  uint32_t off[MINE];   // of a lane's piece within the 16 rows
+  const uint32_t to_v = kv.heads * kv.block_bytes, mask = (1u << kv.page_log2) - 1u;
+  const uint8_t *const heads = kv.base + (uint64_t)kvh * kv.block_bytes;
+  // fp16: a step's fills, K's 16 rows of each half, then V's; the wave's are NW apart.
+  // int8: a step's 16-byte pieces, K's, then V's; the thread's are 256 apart
+  constexpr uint32_t MINE = I8 ? (4u * D + 255u) / 256u : 4u * S::FILLS / NW;
+  uint32_t off[MINE];   // of a piece within its 16 rows
 #pragma unroll
   for (uint32_t k = 0; k < MINE; ++k) {
-    const uint32_t l = NW * k + wave, at = l % S::FILLS * 64u + lane, r = at / S::PIECES;
-    off[k] = l / S::FILLS < 2u ? r * S::ROW + 16u * S::piece(r, at % S::PIECES) : 16u * at;
+    if constexpr (I8) {
+      const uint32_t at = (256u * k + tid) % (2u * D);
+      off[k] = 16u * (at % D);
+    } else {
+      const uint32_t l = NW * k + wave, at = l % S::FILLS * 64u + lane, r = at / S::PIECES, c = at % S::PIECES;
+      off[k] = r * S::ROW + 16u * (l / S::FILLS < 2u ? S::piece(r, c) : S::v_piece(r, c));
+    }
   }
+  // where the lane's parts of the operands lie in a buffer. From 128 wide the places
+  // are those of piece 0 with bits turned, one instruction instead of a register
+  constexpr bool TURN = S::PIECES >= 16u;
+  const uint32_t vr = 4u * g + n / 4u;
+  uint32_t ka[TURN ? 1 : W::KS], va[TURN ? 1 : W::E];
+#pragma unroll
+  for (int c = 0; c < (TURN ? 1 : W::KS); ++c) ka[c] = n * S::ROW + 16u * S::place(n, 4u * c + g);
+#pragma unroll
+  for (int i = 0; i < (TURN ? 1 : W::E); ++i) va[i] = S::V + vr * S::ROW + 32u * S::v_place(vr, i) + 8u * (n & 3u);
+
   uint32_t ids = 0;
   const int steps = t.end > base ? (t.end - base + 31) / 32 : 0;
   bool gone[2] = {};
-  auto issue = [&](int i) {
+  u32x4 raw[I8 ? MINE : 1];
+  uint32_t raw_scale = 0;
+  // Requests step i: into buffer `lds`, or (int8) into registers.
+  const auto issue = [&](int i, const uint8_t *lds) {
     const int t0 = base + 32 * i;
     if ((i & 31) == 0) {
       const int at = t0 + 16 * (int)lane;
       ids = at < t.end ? table[(uint32_t)at >> kv.page_log2] : ~0u;
     }
-    const uint8_t *blk[2];
+    rsrc_t page[2];
     uint32_t slot[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint32_t p = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + u);
       gone[u] = p >= kv.pages;
-      blk[u] = kv.base + (gone[u] ? 0ull : (uint64_t)p * kv.page_bytes) + (uint64_t)kvh * kv.block_bytes;
+      page[u] = __builtin_amdgcn_make_buffer_rsrc((void *)(heads + (gone[u] ? 0ull : (uint64_t)p * kv.page_bytes)), (short)0,
+                                                  (int)(to_v + kv.block_bytes), kRsrcFlags);
       slot[u] = (uint32_t)(t0 + 16 * u) & mask;
     }
-    const uint8_t *lds = buf[i & 1];
+    if constexpr (I8) {
 #pragma unroll
-    for (uint32_t k = 0; k < MINE; ++k) {
-      const uint32_t l = NW * k + wave, which = l / S::FILLS, sub = l % S::FILLS, u = which & 1u;
-      const rsrc_t r = make_rsrc((u ? blk[1] : blk[0]) + (which >> 1 ? to_v : 0ull), kv.block_bytes);
-      const uint32_t row = (u ? slot[1] : slot[0]) * S::ROW;
-      // 16 rows that are no whole number of fills: the last one's upper lanes have none
-      if (S::ROW % 64u == 0u || sub * 64u + lane < S::ROW)
-        dma16(r, lds + which * S::HALF + sub * 1024u, off[k], row);
-    }
-    if constexpr (W::I8) {
-      if (wave == NW - 1u) {
-        const uint32_t u = lane >> 4 & 1u;
-        fill4((u ? blk[1] + slot[1] * 4u : blk[0] + slot[0] * 4u) + ((uint32_t)D << kv.page_log2) + 4u * (lane & 15u) + (lane < 32u ? 0ull : to_v),
-              lds + S::SCALES);
+      for (uint32_t k = 0; k < MINE; ++k) {
+        // 16 rows are D pieces: a wave's 64 may lie in two halves
+        const uint32_t at = 256u * k + tid, which = at / D;
+        if (MINE * 256u > 4u * D && at >= 4u * D) break;
+        const uint32_t o = off[k] + (which >> 1 ? to_v : 0u) + (which & 1u ? slot[1] : slot[0]) * D;
+        if (D % 64u == 0u) raw[k] = __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_readfirstlane(which) & 1u ? page[1] : page[0], (int)o, 0, 0);
+        else if (which & 1u) raw[k] = __builtin_amdgcn_raw_buffer_load_b128(page[1], (int)o, 0, 0);
+        else raw[k] = __builtin_amdgcn_raw_buffer_load_b128(page[0], (int)o, 0, 0);
+      }
+      if (wave == 3u) {   // the scales: K's of the 32 tokens, then V's
+        const uint32_t o = ((uint32_t)D << kv.page_log2) + 4u * (lane & 15u) + (lane < 32u ? 0u : to_v);
+        const uint32_t x = __builtin_amdgcn_raw_buffer_load_b32(page[0], (int)(o + 4u * slot[0]), 0, 0);
+        const uint32_t y = __builtin_amdgcn_raw_buffer_load_b32(page[1], (int)(o + 4u * slot[1]), 0, 0);
+        raw_scale = lane & 16u ? y : x;
+      }
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < MINE; ++k) {
+        const uint32_t l = NW * k + wave, which = l / S::FILLS;
+        dma16(which & 1u ? page[1] : page[0], lds + 1024u * l, off[k], (which & 1u ? slot[1] : slot[0]) * S::ROW + (which >> 1 ? to_v : 0u));
       }
     }
   };
-  if (steps) issue(0);
-#pragma unroll 1
-  for (int i = 0; i < steps; ++i) {
-    const bool was[2] = {gone[0], gone[1]};
-    wait_step();
-    if (i + 1 < steps) issue(i + 1);
-    const int t0 = base + 32 * i;
-    if (t0 >= m.end || t0 + 32 <= m.begin) continue;
-    const uint8_t *lds = buf[i & 1];
+  // int8: what step i's issue() asked for, as fp16 into buffer `lds`.
+  const auto convert = [&](uint8_t *lds) {
+    if constexpr (I8) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint8_t *p = lds + u * S::HALF + n * S::ROW;
-      if constexpr (!W::I8) {
-#pragma unroll
-        for (int c = 0; c < W::KS; ++c) ld_words<4>(w.kw[u] + 4 * c, p + 16u * S::place(n, 4u * c + g));
-      } else {
-#pragma unroll
-        for (int c = 0; c + 1 < W::KS; c += 2) ld_words<4>(w.kw[u] + 2 * c, p + 16u * S::place(n, 2u * c + g));
-        if constexpr (W::KS & 1) ld_words<2>(w.kw[u] + 2 * (W::KS - 1), p + 16u * S::place(n, 2u * (W::KS - 1) + g / 2u) + 8u * (g & 1u));
-        ld_words<4>(w.ks[u], lds + S::SCALES + 64u * u + 16u * g);
+      for (uint32_t k = 0; k < MINE; ++k) {
+        const uint32_t at = 256u * k + tid, which = at / D, r = at % D / (D / 16u), c = at % D % (D / 16u);
+        if (MINE * 256u > 4u * D && at >= 4u * D) break;
+        uint8_t *row = lds + which * S::HALF + r * S::ROW;
+        const half8 x = i8_half8(raw[k][0], raw[k][1]), y = i8_half8(raw[k][2], raw[k][3]);
+        *(half8 *)(row + 16u * (which >> 1 ? 2u * S::v_place(r, c) : S::place(r, 2u * c))) = x;
+        *(half8 *)(row + 16u * (which >> 1 ? 2u * S::v_place(r, c) + 1u : S::place(r, 2u * c + 1u))) = y;
       }
+      if (wave == 3u) *(uint32_t *)(lds + S::SCALES + 4u * lane) = raw_scale;
     }
-    float s[MT][2][4];
-    w.scores(s);
-    __builtin_amdgcn_sched_barrier(0);   // V's registers are K's
-#pragma unroll
-    for (int u = 0; u < 2; ++u) w.load_rows(u, lds + S::V + u * S::HALF, lds + S::SCALES + 128u + 64u * u, n, g);
-    const bool masked = was[0] || was[1] || t0 + 31 > m.first || t0 < m.begin || (window && t0 <= m.last - window);
-    w.step(t0, masked, was, m, window, g, s);
+  };
+  if (steps) {
+    issue(0, buf[0]);
+    convert(buf[0]);
   }
+#pragma unroll 1
+  for (int i0 = 0; i0 < steps; i0 += 2) {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const float l = row_add(w.l[mt]);
-    const uint32_t r = 16u * mt + n;
-    if (r >= m.rows) continue;
-    const float f = l == 0.f ? 0.f : (W::I8 ? w.vref[mt] : 1.f) / l;
-    const uint32_t tok = (m.r0 + r) / group, h = (m.r0 + r) % group;
-    float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D;
+    for (int half = 0; half < 2; ++half) {
+      const int i = i0 + half;
+      if (i >= steps) break;
+      const bool was[2] = {gone[0], gone[1]};
+      wait_step();
+      if (i + 1 < steps) issue(i + 1, buf[1 - half]);
+      const int t0 = base + 32 * i;
+      if (t0 < m.end && t0 + 32 > m.begin) {
+        const uint8_t *lds = buf[half];
+        if constexpr (TURN) __asm__("" : "+v"(ka[0]), "+v"(va[0]));   // computed here, not kept
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int i = 0; i + 3 < W::E; i += 4)
-        *(float4v *)(dst + W::column(g, i, j)) = float4v{w.acc[mt][i][j], w.acc[mt][i + 1][j], w.acc[mt][i + 2][j], w.acc[mt][i + 3][j]} * f;
-      if constexpr (W::E & 2) *(float2v *)(dst + W::column(g, W::E - 2, j)) = float2v{w.acc[mt][W::E - 2][j], w.acc[mt][W::E - 1][j]} * f;
+          for (int c = 0; c < W::KS; ++c) ld_words<4>(w.kw[u] + 4 * c, lds + (TURN ? ka[0] ^ (64u * c) : ka[TURN ? 0 : c]) + u * S::HALF);
+          if constexpr (I8) ld_words<4>(w.ks[u], lds + S::SCALES + 64u * u + 16u * g);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float s[2][4];
+        w.scores(s);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < W::E; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint2 x = ld_turned(lds + (TURN ? va[0] ^ (32u * k) : va[TURN ? 0 : k]) + u * S::HALF);
+            w.vw[k][2 * u] = x.x, w.vw[k][2 * u + 1] = x.y;
+          }
+        if constexpr (I8) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) ld_words<4>(w.vs[u], lds + S::SCALES + 128u + 64u * u + 16u * g);
+        }
+        const bool masked = was[0] || was[1] || t0 + 31 > m.first || t0 < m.begin || (window && t0 <= m.last - window);
+        w.step(t0, masked, was, m, window, g, s);
+      }
+      if (i + 1 < steps) convert(buf[1 - half]);
     }
   }
+  const float l = row_add(w.l);
+  if (n >= m.rows) return;
+  const float f = l == 0.f ? 0.f : (I8 ? w.vref : 1.f) / l;
+  const uint32_t tok = (m.r0 + n) / group, h = (m.r0 + n) % group;
+  float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D;
+#pragma unroll
+  for (int i = 0; i < W::E; ++i) *(float4v *)(dst + W::column(g, i, 0)) = w.acc[i] * f;
 }
 
 // Tiles of R rows for sequences of at most `most` rows, `rows` of them in all.
@@ -906,7 +949,7 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
     const uint64_t g = (uint64_t)p.many_tiles * kv.heads;
     const uint32_t min_rows = b.seqs == 1u ? 1u : kFewRows + 1u;
     if (g > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_rows<TYPE, D, 1, 4>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
+    hipLaunchKernelGGL((k_attn_rows<TYPE, D>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.tiles) return e;
   }
@@ -916,11 +959,11 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
   if constexpr (D < 256) {
     if (p.waves == 8u) {
-      hipLaunchKernelGGL((k_attn<TYPE, D, 1, 8, false>), dim3((uint32_t)grid), dim3(512), 0, s, kv, b, a, p, cnt, part);
+      hipLaunchKernelGGL((k_attn<TYPE, D, 8>), dim3((uint32_t)grid), dim3(512), 0, s, kv, b, a, p, cnt, part);
       return hipGetLastError();
     }
   }
-  hipLaunchKernelGGL((k_attn<TYPE, D, 1, 4, (D == 256)>), dim3((uint32_t)grid), dim3(256), 0, s, kv, b, a, p, cnt, part);
+  hipLaunchKernelGGL((k_attn<TYPE, D, 4>), dim3((uint32_t)grid), dim3(256), 0, s, kv, b, a, p, cnt, part);
   return hipGetLastError();
 }
 
