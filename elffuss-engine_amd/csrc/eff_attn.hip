@@ -168,6 +168,52 @@ __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, 
   return true;
 }
 
+// The walk over a tile's cached tokens: steps of 32 tokens at lo, lo + stride, ... up
+// to hi, each two runs of 16 tokens of one page. The places of the next 32 steps'
+// runs are computed at once, one in each lane; a step takes its two out of them.
+struct AttnWalk {
+  const uint32_t *table;   // the sequence's
+  const uint8_t *heads;    // the first page's K of the head
+  int lo, hi, stride;
+  uint32_t low, high, slots;   // a lane's: address of its run's first row of K, and slot in the page
+  uint64_t none;               // lanes whose run has no page
+  const uint8_t *at[2];
+  uint32_t slot[2];
+  bool gone[2];
+
+  template <int ROW>
+  __device__ __forceinline__ void look(const KvView &kv, int t0) {
+    const uint32_t lane = threadIdx.x & 63u;
+    const int t = t0 + (int)(lane >> 1) * stride + 16 * (int)(lane & 1u);
+    const uint32_t page = t < hi ? table[(uint32_t)t >> kv.page_log2] : ~0u;
+    const bool there = page < kv.pages;
+    none = __ballot(!there);
+    slots = (uint32_t)t & ((1u << kv.page_log2) - 1u);
+    // a run without a page reads the first page's rows, which are masked
+    const uint64_t a = (uint64_t)(uintptr_t)heads + (there ? (uint64_t)page * kv.page_bytes : 0ull) + slots * (uint32_t)ROW;
+    low = (uint32_t)a, high = (uint32_t)(a >> 32);
+  }
+
+  // To step i (in order).
+  template <int ROW>
+  __device__ __forceinline__ void go(const KvView &kv, int i) {
+    if ((i & 31) == 0) look<ROW>(kv, lo + i * stride);
+    const uint32_t l = 2u * (i & 31);
+#pragma unroll
+    for (uint32_t u = 0; u < 2u; ++u) {
+      at[u] = (const uint8_t *)((uint64_t)__builtin_amdgcn_readlane(high, l + u) << 32 | (uint32_t)__builtin_amdgcn_readlane(low, l + u));
+      slot[u] = __builtin_amdgcn_readlane(slots, l + u);
+    }
+    const uint32_t two = (uint32_t)(none >> l) & 3u;
+    gone[0] = two & 1u, gone[1] = two >> 1;
+  }
+
+  // int8 pages: the scales of run u's rows of K.
+  __device__ __forceinline__ const uint8_t *scales(int u, const KvView &kv, uint32_t dim) const {
+    return at[u] + (dim << kv.page_log2) + 4u * slot[u] - dim * slot[u];
+  }
+};
+
 // One wave's share of a tile of 16 rows.
 //   SCALED  rows of the cache have scales
 //   I8      K and V arrive as int8 (else fp16, also where int8 was converted on the way)
@@ -253,9 +299,8 @@ struct AttnWave {
     for (int i = 0; i < E; ++i) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
   }
 
-  // K of the 16 tokens from `blk`'s slot `slot` on, into half u of the step.
-  __device__ __forceinline__ void load_k(int u, const uint8_t *blk, uint32_t slot, uint32_t page_log2, uint32_t n, uint32_t g) {
-    const uint8_t *p = blk + slot * ROW;
+  // K of the 16 tokens from p on, into half u of the step.
+  __device__ __forceinline__ void load_k(int u, const uint8_t *p, const uint8_t *scales, uint32_t n, uint32_t g) {
     if constexpr (!I8) {
 #pragma unroll
       for (int c = 0; c < KS; ++c) ld_words<4>(kw[u] + 4 * c, p + (n * ROW + 16u * g) + 64u * c);
@@ -263,13 +308,12 @@ struct AttnWave {
 #pragma unroll
       for (int c = 0; c + 1 < KS; c += 2) ld_words<4>(kw[u] + 2 * c, p + (n * ROW + 16u * g) + 32u * c);
       if constexpr (KS & 1) ld_words<2>(kw[u] + 2 * (KS - 1), p + (n * ROW + 8u * g) + 32u * (KS - 1));
-      ld_words<4>(ks[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
+      ld_words<4>(ks[u], scales + 16u * g);
     }
   }
 
   // V of the same tokens: the lane's columns of the rows 4 g .. 4 g + 3.
-  __device__ __forceinline__ void load_v(int u, const uint8_t *blk, uint32_t slot, uint32_t page_log2, uint32_t n, uint32_t g) {
-    const uint8_t *p = blk + slot * ROW;
+  __device__ __forceinline__ void load_v(int u, const uint8_t *p, const uint8_t *scales, uint32_t n, uint32_t g) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint8_t *r = p + 4u * g * ROW + j * ROW;
@@ -287,7 +331,7 @@ struct AttnWave {
         ld_words<VW>(o, r + 4u * VW * n);
       }
     }
-    if constexpr (I8) ld_words<4>(vs[u], blk + ((uint32_t)D << page_log2) + (slot + 4u * g) * 4u);
+    if constexpr (I8) ld_words<4>(vs[u], scales + 16u * g);
   }
 
   // Column i of the 8 tokens of the lane as the first operand.
@@ -465,52 +509,28 @@ struct AttnWave {
       for (int w = 0; w < (TR ? 4 : VW); ++w) vw[k][w] &= ~(not_finite(vw[k][w]) / 0x3C00u * 0xFFFFu);
   }
 
-  // The walk over a tile's cached tokens: the steps lo, lo + stride, ... up to hi.
-  // Page numbers are read 32 steps ahead, two in each pair of lanes.
-  struct Walk {
-    const uint32_t *table;
-    const uint8_t *blk[2];   // the pages of the step's two halves
-    bool gone[2];
-    uint32_t ids;
-    int lo, hi, stride;
-  };
-
-  static __device__ __forceinline__ void read_ids(Walk &k, const KvView &kv, int t0) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const int at = t0 + (int)(lane >> 1) * k.stride + 16 * (int)(lane & 1u);
-    k.ids = at < k.hi ? k.table[(uint32_t)at >> kv.page_log2] : ~0u;
-  }
-
-  __device__ __forceinline__ void fetch_k(Walk &k, const KvView &kv, uint32_t kvh, int i, int t0, uint32_t n, uint32_t g) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t p = __builtin_amdgcn_readlane(k.ids, 2 * (i & 31) + u);
-      k.gone[u] = p >= kv.pages;
-      k.blk[u] = kv.base + (k.gone[u] ? 0ull : (uint64_t)p * kv.page_bytes) + (uint64_t)kvh * kv.block_bytes;
-      load_k(u, k.blk[u], (uint32_t)(t0 + 16 * u) & ((1u << kv.page_log2) - 1u), kv.page_log2, n, g);
-    }
-  }
-
-  // The first step's keys are on their way (read_ids, fetch_k).
-  __device__ __forceinline__ void run(Walk &k, const KvView &kv, const AttnTile &t, uint32_t kvh, int window, uint32_t n, uint32_t g) {
-    const uint64_t to_v = (uint64_t)kv.heads * kv.block_bytes;
+  // The steps of `k`, whose first keys are on their way (fetch_k).
+  __device__ __forceinline__ void run(AttnWalk &k, const KvView &kv, const AttnTile &t, int window, uint32_t n, uint32_t g) {
+    const uint32_t to_v = kv.heads * kv.block_bytes;
+    const int full = t.first - 31, from = window ? t.last - window + 1 : 0;   // steps from .. full need no mask
     int i = 0;
 #pragma unroll 1
     for (int t0 = k.lo; t0 < k.hi; t0 += k.stride, ++i) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        load_v(u, k.blk[u] + to_v, (uint32_t)(t0 + 16 * u) & ((1u << kv.page_log2) - 1u), kv.page_log2, n, g);
+      for (int u = 0; u < 2; ++u) load_v(u, k.at[u] + to_v, k.scales(u, kv, D) + to_v, n, g);
       float s[2][4];
       scores(s);
       const bool gone[2] = {k.gone[0], k.gone[1]};
-      const bool masked = gone[0] || gone[1] || t0 + 31 > t.first || t0 < t.begin || (window && t0 <= t.last - window);
-      const int next = t0 + k.stride;
-      if (next < k.hi) {
-        if (((i + 1) & 31) == 0) read_ids(k, kv, next);
-        fetch_k(k, kv, kvh, i + 1, next, n, g);
-      }
+      const bool masked = gone[0] || gone[1] || t0 > full || t0 < from;
+      if (t0 + k.stride < k.hi) fetch_k(k, kv, i + 1, n, g);
       step(t0, masked, gone, t, window, g, s);
     }
+  }
+
+  __device__ __forceinline__ void fetch_k(AttnWalk &k, const KvView &kv, int i, uint32_t n, uint32_t g) {
+    k.go<ROW>(kv, i);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) load_k(u, k.at[u], k.scales(u, kv, D), n, g);
   }
 };
 
@@ -557,16 +577,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   const int lo = base + (int)(chunk * p.chunk), hi = min(lo + (int)p.chunk, t.end);
   W w;
   {
-    typename W::Walk k;
+    AttnWalk k;
     k.table = b.table + (uint64_t)t.seq * b.table_pages;
+    k.heads = kv.base + (uint64_t)kvh * kv.block_bytes;
     k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 32 * NW;
-    W::read_ids(k, kv, k.lo);
     float q[W::KS][8];
     w.load_q(q, a, t, group, kvh, n, g);
-    w.fetch_k(k, kv, kvh, 0, k.lo, n, g);   // of the first page, where the wave has no step
+    w.fetch_k(k, kv, 0, n, g);   // of the first page, where the wave has no step
     w.init(q, a.scale, (uint8_t *)so, wave, NW);
     if constexpr (QL) __syncthreads();
-    w.run(k, kv, t, kvh, window, n, g);
+    w.run(k, kv, t, window, n, g);
     if constexpr (QL) __syncthreads();   // the sums take q's place
   }
   const float wl = row_add(w.l);
@@ -746,21 +766,29 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   w.load_q(q, a, m, group, kvh, n, g);
   w.init(q, a.scale, nullptr, wave, NW);
 
-  const uint32_t *table = b.table + (uint64_t)t.seq * b.table_pages;
-  const uint32_t to_v = kv.heads * kv.block_bytes, mask = (1u << kv.page_log2) - 1u;
-  const uint8_t *const heads = kv.base + (uint64_t)kvh * kv.block_bytes;
+  const uint32_t to_v = kv.heads * kv.block_bytes;
+  AttnWalk k;
+  k.table = b.table + (uint64_t)t.seq * b.table_pages;
+  k.heads = kv.base + (uint64_t)kvh * kv.block_bytes;
+  k.lo = base, k.hi = t.end, k.stride = 32;
   // fp16: a step's fills, K's 16 rows of each half, then V's; the wave's are NW apart.
   // int8: a step's 16-byte pieces, K's, then V's; the thread's are 256 apart
   constexpr uint32_t MINE = I8 ? (4u * D + 255u) / 256u : 4u * S::FILLS / NW;
-  uint32_t off[MINE];   // of a piece within its 16 rows
+  // which of K's halves and V's a fill or piece is of, and its place there: known
+  // when a wave's are whole
+  constexpr bool EVEN = I8 ? D % 256u == 0u : S::FILLS % NW == 0u;
+  constexpr uint32_t PER = EVEN ? (I8 ? D / 256u : S::FILLS / NW) : 1u;
+  uint32_t off[MINE], which[MINE];   // bytes within the 16 rows
 #pragma unroll
-  for (uint32_t k = 0; k < MINE; ++k) {
+  for (uint32_t j = 0; j < MINE; ++j) {
     if constexpr (I8) {
-      const uint32_t at = (256u * k + tid) % (2u * D);
-      off[k] = 16u * (at % D);
+      const uint32_t x = 256u * j + tid;
+      which[j] = EVEN ? j / PER : D % 64u ? x / D : __builtin_amdgcn_readfirstlane(x / D);
+      off[j] = 16u * (x % D);
     } else {
-      const uint32_t l = NW * k + wave, at = l % S::FILLS * 64u + lane, r = at / S::PIECES, c = at % S::PIECES;
-      off[k] = r * S::ROW + 16u * (l / S::FILLS < 2u ? S::piece(r, c) : S::v_piece(r, c));
+      const uint32_t l = NW * j + wave, x = l % S::FILLS * 64u + lane, r = x / S::PIECES, c = x % S::PIECES;
+      which[j] = EVEN ? j / PER : l / S::FILLS;
+      off[j] = r * S::ROW + 16u * (which[j] < 2u ? S::piece(r, c) : S::v_piece(r, c));
     }
   }
   // where the lane's parts of the operands lie in a buffer. From 128 wide the places
@@ -773,68 +801,55 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
 #pragma unroll
   for (int i = 0; i < (TURN ? 1 : W::E); ++i) va[i] = S::V + vr * S::ROW + 32u * S::v_place(vr, i) + 8u * (n & 3u);
 
-  uint32_t ids = 0;
   const int steps = t.end > base ? (t.end - base + 31) / 32 : 0;
-  bool gone[2] = {};
   u32x4 raw[I8 ? MINE : 1];
   uint32_t raw_scale = 0;
   // Requests step i: into buffer `lds`, or (int8) into registers.
   const auto issue = [&](int i, const uint8_t *lds) {
-    const int t0 = base + 32 * i;
-    if ((i & 31) == 0) {
-      const int at = t0 + 16 * (int)lane;
-      ids = at < t.end ? table[(uint32_t)at >> kv.page_log2] : ~0u;
-    }
-    rsrc_t page[2];
-    uint32_t slot[2];
+    k.go<I8 ? D : 2 * D>(kv, i);
+    rsrc_t run[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t p = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + u);
-      gone[u] = p >= kv.pages;
-      page[u] = __builtin_amdgcn_make_buffer_rsrc((void *)(heads + (gone[u] ? 0ull : (uint64_t)p * kv.page_bytes)), (short)0,
-                                                  (int)(to_v + kv.block_bytes), kRsrcFlags);
-      slot[u] = (uint32_t)(t0 + 16 * u) & mask;
-    }
+    for (int u = 0; u < 2; ++u)
+      run[u] = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(k.at[u]), (short)0, (int)(to_v + kv.block_bytes), kRsrcFlags);
     if constexpr (I8) {
 #pragma unroll
-      for (uint32_t k = 0; k < MINE; ++k) {
-        // 16 rows are D pieces: a wave's 64 may lie in two halves
-        const uint32_t at = 256u * k + tid, which = at / D;
-        if (MINE * 256u > 4u * D && at >= 4u * D) break;
-        const uint32_t o = off[k] + (which >> 1 ? to_v : 0u) + (which & 1u ? slot[1] : slot[0]) * D;
-        if (D % 64u == 0u) raw[k] = __builtin_amdgcn_raw_buffer_load_b128(__builtin_amdgcn_readfirstlane(which) & 1u ? page[1] : page[0], (int)o, 0, 0);
-        else if (which & 1u) raw[k] = __builtin_amdgcn_raw_buffer_load_b128(page[1], (int)o, 0, 0);
-        else raw[k] = __builtin_amdgcn_raw_buffer_load_b128(page[0], (int)o, 0, 0);
+      for (uint32_t j = 0; j < MINE; ++j) {
+        if (MINE * 256u > 4u * D && 256u * j + tid >= 4u * D) break;
+        const uint32_t o = off[j] + (which[j] >> 1 ? to_v : 0u);
+        if (D % 64u) {   // a wave's 64 pieces may lie in two halves
+          if (which[j] & 1u) raw[j] = __builtin_amdgcn_raw_buffer_load_b128(run[1], (int)o, 0, 0);
+          else raw[j] = __builtin_amdgcn_raw_buffer_load_b128(run[0], (int)o, 0, 0);
+        } else {
+          raw[j] = __builtin_amdgcn_raw_buffer_load_b128(which[j] & 1u ? run[1] : run[0], (int)o, 0, 0);
+        }
       }
       if (wave == 3u) {   // the scales: K's of the 32 tokens, then V's
-        const uint32_t o = ((uint32_t)D << kv.page_log2) + 4u * (lane & 15u) + (lane < 32u ? 0u : to_v);
-        const uint32_t x = __builtin_amdgcn_raw_buffer_load_b32(page[0], (int)(o + 4u * slot[0]), 0, 0);
-        const uint32_t y = __builtin_amdgcn_raw_buffer_load_b32(page[1], (int)(o + 4u * slot[1]), 0, 0);
-        raw_scale = lane & 16u ? y : x;
+        const uint8_t *p = lane & 16u ? k.scales(1, kv, D) : k.scales(0, kv, D);
+        raw_scale = *(const uint32_t *)(p + 4u * (lane & 15u) + (lane < 32u ? 0u : to_v));
       }
     } else {
 #pragma unroll
-      for (uint32_t k = 0; k < MINE; ++k) {
-        const uint32_t l = NW * k + wave, which = l / S::FILLS;
-        dma16(which & 1u ? page[1] : page[0], lds + 1024u * l, off[k], (which & 1u ? slot[1] : slot[0]) * S::ROW + (which >> 1 ? to_v : 0u));
-      }
+      for (uint32_t j = 0; j < MINE; ++j)
+        dma16(which[j] & 1u ? run[1] : run[0], lds + 1024u * (NW * j + wave), off[j], which[j] >> 1 ? to_v : 0u);
     }
   };
   // int8: what step i's issue() asked for, as fp16 into buffer `lds`.
   const auto convert = [&](uint8_t *lds) {
     if constexpr (I8) {
 #pragma unroll
-      for (uint32_t k = 0; k < MINE; ++k) {
-        const uint32_t at = 256u * k + tid, which = at / D, r = at % D / (D / 16u), c = at % D % (D / 16u);
-        if (MINE * 256u > 4u * D && at >= 4u * D) break;
-        uint8_t *row = lds + which * S::HALF + r * S::ROW;
-        const half8 x = i8_half8(raw[k][0], raw[k][1]), y = i8_half8(raw[k][2], raw[k][3]);
-        *(half8 *)(row + 16u * (which >> 1 ? 2u * S::v_place(r, c) : S::place(r, 2u * c))) = x;
-        *(half8 *)(row + 16u * (which >> 1 ? 2u * S::v_place(r, c) + 1u : S::place(r, 2u * c + 1u))) = y;
+      for (uint32_t j = 0; j < MINE; ++j) {
+        const uint32_t x = 256u * j + tid, r = x % D / (D / 16u), c = x % D % (D / 16u);
+        if (MINE * 256u > 4u * D && x >= 4u * D) break;
+        uint8_t *row = lds + which[j] * S::HALF + r * S::ROW;
+        const uint32_t first = which[j] >> 1 ? 2u * S::v_place(r, c) : S::place(r, 2u * c);
+        const uint32_t second = which[j] >> 1 ? first + 1u : S::place(r, 2u * c + 1u);
+        *(half8 *)(row + 16u * first) = i8_half8(raw[j][0], raw[j][1]);
+        *(half8 *)(row + 16u * second) = i8_half8(raw[j][2], raw[j][3]);
       }
       if (wave == 3u) *(uint32_t *)(lds + S::SCALES + 4u * lane) = raw_scale;
     }
   };
+  const int full = m.first - 31, from = window ? m.last - window + 1 : 0;   // steps from .. full need no mask
   if (steps) {
     issue(0, buf[0]);
     convert(buf[0]);
@@ -845,7 +860,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     for (int half = 0; half < 2; ++half) {
       const int i = i0 + half;
       if (i >= steps) break;
-      const bool was[2] = {gone[0], gone[1]};
+      const bool was[2] = {k.gone[0], k.gone[1]};
       wait_step();
       if (i + 1 < steps) issue(i + 1, buf[1 - half]);
       const int t0 = base + 32 * i;
@@ -863,18 +878,17 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
         w.scores(s);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int k = 0; k < W::E; ++k)
+        for (int c = 0; c < W::E; ++c)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const uint2 x = ld_turned(lds + (TURN ? va[0] ^ (32u * k) : va[TURN ? 0 : k]) + u * S::HALF);
-            w.vw[k][2 * u] = x.x, w.vw[k][2 * u + 1] = x.y;
+            const uint2 x = ld_turned(lds + (TURN ? va[0] ^ (32u * c) : va[TURN ? 0 : c]) + u * S::HALF);
+            w.vw[c][2 * u] = x.x, w.vw[c][2 * u + 1] = x.y;
           }
         if constexpr (I8) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) ld_words<4>(w.vs[u], lds + S::SCALES + 128u + 64u * u + 16u * g);
         }
-        const bool masked = was[0] || was[1] || t0 + 31 > m.first || t0 < m.begin || (window && t0 <= m.last - window);
-        w.step(t0, masked, was, m, window, g, s);
+        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, g, s);
       }
       if (i + 1 < steps) convert(buf[1 - half]);
     }
