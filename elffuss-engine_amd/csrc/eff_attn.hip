@@ -219,8 +219,10 @@ struct AttnWalk {
 //   I8      K and V arrive as int8 (else fp16, also where int8 was converted on the way)
 //   QL      the parts of q are in LDS, shared by the waves of the tile, and read for
 //           each step
-//   TR      V arrives as the operand it is (turned by the LDS read)
-template <int D, bool SCALED, bool I8, bool QL, bool TR>
+//   VIN     V arrives as rows, as the operands that it is (turned by the LDS read), or
+//           is read by the caller as it is used (for want of registers)
+enum { kVRows, kVTurned, kVLater };
+template <int D, bool SCALED, bool I8, bool QL, int VIN>
 struct AttnWave {
   static constexpr int E = D / 16;                     // columns of a lane
   static constexpr int KS = D / 32;                    // matrix steps of a score
@@ -238,13 +240,14 @@ struct AttnWave {
 
   uint32_t kw[2][KS * KW];
   uint32_t ks[2][4];                          // SCALED: the scales of the lane's tokens (f32 bits)
-  uint32_t vw[TR ? E : 8][TR ? 4 : VW];       // V: 8 rows, or the operands of E columns
+  static constexpr int VN = VIN == kVRows ? 8 : VIN == kVTurned ? E : 1, VM = VIN == kVRows ? VW : VIN == kVTurned ? 4 : 1;
+  uint32_t vw[VN][VM];                        // V: 8 rows, or the operands of E columns
   uint32_t vs[2][4];
 
-  // column of acc[i][j] of lane group g: TR, and at D = 96, side by side with the
+  // column of acc[i][j] of lane group g: turned, and at D = 96, side by side with the
   // group's 4 rows; else E side by side
   static __device__ __forceinline__ uint32_t column(uint32_t g, int i, int j) {
-    if constexpr (TR) return 16u * i + 4u * g + j;
+    if constexpr (VIN != kVRows) return 16u * i + 4u * g + j;
     if constexpr (D == 96) return i < 4 ? 4u * (4u * g + j) + i : 64u + 2u * (4u * g + j) + (i - 4);
     return (uint32_t)E * (4u * g + j) + i;
   }
@@ -339,7 +342,7 @@ struct AttnWave {
     u32x4 o;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      if constexpr (TR) {
+      if constexpr (VIN == kVTurned) {
         o[x] = vw[i][x];
       } else if constexpr (I8) {
         const uint32_t w = i / 4, k = i % 4;
@@ -352,24 +355,18 @@ struct AttnWave {
     return o;
   }
 
-  // Takes the tokens whose bit is set out of V.
-  __device__ __forceinline__ void clear_v(uint32_t gone) {
-    if constexpr (TR) {
+  // Takes the tokens out of V whose halves of `keep` are 0.
+  __device__ __forceinline__ void keep_v(u32x4 keep) {
+    if constexpr (VIN == kVTurned) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint32_t keep = (gone >> (2 * x) & 1u ? 0u : 0xFFFFu) | (gone >> (2 * x + 1) & 1u ? 0u : 0xFFFF0000u);
+      for (int i = 0; i < E; ++i)
 #pragma unroll
-        for (int i = 0; i < E; ++i) vw[i][x] &= keep;
-      }
-    } else {
+        for (int x = 0; x < 4; ++x) vw[i][x] &= keep[x];
+    } else if constexpr (VIN == kVRows) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vw[k][w] = gone >> k & 1u ? 0u : vw[k][w];
-    }
-    if constexpr (SCALED) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) vs[k / 4][k % 4] = gone >> k & 1u ? 0u : vs[k / 4][k % 4];
+        for (int w = 0; w < VW; ++w) vw[k][w] = (keep[k / 2] >> 16 * (k & 1) & 1u) ? vw[k][w] : 0u;
     }
   }
 
@@ -401,19 +398,43 @@ struct AttnWave {
 
   static __device__ __forceinline__ bool sees(int pos, int window, int t) { return t <= pos && (window == 0 || t > pos - window); }
 
-  // The weights of the step at token t0, and the weighted sum. `masked`: some row
-  // does not see every one of its 32 tokens (wave-uniform); a half without a page is
-  // `gone`.
-  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[2][4]) {
+  // The weights of the step at token t0, and the weighted sum; v(i) is V's operand of
+  // column i. `masked`: some row does not see every one of its 32 tokens (wave-
+  // uniform); a half without a page is `gone`.
+  template <typename V>
+  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[2][4], V v) {
+    u32x4 keep = {~0u, ~0u, ~0u, ~0u};   // the halves of an operand whose token some row sees
+    bool dirty = false;                  // and whether some of them are not finite
     if (masked) {
-      uint32_t none = 0;   // tokens that no row sees: may be any bits
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int at = t0 + 16 * (k / 4) + 4 * (int)g + k % 4;
         if (gone[k / 4] || !sees(pos, window, at)) s[k / 4][k % 4] = -INFINITY;
-        if (gone[k / 4] || at < t.begin || at >= t.end) none |= 1u << k;
+        // what no row sees may be any bits
+        if (gone[k / 4] || at < t.begin || at >= t.end) {
+          if constexpr (SCALED) vs[k / 4][k % 4] = 0u;
+          else keep[k / 2] &= k & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
       }
-      clear_v(none);
+      // A value that only some rows see and that is not finite: 0 * inf would
+      // reach the others. (int8 values are finite, and their scales go with the weights.)
+      if constexpr (!SCALED) {
+        keep_v(keep);
+        if (t.first != t.last) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < (VIN == kVLater ? E : VN * VM / 4); ++i) {
+            u32x4 o;
+            if constexpr (VIN == kVLater) o = v(i) & keep;
+            else o = u32x4{vw[4 * i / VM][4 * i % VM], vw[(4 * i + 1) / VM][(4 * i + 1) % VM], vw[(4 * i + 2) / VM][(4 * i + 2) % VM], vw[(4 * i + 3) / VM][(4 * i + 3) % VM]};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) top = max(top, max(o[x] & 0x7FFFu, o[x] >> 16 & 0x7FFFu));
+            __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
+          }
+          dirty = __any(top >= 0x7C00u);
+          if (dirty) poison(t0, gone, window, g, keep, v);
+        }
+      }
     }
     float mx = max2(max2(max2(s[0][0], s[0][1]), max2(s[0][2], s[0][3])), max2(max2(s[1][0], s[1][1]), max2(s[1][2], s[1][3])));
     mx = row_max(mx);
@@ -459,27 +480,26 @@ struct AttnWave {
       split2(p[0], p[1], hi[k / 2], lo[k / 2]);
     }
     l += sum;
-    if constexpr (!SCALED) {
-      // A value that only some rows see and that is not finite: 0 * inf would
-      // reach the others.
-      if (masked && t.first != t.last) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < (TR ? E : 8); ++k)
-#pragma unroll
-          for (int w = 0; w < (TR ? 4 : VW); ++w) {
-            const uint32_t x = vw[k][w] & 0x7FFF7FFFu;
-            top = max(top, max(x & 0xFFFFu, x >> 16));
-          }
-        if (__any(top >= 0x7C00u)) poison(t0, gone, window, g);
-      }
-    }
     const half8 ph = join8(hi), pl = join8(lo);
+    if (VIN == kVLater && !SCALED && masked) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        u32x4 o = v(i) & keep;
+        if (dirty) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[x] &= ~not_finite_halves(o[x]);
+        }
+        acc[i] = mfma(__builtin_bit_cast(half8, o), ph, acc[i]);
+        acc[i] = mfma(__builtin_bit_cast(half8, o), pl, acc[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const half8 v = __builtin_bit_cast(half8, v_operand(i));
-      acc[i] = mfma(v, ph, acc[i]);
-      acc[i] = mfma(v, pl, acc[i]);
+      const half8 o = __builtin_bit_cast(half8, v(i));
+      acc[i] = mfma(o, ph, acc[i]);
+      acc[i] = mfma(o, pl, acc[i]);
     }
   }
 
@@ -488,25 +508,32 @@ struct AttnWave {
     return ((w & 0x7C00u) == 0x7C00u ? 0x3C00u : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0x3C000000u : 0u);
   }
 
+  // All bits of such a half.
+  static __device__ __forceinline__ uint32_t not_finite_halves(uint32_t w) { return not_finite(w) / 0x3C00u * 0xFFFFu; }
+
   // The columns of the rows that see a value that is not finite become NaN (the
-  // product of the two indicators says which), and such values are taken out of
-  // the step.
-  __device__ __forceinline__ void poison(int t0, const bool gone[2], int window, uint32_t g) {
+  // product of the two indicators says which), and such values are taken out of the
+  // step (by the product itself where V is read as it is used).
+  template <typename V>
+  __device__ __forceinline__ void poison(int t0, const bool gone[2], int window, uint32_t g, u32x4 keep, V v) {
     half8 seen;
 #pragma unroll
     for (int k = 0; k < 8; ++k) seen[k] = (_Float16)(!gone[k / 4] && sees(pos, window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4) ? 1.f : 0.f);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const u32x4 v = v_operand(i);
-      const u32x4 bad = {not_finite(v[0]), not_finite(v[1]), not_finite(v[2]), not_finite(v[3])};
+      const u32x4 o = v(i) & keep;
+      const u32x4 bad = {not_finite(o[0]), not_finite(o[1]), not_finite(o[2]), not_finite(o[3])};
       const float4v c = mfma(__builtin_bit_cast(half8, bad), seen, float4v{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = c[j] > 0.f ? NAN : acc[i][j];
+      __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
     }
+    if constexpr (VIN != kVLater) {
 #pragma unroll
-    for (int k = 0; k < (TR ? E : 8); ++k)
+      for (int k = 0; k < VN; ++k)
 #pragma unroll
-      for (int w = 0; w < (TR ? 4 : VW); ++w) vw[k][w] &= ~(not_finite(vw[k][w]) / 0x3C00u * 0xFFFFu);
+        for (int w = 0; w < VM; ++w) vw[k][w] &= ~not_finite_halves(vw[k][w]);
+    }
   }
 
   // The steps of `k`, whose first keys are on their way (fetch_k).
@@ -523,7 +550,7 @@ struct AttnWave {
       const bool gone[2] = {k.gone[0], k.gone[1]};
       const bool masked = gone[0] || gone[1] || t0 > full || t0 < from;
       if (t0 + k.stride < k.hi) fetch_k(k, kv, i + 1, n, g);
-      step(t0, masked, gone, t, window, g, s);
+      step(t0, masked, gone, t, window, g, s, [&](int c) { return v_operand(c); });
     }
   }
 
@@ -560,7 +587,7 @@ constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 template <int TYPE, int D, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
   constexpr bool I8 = TYPE == EFF_KV_I8, QL = D == 256;   // 256 wide, q's parts would take a quarter of the registers
-  using W = AttnWave<D, I8, I8, QL, false>;
+  using W = AttnWave<D, I8, I8, QL, kVRows>;
   constexpr uint32_t R = 16u, LD = D + 4u, T = 64u * NW;
   static_assert(!QL || W::KS * 2048u <= NW * R * LD * 4u, "q's parts share the sums' space");
   __shared__ float so[NW][R][LD];
@@ -737,7 +764,7 @@ template <int TYPE, int D>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles,
                                                                       uint32_t per_seq, uint32_t min_rows) {
   constexpr bool I8 = TYPE == EFF_KV_I8;
-  using W = AttnWave<D, I8, false, false, true>;
+  using W = AttnWave<D, I8, false, false, D <= 128 ? kVTurned : kVLater>;
   using S = AttnStage<D>;
   constexpr uint32_t NW = 4u, R = 16u * NW;
   __shared__ __align__(1024) uint8_t buf[2][S::BYTES];
@@ -877,18 +904,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
         float s[2][4];
         w.scores(s);
         __builtin_amdgcn_sched_barrier(0);
+        const auto turned = [&](int c) {
+          const uint8_t *p = lds + (TURN ? va[0] ^ (32u * c) : va[TURN ? 0 : c]);
+          const uint2 x = ld_turned(p), y = ld_turned(p + S::HALF);
+          return u32x4{x.x, x.y, y.x, y.y};
+        };
+        if constexpr (D <= 128) {
 #pragma unroll
-        for (int c = 0; c < W::E; ++c)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint2 x = ld_turned(lds + (TURN ? va[0] ^ (32u * c) : va[TURN ? 0 : c]) + u * S::HALF);
-            w.vw[c][2 * u] = x.x, w.vw[c][2 * u + 1] = x.y;
-          }
+          for (int c = 0; c < W::E; ++c) __builtin_memcpy(w.vw[c], &(const u32x4 &)turned(c), 16);
+        }
         if constexpr (I8) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) ld_words<4>(w.vs[u], lds + S::SCALES + 128u + 64u * u + 16u * g);
         }
-        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, g, s);
+        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); });
       }
       if (i + 1 < steps) convert(buf[1 - half]);
     }
