@@ -105,6 +105,9 @@ __device__ __forceinline__ void split2(float a, float b, half2v &hi, half2v &lo)
   lo = half2v{(_Float16)fmaf((float)hi[0], m, a), (_Float16)fmaf((float)hi[1], m, b)};
 }
 
+constexpr uint32_t kShort = 8;    // units of a share
+constexpr uint32_t kUnit = 128;   // tokens: a step of each of four waves
+
 // The rows of a tile, their tokens and what they see.
 struct AttnTile {
   uint32_t seq, token0;   // the sequence's first new token
@@ -112,6 +115,18 @@ struct AttnTile {
   int first, last;        // positions of the first and last row
   int begin, end;         // the cached tokens that any row sees
 };
+
+// Tile `sub` of a sequence of n new tokens from s0 on, `len` with them.
+template <uint32_t R>
+__device__ __forceinline__ void attn_rows_of(AttnTile &t, uint32_t sub, uint32_t s0, uint32_t n, int len, uint32_t group, uint32_t window) {
+  t.token0 = s0;
+  t.r0 = sub * R;
+  t.rows = min(R, n * group - t.r0);
+  t.first = len - (int)n + (int)(t.r0 / group);
+  t.last = len - (int)n + (int)((t.r0 + t.rows - 1u) / group);
+  t.end = max(t.last + 1, 0);
+  t.begin = window ? max(0, t.first - (int)min(window, 0x40000000u) + 1) : 0;
+}
 
 // The tile of a workgroup, of the sequences that have min_rows .. max_rows rows:
 // `per_seq` tiles of each sequence, or (per_seq = 0) their tiles one after the other.
@@ -156,16 +171,137 @@ __device__ __forceinline__ bool attn_tile(const KvBatchView &b, uint32_t group, 
   const uint32_t s0 = __builtin_amdgcn_readfirstlane(b.starts[t.seq]);
   const uint32_t s1 = min((uint32_t)__builtin_amdgcn_readfirstlane(b.starts[t.seq + 1]), b.tokens);
   const uint32_t n = s1 > s0 ? min(s1 - s0, b.max_new) : 0u;
-  t.token0 = s0;
-  t.r0 = sub * R;
-  if (t.r0 >= n * group || n * group < min_rows || n * group > max_rows) return false;
-  t.rows = min(R, n * group - t.r0);
-  const int len = __builtin_amdgcn_readfirstlane((int)kv_len(b, t.seq));
-  t.first = len - (int)n + (int)(t.r0 / group);
-  t.last = len - (int)n + (int)((t.r0 + t.rows - 1u) / group);
-  t.end = max(t.last + 1, 0);
-  t.begin = window ? max(0, t.first - (int)min(window, 0x40000000u) + 1) : 0;
+  if (sub * R >= n * group || n * group < min_rows || n * group > max_rows) return false;
+  attn_rows_of<R>(t, sub, s0, n, __builtin_amdgcn_readfirstlane((int)kv_len(b, t.seq)), group, window);
   return true;
+}
+
+// A workgroup's share of the cached tokens that all tiles see, in units of 128 tokens,
+// the tiles' one after the other: the next tile of it.
+struct AttnShare {
+  uint32_t each, left;    // units of a workgroup; units that this one has left
+  uint32_t sub, of;       // the tile within its sequence, and units of each of the sequence's tiles
+  uint32_t start, at;     // the tile's first unit of all, and the share's first within the tile
+};
+
+// Units of each tile of a sequence of `len` tokens at most.
+template <uint32_t R>
+__device__ __forceinline__ uint32_t attn_units(uint32_t len, uint32_t group, uint32_t window) {
+  const uint32_t span = window ? min(len, min(window, 0x40000000u) + R / group + 33u) : len;
+  return max((span + kUnit - 1u) / kUnit, 1u);
+}
+
+// The share of workgroup `item` of `items`, `least` units at least: every one has the
+// same work, whatever the lengths are. Each wave adds the sequences up for itself, 64
+// at a time. A share that goes on into the next tile starts anew there, with its
+// loads' latency: short shares end with a tile instead (ENDS: all; there are more
+// items than tiles).
+template <uint32_t R, bool ENDS>
+__device__ __forceinline__ bool attn_share(const KvBatchView &b, uint32_t group, uint32_t window, uint32_t item, uint32_t items,
+                                           uint32_t least, uint32_t max_rows, AttnTile &t, AttnShare &c) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t s0 = 0, n = 0, len = 0, tiles = 0, of = 0;
+  const auto load = [&](uint32_t at) {
+    const uint32_t i = at + lane;
+    n = len = 0;
+    if (i < b.seqs) {
+      s0 = b.starts[i];
+      const uint32_t s1 = min(b.starts[i + 1], b.tokens);
+      len = kv_len(b, i);
+      n = s1 > s0 ? min(s1 - s0, b.max_new) : 0u;
+    }
+    tiles = n * group <= max_rows ? (n * group + R - 1u) / R : 0u;
+    of = attn_units<R>(len, group, window);
+  };
+  if (ENDS && b.seqs == 1u) {   // scalar all the way
+    const uint32_t from = __builtin_amdgcn_readfirstlane(b.starts[0]), to = min((uint32_t)__builtin_amdgcn_readfirstlane(b.starts[1]), b.tokens);
+    const uint32_t l = __builtin_amdgcn_readfirstlane(kv_len(b, 0)), m = to > from ? min(to - from, b.max_new) : 0u;
+    const uint32_t units = attn_units<R>(l, group, window), many = (m * group + R - 1u) / R;
+    if (m * group > max_rows || many >= items) return false;
+    c.each = max((many * units + items - many - 1u) / (items - many), least);
+    c.of = (units + c.each - 1u) / c.each * c.each;
+    c.sub = item * c.each / c.of;
+    if (c.sub >= many) return false;
+    c.start = c.sub * c.of, c.at = item * c.each - c.start, c.left = c.each;
+    t.seq = 0;
+    attn_rows_of<R>(t, c.sub, from, m, (int)l, group, window);
+    return true;
+  }
+  load(0);
+  uint32_t total = 0, count = 0;
+  for (uint32_t at = 0;;) {
+    total += tiles * of;
+    count += tiles;
+    if ((at += 64u) >= b.seqs) break;
+    load(at);
+  }
+  if (b.seqs > 1u) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o), count += __shfl_xor(count, o);
+  }
+  total = __builtin_amdgcn_readfirstlane(total);
+  count = __builtin_amdgcn_readfirstlane(count);
+  uint32_t each = (total + items - 1u) / items, whole = 1;
+  if (ENDS && count >= items) return false;
+  if (ENDS || (each < kShort && count < items)) whole = each = max((total + items - count - 1u) / (items - count), least);
+  each = max(each, least);
+  c.each = __builtin_amdgcn_readfirstlane(each);
+  whole = __builtin_amdgcn_readfirstlane(whole);
+  const uint32_t first = item * c.each;
+  uint32_t base = 0;
+  for (uint32_t at = 0; at < b.seqs; at += 64u) {
+    if (b.seqs > 64u) load(at);
+    if (whole > 1u) of = (of + whole - 1u) / whole * whole;
+    const uint32_t mine = tiles * of;
+    uint32_t sum = mine;
+    if (b.seqs > 1u) {
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(sum, o);
+        if ((int)lane >= o) sum += u;
+      }
+    }
+    const uint64_t past = __ballot(base + sum > first);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      c.of = __builtin_amdgcn_readlane(of, l);
+      const uint32_t before = base + __builtin_amdgcn_readlane(sum - mine, l), i = first - before;
+      c.sub = __builtin_amdgcn_readfirstlane(i / c.of);
+      c.at = i - c.sub * c.of;
+      c.start = first - c.at;
+      c.left = c.each;
+      t.seq = at + l;
+      attn_rows_of<R>(t, c.sub, __builtin_amdgcn_readlane(s0, l), __builtin_amdgcn_readlane(n, l), (int)__builtin_amdgcn_readlane(len, l),
+                      group, window);
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+// To the share's next tile; false: it ends.
+template <uint32_t R>
+__device__ __forceinline__ bool attn_next(const KvBatchView &b, uint32_t group, uint32_t window, uint32_t max_rows, AttnTile &t, AttnShare &c) {
+  const uint32_t took = min(c.left, c.of - c.at);
+  c.left -= took;
+  if (c.left == 0u) return false;
+  c.start += c.of;
+  c.at = 0;
+  ++c.sub;
+  for (;;) {
+    const uint32_t s0 = __builtin_amdgcn_readfirstlane(b.starts[t.seq]);
+    const uint32_t s1 = min((uint32_t)__builtin_amdgcn_readfirstlane(b.starts[t.seq + 1]), b.tokens);
+    const uint32_t len = __builtin_amdgcn_readfirstlane(kv_len(b, t.seq));
+    const uint32_t n = s1 > s0 ? min(s1 - s0, b.max_new) : 0u;
+    if (n * group <= max_rows && c.sub * R < n * group) {
+      c.of = attn_units<R>(len, group, window);
+      attn_rows_of<R>(t, c.sub, s0, n, (int)len, group, window);
+      return true;
+    }
+    if (++t.seq >= b.seqs) return false;
+    c.sub = 0;
+  }
 }
 
 // The walk over a tile's cached tokens: steps of 32 tokens at lo, lo + stride, ... up
@@ -563,157 +699,207 @@ struct AttnWave {
 
 struct AttnPlan {
   uint32_t tiles, per_seq;    // row tiles; tiles of each sequence (0: packed)
-  uint32_t chunk, chunks;     // cached tokens of a workgroup, chunks of a tile at most
+  uint32_t items;             // workgroups of a head that share the cached tokens (0: one a tile)
+  uint32_t least;             // units of a share at least
+  bool on;                    // a share may go on into the next tile
   uint32_t rows;              // rows of a tile at most
   uint32_t waves;             // of a workgroup
   uint32_t max_rows;          // of the sequences taken; those with more go to k_attn_rows:
   uint32_t many_tiles, many_per_seq;   // its tiles (0: none go)
 };
 
-// The joined sums of chunks: per (tile, head) the chunks' weighted sums, then
-// their maxima and sums.
-__host__ __device__ constexpr uint64_t attn_part_floats(const AttnPlan &p, uint32_t dim) {
-  return (uint64_t)p.chunks * p.rows * (dim + 2u);
-}
+// The sums of a tile that several workgroups share: each has two slots for a head, for
+// the tile that it begins in and for the one that it ends in, of `rows` rows'
+// weighted sums and their maxima and sums.
+__host__ __device__ constexpr uint32_t attn_part_floats(const AttnPlan &p, uint32_t dim) { return p.rows * (dim + 2u); }
 
 constexpr uint32_t kFewRows = 64;
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
-// NW waves take the 32-token steps of a chunk in turn; their sums meet in
-// LDS. Where a tile has several chunks, the last workgroup of the tile to arrive
-// joins them, in chunk order; stores and loads of the chunks' sums go past the
-// XCD's L2 (sc1), every wave waits for its stores before the barrier ahead of the
-// counter's increment, and the counter is left at zero for the next launch.
-template <int TYPE, int D, int NW>
+enum { kAttnWhole, kAttnEnds, kAttnOn };   // a workgroup has a tile; a part of one; a share that may go on into the next
+
+// A wave's copy of what a workgroup has in LDS, in scalar registers.
+template <typename T>
+__device__ __forceinline__ void from_lds(T &to, const T &from) {
+  uint32_t w[sizeof(T) / 4];
+  __builtin_memcpy(w, &from, sizeof(T));
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(T) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+  __builtin_memcpy(&to, w, sizeof(T));
+}
+
+// NW waves take the 32-token steps of a tile in turn; their sums meet in LDS. Where
+// a tile has several workgroups, the last of them to arrive joins their sums, in the
+// tokens' order; stores and loads of these go past the XCD's L2 (sc1), every wave
+// waits for its stores before the barrier ahead of the counter's increment, and the
+// counter is left at zero for the next launch.
+template <int TYPE, int D, int NW, int MODE>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
   constexpr bool I8 = TYPE == EFF_KV_I8, QL = D == 256;   // 256 wide, q's parts would take a quarter of the registers
   using W = AttnWave<D, I8, I8, QL, kVRows>;
   constexpr uint32_t R = 16u, LD = D + 4u, T = 64u * NW;
   static_assert(!QL || W::KS * 2048u <= NW * R * LD * 4u, "q's parts share the sums' space");
+  static_assert(MODE == kAttnWhole || kUnit == 32u * NW, "a unit is a step of each wave");
   __shared__ float so[NW][R][LD];
   __shared__ float sm[NW][R], sl[NW][R], sv[NW][R];
   __shared__ uint32_t arrived;
+  __shared__ AttnTile kept_t;
+  __shared__ AttnShare kept_c;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
-  const uint32_t kvh = blockIdx.x % kv.heads, w0 = blockIdx.x / kv.heads, chunk = w0 % p.chunks, tile = w0 / p.chunks;
+  const uint32_t kvh = blockIdx.x % kv.heads, item = blockIdx.x / kv.heads;
+  const int window = (int)min(a.window, 0x40000000u);
+  constexpr bool shared = MODE != kAttnWhole, on = MODE == kAttnOn;
   AttnTile t;
-  if (!attn_tile<R>(b, group, a.window, tile, p.per_seq, 1u, p.max_rows, t)) return;
-  const int window = (int)min(a.window, 0x40000000u), base = t.begin & ~31;
-  const uint32_t chunks = t.end > base ? ((uint32_t)(t.end - base) + p.chunk - 1u) / p.chunk : 1u;
-  if (chunk >= chunks) return;
-  const int lo = base + (int)(chunk * p.chunk), hi = min(lo + (int)p.chunk, t.end);
-  W w;
-  {
-    AttnWalk k;
-    k.table = b.table + (uint64_t)t.seq * b.table_pages;
-    k.heads = kv.base + (uint64_t)kvh * kv.block_bytes;
-    k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 32 * NW;
-    float q[W::KS][8];
-    w.load_q(q, a, t, group, kvh, n, g);
-    w.fetch_k(k, kv, 0, n, g);   // of the first page, where the wave has no step
-    w.init(q, a.scale, (uint8_t *)so, wave, NW);
-    if constexpr (QL) __syncthreads();
-    w.run(k, kv, t, window, n, g);
-    if constexpr (QL) __syncthreads();   // the sums take q's place
+  AttnShare c = {1u, 1u, 0u, 1u, 0u, 0u};
+  if constexpr (shared) {
+    if (!attn_share<R, !on>(b, group, a.window, item, p.items, p.least, p.max_rows, t, c)) return;
+  } else {
+    if (!attn_tile<R>(b, group, a.window, item, p.per_seq, 1u, p.max_rows, t)) return;
   }
-  const float wl = row_add(w.l);
-  if (g == 0u) sm[wave][n] = w.m * w.sc, sl[wave][n] = wl, sv[wave][n] = w.vref;
-#pragma unroll
-  for (int i = 0; i < W::E; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) so[wave][n][W::column(g, i, j)] = w.acc[i][j];
-  __syncthreads();
-  const uint64_t at = ((uint64_t)tile * kv.heads + kvh) * attn_part_floats(p, D);
-  const rsrc_t prs = make_rsrc(part + at, attn_part_floats(p, D) * 4u);
-  const uint32_t ml = p.chunks * p.rows * D;   // where the maxima and sums begin
-  for (uint32_t i = tid; i < t.rows * (D / 4u); i += T) {
-    const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u));
-    float mx = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int v = 0; v < NW; ++v) mx = fmaxf(mx, sm[v][r]);
-    float4v o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int v = 0; v < NW; ++v) {
-      const float f = sm[v][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[v][r] - mx);
-      l += f * sl[v][r];
-      const float4v x = *(const float4v *)&so[v][r][d];
-      o += x * (I8 ? f * sv[v][r] : f);
+  for (;;) {
+    const int base = t.begin & ~31;
+    int lo = base, hi = t.end;
+    if (shared) {
+      lo = base + (int)(c.at * kUnit);
+      hi = min(base + (int)(min(c.at + c.left, c.of) * kUnit), t.end);
+      // the steps take all scalar registers: the rest waits in LDS
+      if (on && tid == 0u) kept_t = t, kept_c = c;
     }
-    if (chunks == 1u) {
-      const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
-      float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
-      *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
-    } else {
-      const uint32_t row = chunk * p.rows + r;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((row * D + d) * 4u), 0, kSc1);
-      if (d == 0u) {
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((ml + 2u * row) * 4u), 0, kSc1);
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((ml + 2u * row + 1u) * 4u), 0, kSc1);
+    const bool mine = lo < hi || lo == base;   // past the end the tile's other workgroups have it all
+    if (mine) {
+      W w;
+      {
+        AttnWalk k;
+        k.table = b.table + (uint64_t)t.seq * b.table_pages;
+        k.heads = kv.base + (uint64_t)kvh * kv.block_bytes;
+        k.lo = lo + 32 * (int)wave, k.hi = hi, k.stride = 32 * NW;
+        float q[W::KS][8];
+        w.load_q(q, a, t, group, kvh, n, g);
+        w.fetch_k(k, kv, 0, n, g);   // of the first page, where the wave has no step
+        w.init(q, a.scale, (uint8_t *)so, wave, NW);
+        if constexpr (QL) __syncthreads();
+        w.run(k, kv, t, window, n, g);
+        if constexpr (QL) __syncthreads();   // the sums take q's place
       }
-    }
-  }
-  if (chunks == 1u) return;
-  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  uint32_t *c = cnt + (uint64_t)tile * kv.heads + kvh;
-  if (tid == 0u) arrived = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (arrived != chunks - 1u) return;
-  if (tid == 0u) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // the chunks' weights relative to the largest maximum, [chunk][row], and the
-  // rows' sums: a wave per row, its lanes over the chunks
-  float *wt = &so[0][0][0], *half = wt + NW * R * LD - 4u * T;
-  for (uint32_t r = wave; r < t.rows; r += NW) {
-    float mx = -INFINITY, l = 0.f;
-    for (uint32_t z = lane; z < chunks; z += 64u)
-      mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((ml + 2u * (z * p.rows + r)) * 4u), 0, kSc1)));
+      const float wl = row_add(w.l);
+      if (g == 0u) sm[wave][n] = w.m * w.sc, sl[wave][n] = wl, sv[wave][n] = w.vref;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    for (uint32_t z = lane; z < chunks; z += 64u) {
-      const int at = (int)((ml + 2u * (z * p.rows + r)) * 4u);
-      const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
-      const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
-      const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
-      wt[z * p.rows + r] = f;
-      l += f * lz;
-    }
-    l = wave_sum(l);
-    if (lane == 0u) sl[0][r] = l;
-  }
-  __syncthreads();
-  // each thread a part of the chunks of 4 columns of a row
-  const uint32_t items = t.rows * (D / 4u), parts = max(1u, T / items);
-  for (uint32_t i0 = 0; i0 < items; i0 += T) {
-    const uint32_t part_i = parts > 1u ? tid / items : 0u, i = parts > 1u ? tid % items : i0 + tid;
-    const bool on = i < items && part_i < parts;
-    const uint32_t r = on ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
-    float4v o = {0.f, 0.f, 0.f, 0.f};
-    if (on) {
-      constexpr uint32_t U = 8;
-      for (uint32_t z = part_i; z < chunks; z += U * parts) {
-        float4v x[U];
+      for (int i = 0; i < W::E; ++i)
 #pragma unroll
-        for (uint32_t k = 0; k < U; ++k) {
-          const uint32_t row = min(z + k * parts, chunks - 1u) * p.rows + r;
-          x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)((row * D + d) * 4u), 0, kSc1));
+        for (int j = 0; j < 4; ++j) so[wave][n][W::column(g, i, j)] = w.acc[i][j];
+    }
+    __syncthreads();
+    uint32_t first = 0, chunks = 1;   // the tile's workgroups
+    if (shared) {
+      if constexpr (on) {
+        from_lds(t, kept_t);
+        from_lds(c, kept_c);
+      }
+      const int tokens = t.end - (t.begin & ~31);
+      const uint32_t units = tokens > 0 ? ((uint32_t)tokens + kUnit - 1u) / kUnit : 1u;
+      first = __builtin_amdgcn_readfirstlane(c.start / c.each);
+      chunks = __builtin_amdgcn_readfirstlane((c.start + units - 1u) / c.each) - first + 1u;
+    }
+    // the head's slots: of a workgroup, the one of the tile that it begins in, then of
+    // the tile that it ends in
+    const uint32_t slot_floats = attn_part_floats(p, D), ml = p.rows * D;   // ml: where a slot's maxima and sums begin
+    const rsrc_t prs = make_rsrc(part + (uint64_t)kvh * p.items * 2u * slot_floats, (uint64_t)p.items * 2u * slot_floats * 4u);
+    const uint32_t slot = (2u * item + (item == first ? 1u : 0u)) * slot_floats;
+    if (mine) {
+      for (uint32_t i = tid; i < t.rows * (D / 4u); i += T) {
+        const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u));
+        float mx = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int v = 0; v < NW; ++v) mx = fmaxf(mx, sm[v][r]);
+        float4v o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < NW; ++v) {
+          const float f = sm[v][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[v][r] - mx);
+          l += f * sl[v][r];
+          const float4v x = *(const float4v *)&so[v][r][d];
+          o += x * (I8 ? f * sv[v][r] : f);
         }
-#pragma unroll
-        for (uint32_t k = 0; k < U; ++k)
-          if (z + k * parts < chunks) o += x[k] * wt[(z + k * parts) * p.rows + r];
+        if (!shared || chunks == 1u) {
+          const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+          float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+          *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+        } else {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((slot + r * D + d) * 4u), 0, kSc1);
+          if (d == 0u) {
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((slot + ml + 2u * r) * 4u), 0, kSc1);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((slot + ml + 2u * r + 1u) * 4u), 0, kSc1);
+          }
+        }
       }
     }
-    if (parts > 1u) {
-      *(float4v *)(half + 4u * tid) = o;
+    if (shared && mine && chunks > 1u) {
+      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (on && part_i == 0u)
-        for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * items));
+      uint32_t *counter = cnt + ((uint64_t)kvh * p.items + first);
+      if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (arrived == chunks - 1u) {
+        if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const auto place = [&](uint32_t z) { return (2u * (first + z) + (z == 0u ? 1u : 0u)) * slot_floats; };
+        // the workgroups' weights relative to the largest maximum, [workgroup][row],
+        // and the rows' sums: a wave per row, its lanes over the workgroups
+        float *wt = &so[0][0][0], *half = wt + NW * R * LD - 4u * T;
+        for (uint32_t r = wave; r < t.rows; r += NW) {
+          float mx = -INFINITY, l = 0.f;
+          for (uint32_t z = lane; z < chunks; z += 64u)
+            mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((place(z) + ml + 2u * r) * 4u), 0, kSc1)));
+#pragma unroll
+          for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+          for (uint32_t z = lane; z < chunks; z += 64u) {
+            const int at = (int)((place(z) + ml + 2u * r) * 4u);
+            const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
+            const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
+            const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
+            wt[z * p.rows + r] = f;
+            l += f * lz;
+          }
+          l = wave_sum(l);
+          if (lane == 0u) sl[0][r] = l;
+        }
+        __syncthreads();
+        // each thread a part of the workgroups' 4 columns of a row
+        const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
+        for (uint32_t i0 = 0; i0 < pieces; i0 += T) {
+          const uint32_t part_i = parts > 1u ? tid / pieces : 0u, i = parts > 1u ? tid % pieces : i0 + tid;
+          const bool on = i < pieces && part_i < parts;
+          const uint32_t r = on ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
+          float4v o = {0.f, 0.f, 0.f, 0.f};
+          if (on) {
+            constexpr uint32_t U = 8;
+            for (uint32_t z = part_i; z < chunks; z += U * parts) {
+              float4v x[U];
+#pragma unroll
+              for (uint32_t k = 0; k < U; ++k)
+                x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(
+                                                       prs, (int)((place(min(z + k * parts, chunks - 1u)) + r * D + d) * 4u), 0, kSc1));
+#pragma unroll
+              for (uint32_t k = 0; k < U; ++k)
+                if (z + k * parts < chunks) o += x[k] * wt[(z + k * parts) * p.rows + r];
+            }
+          }
+          if (parts > 1u) {
+            *(float4v *)(half + 4u * tid) = o;
+            __syncthreads();
+            if (on && part_i == 0u)
+              for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * pieces));
+          }
+          if (on && part_i == 0u) {
+            const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+            const float l = sl[0][r];
+            float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+            *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+          }
+        }
+      }
     }
-    if (on && part_i == 0u) {
-      const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
-      const float l = sl[0][r];
-      float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
-      *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
-    }
+    if (!on || !attn_next<R>(b, group, a.window, p.max_rows, t, c)) return;
+    __syncthreads();   // the next tile's sums take these ones' place
   }
 }
 
@@ -957,32 +1143,37 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
-  // About 256 workgroups, one for each CU, in chunks of 256 tokens at least: below,
-  // a wave has one step, and the join costs more than the steps it takes over
-  // (1 x 8 heads of 128 over 2000 tokens: 256 10.0 us, 512 11.8, one chunk 23). At
-  // most 1024 for several sequences, whose lengths differ by what the host does not
-  // know (64 up to 16384: 384 us, one chunk each 453; 40 of int8 up to 9001 52.9,
-  // 2048 76.2), and 4096 for one (130001: 94.3, 1024 104.4). Where the tiles alone
-  // fill half of the CUs and are short, no chunks: a join takes 5 us (24 x 8 heads
-  // of drafts that see 1024: 17.8 us, chunks of 512 22.5).
-  const uint64_t whole = (span + 127u) / 128u * 128u;
-  uint64_t chunk = std::min<uint64_t>(std::max<uint64_t>((span * wgs / 256u + 127u) / 128u * 128u, 256u), b.seqs > 1u ? 1024u : 4096u);
-  if (wgs >= 128u && whole <= 2176u) chunk = whole;
-  if (wgs >= 4096u) chunk = whole;
-  const uint64_t most_chunks = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;
-  chunk = std::min(std::max(chunk, (span / most_chunks + 128u) / 128u * 128u), whole);
-  if (wgs > kAttnCounters) chunk = whole;
-  p.chunk = (uint32_t)chunk;
-  p.chunks = (uint32_t)((span + chunk - 1u) / chunk);
+  // Where the tiles alone fill half of the CUs and are short, or there are many, a
+  // workgroup has a tile: a join takes 5 us (24 x 8 heads of drafts that see 1024
+  // tokens: 15.8 us, shared 22.5; 32 x 8 heads of one token up to 2000 36.8, shared
+  // 45.8).
+  const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
+  if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > 2u && each * b.seqs * units < 1u << 31) {
+    // Two workgroups to a CU, or one where its waves have enough bytes under way:
+    // rows of 512 bytes (24 x 2 heads up to 8000 50.7 us, two 56.1), or of 256 and
+    // long shares (1 x 8 up to 130001 97.9, two 100.8; 40 x 2 of int8 up to 9001,
+    // short ones, 56.3, two 48.5). Rows of 128 bytes take two (16 x 8 of int8 up to
+    // 30000 102.3, one 124.7).
+    // Shares that may go on into the next tile pay where they are long (64 x 8 up to
+    // 16384 360 us, ending with a tile 415; 24 x 8 up to 6000 71, 92; 40 x 8 of 64 up
+    // to 3000, short, 34.0, 31.2). 256 wide the registers do not suffice for them.
+    uint64_t slots = 512u;
+    const uint64_t share = wgs * units / slots, row = kv.dim * (kv.type == EFF_KV_F16 ? 2u : 1u);
+    if (row >= 512u || (row >= 256u && share >= 12u)) slots = 256u;
+    p.on = kv.dim < 256u && share >= 16u;
+    p.items = (uint32_t)std::max<uint64_t>(slots / kv.heads, p.on ? 1u : 2u * p.tiles);
+    const uint64_t most_wgs = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;   // whose weights fit in the join's LDS
+    p.least = (uint32_t)std::max<uint64_t>(units / (most_wgs - 2u) + 1u, 2u);
+  }
   // 8 waves where a CU has one workgroup and the steps to share (the drafts above:
   // 15.8 us, 4 waves 17.8; 1024 workgroups of 300 tokens 30, 4 waves 21)
-  p.waves = p.chunks == 1u && wgs <= 256u && span >= 512u && kv.dim < 256u ? 8u : 4u;
+  p.waves = !p.items && wgs <= 256u && span >= 512u && kv.dim < 256u ? 8u : 4u;
   return p;
 }
 
 size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a) {
   const AttnPlan p = attn_plan(kv, b, a);
-  return p.chunks > 1u ? kAttnCounters * 4u + (uint64_t)p.tiles * kv.heads * attn_part_floats(p, kv.dim) * 4u : 0u;
+  return p.items ? kAttnCounters * 4u + (uint64_t)p.items * kv.heads * 2u * attn_part_floats(p, kv.dim) * 4u : 0u;
 }
 
 template <int TYPE, int D>
@@ -996,17 +1187,16 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.tiles) return e;
   }
-  const uint64_t grid = (uint64_t)p.tiles * p.chunks * kv.heads;
-  if (grid > 0x7FFFFFFFull || (p.chunks > 1u && !scratch)) return hipErrorInvalidValue;
+  const uint64_t grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
+  if (grid > 0x7FFFFFFFull || (p.items && (grid > kAttnCounters || !scratch))) return hipErrorInvalidValue;
   uint32_t *cnt = (uint32_t *)scratch;
   float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
-  if constexpr (D < 256) {
-    if (p.waves == 8u) {
-      hipLaunchKernelGGL((k_attn<TYPE, D, 8>), dim3((uint32_t)grid), dim3(512), 0, s, kv, b, a, p, cnt, part);
-      return hipGetLastError();
-    }
-  }
-  hipLaunchKernelGGL((k_attn<TYPE, D, 4>), dim3((uint32_t)grid), dim3(256), 0, s, kv, b, a, p, cnt, part);
+  const auto go = [&](auto kernel, uint32_t threads) { hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part); };
+  constexpr int E = D < 256 ? D : 64;   // no kernels of 256 for the two forms that it has not
+  if (p.on) go(k_attn<TYPE, E, 4, kAttnOn>, 256u);
+  else if (p.items) go(k_attn<TYPE, D, 4, kAttnEnds>, 256u);
+  else if (p.waves == 8u) go(k_attn<TYPE, E, 8, kAttnWhole>, 512u);
+  else go(k_attn<TYPE, D, 4, kAttnWhole>, 256u);
   return hipGetLastError();
 }
 

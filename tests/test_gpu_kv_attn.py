@@ -122,6 +122,35 @@ def test_window(ctx, eff, t, window, new, lens):
     run(eff, ctx, window, t, 2, 4, 64, 16, new, lens, window)
 
 
+@pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("dim,group,new,window", [(64, 4, 1, 0), (96, 3, 6, 0), (128, 8, 5, 0), (64, 1, 3, 150), (256, 2, 1, 0)])
+def test_uneven_lengths(ctx, eff, t, dim, group, new, window):
+    """More sequences than a wave has lanes, nearly all short beside the longest: workgroups go on from tile to tile."""
+    rng = np.random.default_rng(dim + new)
+    lens = [2300] + [int(n) for n in rng.integers(0, 400, 75)]
+    lens[40], lens[63], lens[64] = 1500, 128, 129
+    run(eff, ctx, group, t, 8, group, dim, 16, [min(new, n) for n in lens], lens, window)
+
+
+def test_long_shares(ctx, eff):
+    """Sequences that take several workgroups each, which begin and end within tiles."""
+    rng = np.random.default_rng(1)
+    lens = [2300, 129] + [int(n) for n in rng.integers(300, 1300, 22)]
+    run(eff, ctx, 1, F16, 32, 2, 64, 64, [1] * 24, lens)
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("lens", [[1], [700], [20, 5, 300]])
+def test_length_bound(ctx, eff, t, lens):
+    """The bound of the lengths far above them, as a recording has it."""
+    rng = np.random.default_rng(3)
+    b = Batch(rng, [1] * len(lens), lens, 16, table_pages=4096)
+    data, values = make(rng, t, 2, 128, b, np.nan)
+    q = rng.standard_normal((b.tokens, 8, 128)).astype(np.float32)
+    got = launch(eff, ctx, t, 2, 128, b, data, q, 8, 128 ** -0.5, max_len=65536)
+    check(got, attend(values, b.table, b.starts, b.lens, q, 8, 128 ** -0.5, 0, 16), values)
+
+
 def test_mixed_batch(ctx, eff):
     """A prompt among decoding requests, one with no new token, one without a token at all; bounds above the sizes."""
     new, lens = [1, 1, 90, 0, 1, 0, 1, 3], [40, 1, 200, 77, 513, 0, 16, 3]
