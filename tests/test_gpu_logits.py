@@ -72,6 +72,23 @@ def inputs(rng, rows, vocab, history=50, bias=0, masks=0):
     return z, h, pen, b, m, mo
 
 
+def test_quotients_between_two_numbers(ctx, eff):
+    """Repeats for which a logit over the repeat lies next to the middle of two f32 numbers, and the smallest quotients."""
+    rng = np.random.default_rng(5)
+    rows = 4000
+    z = np.exp(rng.uniform(-3, 3, (rows, 4))).astype(np.float32)
+    low = rng.uniform(0.3, 30, rows).astype(np.float32)
+    middle = (low.astype(np.float64) + np.nextafter(low, np.float32(np.inf)).astype(np.float64)) / 2
+    repeat = z[:, 0].astype(np.float64) / middle
+    for step in range(-3, 4):
+        at = np.arange(rows) % 7 == step + 3
+        repeat[at] += step * np.spacing(repeat[at])
+    z[:, 1] *= np.float32(1e-38)
+    z[:, 2] *= -1
+    run(eff, ctx, z, history=[[0, 1, 2, 3]] * rows, penalties=[[x, 0, 0] for x in repeat])
+    run(eff, ctx, z, history=[[0, 1, 2, 3, 3]] * rows, penalties=[[x, 0.25, 0.5] for x in 10.0 ** rng.uniform(-120, 120, rows)])
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 31), (2, 33), (3, 1000), (5, 4096), (2, 4097), (4, 50021), (1, 200003), (70, 300)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_rules(ctx, eff, rows, vocab, in_place):
