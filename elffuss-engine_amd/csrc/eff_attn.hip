@@ -1131,17 +1131,21 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group;
   const uint64_t rows = (uint64_t)b.tokens * group;
   p.max_rows = ~0u;
-  // Sequences with more than 64 rows go to k_attn_rows where their tiles fill half
-  // of the CUs without chunks
-  if (most > kFewRows && rows / 64u * kv.heads >= 128u) {
+  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
+  // Sequences with more than 64 rows go to k_attn_rows where there are enough tiles of
+  // that (1 x 8 heads of 128 over 4000 tokens: 300 rows of new tokens 109 us, k_attn
+  // 106, 400 108 and 133; its int8 pages cost a conversion more for the same tile:
+  // 600 175 and 169, 700 175 and 196). The others go with them where lengths and
+  // new tokens are alike, since a second launch waits for the first (32 x 8, up to
+  // 24 new tokens: 73 us, two launches 97) and a long one's tile is not shared.
+  if (most > kFewRows && rows / 64u * kv.heads >= (kv.type == EFF_KV_F16 ? 176u : 400u)) {
     attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
+    if (b.seqs == 1u || (most * b.seqs <= 3u * rows && seen <= 4096u)) return p;
     p.max_rows = kFewRows;
     most = kFewRows;
-    if (b.seqs == 1u) return p;
   }
   attn_tiles(most, rows, b.seqs, R, &p.tiles, &p.per_seq);
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
-  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
   // Where the tiles alone fill half of the CUs and are short, or there are many, a
   // workgroup has a tile: a join takes 5 us (24 x 8 heads of drafts that see 1024
@@ -1181,7 +1185,7 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   const AttnPlan p = attn_plan(kv, b, a);
   if (p.many_tiles) {
     const uint64_t g = (uint64_t)p.many_tiles * kv.heads;
-    const uint32_t min_rows = b.seqs == 1u ? 1u : kFewRows + 1u;
+    const uint32_t min_rows = p.tiles ? kFewRows + 1u : 1u;
     if (g > 0x7FFFFFFFull) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_attn_rows<TYPE, D>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
     const hipError_t e = hipGetLastError();

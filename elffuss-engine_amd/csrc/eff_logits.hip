@@ -17,12 +17,13 @@
 
 namespace eff {
 
+constexpr uint32_t kThreads = 1024, kItems = 2;   // of a workgroup; groups of 4 logits of a thread
+
 // Rows start wherever the stride puts them: 4-byte aligned.
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // The ids from `a` to `e` of a list, 4 of a thread under way at a time: the first are
 // requested by start(). f(i, id); past the end the id is ~0, past every vocabulary.
-template <uint32_t THREADS>
 struct Ids {
   static constexpr uint32_t U = 4;
   const uint32_t *list;
@@ -30,7 +31,7 @@ struct Ids {
 
   __device__ __forceinline__ void load(uint32_t *o, uint32_t i) const {
 #pragma unroll
-    for (uint32_t k = 0; k < U; ++k) o[k] = i + THREADS * k < e ? list[i + THREADS * k] : ~0u;
+    for (uint32_t k = 0; k < U; ++k) o[k] = i + kThreads * k < e ? list[i + kThreads * k] : ~0u;
   }
   __device__ __forceinline__ void start(const uint32_t *from, uint32_t first, uint32_t end) {
     list = from, a = first, e = end;
@@ -39,29 +40,27 @@ struct Ids {
   template <typename F>
   __device__ __forceinline__ void each(F f) {
     uint32_t i = a + threadIdx.x;
-    for (uint32_t at = a; at < e; at += THREADS * U, i += THREADS * U) {
+    for (uint32_t at = a; at < e; at += kThreads * U, i += kThreads * U) {
       uint32_t next[U];
-      load(next, i + THREADS * U);
+      load(next, i + kThreads * U);
 #pragma unroll
-      for (uint32_t k = 0; k < U; ++k) f(i + THREADS * k, id[k]), id[k] = next[k];
+      for (uint32_t k = 0; k < U; ++k) f(i + kThreads * k, id[k]), id[k] = next[k];
     }
   }
 };
 
-// ITEMS: groups of 4 logits of a thread.
-template <uint32_t THREADS, uint32_t ITEMS>
-__global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles) {
+__global__ __launch_bounds__(kThreads) void k_logits(LogitsArgs a, uint32_t tiles) {
 #pragma clang fp contract(off)
-  constexpr uint32_t T = 4u * THREADS * ITEMS;
+  constexpr uint32_t T = 4u * kThreads * kItems;
   __shared__ __align__(16) float z[T];
   __shared__ __align__(16) uint32_t count[T];
   const uint32_t row = blockIdx.x / tiles, v0 = (blockIdx.x % tiles) * T, n = min(T, a.vocab - v0), tid = threadIdx.x;
   const float *in = a.in + (uint64_t)row * a.stride + v0;
   float *out = a.out + (uint64_t)row * a.stride + v0;
-  float4u x[ITEMS];
+  float4u x[kItems];
 #pragma unroll
-  for (uint32_t k = 0; k < ITEMS; ++k) {
-    const uint32_t v = 4u * (THREADS * k + tid);
+  for (uint32_t k = 0; k < kItems; ++k) {
+    const uint32_t v = 4u * (kThreads * k + tid);
     if (v + 4u <= n) x[k] = *(const float4u *)(in + v);
   }
   // where the row's lists and mask begin, asked for together
@@ -70,25 +69,25 @@ __global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles
   if (a.bias_ids) b0 = a.bias_starts[row], b1 = min(a.bias_starts[row + 1], a.bias_count);
   if (a.mask) m = a.mask_of[row];
   const bool touched = a.history || a.bias_ids;
-  Ids<THREADS> h;
+  Ids h;
   h.start(a.history, h0, h1);
   // the thread's first bias; the rest of a long list is read when it is needed
   uint32_t bias_id = ~0u;
   float bias = 0.f;
   if (b0 + tid < b1) bias_id = a.bias_ids[b0 + tid], bias = a.bias_values[b0 + tid];
   const bool masked = m < a.mask_count;
-  uint32_t bits[ITEMS];
+  uint32_t bits[kItems];
   if (masked) {
     const uint32_t *words = a.mask + (uint64_t)m * ((a.vocab + 31u) / 32u);
 #pragma unroll
-    for (uint32_t k = 0; k < ITEMS; ++k) {
-      const uint32_t v = v0 + 4u * (THREADS * k + tid);   // 4 logits lie in one word: v0 and v are multiples of 4
+    for (uint32_t k = 0; k < kItems; ++k) {
+      const uint32_t v = v0 + 4u * (kThreads * k + tid);   // 4 logits lie in one word: v0 and v are multiples of 4
       bits[k] = words[min(v, a.vocab - 1u) >> 5] >> (v & 31u);
     }
   }
   if (touched) {
 #pragma unroll
-    for (uint32_t k = 0; k < ITEMS; ++k) *(u32x4 *)(count + 4u * (THREADS * k + tid)) = u32x4{0u, 0u, 0u, 0u};
+    for (uint32_t k = 0; k < kItems; ++k) *(u32x4 *)(count + 4u * (kThreads * k + tid)) = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
   }
   if (a.history)
@@ -96,8 +95,8 @@ __global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles
       if (id - v0 < n) atomicAdd(&count[id - v0], 1u);
     });
 #pragma unroll
-  for (uint32_t k = 0; k < ITEMS; ++k) {
-    const uint32_t v = 4u * (THREADS * k + tid);
+  for (uint32_t k = 0; k < kItems; ++k) {
+    const uint32_t v = 4u * (kThreads * k + tid);
     if (v + 4u <= n) {
       *(float4u *)(z + v) = x[k];
     } else {
@@ -117,7 +116,7 @@ __global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles
       inverse = fma(fma(-repeat, inverse, 1.0), inverse, inverse);
       inverse = fma(fma(-repeat, inverse, 1.0), inverse, inverse);
 #pragma unroll 1
-      for (uint32_t v = tid; v < n; v += THREADS) {
+      for (uint32_t v = tid; v < n; v += kThreads) {
         const uint32_t c = count[v];
         if (c == 0u) continue;
         if (a.bias_ids) count[v] = 0u;
@@ -135,13 +134,13 @@ __global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles
     if (a.bias_ids) {
       // of several pairs of one id the last counts: the largest place in the list
       if (bias_id - v0 < n) atomicMax(&count[bias_id - v0], b0 + tid + 1u);
-      for (uint32_t i = b0 + THREADS + tid; i < b1; i += THREADS) {
+      for (uint32_t i = b0 + kThreads + tid; i < b1; i += kThreads) {
         const uint32_t at = a.bias_ids[i] - v0;
         if (at < n) atomicMax(&count[at], i + 1u);
       }
       __syncthreads();
       if (bias_id - v0 < n && count[bias_id - v0] == b0 + tid + 1u) z[bias_id - v0] += bias;
-      for (uint32_t i = b0 + THREADS + tid; i < b1; i += THREADS) {
+      for (uint32_t i = b0 + kThreads + tid; i < b1; i += kThreads) {
         const uint32_t at = a.bias_ids[i] - v0;
         if (at < n && count[at] == i + 1u) z[at] += a.bias_values[i];
       }
@@ -149,8 +148,8 @@ __global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles
     }
   }
 #pragma unroll
-  for (uint32_t k = 0; k < ITEMS; ++k) {
-    const uint32_t v = 4u * (THREADS * k + tid);
+  for (uint32_t k = 0; k < kItems; ++k) {
+    const uint32_t v = 4u * (kThreads * k + tid);
     if (v >= n) break;
     float4u y = *(const float4u *)(z + v);
     if (masked) {
@@ -166,11 +165,12 @@ __global__ __launch_bounds__(THREADS) void k_logits(LogitsArgs a, uint32_t tiles
 }
 
 hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream) {
-  // tiles of 8192 logits where they give every CU a workgroup, else of 2048
-  const uint32_t t4 = (a.vocab + 8191u) / 8192u, t1 = (a.vocab + 2047u) / 2048u;
-  const bool big = (uint64_t)a.rows * t4 >= 256u;
-  if (big) hipLaunchKernelGGL((k_logits<1024, 2>), dim3(t4 * a.rows), dim3(1024), 0, stream, a, t4);
-  else hipLaunchKernelGGL((k_logits<512, 1>), dim3(t1 * a.rows), dim3(512), 0, stream, a, t1);
+  // Tiles of 8192 logits: two workgroups fill a CU, and a history is read once for each
+  // (48 x 50021, histories of 16000: 11.9 us, tiles of 2048 14.1; a single row of 131072
+  // 5.9 and 6.0).
+  constexpr uint32_t T = 4u * kThreads * kItems;
+  const uint32_t tiles = (a.vocab + T - 1u) / T;
+  hipLaunchKernelGGL(k_logits, dim3(tiles * a.rows), dim3(kThreads), 0, stream, a, tiles);
   return hipGetLastError();
 }
 
