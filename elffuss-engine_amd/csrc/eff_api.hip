@@ -89,7 +89,7 @@ struct eff_ctx {
   int64_t sx_min_tokens = 0;        // 0: the measured default (sx_routes)
   void *act_scratch = nullptr;      // x in the CPU path's 8-bit blocks (eff_qmatmul_cpu_path)
   size_t act_scratch_bytes = 0;
-  void *attn_scratch = nullptr;     // counters and sums of eff_kv_attn's chunks
+  void *attn_scratch = nullptr;     // counters and sums of eff_kv_attn's shared tiles
   size_t attn_scratch_bytes = 0;
   // Pinned staging ring of eff_buf_write: the source bytes are copied here on
   // the calling thread and the device copy is enqueued from here, so a write
@@ -1651,7 +1651,7 @@ int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *bat
   if ((uint64_t)b.tokens * q_heads > 0x7FFFFFFFull)
     return fail(ctx, EFF_E_SHAPE, "kv attn: %u tokens of %u heads", b.tokens, q_heads);
   if ((rc = use_device(ctx))) return rc;
-  // the joined chunks' scratch: its counters are zeroed when it is made
+  // the scratch of shared tiles: its counters are zeroed when it is made
   const size_t need = kv_attn_scratch(kv, b, a), before = ctx->attn_scratch_bytes;
   if ((rc = grow(ctx, &ctx->attn_scratch, &ctx->attn_scratch_bytes, need, "attention"))) return rc;
   if (ctx->attn_scratch_bytes != before)

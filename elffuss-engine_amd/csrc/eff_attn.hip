@@ -1183,16 +1183,15 @@ size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs 
 template <int TYPE, int D>
 static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t s) {
   const AttnPlan p = attn_plan(kv, b, a);
-  if (p.many_tiles) {
-    const uint64_t g = (uint64_t)p.many_tiles * kv.heads;
+  const uint64_t many = (uint64_t)p.many_tiles * kv.heads, grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
+  if (!fits(many, 256u) || !fits(grid, 512u)) return hipErrorInvalidConfiguration;
+  if (p.items && (grid > kAttnCounters || !scratch)) return hipErrorInvalidValue;
+  if (many) {
     const uint32_t min_rows = p.tiles ? kFewRows + 1u : 1u;
-    if (g > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_rows<TYPE, D>), dim3((uint32_t)g), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
+    hipLaunchKernelGGL((k_attn_rows<TYPE, D>), dim3((uint32_t)many), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.tiles) return e;
   }
-  const uint64_t grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
-  if (grid > 0x7FFFFFFFull || (p.items && (grid > kAttnCounters || !scratch))) return hipErrorInvalidValue;
   uint32_t *cnt = (uint32_t *)scratch;
   float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
   const auto go = [&](auto kernel, uint32_t threads) { hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part); };

@@ -24,6 +24,9 @@ constexpr uint32_t kv_block_bytes(int type, uint32_t dim, uint32_t page) {
   return page * (type == EFF_KV_F16 ? 2u * dim : dim + 4u);
 }
 
+// A grid's threads are counted in 32 bits.
+inline bool fits(uint64_t wgs, uint32_t threads) { return wgs * threads <= 0xFFFFFFFFull; }
+
 struct KvView {
   uint8_t *base;
   int type;
@@ -68,8 +71,8 @@ struct RopeFreqs {
 hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positions, float scale, float *out,
                              hipStream_t stream);
 hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t stream);
-// The scratch of the joined chunks (0: none): counters, zero before the first
-// launch and left zero by each, then the chunks' sums.
+// The scratch of tiles that several workgroups share (0: none): counters, zero before
+// the first launch and left zero by each, then the workgroups' sums.
 constexpr uint32_t kAttnCounters = 65536;
 size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a);
 hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch,

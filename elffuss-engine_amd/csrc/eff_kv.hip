@@ -6,7 +6,7 @@
 //   rotation  the pair (a, b) at position p and frequency i becomes
 //             (a cos - b sin, a sin + b cos), cos and sin from the table  (the first rope_dim values)
 // k and v rows are then stored as fp16 (round to nearest even), or as int8:
-//   scale = max|x| / 127,  n = round(x * (127 / max|x|)).
+//   scale = max|x| / 127,  n = round(x * (127 / max|x|)), 0 where max|x| < 2^-119.
 // Every operation is a separate f32 rounding (no contraction).
 #include "eff_device.h"
 #include "eff_kv.h"
@@ -162,7 +162,8 @@ __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvA
       for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(y[i]) & 0x7FFFFFFFu);
       const float m = __uint_as_float(group_max<L>(top));
       if (!on || !store) continue;
-      const float inv = m > 0.f ? 127.f / m : 0.f;
+      // the smallest rows' 127 / m would pass the largest number: they become zeros
+      const float inv = m >= 0x1p-119f ? 127.f / m : 0.f;
       int8_t *o = (int8_t *)blk + slot * D;
       uint32_t q[4];
 #pragma unroll
@@ -180,24 +181,26 @@ __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvA
 hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positions, float scale, float *out,
                              hipStream_t stream) {
   const uint64_t n = (uint64_t)pairs * positions;
+  if (!fits((n + 255u) / 256u, 256u)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(k_rope_table, dim3((uint32_t)((n + 255u) / 256u)), dim3(256), 0, stream, f, pairs, positions,
                      scale, out);
   return hipGetLastError();
 }
 
 template <int TYPE, int D, int U>
-static void append_launch(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
+static hipError_t append_launch(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
   constexpr uint32_t rows = (D == 96 ? 8u : 1024u / D) * U;   // of a workgroup
   const uint32_t q = (a.q_heads + rows - 1u) / rows, k = (kv.heads + rows - 1u) / rows;
+  if (!fits((uint64_t)b.tokens * (q + 2u * k), 256u)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((k_kv_append<TYPE, D, U>), dim3(b.tokens * (q + 2u * k)), dim3(256), 0, s, kv, b, a, q, k);
+  return hipGetLastError();
 }
 
 template <int TYPE, int D>
 static hipError_t append_dim(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
   // 4 rows a thread where a CU still has 8 workgroups to take
-  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= 2048ull * 4096u) append_launch<TYPE, D, 4>(kv, b, a, s);
-  else append_launch<TYPE, D, 1>(kv, b, a, s);
-  return hipGetLastError();
+  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= 2048ull * 4096u) return append_launch<TYPE, D, 4>(kv, b, a, s);
+  return append_launch<TYPE, D, 1>(kv, b, a, s);
 }
 
 template <int TYPE>

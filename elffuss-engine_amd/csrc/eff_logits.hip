@@ -170,6 +170,7 @@ hipError_t launch_logits(const LogitsArgs &a, hipStream_t stream) {
   // 5.9 and 6.0).
   constexpr uint32_t T = 4u * kThreads * kItems;
   const uint32_t tiles = (a.vocab + T - 1u) / T;
+  if (!fits((uint64_t)tiles * a.rows, kThreads)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(k_logits, dim3(tiles * a.rows), dim3(kThreads), 0, stream, a, tiles);
   return hipGetLastError();
 }

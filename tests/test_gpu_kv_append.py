@@ -162,6 +162,19 @@ def test_rows_of_zeros(ctx, eff):
     run(eff, ctx, 5, I8, 2, 2, 128, 16, [4], [9], 128, norm=True, edit=edit)
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e-35, 3e-36, 1e-36, 1e-38, 1e-42])
+def test_smallest_int8_rows(ctx, eff, size):
+    """Rows whose largest value is next to the smallest numbers: rounded, or zeros below 2^-119; zeros stay zeros."""
+    def edit(rows):
+        rows[2][:] = np.linspace(-size, size, 64, dtype=np.float32)[None]
+        rows[2][:, 7] = 0
+    b, rows, _, got, _ = run(eff, ctx, 8, I8, 1, 1, 64, 16, [2], [2], 0, edit=edit, place=False)
+    v = decode(I8, got, b.pages, 1, 64, 16)[b.table[0, 0], 1, 0, :2]
+    assert (v[:, 7] == 0).all()
+    step = np.float64(size) / 254 + 2.0 ** -149 * 127 if size > 2.0 ** -119 else size * 1.01
+    assert (np.abs(v - rows[2]) <= step * (1 + 2.0 ** -20)).all()
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 def test_rows_that_are_not_finite(ctx, eff, bad):
     """In int8 the whole row is not finite; in fp16 the value is; other rows are as ever."""
