@@ -1148,11 +1148,13 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
   // Where the tiles alone fill half of the CUs and are short, or there are many, a
-  // workgroup has a tile: a join takes 5 us (24 x 8 heads of drafts that see 1024
+  // workgroup has a tile, as where there are 5 units or fewer (4 at 256 wide): a join
+  // takes time (1 x 8 heads of 64 over 517 tokens: 7.3 us, shared 8.2, over 1000 9.6
+  // and 8.7; 24 x 8 heads of drafts that see 1024
   // tokens: 15.8 us, shared 22.5; 32 x 8 heads of one token up to 2000 36.8, shared
   // 45.8).
   const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
-  if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > 2u && each * b.seqs * units < 1u << 31) {
+  if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
     // Two workgroups to a CU, or one where its waves have enough bytes under way:
     // rows of 512 bytes (24 x 2 heads up to 8000 50.7 us, two 56.1), or of 256 and
     // long shares (1 x 8 up to 130001 97.9, two 100.8; 40 x 2 of int8 up to 9001,
@@ -1170,8 +1172,9 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
     p.least = (uint32_t)std::max<uint64_t>(units / (most_wgs - 2u) + 1u, 2u);
   }
   // 8 waves where a CU has one workgroup and the steps to share (the drafts above:
-  // 15.8 us, 4 waves 17.8; 1024 workgroups of 300 tokens 30, 4 waves 21)
-  p.waves = !p.items && wgs <= 256u && span >= 512u && kv.dim < 256u ? 8u : 4u;
+  // 15.8 us, 4 waves 17.8; 1024 workgroups of 300 tokens 30, 4 waves 21; 128 of up to
+  // 2000 of int8, 256 wide 35.8, 4 waves 41.4; fp16 of that width 47.6 and 45.6)
+  p.waves = !p.items && wgs <= 256u && span >= 512u && (kv.dim < 256u || kv.type == EFF_KV_I8) ? 8u : 4u;
   return p;
 }
 
@@ -1195,10 +1198,10 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   uint32_t *cnt = (uint32_t *)scratch;
   float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
   const auto go = [&](auto kernel, uint32_t threads) { hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part); };
-  constexpr int E = D < 256 ? D : 64;   // no kernels of 256 for the two forms that it has not
+  constexpr int E = D < 256 ? D : 64;   // 256 wide there is no such kernel
   if (p.on) go(k_attn<TYPE, E, 4, kAttnOn>, 256u);
   else if (p.items) go(k_attn<TYPE, D, 4, kAttnEnds>, 256u);
-  else if (p.waves == 8u) go(k_attn<TYPE, E, 8, kAttnWhole>, 512u);
+  else if (p.waves == 8u) go(k_attn<TYPE, TYPE == EFF_KV_I8 ? D : E, 8, kAttnWhole>, 512u);
   else go(k_attn<TYPE, D, 4, kAttnWhole>, 256u);
   return hipGetLastError();
 }
