@@ -350,7 +350,8 @@ struct AttnWalk {
   }
 };
 
-// One wave's share of a tile of 16 rows.
+// One wave's share of a tile of 16 rows: 16, because that is the matrix instruction's
+// side, and a group of query heads seldom has more.
 //   SCALED  rows of the cache have scales
 //   I8      K and V arrive as int8 (else fp16, also where int8 was converted on the way)
 //   QL      the parts of q are in LDS, shared by the waves of the tile, and read for
@@ -562,7 +563,9 @@ struct AttnWave {
           for (int i = 0; i < (VIN == kVLater ? E : VN * VM / 4); ++i) {
             u32x4 o;
             if constexpr (VIN == kVLater) o = v(i) & keep;
-            else o = u32x4{vw[4 * i / VM][4 * i % VM], vw[(4 * i + 1) / VM][(4 * i + 1) % VM], vw[(4 * i + 2) / VM][(4 * i + 2) % VM], vw[(4 * i + 3) / VM][(4 * i + 3) % VM]};
+            else
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[x] = vw[(4 * i + x) / VM][(4 * i + x) % VM];
 #pragma unroll
             for (int x = 0; x < 4; ++x) top = max(top, max(o[x] & 0x7FFFu, o[x] >> 16 & 0x7FFFu));
             __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
@@ -728,11 +731,21 @@ __device__ __forceinline__ void from_lds(T &to, const T &from) {
   __builtin_memcpy(&to, w, sizeof(T));
 }
 
-// NW waves take the 32-token steps of a tile in turn; their sums meet in LDS. Where
-// a tile has several workgroups, the last of them to arrive joins their sums, in the
-// tokens' order; stores and loads of these go past the XCD's L2 (sc1), every wave
-// waits for its stores before the barrier ahead of the counter's increment, and the
-// counter is left at zero for the next launch.
+// Few rows: NW waves take the 32-token steps of a tile in turn; their sums meet in
+// LDS. Where a tile has several workgroups, the last of them to arrive joins their
+// sums, in the tokens' order, so that the bits do not depend on who was last; stores
+// and loads of these go past the XCD's L2 (sc1), every wave waits for its stores before
+// the barrier ahead of the counter's increment, and the counter is left at zero for the
+// next launch.
+//
+// The cache's bytes bound a batch: K and V go from memory to the registers that the
+// matrix unit reads, a step of V and the next step of K under way in each wave, 16 KB
+// of fp16 rows of 128, 64 KB a CU and more (64 sequences up to 16384 long, 32 heads of
+// 128 on 8: 360 us, 5.9 TB/s; one of 130001: 97 us, 5.5 TB/s). The matrix unit is busy
+// 8 % of the time there, so the second parts of q and p are free. int8 rows are half
+// the bytes with as many instructions, which shows where the shares are short (40 up
+// to 9001, 16 heads of 256 on 2: 48 us, 3.4 TB/s). A single short sequence is round
+// trips: lengths, page table, K, V, the join (517 tokens: 7.3 us, an empty launch 3.4).
 template <int TYPE, int D, int NW, int MODE>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
   constexpr bool I8 = TYPE == EFF_KV_I8, QL = D == 256;   // 256 wide, q's parts would take a quarter of the registers
@@ -913,6 +926,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
 // 16 rows of an operand lie in different banks; V's operand comes out of LDS turned
 // (ds_read_b64_tr_b16: of 16 lanes, lane 4 j + q reads 4 values of row j, and lane c
 // gets column c of the 4 rows).
+//
+// Instruction issue bounds it: per step of 32 tokens x 16 rows x 128 a wave has 64
+// matrix instructions of 16 cycles and as many cycles of the softmax's VALU, and three
+// waves a SIMD overlap them to 44 + 44 % of the busy time (3 x 1000 new tokens at lengths up to 3001, 32
+// heads of 128 on 8: 181 us, 440 TFLOP/s of the product itself, 880 with q's and p's
+// second parts, where a large fp16 product reaches 1090). Three buffers, two steps ahead, were
+// no faster (185 us): the loads are not waited for.
 template <int D>
 struct AttnStage {
   static constexpr uint32_t ROW = 2 * D, PIECES = ROW / 16u;
@@ -1150,9 +1170,8 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // Where the tiles alone fill half of the CUs and are short, or there are many, a
   // workgroup has a tile, as where there are 5 units or fewer (4 at 256 wide): a join
   // takes time (1 x 8 heads of 64 over 517 tokens: 7.3 us, shared 8.2, over 1000 9.6
-  // and 8.7; 24 x 8 heads of drafts that see 1024
-  // tokens: 15.8 us, shared 22.5; 32 x 8 heads of one token up to 2000 36.8, shared
-  // 45.8).
+  // and 8.7; 24 x 8 heads of drafts that see 1024 tokens 15.8, shared 22.5; 32 x 8
+  // heads of one token up to 2000 36.8, shared 45.8).
   const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
   if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
     // Two workgroups to a CU, or one where its waves have enough bytes under way:
@@ -1197,7 +1216,9 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   }
   uint32_t *cnt = (uint32_t *)scratch;
   float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
-  const auto go = [&](auto kernel, uint32_t threads) { hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part); };
+  const auto go = [&](auto kernel, uint32_t threads) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part);
+  };
   constexpr int E = D < 256 ? D : 64;   // 256 wide there is no such kernel
   if (p.on) go(k_attn<TYPE, E, 4, kAttnOn>, 256u);
   else if (p.items) go(k_attn<TYPE, D, 4, kAttnEnds>, 256u);

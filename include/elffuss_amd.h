@@ -559,7 +559,8 @@ int eff_rope_table(eff_ctx *ctx, const double *freqs, uint32_t n, uint32_t posit
 
 /* Norm (optional) and rotation of the new tokens' q and k, q to q_out, k and v
  * into the cache. An int8 row: scale = max|x| * (1 / 127), n = round(x * (127 /
- * max|x|)), ties to even; a row with a NaN or an infinity has no finite value. */
+ * max|x|)), ties to even, 0 where max|x| < 2^-119; a row with a NaN or an
+ * infinity has no finite value. */
 int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *rows);
 
 /* out [tokens][q_heads * head_dim] = attention of q (rows as in eff_kv_rows,
