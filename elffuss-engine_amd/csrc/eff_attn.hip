@@ -28,7 +28,6 @@
 namespace eff {
 
 typedef float float4v __attribute__((ext_vector_type(4)));
-typedef float float2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {

@@ -132,6 +132,17 @@ def test_uneven_lengths(ctx, eff, t, dim, group, new, window):
     run(eff, ctx, group, t, 8, group, dim, 16, [min(new, n) for n in lens], lens, window)
 
 
+@pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("group,new,window", [(1, 1, 0), (4, 1, 200), (3, 6, 0)])
+def test_whole_tiles(ctx, eff, t, dim, group, new, window):
+    """Enough short tiles for a workgroup each: of eight waves where they are few."""
+    rng = np.random.default_rng(dim + group)
+    lens = [900, 0, 1, 511, 512, 513] + [int(n) for n in rng.integers(1, 900, 11)]
+    run(eff, ctx, dim, t, 8, group, dim, 32, [min(new, n) for n in lens], lens, window)
+    run(eff, ctx, dim, t, 3, group, dim, 16, [new], [599], window)
+
+
 def test_long_shares(ctx, eff):
     """Sequences that take several workgroups each, which begin and end within tiles."""
     rng = np.random.default_rng(1)
@@ -214,6 +225,36 @@ def test_missing_pages(ctx, eff):
         got = launch(eff, ctx, t, 2, 64, b, data, q, 6, 0.2)
         check(got, attend(values, b.table, b.starts, b.lens, q, 6, 0.2, 0, 16), values)
         assert not got[4].any()
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("heads,group,new,lens,window", [
+    (8, 8, [500, 33], [1100, 200], 0), (4, 16, [450, 1, 300], [1500, 50, 300], 100), (16, 1, [1500, 700], [1500, 1222], 0),
+    (7, 3, [1301], [1301], 0)])
+def test_many_rows(ctx, eff, t, dim, heads, group, new, lens, window):
+    """Enough rows for the kernel of many rows, of int8 too; all sequences in one launch."""
+    run(eff, ctx, dim, t, heads, group, dim, 32, new, lens, window)
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+def test_many_rows_in_a_batch(ctx, eff, t):
+    """Prompts and decoding requests together, in two launches."""
+    new, lens = [1, 900, 0, 5, 1, 16, 17, 300, 1], [3000, 900, 10, 77, 0, 16, 2000, 5000, 1]
+    run(eff, ctx, 31, t, 8, 4, 64, 16, new, lens)
+    run(eff, ctx, 32, t, 8, 4, 128, 64, new, lens, 500, max_new=4000, max_len=5001)
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("bad", [np.nan, -np.inf])
+@pytest.mark.parametrize("where", [0, 1])
+def test_later_tokens_of_many_rows(ctx, eff, t, bad, where):
+    test_later_tokens_do_not_reach_earlier_rows(ctx, eff, t, bad, where, 1650, 16)
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+def test_what_many_rows_do_not_see(ctx, eff, t):
+    test_what_is_not_seen(ctx, eff, t, 1800)
 
 
 def test_more_new_tokens_than_length(ctx, eff):
