@@ -67,6 +67,23 @@ __device__ __forceinline__ void ld_words(uint32_t *o, const uint8_t *p) {
   }
 }
 
+// The same of the cache. An address made of two words may be LDS for all the compiler
+// knows: without its space named the loads would be counted with LDS's, and a wait for
+// one of them would wait for all that are under way.
+template <typename T>
+using cached = const __attribute__((address_space(1))) T *;
+template <int N>
+__device__ __forceinline__ void ld_cache(uint32_t *o, const uint8_t *p) {
+  typedef uint32_t words __attribute__((ext_vector_type(N == 1 ? 2 : N)));
+  if constexpr (N == 1) {
+    *o = *(cached<uint32_t>)p;
+  } else {
+    const words v = *(cached<words>)p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = v[i];
+  }
+}
+
 // A constant that the compiler does not see, so that it keeps the instruction
 // around it.
 __device__ __forceinline__ float unseen(float v) {
@@ -442,12 +459,12 @@ struct AttnWave {
   __device__ __forceinline__ void load_k(int u, const uint8_t *p, const uint8_t *scales, uint32_t n, uint32_t g) {
     if constexpr (!I8) {
 #pragma unroll
-      for (int c = 0; c < KS; ++c) ld_words<4>(kw[u] + 4 * c, p + (n * ROW + 16u * g) + 64u * c);
+      for (int c = 0; c < KS; ++c) ld_cache<4>(kw[u] + 4 * c, p + (n * ROW + 16u * g) + 64u * c);
     } else {
 #pragma unroll
-      for (int c = 0; c + 1 < KS; c += 2) ld_words<4>(kw[u] + 2 * c, p + (n * ROW + 16u * g) + 32u * c);
-      if constexpr (KS & 1) ld_words<2>(kw[u] + 2 * (KS - 1), p + (n * ROW + 8u * g) + 32u * (KS - 1));
-      ld_words<4>(ks[u], scales + 16u * g);
+      for (int c = 0; c + 1 < KS; c += 2) ld_cache<4>(kw[u] + 2 * c, p + (n * ROW + 16u * g) + 32u * c);
+      if constexpr (KS & 1) ld_cache<2>(kw[u] + 2 * (KS - 1), p + (n * ROW + 8u * g) + 32u * (KS - 1));
+      ld_cache<4>(ks[u], scales + 16u * g);
     }
   }
 
@@ -458,19 +475,19 @@ struct AttnWave {
       const uint8_t *r = p + 4u * g * ROW + j * ROW;
       uint32_t *o = vw[4 * u + j];
       if constexpr (D == 96 && I8) {
-        o[0] = *(const uint32_t *)(r + 4u * n);
-        o[1] = *(const uint16_t *)(r + 64 + 2u * n);
+        o[0] = *(cached<uint32_t>)(r + 4u * n);
+        o[1] = *(cached<uint16_t>)(r + 64 + 2u * n);
       } else if constexpr (D == 96) {
-        ld_words<2>(o, r + 8u * n);
-        o[2] = *(const uint32_t *)(r + 128 + 4u * n);
+        ld_cache<2>(o, r + 8u * n);
+        o[2] = *(cached<uint32_t>)(r + 128 + 4u * n);
       } else if constexpr (VW == 8) {
-        ld_words<4>(o, r + 32u * n);
-        ld_words<4>(o + 4, r + 32u * n + 16);
+        ld_cache<4>(o, r + 32u * n);
+        ld_cache<4>(o + 4, r + 32u * n + 16);
       } else {
-        ld_words<VW>(o, r + 4u * VW * n);
+        ld_cache<VW>(o, r + 4u * VW * n);
       }
     }
-    if constexpr (I8) ld_words<4>(vs[u], scales + 16u * g);
+    if constexpr (I8) ld_cache<4>(vs[u], scales + 16u * g);
   }
 
   // Column i of the 8 tokens of the lane as the first operand.
@@ -1057,7 +1074,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
       }
       if (wave == 3u) {   // the scales: K's of the 32 tokens, then V's
         const uint8_t *p = lane & 16u ? k.scales(1, kv, D) : k.scales(0, kv, D);
-        raw_scale = *(const uint32_t *)(p + 4u * (lane & 15u) + (lane < 32u ? 0u : to_v));
+        raw_scale = *(cached<uint32_t>)(p + 4u * (lane & 15u) + (lane < 32u ? 0u : to_v));
       }
     } else {
 #pragma unroll
