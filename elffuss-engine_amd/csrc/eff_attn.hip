@@ -527,6 +527,9 @@ struct AttnWave {
   // so that a matrix step does not wait for the one before it.
   __device__ __forceinline__ void scores(float s[2][4]) const {
     float4v c[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    uint32_t nothing = 0;
+    if constexpr (QL) __asm__ volatile("" : "+v"(nothing));   // q is read here, not kept from step to step
+    const uint8_t *parts = qs + nothing;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       half8 a[2];
@@ -536,7 +539,7 @@ struct AttnWave {
         else a[u] = __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
       }
       half8 h, r;
-      if constexpr (QL) h = *(const half8 *)(qs + k * 2048), r = *(const half8 *)(qs + k * 2048 + 1024);
+      if constexpr (QL) h = *(const half8 *)(parts + k * 2048), r = *(const half8 *)(parts + k * 2048 + 1024);
       else h = qh[k], r = ql[k];
 #pragma unroll
       for (int u = 0; u < 2; ++u) c[u] = mfma(a[u], h, c[u]);
@@ -691,22 +694,33 @@ struct AttnWave {
     }
   }
 
-  // The steps of `k`, whose first keys are on their way (fetch_k).
+  // The steps of `k`, whose first keys are on their way (fetch_k). The last one is on
+  // its own: behind a branch that may or may not ask for the next keys, a wait for V
+  // would be one for whatever is under way.
   __device__ __forceinline__ void run(AttnWalk &k, const KvView &kv, const AttnTile &t, int window, uint32_t n, uint32_t g) {
+    int t0 = k.lo, i = 0;
+    if (t0 >= k.hi) return;
+#pragma unroll 1
+    for (; t0 + k.stride < k.hi; t0 += k.stride, ++i) one<false>(k, kv, t, window, n, g, t0, i);
+    one<true>(k, kv, t, window, n, g, t0, i);
+  }
+
+  template <bool LAST>
+  __device__ __forceinline__ void one(AttnWalk &k, const KvView &kv, const AttnTile &t, int window, uint32_t n, uint32_t g, int t0, int i) {
     const uint32_t to_v = kv.heads * kv.block_bytes;
     const int full = t.first - 31, from = window ? t.last - window + 1 : 0;   // steps from .. full need no mask
-    int i = 0;
-#pragma unroll 1
-    for (int t0 = k.lo; t0 < k.hi; t0 += k.stride, ++i) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) load_v(u, k.at[u] + to_v, k.scales(u, kv, D) + to_v, n, g);
-      float s[2][4];
-      scores(s);
-      const bool gone[2] = {k.gone[0], k.gone[1]};
-      const bool masked = gone[0] || gone[1] || t0 > full || t0 < from;
-      if (t0 + k.stride < k.hi) fetch_k(k, kv, i + 1, n, g);
-      step(t0, masked, gone, t, window, g, s, [&](int c) { return v_operand(c); });
+    for (int u = 0; u < 2; ++u) load_v(u, k.at[u] + to_v, k.scales(u, kv, D) + to_v, n, g);
+    __builtin_amdgcn_sched_barrier(0);   // requested before the scores
+    float s[2][4];
+    scores(s);
+    const bool gone[2] = {k.gone[0], k.gone[1]};
+    const bool masked = gone[0] || gone[1] || t0 > full || t0 < from;
+    if constexpr (!LAST) {
+      fetch_k(k, kv, i + 1, n, g);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    step(t0, masked, gone, t, window, g, s, [&](int c) { return v_operand(c); });
   }
 
   __device__ __forceinline__ void fetch_k(AttnWalk &k, const KvView &kv, int i, uint32_t n, uint32_t g) {
