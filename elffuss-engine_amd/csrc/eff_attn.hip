@@ -1204,18 +1204,20 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // heads of one token up to 2000 36.8, shared 45.8).
   const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
   if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
-    // Two workgroups to a CU, or one where its waves have enough bytes under way:
-    // rows of 512 bytes (24 x 2 heads up to 8000 50.7 us, two 56.1), or of 256 and
-    // long shares (1 x 8 up to 130001 97.9, two 100.8; 40 x 2 of int8 up to 9001,
-    // short ones, 56.3, two 48.5). Rows of 128 bytes take two (16 x 8 of int8 up to
-    // 30000 102.3, one 124.7).
+    // Two workgroups to a CU, or one where its waves have enough bytes under way: 256
+    // wide (24 x 2 heads up to 8000 50.4 us, two 55.9; of int8 33.5 and 35.8), or fp16
+    // rows of 128 and long shares (1 x 8 up to 130001 96.7, two 99.4; 8 x 8 drafts up to
+    // 5000, short ones, 30.8 and 28.1). Less wide they take two (16 x 8 of int8 up to
+    // 30000 106, two 100).
     // Shares that may go on into the next tile pay where they are long (64 x 8 up to
-    // 16384 360 us, ending with a tile 415; 24 x 8 up to 6000 71, 92; 40 x 8 of 64 up
-    // to 3000, short, 34.0, 31.2). 256 wide the registers do not suffice for them.
+    // 16384 359 us, ending with a tile 411; 24 x 8 up to 6000 69, 94); 256 wide, where
+    // the scalar registers of that take vector ones, only with many tiles (100 x 2 of
+    // int8 up to 9000 112, 157; 24 x 2 up to 30000 77, 73).
     uint64_t slots = 512u;
-    const uint64_t share = wgs * units / slots, row = kv.dim * (kv.type == EFF_KV_F16 ? 2u : 1u);
-    if (row >= 512u || (row >= 256u && share >= 12u)) slots = 256u;
-    p.on = kv.dim < 256u && share >= 16u;
+    const uint64_t share = wgs * units / slots;
+    const bool wide = kv.dim >= 256u;
+    if (wide || (kv.dim == 128u && kv.type == EFF_KV_F16 && share >= 12u)) slots = 256u;
+    p.on = share >= 16u && (!wide || wgs * 4u > slots);
     p.items = (uint32_t)std::max<uint64_t>(slots / kv.heads, p.on ? 1u : 2u * p.tiles);
     const uint64_t most_wgs = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;   // whose weights fit in the join's LDS
     p.least = (uint32_t)std::max<uint64_t>(units / (most_wgs - 2u) + 1u, 2u);
@@ -1249,10 +1251,10 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   const auto go = [&](auto kernel, uint32_t threads) {
     hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part);
   };
-  constexpr int E = D < 256 ? D : 64;   // 256 wide there is no such kernel
-  if (p.on) go(k_attn<TYPE, E, 4, kAttnOn>, 256u);
+  constexpr int E = D < 256 || TYPE == EFF_KV_I8 ? D : 64;   // no fp16 tiles 256 wide of eight waves
+  if (p.on) go(k_attn<TYPE, D, 4, kAttnOn>, 256u);
   else if (p.items) go(k_attn<TYPE, D, 4, kAttnEnds>, 256u);
-  else if (p.waves == 8u) go(k_attn<TYPE, TYPE == EFF_KV_I8 ? D : E, 8, kAttnWhole>, 512u);
+  else if (p.waves == 8u) go(k_attn<TYPE, E, 8, kAttnWhole>, 512u);
   else go(k_attn<TYPE, D, 4, kAttnWhole>, 256u);
   return hipGetLastError();
 }
