@@ -121,7 +121,7 @@ __device__ __forceinline__ void split2(float a, float b, half2v &hi, half2v &lo)
   lo = half2v{(_Float16)fmaf((float)hi[0], m, a), (_Float16)fmaf((float)hi[1], m, b)};
 }
 
-constexpr uint32_t kShort = 8;    // units of a share
+constexpr uint32_t kLeast = 2, kShort = 8;   // units of a share
 constexpr uint32_t kUnit = 128;   // tokens: a step of each of four waves
 
 // The rows of a tile, their tokens and what they see.
@@ -207,14 +207,14 @@ __device__ __forceinline__ uint32_t attn_units(uint32_t len, uint32_t group, uin
   return max((span + kUnit - 1u) / kUnit, 1u);
 }
 
-// The share of workgroup `item` of `items`, `least` units at least: every one has the
+// The share of workgroup `item` of `items`, kLeast units at least: every one has the
 // same work, whatever the lengths are. Each wave adds the sequences up for itself, 64
 // at a time. A share that goes on into the next tile starts anew there, with its
 // loads' latency: short shares end with a tile instead (ENDS: all; there are more
 // items than tiles).
 template <uint32_t R, bool ENDS>
 __device__ __forceinline__ bool attn_share(const KvBatchView &b, uint32_t group, uint32_t window, uint32_t item, uint32_t items,
-                                           uint32_t least, uint32_t max_rows, AttnTile &t, AttnShare &c) {
+                                           uint32_t max_rows, AttnTile &t, AttnShare &c) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t s0 = 0, n = 0, len = 0, tiles = 0, of = 0;
   const auto load = [&](uint32_t at) {
@@ -234,7 +234,7 @@ __device__ __forceinline__ bool attn_share(const KvBatchView &b, uint32_t group,
     const uint32_t l = __builtin_amdgcn_readfirstlane(kv_len(b, 0)), m = to > from ? min(to - from, b.max_new) : 0u;
     const uint32_t units = attn_units<R>(l, group, window), many = (m * group + R - 1u) / R;
     if (m * group > max_rows || many >= items) return false;
-    c.each = max((many * units + items - many - 1u) / (items - many), least);
+    c.each = max((many * units + items - many - 1u) / (items - many), kLeast);
     c.of = (units + c.each - 1u) / c.each * c.each;
     c.sub = item * c.each / c.of;
     if (c.sub >= many) return false;
@@ -259,8 +259,8 @@ __device__ __forceinline__ bool attn_share(const KvBatchView &b, uint32_t group,
   count = __builtin_amdgcn_readfirstlane(count);
   uint32_t each = (total + items - 1u) / items, whole = 1;
   if (ENDS && count >= items) return false;
-  if (ENDS || (each < kShort && count < items)) whole = each = max((total + items - count - 1u) / (items - count), least);
-  each = max(each, least);
+  if (ENDS || (each < kShort && count < items)) whole = each = max((total + items - count - 1u) / (items - count), kLeast);
+  each = max(each, kLeast);
   c.each = __builtin_amdgcn_readfirstlane(each);
   whole = __builtin_amdgcn_readfirstlane(whole);
   const uint32_t first = item * c.each;
@@ -733,7 +733,6 @@ struct AttnWave {
 struct AttnPlan {
   uint32_t tiles, per_seq;    // row tiles; tiles of each sequence (0: packed)
   uint32_t items;             // workgroups of a head that share the cached tokens (0: one a tile)
-  uint32_t least;             // units of a share at least
   bool on;                    // a share may go on into the next tile
   uint32_t rows;              // rows of a tile at most
   uint32_t waves;             // of a workgroup
@@ -747,6 +746,10 @@ struct AttnPlan {
 __host__ __device__ constexpr uint32_t attn_part_floats(const AttnPlan &p, uint32_t dim) { return p.rows * (dim + 2u); }
 
 constexpr uint32_t kFewRows = 64;
+// Values that one join reads: of more than these it takes longer than the second round
+// trip of two (32 workgroups x 8 rows x 128: 16.3 us, in two 16.6; 128 x 8 x 256 46.5
+// and 25.8).
+constexpr uint32_t kJoin = 65536;
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
 enum { kAttnWhole, kAttnEnds, kAttnOn };   // a workgroup has a tile; a part of one; a share that may go on into the next
@@ -796,7 +799,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   AttnTile t;
   AttnShare c = {1u, 1u, 0u, 1u, 0u, 0u};
   if constexpr (shared) {
-    if (!attn_share<R, !on>(b, group, a.window, item, p.items, p.least, p.max_rows, t, c)) return;
+    if (!attn_share<R, !on>(b, group, a.window, item, p.items, p.max_rows, t, c)) return;
   } else {
     if (!attn_tile<R>(b, group, a.window, item, p.per_seq, 1u, p.max_rows, t)) return;
   }
@@ -877,68 +880,87 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
       }
     }
     if (shared && mine && chunks > 1u) {
-      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      uint32_t *counter = cnt + ((uint64_t)kvh * p.items + first);
-      if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      if (arrived == chunks - 1u) {
+      const auto place = [&](uint32_t z) { return 2u * (first + z) + (z == 0u ? 1u : 0u); };   // the slot of the tile's workgroup z
+      // one join, or where there is much to read, one of each group of about sqrt(chunks)
+      // workgroups, whose sums take its first one's slot, and one of the groups
+      const uint32_t side = chunks * p.rows * D <= kJoin ? chunks : __builtin_amdgcn_readfirstlane((uint32_t)ceilf(sqrtf((float)chunks)));
+      const uint32_t groups = (chunks + side - 1u) / side;
+      uint32_t z0 = (item - first) / side * side, step = 1u, count = min(side, chunks - z0);
+      for (bool last = groups == 1u;; last = true) {
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint32_t *counter = cnt + (step == 1u ? 0u : kAttnCounters / 2u) + (uint64_t)kvh * p.items * 2u + place(z0);
+        if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived != count - 1u) break;
         if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const auto place = [&](uint32_t z) { return (2u * (first + z) + (z == 0u ? 1u : 0u)) * slot_floats; };
         // the workgroups' weights relative to the largest maximum, [workgroup][row],
         // and the rows' sums: a wave per row, its lanes over the workgroups
         float *wt = &so[0][0][0], *half = wt + NW * R * LD - 4u * T;
         for (uint32_t r = wave; r < t.rows; r += NW) {
+          const auto maximum = [&](uint32_t z) { return (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u); };
           float mx = -INFINITY, l = 0.f;
-          for (uint32_t z = lane; z < chunks; z += 64u)
-            mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, (int)((place(z) + ml + 2u * r) * 4u), 0, kSc1)));
+          for (uint32_t z = lane; z < count; z += 64u)
+            mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, maximum(z), 0, kSc1)));
 #pragma unroll
           for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-          for (uint32_t z = lane; z < chunks; z += 64u) {
-            const int at = (int)((place(z) + ml + 2u * r) * 4u);
-            const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
-            const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
+          for (uint32_t z = lane; z < count; z += 64u) {
+            const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, maximum(z), 0, kSc1));
+            const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, maximum(z) + 4, 0, kSc1));
             const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
             wt[z * p.rows + r] = f;
             l += f * lz;
           }
           l = wave_sum(l);
-          if (lane == 0u) sl[0][r] = l;
+          if (lane == 0u) sl[0][r] = l, sm[0][r] = mx;
         }
         __syncthreads();
         // each thread a part of the workgroups' 4 columns of a row
         const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
         for (uint32_t i0 = 0; i0 < pieces; i0 += T) {
           const uint32_t part_i = parts > 1u ? tid / pieces : 0u, i = parts > 1u ? tid % pieces : i0 + tid;
-          const bool on = i < pieces && part_i < parts;
-          const uint32_t r = on ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
+          const bool here = i < pieces && part_i < parts;
+          const uint32_t r = here ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
           float4v o = {0.f, 0.f, 0.f, 0.f};
-          if (on) {
+          if (here) {
             constexpr uint32_t U = 8;
-            for (uint32_t z = part_i; z < chunks; z += U * parts) {
+            for (uint32_t z = part_i; z < count; z += U * parts) {
               float4v x[U];
 #pragma unroll
-              for (uint32_t k = 0; k < U; ++k)
-                x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(
-                                                       prs, (int)((place(min(z + k * parts, chunks - 1u)) + r * D + d) * 4u), 0, kSc1));
+              for (uint32_t k = 0; k < U; ++k) {
+                const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + r * D + d;
+                x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
+              }
 #pragma unroll
               for (uint32_t k = 0; k < U; ++k)
-                if (z + k * parts < chunks) o += x[k] * wt[(z + k * parts) * p.rows + r];
+                if (z + k * parts < count) o += x[k] * wt[(z + k * parts) * p.rows + r];
             }
           }
           if (parts > 1u) {
             *(float4v *)(half + 4u * tid) = o;
             __syncthreads();
-            if (on && part_i == 0u)
+            if (here && part_i == 0u)
               for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * pieces));
           }
-          if (on && part_i == 0u) {
+          if (!here || part_i != 0u) continue;
+          const float l = sl[0][r];
+          if (last) {
             const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
-            const float l = sl[0][r];
             float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
             *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+          } else {
+            const uint32_t at = place(z0) * slot_floats;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((at + r * D + d) * 4u), 0, kSc1);
+            if (d == 0u) {
+              // a sum that is not a number is not nothing
+              const float mx = sm[0][r] == -INFINITY && l != 0.f ? 0.f : sm[0][r];
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((at + ml + 2u * r) * 4u), 0, kSc1);
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((at + ml + 2u * r + 1u) * 4u), 0, kSc1);
+            }
           }
         }
+        if (last) break;
+        z0 = 0u, step = side, count = groups;
       }
     }
     if (!on || !attn_next<R>(b, group, a.window, p.max_rows, t, c)) return;
@@ -1219,8 +1241,6 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
     if (wide || (kv.dim == 128u && kv.type == EFF_KV_F16 && share >= 12u)) slots = 256u;
     p.on = share >= 16u && (!wide || wgs * 4u > slots);
     p.items = (uint32_t)std::max<uint64_t>(slots / kv.heads, p.on ? 1u : 2u * p.tiles);
-    const uint64_t most_wgs = (4u * R * (kv.dim + 4u) - 1024u) / p.rows;   // whose weights fit in the join's LDS
-    p.least = (uint32_t)std::max<uint64_t>(units / (most_wgs - 2u) + 1u, 2u);
   }
   // 8 waves where a CU has one workgroup and the steps to share (the drafts above:
   // 15.8 us, 4 waves 17.8; 1024 workgroups of 300 tokens 30, 4 waves 21; 128 of up to
@@ -1239,7 +1259,7 @@ static hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnAr
   const AttnPlan p = attn_plan(kv, b, a);
   const uint64_t many = (uint64_t)p.many_tiles * kv.heads, grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
   if (!fits(many, 256u) || !fits(grid, 512u)) return hipErrorInvalidConfiguration;
-  if (p.items && (grid > kAttnCounters || !scratch)) return hipErrorInvalidValue;
+  if (p.items && (grid > kAttnCounters / 4u || !scratch)) return hipErrorInvalidValue;
   if (many) {
     const uint32_t min_rows = p.tiles ? kFewRows + 1u : 1u;
     hipLaunchKernelGGL((k_attn_rows<TYPE, D>), dim3((uint32_t)many), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows);

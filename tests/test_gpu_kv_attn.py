@@ -151,6 +151,28 @@ def test_long_shares(ctx, eff):
 
 
 @pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("dim,heads,group,new,lens,window", [
+    (256, 2, 8, [1], [20011], 0), (128, 1, 16, [1], [33000], 0), (64, 2, 16, [1, 2], [16000, 9000], 0),
+    (128, 2, 8, [5, 1], [19000, 17000], 18001), (96, 1, 5, [1], [40001], 0)])
+def test_many_workgroups_to_a_tile(ctx, eff, t, dim, heads, group, new, lens, window):
+    """More of their sums than are joined at once."""
+    run(eff, ctx, dim, t, heads, group, dim, 64, new, lens, window)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("where", [0, 1])
+def test_not_finite_in_a_long_tile(ctx, eff, bad, where):
+    """A key or value that is not finite, in one of many workgroups' tokens: the rows that see it are not finite."""
+    rng = np.random.default_rng(6)
+    b = Batch(rng, [2], [20000], 64)
+    rows = rng.standard_normal((b.pages, 2, 1, 64, 128)).astype(np.float32)
+    rows[b.table[0, 7000 // 64], where, 0, 7000 % 64, 5] = bad
+    q = np.abs(rng.standard_normal((2, 16, 128))).astype(np.float32)
+    out = launch(eff, ctx, F16, 1, 128, b, encode(F16, rows)[0], q, 16, 0.1)
+    assert not np.isfinite(out).all(-1).any()
+
+
+@pytest.mark.parametrize("t", [F16, I8])
 @pytest.mark.parametrize("lens", [[1], [700], [20, 5, 300]])
 def test_length_bound(ctx, eff, t, lens):
     """The bound of the lengths far above them, as a recording has it."""
