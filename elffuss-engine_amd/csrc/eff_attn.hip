@@ -766,15 +766,15 @@ __device__ __forceinline__ void from_lds(T &to, const T &from) {
 
 // Few rows: NW waves take the 32-token steps of a tile in turn; their sums meet in
 // LDS. Where a tile has several workgroups, the last of them to arrive joins their
-// sums, in the tokens' order, so that the bits do not depend on who was last; stores
-// and loads of these go past the XCD's L2 (sc1), every wave waits for its stores before
-// the barrier ahead of the counter's increment, and the counter is left at zero for the
-// next launch.
+// sums, in the tokens' order, so that the bits do not depend on who was last (many in
+// two steps, groups first); stores and loads of these go past the XCD's L2 (sc1), every
+// wave waits for its stores before the barrier ahead of the counter's increment, and
+// the counters are left at zero for the next launch.
 //
 // The cache's bytes bound a batch: K and V go from memory to the registers that the
 // matrix unit reads, a step of V and the next step of K under way in each wave, 16 KB
 // of fp16 rows of 128, 64 KB a CU and more (64 sequences up to 16384 long, 32 heads of
-// 128 on 8: 360 us, 5.9 TB/s; one of 130001: 97 us, 5.5 TB/s). The matrix unit is busy
+// 128 on 8: 359 us, 5.9 TB/s; one of 130001: 97 us, 5.5 TB/s). The matrix unit is busy
 // 8 % of the time there, so the second parts of q and p are free. int8 rows are half
 // the bytes with as many instructions, which shows where the shares are short (40 up
 // to 9001, 16 heads of 256 on 2: 48 us, 3.4 TB/s). A single short sequence is round
