@@ -1205,11 +1205,11 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   p.max_rows = ~0u;
   const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
   // Sequences with more than 64 rows go to k_attn_rows where there are enough tiles of
-  // that (1 x 8 heads of 128 over 4000 tokens: 300 rows of new tokens 109 us, k_attn
-  // 106, 400 108 and 133; its int8 pages cost a conversion more for the same tile:
-  // 600 175 and 169, 700 175 and 196). The others go with them where lengths and
-  // new tokens are alike, since a second launch waits for the first (32 x 8, up to
-  // 24 new tokens: 73 us, two launches 97) and a long one's tile is not shared.
+  // that (1 x 32 heads of 128 on 8 over 4000 tokens: 300 new tokens 108 us, k_attn 104,
+  // 400 108 and 131; int8 pages cost a conversion more for the same tile: 600 174 and
+  // 160, 800 175 and 201). The others go with them where lengths and new tokens are
+  // alike, since a second launch waits for the first (32 of up to 24 new tokens: 71 us,
+  // two launches 97); a long one's tile there is not shared.
   if (most > kFewRows && rows / 64u * kv.heads >= (kv.type == EFF_KV_F16 ? 176u : 400u)) {
     attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
     if (b.seqs == 1u || (most * b.seqs <= 3u * rows && seen <= 4096u)) return p;
@@ -1221,20 +1221,20 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
   // Where the tiles alone fill half of the CUs and are short, or there are many, a
   // workgroup has a tile, as where there are 5 units or fewer (4 at 256 wide): a join
-  // takes time (1 x 8 heads of 64 over 517 tokens: 7.3 us, shared 8.2, over 1000 9.6
-  // and 8.7; 24 x 8 heads of drafts that see 1024 tokens 15.8, shared 22.5; 32 x 8
-  // heads of one token up to 2000 36.8, shared 45.8).
+  // takes time (1 x 8 heads of 64 over 517 tokens: 6.9 us, shared 7.8, over 1000 9.3
+  // and 8.3; 24 x 8 heads of drafts that see 1024 tokens 14.7, shared 23.4; 32 x 8
+  // heads of one token up to 2000 36.4, shared 45.8).
   const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
   if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
     // Two workgroups to a CU, or one where its waves have enough bytes under way: 256
-    // wide (24 x 2 heads up to 8000 50.4 us, two 55.9; of int8 33.5 and 35.8), or fp16
+    // wide (24 x 2 heads up to 8000 48.9 us, two 54.1; of int8 33.6 and 35.0), or fp16
     // rows of 128 and long shares (1 x 8 up to 130001 96.7, two 99.4; 8 x 8 drafts up to
-    // 5000, short ones, 30.8 and 28.1). Less wide they take two (16 x 8 of int8 up to
-    // 30000 106, two 100).
+    // 5000, short ones, 30.6 and 28.1). Less wide they take two (16 x 8 of int8 up to
+    // 30000 102, two 99).
     // Shares that may go on into the next tile pay where they are long (64 x 8 up to
-    // 16384 359 us, ending with a tile 411; 24 x 8 up to 6000 69, 94); 256 wide, where
+    // 16384 357 us, ending with a tile 411; 24 x 8 up to 6000 69, 93); 256 wide, where
     // the scalar registers of that take vector ones, only with many tiles (100 x 2 of
-    // int8 up to 9000 112, 157; 24 x 2 up to 30000 77, 73).
+    // int8 up to 9000 115, 156; 24 x 2 up to 30000 76, 73).
     uint64_t slots = 512u;
     const uint64_t share = wgs * units / slots;
     const bool wide = kv.dim >= 256u;
@@ -1243,8 +1243,8 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
     p.items = (uint32_t)std::max<uint64_t>(slots / kv.heads, p.on ? 1u : 2u * p.tiles);
   }
   // 8 waves where a CU has one workgroup and the steps to share (the drafts above:
-  // 15.8 us, 4 waves 17.8; 1024 workgroups of 300 tokens 30, 4 waves 21; 128 of up to
-  // 2000 of int8, 256 wide 35.8, 4 waves 41.4; fp16 of that width 47.6 and 45.6)
+  // 14.7 us, 4 waves 15.5; 128 of up to 2000 of int8, 256 wide, 32.3 and 35.6; fp16 of
+  // that width 46.8 and 45.7; 1024 workgroups of up to 300 tokens 20.5 and 20.2)
   p.waves = !p.items && wgs <= 256u && span >= 512u && (kv.dim < 256u || kv.type == EFF_KV_I8) ? 8u : 4u;
   return p;
 }
