@@ -390,6 +390,26 @@ def test_same_bits(ctx, eff):
         assert np.array_equal(first.view(np.uint32), launch(eff, ctx, F16, 2, 128, b, data, q, 8, 0.09).view(np.uint32))
 
 
+@pytest.mark.parametrize("t,heads,group,dim,lens", [
+    (F16, 8, 2, 64, [2300] + list(range(1, 380, 5))), (I8, 2, 8, 256, [20000]), (I8, 8, 4, 128, [2300] + [700] * 70)])
+def test_same_bits_shared(ctx, eff, t, heads, group, dim, lens):
+    """Tiles that workgroups share, in one order of joining: the same bits again and again."""
+    rng = np.random.default_rng(13)
+    b = Batch(rng, [1] * len(lens), lens, 64)
+    data, _ = make(rng, t, heads, dim, b)
+    q = rng.standard_normal((len(lens), heads * group, dim)).astype(np.float32)
+    cb, qb, out = ctx.upload(data), ctx.upload(q), ctx.alloc(q.nbytes)
+    cache, batch = eff.KvCache(t, heads, dim, 64, b.pages, cb), b.upload(eff, ctx)
+    got = []
+    for _ in range(6):
+        out.write(np.full(q.shape, 9, np.float32))
+        ctx.kv_attn(cache, batch, qb, out, heads * group, 0.1)
+        got.append(out.read(np.uint32).copy())
+    assert all(np.array_equal(got[0], g) for g in got[1:])
+    for x in [cb, qb, out] + batch.buffers:
+        x.free()
+
+
 def test_recorded(ctx, eff):
     """A recorded call takes the next steps' lengths and pages; each replay gives the eager call's bits."""
     rng = np.random.default_rng(14)
