@@ -1028,7 +1028,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   __shared__ __align__(1024) uint8_t buf[2][S::BYTES];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
-  // the last tiles of a sequence see the most: first
+  // The last tiles of a sequence see the most: first; sequence after sequence, and a
+  // head to an XCD where there are 8, so that tiles which run together read the same
+  // rows out of its L2 (the sequences in turn, longest tiles of all first: 199 us
+  // for the above, 371 -> 453 for 4 x 500 over up to 8000)
   const uint32_t kvh = blockIdx.x % kv.heads, tile = tiles - 1u - blockIdx.x / kv.heads;
   AttnTile t;
   if (!attn_tile<R>(b, group, a.window, tile, per_seq, min_rows, ~0u, t)) return;
