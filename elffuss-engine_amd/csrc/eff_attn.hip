@@ -894,19 +894,38 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
         __syncthreads();
         if (arrived != count - 1u) break;
         if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // each thread a part of the workgroups' 4 columns of a row, U of them under way,
+        // the first before the weights are known
+        constexpr uint32_t U = 8;
+        const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
+        const uint32_t part_i = parts > 1u ? tid / pieces : 0u, p0 = parts > 1u ? tid % pieces : tid;
+        float4v x[U] = {};   // (else live from tile to tile)
+        const auto request = [&](uint32_t i, uint32_t z) {
+#pragma unroll
+          for (uint32_t k = 0; k < U; ++k) {
+            const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + i / (D / 4u) * D + 4u * (i % (D / 4u));
+            x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
+          }
+        };
+        if (p0 < pieces && part_i < parts) request(p0, part_i);
         // the workgroups' weights relative to the largest maximum, [workgroup][row],
         // and the rows' sums: a wave per row, its lanes over the workgroups
         float *wt = &so[0][0][0], *half = wt + NW * R * LD - 4u * T;
         for (uint32_t r = wave; r < t.rows; r += NW) {
-          const auto maximum = [&](uint32_t z) { return (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u); };
-          float mx = -INFINITY, l = 0.f;
-          for (uint32_t z = lane; z < count; z += 64u)
-            mx = fmaxf(mx, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, maximum(z), 0, kSc1)));
+          const auto both = [&](uint32_t z, float &mz, float &lz) {
+            const int at = (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u);
+            mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
+            lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
+          };
+          float m0 = -INFINITY, l0 = 0.f, mz, lz;
+          if (lane < count) both(lane, m0, l0);
+          float mx = m0, l = 0.f;
+          for (uint32_t z = lane + 64u; z < count; z += 64u) both(z, mz, lz), mx = fmaxf(mx, mz);
 #pragma unroll
           for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
           for (uint32_t z = lane; z < count; z += 64u) {
-            const float mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, maximum(z), 0, kSc1));
-            const float lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, maximum(z) + 4, 0, kSc1));
+            if (z < 64u) mz = m0, lz = l0;
+            else both(z, mz, lz);
             const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
             wt[z * p.rows + r] = f;
             l += f * lz;
@@ -915,22 +934,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
           if (lane == 0u) sl[0][r] = l, sm[0][r] = mx;
         }
         __syncthreads();
-        // each thread a part of the workgroups' 4 columns of a row
-        const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
-        for (uint32_t i0 = 0; i0 < pieces; i0 += T) {
-          const uint32_t part_i = parts > 1u ? tid / pieces : 0u, i = parts > 1u ? tid % pieces : i0 + tid;
+        for (uint32_t i = p0; i < (parts > 1u ? p0 + 1u : (pieces + T - 1u) / T * T); i += T) {
           const bool here = i < pieces && part_i < parts;
           const uint32_t r = here ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
           float4v o = {0.f, 0.f, 0.f, 0.f};
           if (here) {
-            constexpr uint32_t U = 8;
             for (uint32_t z = part_i; z < count; z += U * parts) {
-              float4v x[U];
-#pragma unroll
-              for (uint32_t k = 0; k < U; ++k) {
-                const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + r * D + d;
-                x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
-              }
+              if (i != p0 || z != part_i) request(i, z);
 #pragma unroll
               for (uint32_t k = 0; k < U; ++k)
                 if (z + k * parts < count) o += x[k] * wt[(z + k * parts) * p.rows + r];
