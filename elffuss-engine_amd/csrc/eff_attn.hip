@@ -747,9 +747,9 @@ __host__ __device__ constexpr uint32_t attn_part_floats(const AttnPlan &p, uint3
 
 constexpr uint32_t kFewRows = 64;
 // Values that one join reads: of more than these it takes longer than the second round
-// trip of two (32 workgroups x 8 rows x 128: 16.3 us, in two 16.6; 128 x 8 x 256 46.5
-// and 25.8).
-constexpr uint32_t kJoin = 65536;
+// trip of two (32 workgroups x 8 rows x 128: 14.7 us, in two 15.3; 64 x 8 x 128 22.3 and
+// 20.3; 128 x 8 x 128 40.9 and 26.9).
+constexpr uint32_t kJoin = 32768;
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
 enum { kAttnWhole, kAttnEnds, kAttnOn };   // a workgroup has a tile; a part of one; a share that may go on into the next
@@ -1232,13 +1232,13 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   attn_tiles(most, rows, b.seqs, R, &p.tiles, &p.per_seq);
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
-  // Where the tiles alone fill half of the CUs and are short, or there are many, a
+  // Where the tiles alone fill two thirds of the CUs and are short, or there are many, a
   // workgroup has a tile, as where there are 5 units or fewer (4 at 256 wide): a join
-  // takes time (1 x 8 heads of 64 over 517 tokens: 6.9 us, shared 7.8, over 1000 9.3
-  // and 8.3; 24 x 8 heads of drafts that see 1024 tokens 14.7, shared 23.4; 32 x 8
-  // heads of one token up to 2000 36.4, shared 45.8).
+  // takes time (1 x 8 heads of 64 over 517 tokens: 6.8 us, shared 7.6, over 1000 9.3
+  // and 8.0; 24 x 8 heads of drafts that see 1024 tokens 14.7, shared 22.0; heads of one
+  // token up to 2000: 16 x 8 22.6, shared 18.3, 32 x 8 35.5 and 45.5).
   const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
-  if ((wgs < 128u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
+  if ((wgs < 171u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
     // Two workgroups to a CU, or one where its waves have enough bytes under way: 256
     // wide (24 x 2 heads up to 8000 48.9 us, two 54.1; of int8 33.6 and 35.0), or fp16
     // rows of 128 and long shares (1 x 8 up to 130001 96.7, two 99.4; 8 x 8 drafts up to

@@ -139,7 +139,8 @@ def test_whole_tiles(ctx, eff, t, dim, group, new, window):
     """Enough short tiles for a workgroup each: of eight waves where they are few."""
     rng = np.random.default_rng(dim + group)
     lens = [900, 0, 1, 511, 512, 513] + [int(n) for n in rng.integers(1, 900, 11)]
-    run(eff, ctx, dim, t, 8, group, dim, 32, [min(new, n) for n in lens], lens, window)
+    for heads in (8, 12):
+        run(eff, ctx, dim, t, heads, group, dim, 32, [min(new, n) for n in lens], lens, window)
     run(eff, ctx, dim, t, 3, group, dim, 16, [new], [599], window)
 
 
