@@ -774,7 +774,7 @@ __device__ __forceinline__ void from_lds(T &to, const T &from) {
 // The cache's bytes bound a batch: K and V go from memory to the registers that the
 // matrix unit reads, a step of V and the next step of K under way in each wave, 16 KB
 // of fp16 rows of 128, 64 KB a CU and more (64 sequences up to 16384 long, 32 heads of
-// 128 on 8: 359 us, 5.9 TB/s; one of 130001: 97 us, 5.5 TB/s). The matrix unit is busy
+// 128 on 8: 358 us, 5.9 TB/s; one of 130001: 95 us, 5.6 TB/s). The matrix unit is busy
 // 8 % of the time there, so the second parts of q and p are free. int8 rows are half
 // the bytes with as many instructions, which shows where the shares are short (40 up
 // to 9001, 16 heads of 256 on 2: 48 us, 3.4 TB/s). A single short sequence is round
