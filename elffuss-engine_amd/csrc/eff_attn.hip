@@ -18,8 +18,9 @@
 // Precision. q (scaled by a power of two to a row maximum of 2^13) and p (scaled
 // by 2^14) are split in two fp16 parts, 22 bits, each its own matrix step; the
 // cached fp16 or int8 values are exact operands; sums are f32. An int8 row's scale
-// multiplies its scores, and its weight relative to the largest value scale
-// the row has seen (so that the weight's fp16 parts stay in range).
+// (of either sign) multiplies its scores, and its weight relative to the largest
+// magnitude of a value scale the row has seen (so that the weight's fp16 parts stay
+// in range).
 #include <algorithm>
 
 #include "eff_device.h"
@@ -388,7 +389,7 @@ struct AttnWave {
   float sc;             // > 0: what a raw score of row n is multiplied by (log2 e included)
   int pos;              // the row's position, -1 for none
   float m, l;           // running maximum (of raw scores), and this lane's share of the sum
-  float vref, vinv;     // SCALED: the largest value scale so far, and its reciprocal
+  float vref, vinv;     // SCALED: the largest magnitude of a value scale so far, and its reciprocal
   float4v acc[E];
 
   uint32_t kw[2][KS * KW];
@@ -602,7 +603,7 @@ struct AttnWave {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vx = fmaxf(vx, !masked || s[u][j] != -INFINITY ? __uint_as_float(vs[u][j]) : 0.f);
+        for (int j = 0; j < 4; ++j) vx = fmaxf(vx, !masked || s[u][j] != -INFINITY ? fabsf(__uint_as_float(vs[u][j])) : 0.f);
       vx = row_max(vx);
     }
     if (__any(mx > m || (SCALED && vx > vref))) {

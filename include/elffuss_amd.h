@@ -499,7 +499,8 @@ size_t eff_topk_out_bytes(void);
  * 16..1024) for `heads` key/value heads of `head_dim` (64, 96, 128 or 256)
  * values, in `buf`. Page p starts at p * eff_kv_page_bytes: its K, then its V,
  * each [head][token][head_dim] in fp16 (EFF_KV_F16), or per head the int8 rows
- * and after them the rows' f32 scales (EFF_KV_I8; a value is int8 * scale).
+ * and after them the rows' f32 scales (EFF_KV_I8; a value is int8 * scale, of
+ * either sign).
  * The reference's cache is one fp16 buffer per layer (README.md:101); pages let
  * requests of different lengths share the memory, and give it back. */
 typedef struct eff_kv_cache {
