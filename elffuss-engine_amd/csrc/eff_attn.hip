@@ -96,6 +96,21 @@ __device__ __forceinline__ float unseen(float v) {
 // signalling NaN, an instruction each; a NaN here makes the row's sum NaN anyway.)
 __device__ __forceinline__ float max2(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, unseen(INFINITY)); }
 
+// Of 8 numbers, NaN if one is: three operands an instruction.
+__device__ __forceinline__ float max8(const float s[2][4]) {
+  float m = s[0][0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) m = __builtin_elementwise_maximum(m, s[k / 4][k % 4]);
+  return m;
+}
+
+__device__ __forceinline__ float min8(const float s[2][4]) {
+  float m = s[0][0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) m = __builtin_elementwise_minimum(m, s[k / 4][k % 4]);
+  return m;
+}
+
 // Maximum and sum over the 4 lanes that hold a row (lane % 16). The swaps leave
 // the two halves (two 16-lane rows) of v side by side in two registers.
 __device__ __forceinline__ float row_max(float v) {
@@ -558,15 +573,22 @@ struct AttnWave {
   // The weights of the step at token t0, and the weighted sum; v(i) is V's operand of
   // column i. `masked`: some row does not see every one of its 32 tokens (wave-
   // uniform); a half without a page is `gone`.
+  // A score of -inf says that a row does not see the token. That of a token it sees is
+  // -inf where the key is not finite (or the score passes f32): the row's sum becomes
+  // NaN, as it does with +inf.
   template <typename V>
   __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[2][4], V v) {
     u32x4 keep = {~0u, ~0u, ~0u, ~0u};   // the halves of an operand whose token some row sees
     bool dirty = false;                  // and whether some of them are not finite
+    float low = 0.f;                     // the smallest score that the row sees (a NaN hides it: no matter)
     if (masked) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int at = t0 + 16 * (k / 4) + 4 * (int)g + k % 4;
-        if (gone[k / 4] || !sees(pos, window, at)) s[k / 4][k % 4] = -INFINITY;
+        float &y = s[k / 4][k % 4];
+        const bool seen = !gone[k / 4] && sees(pos, window, at);
+        low = seen ? __builtin_elementwise_minimum(low, y) : low;
+        y = seen ? y : -INFINITY;
         // what no row sees may be any bits
         if (gone[k / 4] || at < t.begin || at >= t.end) {
           if constexpr (SCALED) vs[k / 4][k % 4] = 0u;
@@ -578,7 +600,7 @@ struct AttnWave {
       if constexpr (!SCALED) {
         keep_v(keep);
         if (t.first != t.last) {
-          uint32_t top = 0;
+          uint32_t most = 0;
 #pragma unroll
           for (int i = 0; i < (VIN == kVLater ? E : VN * VM / 4); ++i) {
             u32x4 o;
@@ -587,16 +609,17 @@ struct AttnWave {
 #pragma unroll
               for (int x = 0; x < 4; ++x) o[x] = vw[(4 * i + x) / VM][(4 * i + x) % VM];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) top = max(top, max(o[x] & 0x7FFFu, o[x] >> 16 & 0x7FFFu));
+            for (int x = 0; x < 4; ++x) most = max(most, max(o[x] & 0x7FFFu, o[x] >> 16 & 0x7FFFu));
             __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
           }
-          dirty = __any(top >= 0x7C00u);
+          dirty = __any(most >= 0x7C00u);
           if (dirty) poison(t0, gone, window, g, keep, v);
         }
       }
+    } else {
+      low = min8(s);
     }
-    float mx = max2(max2(max2(s[0][0], s[0][1]), max2(s[0][2], s[0][3])), max2(max2(s[1][0], s[1][1]), max2(s[1][2], s[1][3])));
-    mx = row_max(mx);
+    const float mx = row_max(max8(s));
     float vx = 0.f;
     if constexpr (SCALED) {
       // of the tokens that the row sees only: another row's may not be finite
@@ -623,7 +646,7 @@ struct AttnWave {
       for (int i = 0; i < E; ++i) acc[i] *= f;
     }
     const float up = m == -INFINITY ? 0.f : 14.f - m * sc;
-    float sum = 0.f;
+    float sum = low == -INFINITY ? NAN : 0.f;
     half2v hi[4], lo[4];
 #pragma unroll
     for (int k = 0; k < 8; k += 2) {
@@ -1196,7 +1219,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   }
   const float l = row_add(w.l);
   if (n >= m.rows) return;
-  const float f = l == 0.f ? 0.f : (I8 ? w.vref : 1.f) / l;
+  // no weight: nothing seen, or the largest score past f32
+  const float f = l == 0.f ? (w.m == -INFINITY ? 0.f : NAN) : (I8 ? w.vref : 1.f) / l;
   const uint32_t tok = (m.r0 + n) / group, h = (m.r0 + n) % group;
   float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D;
 #pragma unroll

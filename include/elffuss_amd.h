@@ -571,7 +571,8 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
  * (the append comes first). softmax(scale * q . k) in f32; a token that sees
  * nothing gives zeros. What lies in the cache at positions it does not see does
  * not reach its output, whatever bits it has; a NaN or an infinity among what
- * it sees does. q and out may not overlap. f32-accurate. */
+ * it sees does, and so does a score past f32's range: the row's output is not
+ * finite. q and out may not overlap. f32-accurate. */
 int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
                 uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window);
 
