@@ -18,9 +18,10 @@
 // Precision. q (scaled by a power of two to a row maximum of 2^13) and p (scaled
 // by 2^14) are split in two fp16 parts, 22 bits, each its own matrix step; the
 // cached fp16 or int8 values are exact operands; sums are f32. An int8 row's scale
-// (of either sign) multiplies its scores, and its weight relative to the largest
-// magnitude of a value scale the row has seen (so that the weight's fp16 parts stay
-// in range).
+// (of either sign) multiplies its scores, and its weights: the fp16 parts are of the
+// products, in units of 2^-14 of the largest one the row has met, which shrinks with
+// the weights as the maximum grows. (Not of the largest scale: a token of no weight
+// and a large scale would take the others' bits.)
 #include <algorithm>
 
 #include "eff_device.h"
@@ -139,6 +140,7 @@ __device__ __forceinline__ void split2(float a, float b, half2v &hi, half2v &lo)
 
 constexpr uint32_t kLeast = 2, kShort = 8;   // units of a share
 constexpr uint32_t kUnit = 128;   // tokens: a step of each of four waves
+constexpr float kLeastUnit = 0x1p-100f;   // of weights times scales
 
 // The rows of a tile, their tokens and what they see.
 struct AttnTile {
@@ -404,7 +406,7 @@ struct AttnWave {
   float sc;             // > 0: what a raw score of row n is multiplied by (log2 e included)
   int pos;              // the row's position, -1 for none
   float m, l;           // running maximum (of raw scores), and this lane's share of the sum
-  float vref, vinv;     // SCALED: the largest magnitude of a value scale so far, and its reciprocal
+  float unit, inv;      // SCALED: what 1 in acc stands for, and its reciprocal
   float4v acc[E];
 
   uint32_t kw[2][KS * KW];
@@ -466,7 +468,7 @@ struct AttnWave {
         *(half8 *)(const_cast<uint8_t *>(qs) + c * 2048 + 1024) = r;
       }
     }
-    m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;
+    m = -INFINITY, l = 0.f, unit = 0.f, inv = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
   }
@@ -571,13 +573,13 @@ struct AttnWave {
   static __device__ __forceinline__ bool sees(int pos, int window, int t) { return t <= pos && (window == 0 || t > pos - window); }
 
   // The weights of the step at token t0, and the weighted sum; v(i) is V's operand of
-  // column i. `masked`: some row does not see every one of its 32 tokens (wave-
-  // uniform); a half without a page is `gone`.
+  // column i, scales(u) the lane's value scales of half u. `masked`: some row does not
+  // see every one of its 32 tokens (wave-uniform); a half without a page is `gone`.
   // A score of -inf says that a row does not see the token. That of a token it sees is
   // -inf where the key is not finite (or the score passes f32): the row's sum becomes
   // NaN, as it does with +inf.
-  template <typename V>
-  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[2][4], V v) {
+  template <typename V, typename S>
+  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const AttnTile &t, int window, uint32_t g, float s[2][4], V v, S scales) {
     u32x4 keep = {~0u, ~0u, ~0u, ~0u};   // the halves of an operand whose token some row sees
     bool dirty = false;                  // and whether some of them are not finite
     float low = 0.f;                     // the smallest score that the row sees (a NaN hides it: no matter)
@@ -589,11 +591,8 @@ struct AttnWave {
         const bool seen = !gone[k / 4] && sees(pos, window, at);
         low = seen ? __builtin_elementwise_minimum(low, y) : low;
         y = seen ? y : -INFINITY;
-        // what no row sees may be any bits
-        if (gone[k / 4] || at < t.begin || at >= t.end) {
-          if constexpr (SCALED) vs[k / 4][k % 4] = 0u;
-          else keep[k / 2] &= k & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-        }
+        // what no row sees may be any bits (int8 are numbers whatever they are)
+        if (!SCALED && (gone[k / 4] || at < t.begin || at >= t.end)) keep[k / 2] &= k & 1 ? 0x0000FFFFu : 0xFFFF0000u;
       }
       // A value that only some rows see and that is not finite: 0 * inf would
       // reach the others. (int8 values are finite, and their scales go with the weights.)
@@ -620,48 +619,52 @@ struct AttnWave {
       low = min8(s);
     }
     const float mx = row_max(max8(s));
-    float vx = 0.f;
-    if constexpr (SCALED) {
-      // of the tokens that the row sees only: another row's may not be finite
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) vx = fmaxf(vx, !masked || s[u][j] != -INFINITY ? fabsf(__uint_as_float(vs[u][j])) : 0.f);
-      vx = row_max(vx);
-    }
-    if (__any(mx > m || (SCALED && vx > vref))) {
+    if (__any(mx > m)) {
       const float mn = fmaxf(m, mx);
-      float f = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * sc);
+      const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * sc);
       m = mn;
       l *= f;
       if constexpr (SCALED) {
-        if (vx > vref) {
-          const float vn = fmaxf(vx, 1e-30f);
-          f *= vref / vn;
-          vref = vn;
-          vinv = 1.f / vn;
-        }
-      }
+        unit *= f;
+        inv = 1.f / unit;
+      } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) acc[i] *= f;
+        for (int i = 0; i < E; ++i) acc[i] *= f;
+      }
     }
-    const float up = m == -INFINITY ? 0.f : 14.f - m * sc;
+    const float up = m == -INFINITY ? 0.f : SCALED ? -(m * sc) : 14.f - m * sc;
     float sum = low == -INFINITY ? NAN : 0.f;
-    half2v hi[4], lo[4];
+    float p[8];
+    u32x4 scale = {};
 #pragma unroll
-    for (int k = 0; k < 8; k += 2) {
-      float p[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float y = s[k / 4][k % 4 + x];
-        p[x] = __builtin_amdgcn_exp2f(fmaf(y, sc, up));
-        sum += p[x];
-        // a weight of nothing takes nothing of a scale that is not finite
-        if constexpr (SCALED) p[x] = masked && y == -INFINITY ? 0.f : p[x] * (__uint_as_float(vs[k / 4][k % 4 + x]) * vinv);
-      }
-      split2(p[0], p[1], hi[k / 2], lo[k / 2]);
+    for (int k = 0; k < 8; ++k) {
+      if (SCALED && k % 4 == 0) scale = scales(k / 4);
+      const float y = s[k / 4][k % 4];
+      p[k] = __builtin_amdgcn_exp2f(fmaf(y, sc, up));
+      sum += p[k];
+      // a weight of nothing takes nothing of a scale that is not finite
+      if constexpr (SCALED) p[k] = masked && y == -INFINITY ? 0.f : p[k] * __uint_as_float(scale[k % 4]);
     }
     l += sum;
+    if constexpr (SCALED) {
+      // the weights with their scales, in units that leave fp16 a factor of 2 to grow
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(p[k]));
+      if (__any(top * inv > 0x1p15f || unit < kLeastUnit)) {
+        top = row_max(top);
+        const float un = fmaxf(top * inv > 0x1p15f ? top * 0x1p-14f : unit, kLeastUnit), f = unit / un;
+        unit = un;
+        inv = 1.f / un;
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] *= f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) p[k] *= inv;
+    }
+    half2v hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) split2(p[k], p[k + 1], hi[k / 2], lo[k / 2]);
     const half8 ph = join8(hi), pl = join8(lo);
     if (VIN == kVLater && !SCALED && masked) {
 #pragma unroll
@@ -744,7 +747,8 @@ struct AttnWave {
       fetch_k(k, kv, i + 1, n, g);
       __builtin_amdgcn_sched_barrier(0);
     }
-    step(t0, masked, gone, t, window, g, s, [&](int c) { return v_operand(c); });
+    step(t0, masked, gone, t, window, g, s, [&](int c) { return v_operand(c); },
+         [&](int u) { return u32x4{vs[u][0], vs[u][1], vs[u][2], vs[u][3]}; });
   }
 
   __device__ __forceinline__ void fetch_k(AttnWalk &k, const KvView &kv, int i, uint32_t n, uint32_t g) {
@@ -853,7 +857,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
         if constexpr (QL) __syncthreads();   // the sums take q's place
       }
       const float wl = row_add(w.l);
-      if (g == 0u) sm[wave][n] = w.m * w.sc, sl[wave][n] = wl, sv[wave][n] = w.vref;
+      if (g == 0u) sm[wave][n] = w.m * w.sc, sl[wave][n] = wl, sv[wave][n] = w.unit;
 #pragma unroll
       for (int i = 0; i < W::E; ++i)
 #pragma unroll
@@ -1208,11 +1212,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
 #pragma unroll
           for (int c = 0; c < W::E; ++c) __builtin_memcpy(w.vw[c], &(const u32x4 &)turned(c), 16);
         }
-        if constexpr (I8) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) ld_words<4>(w.vs[u], lds + S::SCALES + 128u + 64u * u + 16u * g);
-        }
-        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); });
+        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); },
+               [&](int u) { return *(const u32x4 *)(lds + S::SCALES + 128u + 64u * u + 16u * g); });   // late: no register waits for it
       }
       if (i + 1 < steps) convert(buf[1 - half]);
     }
@@ -1220,7 +1221,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   const float l = row_add(w.l);
   if (n >= m.rows) return;
   // no weight: nothing seen, or the largest score past f32
-  const float f = l == 0.f ? (w.m == -INFINITY ? 0.f : NAN) : (I8 ? w.vref : 1.f) / l;
+  const float f = l == 0.f ? (w.m == -INFINITY ? 0.f : NAN) : (I8 ? w.unit : 1.f) / l;
   const uint32_t tok = (m.r0 + n) / group, h = (m.r0 + n) % group;
   float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D;
 #pragma unroll

@@ -46,3 +46,33 @@ def test_negative_scales(ctx, eff, dim, heads, group, new, lens, signs):
     q = rng.standard_normal((b.tokens, heads * group, dim)).astype(np.float32)
     got = launch(eff, ctx, I8, heads, dim, b, data, q, heads * group, dim ** -0.5)
     near(got, decode(I8, data, b.pages, heads, dim, 32), b, q, heads * group, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,group,new,lens", FORMS)
+@pytest.mark.parametrize("where", [0.0, 0.4, 1.0])
+@pytest.mark.parametrize("size", [1e7, 1e12])
+def test_large_scale_of_a_small_weight(ctx, eff, dim, heads, group, new, lens, where, size):
+    """A value far larger than the others whose token has e^-60 of the others' weight: it takes no bits from them. Before,
+    among and after them."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, new, lens, 32)
+    rows = rng.standard_normal((b.pages, 2, heads, 32, dim)).astype(np.float32)
+    along = np.sign(rng.standard_normal(dim)).astype(np.float32)
+    for s, (n, length) in enumerate(zip(new, lens)):
+        at = int(where * (length - n))        # seen by all of the sequence's new tokens
+        page, slot = b.table[s, at // 32], at % 32
+        rows[page, 0, :, slot] = -along
+        rows[page, 1, :, slot] *= size
+    data, values = encode(I8, rows)
+    # scores of about -60 there, within 4 of 0 elsewhere
+    q = (60 * dim ** -0.5 * along + 0.01 * rng.standard_normal((b.tokens, heads * group, dim))).astype(np.float32)
+    rows_k = data.reshape(b.pages, 2, heads, -1)[:, 0]
+    keep = {(b.table[s, int(where * (n - m)) // 32], int(where * (n - m)) % 32) for s, (m, n) in enumerate(zip(new, lens))}
+    scales = rows_k[..., 32 * dim:].view(np.float32)
+    for p in range(b.pages):
+        for slot in range(32):
+            if (p, slot) not in keep:
+                scales[p, :, slot] *= 0.02
+    got = launch(eff, ctx, I8, heads, dim, b, data, q, heads * group, dim ** -0.5)
+    near(got, decode(I8, data, b.pages, heads, dim, 32), b, q, heads * group, dim ** -0.5)
