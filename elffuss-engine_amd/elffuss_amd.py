@@ -238,6 +238,8 @@ def blocks_from_buffer(nbytes):
 # ---- device ------------------------------------------------------------------
 
 class Buffer:
+    given_back = 0   # buffers freed or retired so far: what holds handles looks at its own again
+
     def __init__(self, ctx, handle, size):
         self.ctx, self.handle, self.size = ctx, handle, size
 
@@ -280,23 +282,36 @@ class Buffer:
         if self.handle:
             self.ctx._check(lib().eff_buf_free(self.ctx.h, self.handle))
             self.handle = None
+            Buffer.given_back += 1
 
     def retire(self):
         """Give the buffer back in stream order, without waiting (eff_buf_retire)."""
         if self.handle:
             self.ctx._check(lib().eff_buf_retire(self.ctx.h, self.handle))
             self.handle = None
+            Buffer.given_back += 1
 
 
 class _Described:
     """A C description of a call's buffers and sizes, made once and given to many calls.
 
-    The buffers stay referenced here; `ref` is what the library takes."""
+    The buffers stay referenced here; `ref` is what the library takes, an error once one of them was given back."""
 
     def _describe(self, struct, **values):
-        self.buffers = [v for v in values.values() if isinstance(v, Buffer)]
+        self._named = {k: v for k, v in values.items() if isinstance(v, Buffer)}
+        self.buffers = list(self._named.values())
         self.c = struct(**{k: v.handle if isinstance(v, Buffer) else v for k, v in values.items()})
-        self.ref = ctypes.addressof(self.c)
+        self._ref, self._seen = ctypes.addressof(self.c), None
+
+    @property
+    def ref(self):
+        if self._seen != Buffer.given_back:
+            seen = Buffer.given_back
+            for k, b in self._named.items():
+                if not b.handle:
+                    raise EffError(E_INVALID, f"{type(self).__name__}: the buffer {k} was freed")
+            self._seen = seen
+        return self._ref
 
 
 class _KvCache(ctypes.Structure):
