@@ -692,17 +692,52 @@ napi_value prop(napi_env env, napi_value o, const char *name) {
   return v;
 }
 
+// A call's properties and numbers. What is undefined or null is not there; anything else
+// that is not what it should be throws (a norm or a mask is never left out without a word),
+// and the call ends where one did.
+bool absent(napi_env env, napi_value v) {
+  napi_valuetype t;
+  return napi_typeof(env, v, &t) != napi_ok || t == napi_undefined || t == napi_null;
+}
+
+bool thrown(napi_env env) {
+  bool is = false;
+  napi_is_exception_pending(env, &is);
+  return is;
+}
+
 // A buffer of a description: null where it has none.
 eff_buf *buf_prop(napi_env env, napi_value o, const char *name) {
   napi_value v = prop(env, o, name);
-  napi_valuetype t;
-  return napi_typeof(env, v, &t) == napi_ok && t == napi_external ? external<eff_buf>(env, v) : nullptr;
+  if (absent(env, v)) return nullptr;
+  eff_buf *b = external<eff_buf>(env, v);
+  if (!b) throw_msg(env, std::string(name) + ": not a buffer");
+  return b;
 }
 
-uint32_t u32_prop(napi_env env, napi_value o, const char *name) { return (uint32_t)i64(env, prop(env, o, name)); }
+uint64_t whole(napi_env env, napi_value v, const char *name, double most) {
+  if (absent(env, v)) return 0;
+  const double d = f64(env, v, -1.0);
+  if (d >= 0.0 && d <= most && d == (double)(uint64_t)d) return (uint64_t)d;
+  throw_msg(env, std::string(name) + ": not a whole number in its range");
+  return 0;
+}
+
+uint32_t u32(napi_env env, napi_value v, const char *name) { return (uint32_t)whole(env, v, name, 4294967295.0); }
+uint32_t u32_prop(napi_env env, napi_value o, const char *name) { return u32(env, prop(env, o, name), name); }
+uint64_t offset(napi_env env, napi_value v, const char *name) { return whole(env, v, name, 9007199254740991.0); }
+
+// A number that is there, or `dflt`.
+double number(napi_env env, napi_value v, const char *name, double dflt) {
+  if (absent(env, v)) return dflt;
+  napi_valuetype t;
+  if (napi_typeof(env, v, &t) == napi_ok && t == napi_number) return f64(env, v);
+  throw_msg(env, std::string(name) + ": not a number");
+  return dflt;
+}
 
 eff_kv_cache kv_cache(napi_env env, napi_value o) {
-  return {(int32_t)i64(env, prop(env, o, "type")), u32_prop(env, o, "heads"), u32_prop(env, o, "headDim"),
+  return {(int32_t)u32_prop(env, o, "type"), u32_prop(env, o, "heads"), u32_prop(env, o, "headDim"),
           u32_prop(env, o, "pageTokens"), u32_prop(env, o, "pages"), buf_prop(env, o, "buf")};
 }
 
@@ -742,16 +777,17 @@ napi_value KvAppend(napi_env env, napi_callback_info info) {
   const eff_kv_batch b = kv_batch(env, a[2]);
   eff_kv_rows r{};
   r.q = buf_prop(env, a[3], "q"), r.k = buf_prop(env, a[3], "k"), r.v = buf_prop(env, a[3], "v");
-  r.q_offset = (uint64_t)i64(env, prop(env, a[3], "qOffset"));
-  r.k_offset = (uint64_t)i64(env, prop(env, a[3], "kOffset"));
-  r.v_offset = (uint64_t)i64(env, prop(env, a[3], "vOffset"));
+  r.q_offset = offset(env, prop(env, a[3], "qOffset"), "qOffset");
+  r.k_offset = offset(env, prop(env, a[3], "kOffset"), "kOffset");
+  r.v_offset = offset(env, prop(env, a[3], "vOffset"), "vOffset");
   r.q_stride = u32_prop(env, a[3], "qStride"), r.k_stride = u32_prop(env, a[3], "kStride");
   r.v_stride = u32_prop(env, a[3], "vStride"), r.q_heads = u32_prop(env, a[3], "qHeads");
   r.q_out = buf_prop(env, a[3], "qOut"), r.rope = buf_prop(env, a[3], "rope");
   r.rope_positions = u32_prop(env, a[3], "ropePositions"), r.rope_dim = u32_prop(env, a[3], "ropeDim");
   r.rope_mode = u32_prop(env, a[3], "ropeMode");
   r.q_norm = buf_prop(env, a[3], "qNorm"), r.k_norm = buf_prop(env, a[3], "kNorm");
-  r.norm_eps = (float)f64(env, prop(env, a[3], "normEps"), 1e-6);
+  r.norm_eps = (float)number(env, prop(env, a[3], "normEps"), "normEps", 1e-6);
+  if (thrown(env)) return nullptr;
   return status(env, ctx, eff_kv_append(ctx, &c, &b, &r));
 }
 
@@ -762,9 +798,12 @@ napi_value KvAttn(napi_env env, napi_callback_info info) {
   eff_ctx *ctx = external<eff_ctx>(env, a[0]);
   const eff_kv_cache c = kv_cache(env, a[1]);
   const eff_kv_batch b = kv_batch(env, a[2]);
-  return status(env, ctx, eff_kv_attn(ctx, &c, &b, external<eff_buf>(env, a[3]), (uint64_t)i64(env, a[4]),
-                                      (uint32_t)i64(env, a[5]), external<eff_buf>(env, a[6]), (uint32_t)i64(env, a[7]),
-                                      (float)f64(env, a[8]), (uint32_t)i64(env, a[9])));
+  const uint64_t q_offset = offset(env, a[4], "qOffset");
+  const uint32_t q_stride = u32(env, a[5], "qStride"), q_heads = u32(env, a[7], "qHeads"), window = u32(env, a[9], "window");
+  const float scale = (float)number(env, a[8], "scale", 0.0);
+  if (thrown(env)) return nullptr;
+  return status(env, ctx, eff_kv_attn(ctx, &c, &b, external<eff_buf>(env, a[3]), q_offset, q_stride, external<eff_buf>(env, a[6]),
+                                      q_heads, scale, window));
 }
 
 // logitsApply(ctx, in, out, rows, vocab, stride, rules)
@@ -776,8 +815,9 @@ napi_value LogitsApply(napi_env env, napi_callback_info info) {
                               buf_prop(env, a[6], "penalties"), buf_prop(env, a[6], "biasIds"),
                               buf_prop(env, a[6], "biasValues"), buf_prop(env, a[6], "biasStarts"),
                               buf_prop(env, a[6], "mask"), buf_prop(env, a[6], "maskOf"), u32_prop(env, a[6], "maskCount")};
-  return status(env, ctx, eff_logits_apply(ctx, external<eff_buf>(env, a[1]), external<eff_buf>(env, a[2]),
-                                           (uint32_t)i64(env, a[3]), (uint32_t)i64(env, a[4]), (uint32_t)i64(env, a[5]), &r));
+  const uint32_t rows = u32(env, a[3], "rows"), vocab = u32(env, a[4], "vocab"), stride = u32(env, a[5], "stride");
+  if (thrown(env)) return nullptr;
+  return status(env, ctx, eff_logits_apply(ctx, external<eff_buf>(env, a[1]), external<eff_buf>(env, a[2]), rows, vocab, stride, &r));
 }
 
 napi_value Register(napi_env env, napi_value exports) {

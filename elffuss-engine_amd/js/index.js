@@ -901,7 +901,28 @@ const KV_TIPOS = { F16: 1, I8: 24 };
 const ROPE = { PARES: 0, MITADES: 1 };
 const SIN_PAGINA = 0xFFFFFFFF;
 
-const manejador = (buf) => (buf ? buf._h : undefined);
+function invalido(mensaje) {
+  const e = new Error(mensaje);
+  e.code = STATUS.E_INVALID;
+  return e;
+}
+
+// The handle of a buffer that a call may leave out (undefined or null), which is an error where it is something else.
+function manejador(buf, nombre) {
+  if (buf === undefined || buf === null) return undefined;
+  if (!buf._h || buf._alive === false) throw invalido(`${nombre}: no es un búfer vivo`);
+  return buf._h;
+}
+
+// Descriptions whose properties may be left out: a name that none of them has is an error, not a norm or a mask left out.
+function soloEstas(o, nombres, que) {
+  for (const k of Object.keys(o)) if (!nombres.includes(k)) throw invalido(`${que}: no hay «${k}»`);
+  return o;
+}
+const DE_FILAS = ['q', 'k', 'v', 'desdeQ', 'desdeK', 'desdeV', 'pasoQ', 'pasoK', 'pasoV', 'cabezasQ', 'rope', 'posicionesRope',
+  'dimRope', 'modoRope', 'normaQ', 'normaK', 'eps'];
+const DE_REGLAS = ['historia', 'iniciosHistoria', 'castigos', 'idsSesgo', 'valoresSesgo', 'iniciosSesgo', 'mascara', 'mascaraDe',
+  'mascaras'];
 
 // A cache as the addon takes it.
 function descCache(c) {
@@ -911,13 +932,13 @@ function descCache(c) {
     e.code = STATUS.E_TYPE;
     throw e;
   }
-  return { type, heads: c.cabezas, headDim: c.dim, pageTokens: c.tokensPagina, pages: c.paginas, buf: manejador(c.buf) };
+  return { type, heads: c.cabezas, headDim: c.dim, pageTokens: c.tokensPagina, pages: c.paginas, buf: manejador(c.buf, 'buf') };
 }
 
 // A batch: { tabla, inicios, largos (u32 buffers), secuencias, tokens, paginasTabla, maxNuevos, maxLargo }.
 function descLote(l) {
-  return { table: manejador(l.tabla), starts: manejador(l.inicios), lens: manejador(l.largos), seqs: l.secuencias,
-    tokens: l.tokens, tablePages: l.paginasTabla, maxNew: l.maxNuevos, maxLen: l.maxLargo };
+  return { table: manejador(l.tabla, 'tabla'), starts: manejador(l.inicios, 'inicios'), lens: manejador(l.largos, 'largos'),
+    seqs: l.secuencias, tokens: l.tokens, tablePages: l.paginasTabla, maxNew: l.maxNuevos, maxLen: l.maxLargo };
 }
 
 function createKvOps(device, deps) {
@@ -944,20 +965,23 @@ function createKvOps(device, deps) {
     // filas: { q, k, v, desdeQ, desdeK, desdeV, pasoQ, pasoK, pasoV, cabezasQ, rope, posicionesRope, dimRope,
     // modoRope, normaQ, normaK, eps }.
     anade(cache, lote, filas) {
-      const f = filas;
+      const f = soloEstas(filas, DE_FILAS, 'filas');
+      const d = { q: manejador(f.q, 'q'), k: manejador(f.k, 'k'), v: manejador(f.v, 'v'), qOffset: f.desdeQ, kOffset: f.desdeK,
+        vOffset: f.desdeV, qStride: f.pasoQ, kStride: f.pasoK, vStride: f.pasoV, qHeads: f.q ? f.cabezasQ : 0,
+        rope: manejador(f.rope, 'rope'), ropePositions: f.posicionesRope, ropeDim: f.dimRope, ropeMode: f.modoRope,
+        qNorm: manejador(f.normaQ, 'normaQ'), kNorm: manejador(f.normaK, 'normaK'), normEps: f.eps };
+      const c = descCache(cache), l = descLote(lote);
       const q = f.q ? ctx.alloc(lote.tokens * f.cabezasQ * cache.dim * 4, 'kv.q') : null;
-      native.kvAppend(device._ctx, descCache(cache), descLote(lote), { q: manejador(f.q), k: manejador(f.k), v: manejador(f.v),
-        qOffset: f.desdeQ, kOffset: f.desdeK, vOffset: f.desdeV, qStride: f.pasoQ, kStride: f.pasoK, vStride: f.pasoV,
-        qHeads: f.q ? f.cabezasQ : 0, qOut: manejador(q), rope: manejador(f.rope), ropePositions: f.posicionesRope,
-        ropeDim: f.dimRope, ropeMode: f.modoRope, qNorm: manejador(f.normaQ), kNorm: manejador(f.normaK), normEps: f.eps });
+      d.qOut = manejador(q, 'q');
+      native.kvAppend(device._ctx, c, l, d);
       return Promise.resolve(q);
     },
     // Attention of the new tokens over the cache, into a pooled buffer. opts: { ventana, desdeQ, pasoQ }.
     atiende(cache, lote, q, cabezasQ, escala, opts) {
-      const o = opts || {};
+      const o = soloEstas(opts || {}, ['ventana', 'desdeQ', 'pasoQ'], 'opts');
+      const c = descCache(cache), l = descLote(lote), h = manejador(q, 'q');
       const out = ctx.alloc(lote.tokens * cabezasQ * cache.dim * 4, 'kv.atencion');
-      native.kvAttn(device._ctx, descCache(cache), descLote(lote), q._h, o.desdeQ || 0, o.pasoQ || 0, out._h, cabezasQ, escala,
-        o.ventana || 0);
+      native.kvAttn(device._ctx, c, l, h, o.desdeQ, o.pasoQ, out._h, cabezasQ, escala, o.ventana);
       return Promise.resolve(out);
     },
   };
@@ -970,14 +994,15 @@ function createLogitsOps(device, deps) {
   const ctx = deps.ctx;
   return {
     aplica(logits, filas, vocab, reglas, opts) {
-      const o = opts || {};
-      const r = reglas;
-      const paso = o.paso || vocab;
+      const o = soloEstas(opts || {}, ['paso', 'salida'], 'opts');
+      const r = soloEstas(reglas, DE_REGLAS, 'reglas');
+      const d = { history: manejador(r.historia, 'historia'), historyStarts: manejador(r.iniciosHistoria, 'iniciosHistoria'),
+        penalties: manejador(r.castigos, 'castigos'), biasIds: manejador(r.idsSesgo, 'idsSesgo'),
+        biasValues: manejador(r.valoresSesgo, 'valoresSesgo'), biasStarts: manejador(r.iniciosSesgo, 'iniciosSesgo'),
+        mask: manejador(r.mascara, 'mascara'), maskOf: manejador(r.mascaraDe, 'mascaraDe'), maskCount: r.mascaras };
+      const z = manejador(logits, 'logits'), paso = o.paso || vocab;
       const out = o.salida || ctx.alloc(Math.max(1, filas) * paso * 4, 'logits');
-      native.logitsApply(device._ctx, logits._h, out._h, filas, vocab, paso, { history: manejador(r.historia),
-        historyStarts: manejador(r.iniciosHistoria), penalties: manejador(r.castigos), biasIds: manejador(r.idsSesgo),
-        biasValues: manejador(r.valoresSesgo), biasStarts: manejador(r.iniciosSesgo), mask: manejador(r.mascara),
-        maskOf: manejador(r.mascaraDe), maskCount: r.mascaras });
+      native.logitsApply(device._ctx, z, manejador(out, 'salida'), filas, vocab, paso, d);
       return Promise.resolve(out);
     },
   };
