@@ -762,10 +762,14 @@ napi_value RopeTable(napi_env env, napi_callback_info info) {
   eff_ctx *ctx = external<eff_ctx>(env, a[0]);
   void *f = nullptr;
   size_t len = 0;
-  if (!bytes_of(env, a[1], &f, &len) || len % 8 || ((uintptr_t)f & 7))
+  napi_typedarray_type t;
+  if (napi_get_typedarray_info(env, a[1], &t, nullptr, nullptr, nullptr, nullptr) != napi_ok || t != napi_float64_array ||
+      !bytes_of(env, a[1], &f, &len))
     return throw_msg(env, "ropeTable: the frequencies must be a Float64Array");
-  return status(env, ctx, eff_rope_table(ctx, (const double *)f, (uint32_t)(len / 8), (uint32_t)i64(env, a[2]),
-                                         (float)f64(env, a[3], 1.0), external<eff_buf>(env, a[4])));
+  const uint32_t positions = u32(env, a[2], "positions");
+  const float scale = (float)number(env, a[3], "scale", 1.0);
+  if (thrown(env)) return nullptr;
+  return status(env, ctx, eff_rope_table(ctx, (const double *)f, (uint32_t)(len / 8), positions, scale, external<eff_buf>(env, a[4])));
 }
 
 // kvAppend(ctx, cache, batch, rows)

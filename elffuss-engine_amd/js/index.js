@@ -955,10 +955,11 @@ function createKvOps(device, deps) {
       }
       return Object.assign({}, o, { buf: device.createBuffer({ size: bytes * o.paginas, label: 'kv' }) });
     },
-    // cos and sin of position * freqs[i], once per model.
+    // cos and sin of position * freqs[i] (a Float64Array), once per model.
     tablaRope(freqs, posiciones, escala) {
+      if (!freqs || freqs[Symbol.toStringTag] !== 'Float64Array') throw invalido('tablaRope: las frecuencias van en un Float64Array');
       const out = device.createBuffer({ size: posiciones * freqs.length * 8, label: 'rope' });
-      native.ropeTable(device._ctx, freqs, posiciones, escala === undefined ? 1 : escala, out._h);
+      native.ropeTable(device._ctx, freqs, posiciones, escala, out._h);
       return out;
     },
     // New k, v rows into the cache; q rotated into a pooled buffer, which it resolves to (null without q).

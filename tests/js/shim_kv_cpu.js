@@ -57,4 +57,13 @@ invalido(() => native.kvAttn(undefined, {}, {}, undefined, 0, 0, undefined, 1, '
 invalido(() => native.kvAppend(undefined, {}, {}, { q: null, qNorm: undefined, ropeDim: null }), /elffuss_amd error/);
 invalido(() => native.kvAttn(undefined, {}, {}, undefined, undefined, undefined, undefined, 1, 1), /elffuss_amd error/);
 invalido(() => native.logitsApply(undefined, undefined, undefined, 1, 64, undefined, {}), /elffuss_amd error/);
+
+// the rotation's frequencies are 64-bit numbers: the bytes of other arrays are not read as such
+for (const mal of [new Float32Array(8), new Uint32Array(8), new Uint8Array(64), new ArrayBuffer(64), new DataView(new ArrayBuffer(64)), [1, 2], undefined]) {
+  invalido(() => native.ropeTable(undefined, mal, 16, 1, undefined), /Float64Array/);
+  invalido(() => kv.tablaRope(mal, 16), /Float64Array/);
+}
+for (const mal of ['16', -1, 0.5]) invalido(() => native.ropeTable(undefined, new Float64Array(4), mal, 1, undefined), /^positions:/);
+invalido(() => native.ropeTable(undefined, new Float64Array(4), 16, '1', undefined), /^scale:/);
+invalido(() => native.ropeTable(undefined, new Float64Array(4), 16, undefined, undefined), /elffuss_amd error/);
 console.log('shim_kv_cpu ok');
