@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <chrono>
 #include <deque>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -1540,6 +1541,24 @@ bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
   return an && bn && x < y + bn && y < x + an;
 }
 
+// What a call reads or writes.
+struct Span {
+  const void *p;
+  uint64_t n;
+};
+
+// Whether a call writes `out` where it reads: in any order of its workgroups.
+bool over(const Span &out, std::initializer_list<Span> in) {
+  for (const Span &s : in)
+    if (overlap(out.p, out.n, s.p, s.n)) return true;
+  return false;
+}
+
+Span kv_span(const KvView &kv) { return {kv.base, kv.pages * kv.page_bytes}; }
+bool over_batch(const Span &out, const KvBatchView &b) {
+  return over(out, {{b.table, 4ull * b.seqs * b.table_pages}, {b.starts, 4ull * (b.seqs + 1ull)}, {b.lens, 4ull * b.seqs}});
+}
+
 // Bytes from a row view's first float to its last.
 uint64_t row_span(uint32_t stride, uint64_t n, uint32_t tokens) {
   return tokens ? ((uint64_t)(tokens - 1u) * stride + n) * 4u : 0u;
@@ -1616,6 +1635,14 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
   a.k_norm = r->k_norm ? (const float *)r->k_norm->ptr : nullptr;
   a.eps = r->norm_eps;
   if (b.tokens == 0) return EFF_OK;
+  const Span cached = kv_span(kv), turned = {a.q_out, (uint64_t)b.tokens * nq * 4u};
+  const Span rope = {a.rope, 4ull * r->rope_positions * a.rope_dim}, qn = {a.q_norm, 4ull * kv.dim}, kn = {a.k_norm, 4ull * kv.dim};
+  if (over(cached, {{a.k, row_span(a.k_stride, nk, b.tokens)}, {a.v, row_span(a.v_stride, nk, b.tokens)},
+                    {a.q, a.q ? row_span(a.q_stride, nq, b.tokens) : 0u}, turned, rope, qn, kn}) ||
+      over_batch(cached, b))
+    return fail(ctx, EFF_E_INVALID, "kv append: the cache overlaps what the call reads, or q_out");
+  if (over(turned, {rope, qn, kn}) || over_batch(turned, b))
+    return fail(ctx, EFF_E_INVALID, "kv append: q_out overlaps what the call reads");
   if ((uint64_t)b.tokens * (r->q_heads + 2ull * kv.heads) > 0x7FFFFFFFull)
     return fail(ctx, EFF_E_SHAPE, "kv append: %u tokens of %u + 2 x %u heads", b.tokens, r->q_heads, kv.heads);
   if ((rc = use_device(ctx))) return rc;
@@ -1644,6 +1671,9 @@ int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *bat
   a.out = (float *)out->ptr;
   if (overlap(a.q, row_span(a.q_stride, n, b.tokens), a.out, (uint64_t)b.tokens * n * 4u))
     return fail(ctx, EFF_E_INVALID, "kv attn: q and out overlap");
+  const Span rows = {a.out, (uint64_t)b.tokens * n * 4u};
+  if (over(rows, {kv_span(kv)}) || over_batch(rows, b))
+    return fail(ctx, EFF_E_INVALID, "kv attn: out overlaps the cache or the batch");
   a.q_heads = q_heads;
   a.scale = scale;
   a.window = window;

@@ -534,7 +534,8 @@ typedef struct eff_kv_batch {
  * the buffer's start, a stride in floats from token to token (0: the row's
  * own size); both multiples of 4. One buffer may hold q, k and v (the output
  * of one projection). q may be NULL with q_heads = 0. q_out is [tokens][q_heads * head_dim]; it
- * may be q's own buffer only where q has that layout.
+ * may be q's own buffer only where q has that layout. What the call writes (the
+ * cache's pages, q_out) may not overlap anything else that it reads.
  *   q_norm, k_norm  f32 [head_dim] or NULL: RMS norm weights, with norm_eps
  *   rope            f32 [rope_positions][2][rope_dim / 2], cos then sin
  *                   (eff_rope_table); NULL with rope_dim = 0: no rotation.
@@ -572,7 +573,7 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
  * nothing gives zeros. What lies in the cache at positions it does not see does
  * not reach its output, whatever bits it has; a NaN or an infinity among what
  * it sees does, and so does a score past f32's range: the row's output is not
- * finite. q and out may not overlap. f32-accurate. */
+ * finite. out may not overlap q, the cache or the batch's buffers. f32-accurate. */
 int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
                 uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window);
 
