@@ -1611,7 +1611,7 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
     a.q_heads = r->q_heads;
     // in place a row is read by the lanes that write it, if it is where it was
     const uint64_t out = (uint64_t)b.tokens * nq * 4u;
-    const bool same = a.q == a.q_out && a.q_stride == nq;
+    const bool same = a.q == a.q_out && (a.q_stride == nq || b.tokens == 1u);
     if ((!same && overlap(a.q, row_span(a.q_stride, nq, b.tokens), a.q_out, out)) ||
         overlap(a.k, row_span(a.k_stride, nk, b.tokens), a.q_out, out) ||
         overlap(a.v, row_span(a.v_stride, nk, b.tokens), a.q_out, out))

@@ -534,7 +534,7 @@ typedef struct eff_kv_batch {
  * the buffer's start, a stride in floats from token to token (0: the row's
  * own size); both multiples of 4. One buffer may hold q, k and v (the output
  * of one projection). q may be NULL with q_heads = 0. q_out is [tokens][q_heads * head_dim]; it
- * may be q's own buffer only where q has that layout. What the call writes (the
+ * may be q's own buffer only where q has that layout (one token's always has). What the call writes (the
  * cache's pages, q_out) may not overlap anything else that it reads.
  *   q_norm, k_norm  f32 [head_dim] or NULL: RMS norm weights, with norm_eps
  *   rope            f32 [rope_positions][2][rope_dim / 2], cos then sin

@@ -93,3 +93,24 @@ def test_no_tokens(ctx, eff):
     cache = eff.KvCache(F16, HEADS, DIM, PAGE, PAGES, x)
     ctx.kv_append(cache, batch, eff.KvRows(k=x, v=x))
     ctx.kv_attn(cache, batch, x, x, Q_HEADS, 0.1)
+
+
+def test_one_token_in_place(ctx, eff):
+    """q turned within a fused row: a single token's q is its buffer's first floats whatever the stride."""
+    rng = np.random.default_rng(1)
+    fused = (Q_HEADS + 2 * HEADS) * DIM
+    row = rng.standard_normal(fused).astype(np.float32)
+    x, kept = ctx.upload(row), ctx.upload(row)
+    rope, other = ctx.rope_table(1e4 ** (-np.arange(0, DIM, 2) / DIM), LEN), ctx.alloc(Q_HEADS * DIM * 4)
+    b = [ctx.upload(np.array(v, np.uint32)) for v in ([1], [0, 1], [5])]
+    batch = eff.KvBatch(*b, seqs=1, tokens=1, table_pages=1, max_new=1, max_len=LEN)
+    got = []
+    for rows, q_out in ((kept, other), (x, x)):
+        buf = ctx.alloc(CACHE)
+        ctx.kv_append(eff.KvCache(F16, HEADS, DIM, PAGE, PAGES, buf), batch,
+                      eff.KvRows(q=rows, k=(rows, Q_HEADS * DIM), v=(rows, (Q_HEADS + HEADS) * DIM), q_stride=fused, k_stride=fused,
+                                 v_stride=fused, q_heads=Q_HEADS, q_out=q_out, rope=rope, rope_positions=LEN, rope_dim=DIM))
+        got.append((q_out.read(np.float32, Q_HEADS * DIM), buf.read()))
+    assert np.array_equal(got[0][0], got[1][0]) and np.array_equal(got[0][1], got[1][1]) and got[0][1].any()
+    assert not np.array_equal(got[0][0], row[:Q_HEADS * DIM])
+    assert np.array_equal(x.read(np.float32)[Q_HEADS * DIM:], row[Q_HEADS * DIM:])
