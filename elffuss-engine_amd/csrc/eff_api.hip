@@ -1541,7 +1541,7 @@ bool overlap(const void *a, uint64_t an, const void *b, uint64_t bn) {
   return an && bn && x < y + bn && y < x + an;
 }
 
-// What a call reads or writes.
+// What a call reads or writes (null: nothing).
 struct Span {
   const void *p;
   uint64_t n;
@@ -1550,7 +1550,7 @@ struct Span {
 // Whether a call writes `out` where it reads: in any order of its workgroups.
 bool over(const Span &out, std::initializer_list<Span> in) {
   for (const Span &s : in)
-    if (overlap(out.p, out.n, s.p, s.n)) return true;
+    if (s.p && overlap(out.p, out.n, s.p, s.n)) return true;
   return false;
 }
 
@@ -1638,7 +1638,7 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
   const Span cached = kv_span(kv), turned = {a.q_out, (uint64_t)b.tokens * nq * 4u};
   const Span rope = {a.rope, 4ull * r->rope_positions * a.rope_dim}, qn = {a.q_norm, 4ull * kv.dim}, kn = {a.k_norm, 4ull * kv.dim};
   if (over(cached, {{a.k, row_span(a.k_stride, nk, b.tokens)}, {a.v, row_span(a.v_stride, nk, b.tokens)},
-                    {a.q, a.q ? row_span(a.q_stride, nq, b.tokens) : 0u}, turned, rope, qn, kn}) ||
+                    {a.q, row_span(a.q_stride, nq, b.tokens)}, turned, rope, qn, kn}) ||
       over_batch(cached, b))
     return fail(ctx, EFF_E_INVALID, "kv append: the cache overlaps what the call reads, or q_out");
   if (over(turned, {rope, qn, kn}) || over_batch(turned, b))
@@ -1733,6 +1733,10 @@ int eff_logits_apply(eff_ctx *ctx, eff_buf *in, eff_buf *out, uint32_t rows, uin
     a.mask_count = r->mask_count;
   }
   if (rows == 0) return EFF_OK;
+  // (where the lists of history and biases end is for the device to say)
+  if (over({a.out, bytes}, {{a.history_starts, 4ull * (rows + 1ull)}, {a.penalties, 24ull * rows}, {a.bias_starts, 4ull * (rows + 1ull)},
+                            {a.mask, (uint64_t)a.mask_count * ((vocab + 31ull) / 32u) * 4u}, {a.mask_of, 4ull * rows}}))
+    return fail(ctx, EFF_E_INVALID, "logits: out overlaps what the rules read");
   if ((uint64_t)rows * (vocab / 1024u + 1ull) > 0x7FFFFFFFull)
     return fail(ctx, EFF_E_SHAPE, "logits: %u rows of %u", rows, vocab);
   if ((rc = use_device(ctx))) return rc;

@@ -599,7 +599,8 @@ typedef struct eff_logits_rules {
 /* out[r][v] from in[r][v], f32 rows `stride` floats apart (0: vocab): for a token c > 0 times
  * in the history z = z > 0 ? z / repeat : z * repeat, then z -= frequency * c +
  * presence (each in 64 bits, rounded to f32); then z += bias; then -inf where the
- * mask does not allow it. out may be in (the same buffer). With frequency = 0
+ * mask does not allow it. out may be in (the same buffer), and may not overlap
+ * anything else that the call reads. With frequency = 0
  * the penalties are sample()'s (sample.js:78-153), bit for bit, over a window
  * that the caller cuts; eff_topk reads a row (base = r * stride). */
 int eff_logits_apply(eff_ctx *ctx, eff_buf *in, eff_buf *out, uint32_t rows, uint32_t vocab, uint32_t stride,
