@@ -116,6 +116,8 @@ class Decoder:
 
 def decode(eff, ctx, model, prompts, steps, rules):
     """The tokens of `steps` steps of each prompt, and the processed logits of each step [steps][requests][vocab]."""
+    if not prompts or not all(len(p) for p in prompts) or steps < 1:
+        raise ValueError("decode: prompts of one token or more, and a step or more")   # the first step reads a prompt's last row
     n, max_len = len(prompts), max(len(p) for p in prompts) + steps
     d = Decoder(eff, ctx, model, n, max_len, rules)
     sequences, logits = [list(p) for p in prompts], []
