@@ -55,21 +55,14 @@ __device__ __forceinline__ half8 join8(const half2v v[4]) {
   return half8{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
 }
 
-template <int N>
-__device__ __forceinline__ void ld_words(uint32_t *o, const uint8_t *p) {
-  if constexpr (N == 1) {
-    *o = *(const uint32_t *)p;
-  } else if constexpr (N == 2) {
-    const uint2 v = *(const uint2 *)p;
-    o[0] = v.x, o[1] = v.y;
-  } else {
-    const u32x4 v = *(const u32x4 *)p;
+// 16 bytes of LDS.
+__device__ __forceinline__ void ld_lds(uint32_t *o, const uint8_t *p) {
+  const u32x4 v = *(const u32x4 *)p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = v[i];
-  }
+  for (int i = 0; i < 4; ++i) o[i] = v[i];
 }
 
-// The same of the cache. An address made of two words may be LDS for all the compiler
+// 4 N bytes of the cache. An address made of two words may be LDS for all the compiler
 // knows: without its space named the loads would be counted with LDS's, and a wait for
 // one of them would wait for all that are under way.
 template <typename T>
@@ -1196,8 +1189,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int c = 0; c < W::KS; ++c) ld_words<4>(w.kw[u] + 4 * c, lds + (TURN ? ka[0] ^ (64u * c) : ka[TURN ? 0 : c]) + u * S::HALF);
-          if constexpr (I8) ld_words<4>(w.ks[u], lds + S::SCALES + 64u * u + 16u * g);
+          for (int c = 0; c < W::KS; ++c) ld_lds(w.kw[u] + 4 * c, lds + (TURN ? ka[0] ^ (64u * c) : ka[TURN ? 0 : c]) + u * S::HALF);
+          if constexpr (I8) ld_lds(w.ks[u], lds + S::SCALES + 64u * u + 16u * g);
         }
         __builtin_amdgcn_sched_barrier(0);
         float s[2][4];
