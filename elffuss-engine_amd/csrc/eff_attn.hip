@@ -393,6 +393,12 @@ struct AttnWave {
   static constexpr int KW = I8 ? 2 : 4;                // words of a lane's part of a step of K
   static constexpr int VW = I8 ? (E + 3) / 4 : E / 2;  // words of a lane's part of a row of V
   static constexpr int ROW = I8 ? D : 2 * D;           // bytes of a row as it arrives
+  // fp16 weights are scaled by 2^14, in the exponent itself where instruction issue
+  // bounds the kernel (V not in rows: prompts of 64-wide heads 123 us, else 130). Next
+  // to 14 the exponent has 4 bits less than next to 0, where it is computed elsewhere:
+  // 9.2e-8 -> 6.2e-8 of 3 tokens' output, 2.4e-7 -> 2.0e-7 of 150's (f32 throughout
+  // 5.0e-8 and 3.8e-7); of prompts' 2.6e-7 -> 2.3e-7 (3.4e-7).
+  static constexpr bool RAISED = !SCALED && VIN != kVRows;
 
   half8 qh[QL ? 1 : KS], ql[QL ? 1 : KS];
   const uint8_t *qs;    // QL: [step][part][lane] of 16 bytes
@@ -625,7 +631,7 @@ struct AttnWave {
         for (int i = 0; i < E; ++i) acc[i] *= f;
       }
     }
-    const float up = m == -INFINITY ? 0.f : SCALED ? -(m * sc) : 14.f - m * sc;
+    const float up = m == -INFINITY ? 0.f : RAISED ? 14.f - m * sc : -(m * sc);
     float sum = low == -INFINITY ? NAN : 0.f;
     float p[8];
     u32x4 scale = {};
@@ -634,6 +640,7 @@ struct AttnWave {
       if (SCALED && k % 4 == 0) scale = scales(k / 4);
       const float y = s[k / 4][k % 4];
       p[k] = __builtin_amdgcn_exp2f(fmaf(y, sc, up));
+      if constexpr (!SCALED && !RAISED) p[k] *= 0x1p14f;
       sum += p[k];
       // a weight of nothing takes nothing of a scale that is not finite
       if constexpr (SCALED) p[k] = masked && y == -INFINITY ? 0.f : p[k] * __uint_as_float(scale[k % 4]);
