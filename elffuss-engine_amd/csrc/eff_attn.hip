@@ -805,8 +805,10 @@ __device__ __forceinline__ void from_lds(T &to, const T &from) {
 // 128 on 8: 358 us, 5.9 TB/s; one of 130001: 95 us, 5.6 TB/s). The matrix unit is busy
 // 8 % of the time there, so the second parts of q and p are free. int8 rows are half
 // the bytes with as many instructions, which shows where the shares are short (40 up
-// to 9001, 16 heads of 256 on 2: 48 us, 3.4 TB/s). A single short sequence is round
-// trips: lengths, page table, K, V, the join (517 tokens: 7.3 us, an empty launch 3.4).
+// to 9001, 16 heads of 256 on 2: 43 to 46 us, 3.6 to 3.9 TB/s). A single short sequence
+// is round trips: lengths, page table, K, V, the join (517 tokens: 6.3 to 6.8 us, an
+// empty launch 3.4). Shares that go on keep 26 to 47 scalar registers in vector ones
+// (3 of those in scratch for fp16 256 wide), outside the steps.
 template <int TYPE, int D, int NW, int MODE>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part) {
   constexpr bool I8 = TYPE == EFF_KV_I8, QL = D == 256;   // 256 wide, q's parts would take a quarter of the registers
@@ -1013,16 +1015,20 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
 // next. fp16 pages go straight to LDS; int8 ones are requested before the step and
 // converted after it, once for the four waves.
 // K's 16-byte pieces are turned within their row, and V's 32-byte ones, so that the
-// 16 rows of an operand lie in different banks; V's operand comes out of LDS turned
-// (ds_read_b64_tr_b16: of 16 lanes, lane 4 j + q reads 4 values of row j, and lane c
-// gets column c of the 4 rows).
+// rows of an operand lie in different banks (V's 16 all do; K's, turned by 8 places, two
+// to a bank from 128 wide on, a third of the LDS's active cycles: with 16 places there
+// were no conflicts, and 186 -> 185 us of the prompts below, 237 -> 232 of int8); V's
+// operand comes out of LDS turned (ds_read_b64_tr_b16: of 16 lanes, lane 4 j + q reads 4
+// values of row j, and lane c gets column c of the 4 rows).
 //
-// Instruction issue bounds it: per step of 32 tokens x 16 rows x 128 a wave has 64
-// matrix instructions of 16 cycles and as many cycles of the softmax's VALU, and three
-// waves a SIMD overlap them to 44 + 44 % of the busy time (3 x 1000 new tokens at lengths up to 3001, 32
-// heads of 128 on 8: 181 us, 440 TFLOP/s of the product itself, 880 with q's and p's
-// second parts, where a large fp16 product reaches 1090). Three buffers, two steps ahead, were
-// no faster (185 us): the loads are not waited for.
+// Instruction issue bounds it: per step of 32 tokens x 16 rows x 128 a wave has 32
+// matrix instructions of 16 cycles and 106 of the softmax, the operands and the walk of
+// 4 and more, and three waves a SIMD overlap them to 44 and 37 % of the busy time (3 x
+// 1000 new tokens at lengths up to 3001, 32 heads of 128 on 8: 181 to 190 us, 440
+// TFLOP/s of the product itself, 880 with q's and p's second parts, where a large fp16
+// product reaches 1090; of int8 239, where the conversions are VALU work too). Three
+// buffers, two steps ahead, were no faster (185 us): the loads are not waited for. At
+// 256 wide 2 (fp16) and 9 (int8) registers are in scratch.
 template <int D>
 struct AttnStage {
   static constexpr uint32_t ROW = 2 * D, PIECES = ROW / 16u;
@@ -1262,18 +1268,22 @@ static AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // workgroup has a tile, as where there are 5 units or fewer (4 at 256 wide): a join
   // takes time (1 x 8 heads of 64 over 517 tokens: 6.8 us, shared 7.6, over 1000 9.3
   // and 8.0; 24 x 8 heads of drafts that see 1024 tokens 14.7, shared 22.0; heads of one
-  // token up to 2000: 16 x 8 22.6, shared 18.3, 32 x 8 35.5 and 45.5).
+  // token up to 2000: 16 x 8 22.6, shared 18.3, 32 x 8 35.5 and 45.5; 24 x 8 up to 1500
+  // 19.4, shared 22.5, up to 3000 44.6 and 42.3, in between either way; 480 x 8 heads of
+  // 64 up to 3000 287, shared 288, 1000 x 8 552 and 567).
   const uint64_t units = (span + kUnit - 1u) / kUnit, each = (most + R - 1u) / R;
   if ((wgs < 171u || span > 2176u) && wgs < 4096u && units > (kv.dim < 256u ? 5u : 4u) && each * b.seqs * units < 1u << 31) {
     // Two workgroups to a CU, or one where its waves have enough bytes under way: 256
     // wide (24 x 2 heads up to 8000 48.9 us, two 54.1; of int8 33.6 and 35.0), or fp16
-    // rows of 128 and long shares (1 x 8 up to 130001 96.7, two 99.4; 8 x 8 drafts up to
-    // 5000, short ones, 30.6 and 28.1). Less wide they take two (16 x 8 of int8 up to
-    // 30000 102, two 99).
+    // rows of 128 and long shares (1 x 8 up to 130001 96.7, two 99.4; 24 x 8 up to 6000
+    // 69.2 and 71.1; 8 x 8 drafts up to 5000, short ones, 30.6 and 28.1; next to the
+    // limit, 16 x 8 up to 8000, 68.8 and 63.5). Less wide they take two (16 x 8 of int8
+    // up to 30000 102, two 99).
     // Shares that may go on into the next tile pay where they are long (64 x 8 up to
-    // 16384 357 us, ending with a tile 411; 24 x 8 up to 6000 69, 93); 256 wide, where
-    // the scalar registers of that take vector ones, only with many tiles (100 x 2 of
-    // int8 up to 9000 115, 156; 24 x 2 up to 30000 76, 73).
+    // 16384 357 us, ending with a tile 411; 24 x 8 up to 6000 70, 93, up to 3000 42.1,
+    // 41.5; below the limit from shares of 12 on they would too, up to 4000 55, 77); 256
+    // wide, where the scalar registers of that take vector ones, only with many tiles
+    // (100 x 2 of int8 up to 9000 115, 156; 24 x 2 up to 30000 76, 73).
     uint64_t slots = 512u;
     const uint64_t share = wgs * units / slots;
     const bool wide = kv.dim >= 256u;
