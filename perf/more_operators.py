@@ -412,7 +412,8 @@ def _handles(case, s):
     p = {"buffers": b}
     if case["op"] in ("fork", "keep"):
         each = s["cache"][0].numel() * s["cache"].element_size()
-        p["layers"] = [eff.KvCache(t, kv, d, page, s["cache"].shape[1], _buffer(s["cache"].data_ptr() + i * each, each)) for i in range(case["layers"])]
+        p["layers"] = eff.KvLayers(eff.KvCache(t, kv, d, page, s["cache"].shape[1], _buffer(s["cache"].data_ptr() + i * each, each))
+                                   for i in range(case["layers"]))
     if case["op"] == "fork":
         return p
     p["batch"] = eff.KvBatch(b["table"], b["starts"], b["lens"], seqs=case["seqs"], tokens=s["seq"].numel(), table_pages=s["table"].shape[1],
