@@ -1482,16 +1482,31 @@ int eff_topk_noalloc(eff_ctx *ctx, eff_buf *logits, uint32_t base, uint32_t voca
 
 namespace {
 
-// The view of a cache and the batch of a call, checked. `who` names the call.
-int kv_views(eff_ctx *ctx, const eff_kv_cache *c, const eff_kv_batch *b, KvView &kv, KvBatchView &bv, const char *who) {
-  if (!c || !b) return fail(ctx, EFF_E_INVALID, "%s: null cache or batch", who);
+// The view of a cache, checked. `who` names the call.
+int kv_cache_view(eff_ctx *ctx, const eff_kv_cache *c, KvView &kv, const char *who) {
   if (!kv_type_known(c->type)) return fail(ctx, EFF_E_TYPE, "%s: unsupported cache type %d", who, c->type);
   const size_t page = eff_kv_page_bytes(c->type, c->heads, c->head_dim, c->page_tokens);
   if (!page)
     return fail(ctx, EFF_E_SHAPE, "%s: no cache of %u heads of %u values in pages of %u tokens", who, c->heads,
                 c->head_dim, c->page_tokens);
   if (c->pages == 0) return fail(ctx, EFF_E_INVALID, "%s: a cache without pages", who);
-  int rc = check_out(ctx, c->buf, (uint64_t)c->pages * page, who);
+  const int rc = check_out(ctx, c->buf, (uint64_t)c->pages * page, who);
+  if (rc) return rc;
+  kv.base = (uint8_t *)c->buf->ptr;
+  kv.type = c->type;
+  kv.heads = c->heads;
+  kv.dim = c->head_dim;
+  kv.page_log2 = (uint32_t)__builtin_ctz(c->page_tokens);
+  kv.pages = c->pages;
+  kv.block_bytes = kv_block_bytes(c->type, c->head_dim, c->page_tokens);
+  kv.page_bytes = page;
+  return EFF_OK;
+}
+
+// The same of the batch of a call too.
+int kv_views(eff_ctx *ctx, const eff_kv_cache *c, const eff_kv_batch *b, KvView &kv, KvBatchView &bv, const char *who) {
+  if (!c || !b) return fail(ctx, EFF_E_INVALID, "%s: null cache or batch", who);
+  int rc = kv_cache_view(ctx, c, kv, who);
   if (rc) return rc;
   if (b->seqs == 0 || b->table_pages == 0 || b->max_new == 0 || b->max_len == 0)
     return fail(ctx, EFF_E_INVALID, "%s: empty batch seqs=%u table_pages=%u max_new=%u max_len=%u", who, b->seqs,
@@ -1505,14 +1520,6 @@ int kv_views(eff_ctx *ctx, const eff_kv_cache *c, const eff_kv_batch *b, KvView 
       (rc = check_out(ctx, b->starts, 4ull * (b->seqs + 1ull), who)) ||
       (rc = check_out(ctx, b->lens, 4ull * b->seqs, who)))
     return rc;
-  kv.base = (uint8_t *)c->buf->ptr;
-  kv.type = c->type;
-  kv.heads = c->heads;
-  kv.dim = c->head_dim;
-  kv.page_log2 = (uint32_t)__builtin_ctz(c->page_tokens);
-  kv.pages = c->pages;
-  kv.block_bytes = kv_block_bytes(c->type, c->head_dim, c->page_tokens);
-  kv.page_bytes = page;
   bv = {(const uint32_t *)b->table->ptr, (const uint32_t *)b->starts->ptr, (const uint32_t *)b->lens->ptr,
         b->seqs, b->tokens, b->table_pages, b->max_new, b->max_len};
   return EFF_OK;
@@ -1589,6 +1596,11 @@ int eff_rope_table(eff_ctx *ctx, const double *freqs, uint32_t n, uint32_t posit
 }
 
 int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *r) {
+  return eff_kv_append_at(ctx, cache, batch, r, nullptr);
+}
+
+int eff_kv_append_at(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *r,
+                     const eff_kv_turns *turns) {
   if (!ctx) return EFF_E_INVALID;
   KvView kv;
   KvBatchView b;
@@ -1622,12 +1634,26 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
       return fail(ctx, EFF_E_SHAPE, "kv append: rope_dim=%u must be a multiple of 4 up to %u", r->rope_dim, kv.dim);
     if (r->rope_mode > EFF_ROPE_HALVES) return fail(ctx, EFF_E_INVALID, "kv append: rope_mode=%u", r->rope_mode);
     if ((rc = check_out(ctx, r->rope, 4ull * r->rope_positions * r->rope_dim, "kv append rope"))) return rc;
-    if (r->rope_positions < b.max_len)
+    if (turns && r->rope_positions == 0) return fail(ctx, EFF_E_BOUNDS, "kv append: a rope table without positions");
+    if (!turns && r->rope_positions < b.max_len)
       return fail(ctx, EFF_E_BOUNDS, "kv append: the rope table has %u positions and max_len=%u", r->rope_positions,
                   b.max_len);
     a.rope = (const float *)r->rope->ptr;
     a.rope_dim = r->rope_dim;
     a.halves = r->rope_mode == EFF_ROPE_HALVES;
+  }
+  KvTurnsView tv{};
+  if (turns) {
+    if (!r->rope_dim) return fail(ctx, EFF_E_INVALID, "kv append: positions to turn by, and no rotation");
+    if (turns->axes == 0 || turns->axes > EFF_KV_AXES_MAX)
+      return fail(ctx, EFF_E_SHAPE, "kv append: axes=%u (1..%u)", turns->axes, EFF_KV_AXES_MAX);
+    for (uint32_t i = 0; i < r->rope_dim / 2u; ++i)
+      if (turns->axis[i] >= turns->axes)
+        return fail(ctx, EFF_E_INVALID, "kv append: pair %u turns by axis %u of %u", i, turns->axis[i], turns->axes);
+    if ((rc = check_out(ctx, turns->at, 4ull * turns->axes * b.tokens, "kv append positions"))) return rc;
+    tv.at = (const uint32_t *)turns->at->ptr;
+    tv.tokens = b.tokens, tv.positions = r->rope_positions;
+    memcpy(tv.axis, turns->axis, r->rope_dim / 2u);
   }
   if (r->q_norm && (rc = check_out(ctx, r->q_norm, 4ull * kv.dim, "kv append q_norm"))) return rc;
   if (r->k_norm && (rc = check_out(ctx, r->k_norm, 4ull * kv.dim, "kv append k_norm"))) return rc;
@@ -1637,16 +1663,17 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
   if (b.tokens == 0) return EFF_OK;
   const Span cached = kv_span(kv), turned = {a.q_out, (uint64_t)b.tokens * nq * 4u};
   const Span rope = {a.rope, 4ull * r->rope_positions * a.rope_dim}, qn = {a.q_norm, 4ull * kv.dim}, kn = {a.k_norm, 4ull * kv.dim};
+  const Span at = {tv.at, turns ? 4ull * turns->axes * b.tokens : 0u};
   if (over(cached, {{a.k, row_span(a.k_stride, nk, b.tokens)}, {a.v, row_span(a.v_stride, nk, b.tokens)},
-                    {a.q, row_span(a.q_stride, nq, b.tokens)}, turned, rope, qn, kn}) ||
+                    {a.q, row_span(a.q_stride, nq, b.tokens)}, turned, rope, qn, kn, at}) ||
       over_batch(cached, b))
     return fail(ctx, EFF_E_INVALID, "kv append: the cache overlaps what the call reads, or q_out");
-  if (over(turned, {rope, qn, kn}) || over_batch(turned, b))
+  if (over(turned, {rope, qn, kn, at}) || over_batch(turned, b))
     return fail(ctx, EFF_E_INVALID, "kv append: q_out overlaps what the call reads");
   if ((uint64_t)b.tokens * (r->q_heads + 2ull * kv.heads) > 0x7FFFFFFFull)
     return fail(ctx, EFF_E_SHAPE, "kv append: %u tokens of %u + 2 x %u heads", b.tokens, r->q_heads, kv.heads);
   if ((rc = use_device(ctx))) return rc;
-  hipError_t e = launch_kv_append(kv, b, a, ctx->stream);
+  hipError_t e = launch_kv_append(kv, b, a, turns ? &tv : nullptr, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "kv append launch");
   ++ctx->stats.kv_append;
   return EFF_OK;
@@ -1690,6 +1717,100 @@ int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *bat
   if (e != hipSuccess) return hip_fail(ctx, e, "kv attn launch");
   ++ctx->stats.kv_attn;
   return EFF_OK;
+}
+
+namespace {
+
+// The caches of a call's layers, checked: `each` of them as the first, but for its
+// memory, which none shares with another.
+int kv_layers(eff_ctx *ctx, const eff_kv_cache *c, uint32_t layers, KvView &kv, std::vector<uint8_t *> &bases, const char *who) {
+  if (!c || layers == 0 || layers > 65536u) return fail(ctx, EFF_E_INVALID, "%s: null caches or layers=%u", who, layers);
+  for (uint32_t i = 0; i < layers; ++i) {
+    if (c[i].type != c->type || c[i].heads != c->heads || c[i].head_dim != c->head_dim || c[i].page_tokens != c->page_tokens ||
+        c[i].pages != c->pages)
+      return fail(ctx, EFF_E_SHAPE, "%s: the cache of layer %u is not like the first", who, i);
+    KvView v;
+    const int rc = kv_cache_view(ctx, &c[i], v, who);
+    if (rc) return rc;
+    if (i == 0) kv = v;
+    bases.push_back(v.base);
+  }
+  std::vector<uint8_t *> order(bases);
+  std::sort(order.begin(), order.end());
+  for (uint32_t i = 1; i < layers; ++i)
+    if ((uint64_t)(order[i] - order[i - 1u]) < kv.pages * kv.page_bytes)
+      return fail(ctx, EFF_E_INVALID, "%s: the caches of two layers overlap", who);
+  return EFF_OK;
+}
+
+// Whether a call that writes the layers' caches reads one of `in` there.
+bool over_layers(const KvView &kv, const std::vector<uint8_t *> &bases, std::initializer_list<Span> in) {
+  for (uint8_t *p : bases)
+    if (over({p, kv.pages * kv.page_bytes}, in)) return true;
+  return false;
+}
+
+// A launch for each group of layers.
+template <typename F>
+hipError_t each_layers(const std::vector<uint8_t *> &bases, F launch) {
+  for (size_t at = 0; at < bases.size(); at += kKvLayers) {
+    const uint32_t n = (uint32_t)std::min<size_t>(kKvLayers, bases.size() - at);
+    KvLayers l{};
+    std::copy_n(bases.begin() + at, n, l.base);
+    const hipError_t e = launch(l, n, at == 0);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+int eff_kv_copy(eff_ctx *ctx, const eff_kv_cache *caches, uint32_t layers, eff_buf *copies, uint32_t count) try {
+  if (!ctx) return EFF_E_INVALID;
+  KvView kv;
+  std::vector<uint8_t *> bases;
+  int rc = kv_layers(ctx, caches, layers, kv, bases, "kv copy");
+  if (rc || (rc = check_out(ctx, copies, 12ull * count, "kv copy"))) return rc;
+  if (count == 0) return EFF_OK;
+  if (over_layers(kv, bases, {{copies->ptr, 12ull * count}}))
+    return fail(ctx, EFF_E_INVALID, "kv copy: a cache overlaps the list of copies");
+  if ((rc = use_device(ctx))) return rc;
+  const hipError_t e = each_layers(bases, [&](const KvLayers &l, uint32_t n, bool) {
+    return launch_kv_copy(kv, l, n, (const uint32_t *)copies->ptr, count, ctx->stream);
+  });
+  if (e != hipSuccess) return hip_fail(ctx, e, "kv copy launch");
+  ++ctx->stats.kv_copy;
+  return EFF_OK;
+} catch (const std::exception &e) {
+  return fail(ctx, EFF_E_NOMEM, "kv copy: %s", e.what());
+}
+
+int eff_kv_keep(eff_ctx *ctx, const eff_kv_cache *caches, uint32_t layers, const eff_kv_batch *batch, eff_buf *kept,
+                eff_buf *counts, eff_buf *new_lens) try {
+  if (!ctx) return EFF_E_INVALID;
+  KvView kv;
+  KvBatchView b;
+  std::vector<uint8_t *> bases;
+  int rc = kv_layers(ctx, caches, layers, kv, bases, "kv keep");
+  if (rc || (rc = kv_views(ctx, caches, batch, kv, b, "kv keep")) ||
+      (rc = check_out(ctx, kept, 4ull * b.tokens, "kv keep kept")) || (rc = check_out(ctx, counts, 4ull * b.seqs, "kv keep counts")) ||
+      (new_lens && (rc = check_out(ctx, new_lens, 4ull * b.seqs, "kv keep new_lens"))))
+    return rc;
+  const Span lens = {new_lens ? new_lens->ptr : nullptr, 4ull * b.seqs}, k = {kept->ptr, 4ull * b.tokens}, n = {counts->ptr, 4ull * b.seqs};
+  if (over_layers(kv, bases, {lens, k, n, {b.table, 4ull * b.seqs * b.table_pages}, {b.starts, 4ull * (b.seqs + 1ull)}, {b.lens, 4ull * b.seqs}}))
+    return fail(ctx, EFF_E_INVALID, "kv keep: a cache overlaps what the call reads, or new_lens");
+  if (lens.p && (over(lens, {k, n}) || over_batch(lens, b)))
+    return fail(ctx, EFF_E_INVALID, "kv keep: new_lens overlaps what the call reads");
+  if ((rc = use_device(ctx))) return rc;
+  const hipError_t e = each_layers(bases, [&](const KvLayers &l, uint32_t layers_here, bool first) {
+    return launch_kv_keep(kv, l, layers_here, b, (const uint32_t *)kept->ptr, (const uint32_t *)counts->ptr,
+                          first ? (uint32_t *)lens.p : nullptr, ctx->stream);
+  });
+  if (e != hipSuccess) return hip_fail(ctx, e, "kv keep launch");
+  ++ctx->stats.kv_keep;
+  return EFF_OK;
+} catch (const std::exception &e) {
+  return fail(ctx, EFF_E_NOMEM, "kv keep: %s", e.what());
 }
 
 int eff_logits_apply(eff_ctx *ctx, eff_buf *in, eff_buf *out, uint32_t rows, uint32_t vocab, uint32_t stride,

@@ -55,6 +55,13 @@ struct KvAppendArgs {
   float eps;
 };
 
+// Positions to turn by, of the new tokens on each axis, and the axis of each pair.
+struct KvTurnsView {
+  const uint32_t *at;                // [axes][tokens]
+  uint32_t tokens, positions;        // of the rope table
+  uint8_t axis[128];
+};
+
 struct KvAttnArgs {
   const float *q;
   uint32_t q_stride;
@@ -70,7 +77,18 @@ struct RopeFreqs {
 };
 hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positions, float scale, float *out,
                              hipStream_t stream);
-hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t stream);
+hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const KvTurnsView *turns,
+                            hipStream_t stream);   // turns null: by the place in the cache
+
+// The caches of a group of layers, alike but for their memory (`kv.base` is not used).
+constexpr uint32_t kKvLayers = 64;
+struct KvLayers {
+  uint8_t *base[kKvLayers];
+};
+hipError_t launch_kv_copy(const KvView &kv, const KvLayers &l, uint32_t layers, const uint32_t *copies, uint32_t count,
+                          hipStream_t stream);
+hipError_t launch_kv_keep(const KvView &kv, const KvLayers &l, uint32_t layers, const KvBatchView &b, const uint32_t *kept,
+                          const uint32_t *counts, uint32_t *new_lens, hipStream_t stream);
 // The scratch of tiles that several workgroups share (0: none): counters, zero before
 // the first launch and left zero by each, then the workgroups' sums.
 constexpr uint32_t kAttnCounters = 65536;

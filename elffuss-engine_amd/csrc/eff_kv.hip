@@ -5,6 +5,8 @@
 //   norm      x_i <- x_i * (1 / sqrt(sum x^2 / D + eps)) * w_i            (optional)
 //   rotation  the pair (a, b) at position p and frequency i becomes
 //             (a cos - b sin, a sin + b cos), cos and sin from the table  (the first rope_dim values)
+//             p is the token's place in the cache, or of each pair the token's position
+//             on the pair's axis (TURNS)
 // k and v rows are then stored as fp16 (round to nearest even), or as int8:
 //   scale = max|x| / 127,  n = round(x * (127 / max|x|)), 0 where max|x| < 2^-119.
 // Every operation is a separate f32 rounding (no contraction).
@@ -72,6 +74,23 @@ __device__ __forceinline__ void load4(float x[4], const float *p, bool apart, ui
   }
 }
 
+// Where the rotation goes by the token's place in the cache.
+struct ByPlace {};
+
+// cos and sin of the lane's pairs 2 l and 2 l + 1, each by its own axis: they do not
+// wait for the token's place. A position that the table does not have is not read.
+template <typename TURNS>
+__device__ __forceinline__ void turn_at(const TURNS &turned, const KvAppendArgs &a, uint32_t t, uint32_t half, uint32_t l, float2 &c, float2 &d) {
+  float *cs[2] = {&c.x, &c.y}, *ds[2] = {&d.x, &d.y};
+#pragma unroll
+  for (uint32_t i = 0; i < 2u; ++i) {
+    const uint32_t pair = 2u * l + i, p = turned.at[(uint64_t)turned.axis[pair] * turned.tokens + t];
+    const float *row = a.rope + (uint64_t)min(p, turned.positions - 1u) * a.rope_dim + pair;
+    const float x = row[0], y = row[half];
+    *cs[i] = p < turned.positions ? x : NAN, *ds[i] = p < turned.positions ? y : NAN;
+  }
+}
+
 // A workgroup takes rows of one token and of one kind (q, k or v: what differs
 // between them is then scalar); L lanes take a row, 4 values each: the pairs 2 l
 // and 2 l + 1 of the row's D / 2 pairs. Its bytes bound a long append, round trips a
@@ -80,10 +99,11 @@ __device__ __forceinline__ void load4(float x[4], const float *p, bool apart, ui
 // under way (us, U = 1 / 4: 4780 tokens of 24 heads of 256 with norms 72.2 / 56.9, 3.9
 // TB/s; 4780 of 48 heads of 128 54.4 / 48.8, 4.6 TB/s; 1340 tokens 14.9 / 16.1, 270
 // 6.8 / 7.1).
-template <int TYPE, int D, int U>
-__global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t q_wgs, uint32_t k_wgs) {
+template <int TYPE, int D, int U, typename TURNS>
+__global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t q_wgs, uint32_t k_wgs, TURNS turned) {
 #pragma clang fp contract(off)
   constexpr uint32_t L = D == 96 ? 32u : D / 4u, ROWS = 256u / L;
+  constexpr bool TURNED = !__is_same(TURNS, ByPlace);
   const uint32_t wgs = q_wgs + 2u * k_wgs, t = blockIdx.x / wgs, w = blockIdx.x % wgs, l = (threadIdx.x & 63u) % L;
   const bool is_q = w < q_wgs, is_v = w >= q_wgs + k_wgs;
   const uint32_t heads = is_q ? a.q_heads : kv.heads, h0 = (is_q ? w : is_v ? w - q_wgs - k_wgs : w - q_wgs) * ROWS * U + threadIdx.x / L;
@@ -99,6 +119,10 @@ __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvA
   }
   float weight[4] = {};
   if (norm && in) load4(weight, norm, apart, half, l);
+  float2 c = make_float2(1.f, 1.f), d = make_float2(0.f, 0.f);
+  if constexpr (TURNED) {
+    if (turns) turn_at(turned, a, t, half, l, c, d);
+  }
   KvSeq s;
   if (!kv_seq_of(b, t, s)) return;
   const uint32_t back = s.next - t;   // positions from the sequence's end
@@ -107,8 +131,7 @@ __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvA
   // a page number past the cache holds nothing
   uint32_t page = ~0u;
   if (placed && !is_q) page = b.table[(uint64_t)s.seq * b.table_pages + (pos >> kv.page_log2)];
-  float2 c = make_float2(1.f, 1.f), d = make_float2(0.f, 0.f);
-  if (turns) {
+  if (!TURNED && turns) {
     const float *p = a.rope + (uint64_t)pos * a.rope_dim + 2u * l;
     c = *(const float2 *)p, d = *(const float2 *)(p + half);
   }
@@ -188,35 +211,36 @@ hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positi
   return hipGetLastError();
 }
 
-template <int TYPE, int D, int U>
-static hipError_t append_launch(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
+template <int TYPE, int D, int U, typename TURNS>
+static hipError_t append_launch(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const TURNS &turned, hipStream_t s) {
   constexpr uint32_t rows = (D == 96 ? 8u : 1024u / D) * U;   // of a workgroup
   const uint32_t q = (a.q_heads + rows - 1u) / rows, k = (kv.heads + rows - 1u) / rows;
   if (!fits((uint64_t)b.tokens * (q + 2u * k), 256u)) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((k_kv_append<TYPE, D, U>), dim3(b.tokens * (q + 2u * k)), dim3(256), 0, s, kv, b, a, q, k);
+  hipLaunchKernelGGL((k_kv_append<TYPE, D, U, TURNS>), dim3(b.tokens * (q + 2u * k)), dim3(256), 0, s, kv, b, a, q, k, turned);
   return hipGetLastError();
 }
 
-template <int TYPE, int D>
-static hipError_t append_dim(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
+template <int TYPE, int D, typename TURNS>
+static hipError_t append_dim(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const TURNS &turned, hipStream_t s) {
   // 4 rows a thread where a CU still has 8 workgroups to take
-  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= 2048ull * 4096u) return append_launch<TYPE, D, 4>(kv, b, a, s);
-  return append_launch<TYPE, D, 1>(kv, b, a, s);
+  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= 2048ull * 4096u) return append_launch<TYPE, D, 4>(kv, b, a, turned, s);
+  return append_launch<TYPE, D, 1>(kv, b, a, turned, s);
 }
 
-template <int TYPE>
-static hipError_t append_go(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t s) {
+template <int TYPE, typename TURNS>
+static hipError_t append_go(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const TURNS &turned, hipStream_t s) {
   switch (kv.dim) {
-    case 64: return append_dim<TYPE, 64>(kv, b, a, s);
-    case 96: return append_dim<TYPE, 96>(kv, b, a, s);
-    case 128: return append_dim<TYPE, 128>(kv, b, a, s);
-    case 256: return append_dim<TYPE, 256>(kv, b, a, s);
+    case 64: return append_dim<TYPE, 64>(kv, b, a, turned, s);
+    case 96: return append_dim<TYPE, 96>(kv, b, a, turned, s);
+    case 128: return append_dim<TYPE, 128>(kv, b, a, turned, s);
+    case 256: return append_dim<TYPE, 256>(kv, b, a, turned, s);
     default: return hipErrorInvalidValue;
   }
 }
 
-hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, hipStream_t stream) {
-  return kv.type == EFF_KV_F16 ? append_go<EFF_KV_F16>(kv, b, a, stream) : append_go<EFF_KV_I8>(kv, b, a, stream);
+hipError_t launch_kv_append(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const KvTurnsView *turns, hipStream_t stream) {
+  if (turns) return kv.type == EFF_KV_F16 ? append_go<EFF_KV_F16>(kv, b, a, *turns, stream) : append_go<EFF_KV_I8>(kv, b, a, *turns, stream);
+  return kv.type == EFF_KV_F16 ? append_go<EFF_KV_F16>(kv, b, a, ByPlace{}, stream) : append_go<EFF_KV_I8>(kv, b, a, ByPlace{}, stream);
 }
 
 }  // namespace eff

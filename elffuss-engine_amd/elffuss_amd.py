@@ -47,7 +47,8 @@ class Stats(ctypes.Structure):
                 ("dequant", ctypes.c_uint64), ("topk", ctypes.c_uint64), ("not_applicable", ctypes.c_uint64),
                 ("split", ctypes.c_uint64), ("fused", ctypes.c_uint64), ("gather", ctypes.c_uint64),
                 ("gemm_x", ctypes.c_uint64), ("split_x", ctypes.c_uint64), ("cpu_path", ctypes.c_uint64),
-                ("kv_append", ctypes.c_uint64), ("kv_attn", ctypes.c_uint64), ("logits", ctypes.c_uint64)]
+                ("kv_append", ctypes.c_uint64), ("kv_attn", ctypes.c_uint64), ("logits", ctypes.c_uint64),
+                ("kv_copy", ctypes.c_uint64), ("kv_keep", ctypes.c_uint64)]
 
 
 class SplitPlan(ctypes.Structure):
@@ -135,6 +136,9 @@ def lib():
         "eff_kv_page_bytes": ([i32, u32, u32, u32], sz),
         "eff_rope_table": ([p, p, u32, u32, ctypes.c_float, p], i32),
         "eff_kv_append": ([p, p, p, p], i32),
+        "eff_kv_append_at": ([p, p, p, p, p], i32),
+        "eff_kv_copy": ([p, p, u32, p, u32], i32),
+        "eff_kv_keep": ([p, p, u32, p, p, p, p], i32),
         "eff_kv_attn": ([p, p, p, p, u64, u32, p, u32, ctypes.c_float, u32], i32),
         "eff_logits_apply": ([p, p, p, u32, u32, u32, p], i32),
     }
@@ -154,7 +158,7 @@ EXPORTED = ("eff_type_from_name eff_type_name eff_type_geometry eff_init eff_shu
             "eff_bytes_reordered eff_bytes_buffer_r eff_blocks_from_buffer eff_scales_from eff_buf_mark_r "
             "eff_buf_blocks_r eff_buf_write_r eff_repack eff_unrepack eff_quantize eff_fill_normal eff_qmatmul eff_qgemv "
             "eff_qgemm eff_qgemm_planned eff_gemm_x_layout eff_gemm_prepare_x eff_qgemm_prepared eff_qmatmul_x_layout eff_qmatmul_prepare_x eff_qmatmul_prepared eff_split_plan eff_qmatmul_cpu_path eff_qgemv_multi eff_dequant eff_gather eff_gather_norm eff_topk eff_topk_noalloc eff_qgemv_topk eff_topk_out_bytes eff_read_floor "
-            "eff_kv_page_bytes eff_rope_table eff_kv_append eff_kv_attn eff_logits_apply").split()
+            "eff_kv_page_bytes eff_rope_table eff_kv_append eff_kv_append_at eff_kv_attn eff_kv_copy eff_kv_keep eff_logits_apply").split()
 
 
 def type_code(t):
@@ -334,6 +338,10 @@ class _KvRows(ctypes.Structure):
                 ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("norm_eps", ctypes.c_float)]
 
 
+class _KvTurns(ctypes.Structure):
+    _fields_ = [("at", ctypes.c_void_p), ("axes", ctypes.c_uint32), ("axis", ctypes.c_uint8 * 128)]
+
+
 class _LogitsRules(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("history", "history_starts", "penalties", "bias_ids", "bias_values",
                                                "bias_starts", "mask", "mask_of")] + [("mask_count", ctypes.c_uint32)]
@@ -349,6 +357,20 @@ class KvCache(_Described):
 
     def __init__(self, t, heads, head_dim, page_tokens, pages, buf):
         self._describe(_KvCache, type=t, heads=heads, head_dim=head_dim, page_tokens=page_tokens, pages=pages, buf=buf)
+
+
+class KvLayers(_Described):
+    """The caches of a model's layers side by side, for the calls that go over all of them; alike but for their buffers."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        self.c = (_KvCache * len(self.caches))(*[c.c for c in self.caches])
+        self.buffers = [b for c in self.caches for b in c.buffers]
+        self._named = {f"of layer {i}": c._named["buf"] for i, c in enumerate(self.caches)}
+        self._ref, self._seen = ctypes.addressof(self.c), None
+
+    def __len__(self):
+        return len(self.caches)
 
 
 class KvBatch(_Described):
@@ -369,6 +391,16 @@ class KvRows(_Described):
                        v_offset=at[2][1], q_stride=q_stride, k_stride=k_stride, v_stride=v_stride, q_heads=q_heads,
                        q_out=q_out, rope=rope, rope_positions=rope_positions, rope_dim=rope_dim, rope_mode=rope_mode,
                        q_norm=q_norm, k_norm=k_norm, norm_eps=eps)
+
+
+class KvTurns(_Described):
+    """Positions to turn by (eff_kv_turns): `at` u32 [axes][tokens], `axis` the axis of each pair of rotated channels."""
+
+    def __init__(self, at, axis=(), *, axes=1):
+        axis = [int(a) for a in axis]
+        if len(axis) > 128 or not all(0 <= a < 256 for a in axis):
+            raise EffError(E_INVALID, "KvTurns: axis is up to 128 small numbers")
+        self._describe(_KvTurns, at=at, axes=axes, axis=(ctypes.c_uint8 * 128)(*axis))
 
 
 class LogitsRules(_Described):
@@ -588,9 +620,21 @@ class Context:
         self._check(lib().eff_rope_table(self.h, f.ctypes.data, f.size, positions, scale, out.handle))
         return out
 
-    def kv_append(self, cache, batch, rows):
-        """The new tokens' k and v into the cache, q and k normed and rotated (eff_kv_append)."""
-        self._check(lib().eff_kv_append(self.h, cache.ref, batch.ref, rows.ref))
+    def kv_append(self, cache, batch, rows, turns=None):
+        """The new tokens' k and v into the cache, q and k normed and rotated (eff_kv_append, with turns eff_kv_append_at)."""
+        if turns is None:
+            self._check(lib().eff_kv_append(self.h, cache.ref, batch.ref, rows.ref))
+        else:
+            self._check(lib().eff_kv_append_at(self.h, cache.ref, batch.ref, rows.ref, turns.ref))
+
+    def kv_copy(self, layers, copies, count):
+        """Pages to others in the caches of all layers (KvLayers; eff_kv_copy); copies: u32 [count][3], from, to, tokens."""
+        self._check(lib().eff_kv_copy(self.h, layers.ref, len(layers), copies.handle, count))
+
+    def kv_keep(self, layers, batch, kept, counts, new_lens=None):
+        """The drafts that stay move up in the caches of all layers (KvLayers; eff_kv_keep)."""
+        self._check(lib().eff_kv_keep(self.h, layers.ref, len(layers), batch.ref, kept.handle, counts.handle,
+                                      new_lens.handle if new_lens else None))
 
     def kv_attn(self, cache, batch, q, out, q_heads, scale, window=0, q_offset=0, q_stride=0):
         """Attention of the new tokens over the cache (eff_kv_attn)."""

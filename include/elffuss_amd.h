@@ -116,9 +116,11 @@ typedef struct eff_stats {
                            split-x router call but those of up to 8 tokens that prepare x inside the
                            product: eff_split_plan's prepares_x; one per eff_qmatmul_prepare_x for it) */
   uint64_t cpu_path;    /* products with the reference CPU path's arithmetic (eff_qmatmul_cpu_path) */
-  uint64_t kv_append;   /* eff_kv_append launches */
-  uint64_t kv_attn;     /* eff_kv_attn launches */
+  uint64_t kv_append;   /* eff_kv_append and eff_kv_append_at launches */
+  uint64_t kv_attn;     /* eff_kv_attn and eff_kv_attn_rules launches */
   uint64_t logits;      /* eff_logits_apply launches */
+  uint64_t kv_copy;     /* eff_kv_copy launches */
+  uint64_t kv_keep;     /* eff_kv_keep launches */
 } eff_stats;
 
 /* ---- types and geometry -------------------------------------------------- */
@@ -565,6 +567,25 @@ int eff_rope_table(eff_ctx *ctx, const double *freqs, uint32_t n, uint32_t posit
  * infinity has no finite value. */
 int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *rows);
 
+/* Positions to turn by where they are not the cache's: drafts of a tree (the
+ * position of their depth), patches of an image or a video (time, row, column).
+ *   at     u32 [axes][tokens]: the new tokens' positions on each of 1 .. 4 axes
+ *   axis   of pair i of the rotated channels (i < rope_dim / 2): its axis, < axes
+ * A pair whose position the rope table does not have (>= rope_positions)
+ * becomes NaN. */
+#define EFF_KV_AXES_MAX 4u
+typedef struct eff_kv_turns {
+  eff_buf *at;
+  uint32_t axes;
+  uint8_t axis[128];
+} eff_kv_turns;
+
+/* eff_kv_append with q and k turned by `turns` (NULL: by their place in the
+ * cache, as there); where they are cached stays a matter of `batch`. rows->rope
+ * has rope_positions >= 1 positions, whatever max_len is. */
+int eff_kv_append_at(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, const eff_kv_rows *rows,
+                     const eff_kv_turns *turns);
+
 /* out [tokens][q_heads * head_dim] = attention of q (rows as in eff_kv_rows,
  * rotated: eff_kv_append's q_out) over the cache: q head h reads key/value head
  * h / (q_heads / heads). A new token at position p sees the cached tokens of
@@ -576,6 +597,31 @@ int eff_kv_append(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *b
  * finite. out may not overlap q, the cache or the batch's buffers. f32-accurate. */
 int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
                 uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window);
+
+/* ---- paged key/value cache: copies, drafts that stay ----------------------- */
+
+/* Of `copies` (u32 [count][3]: from page, to page, tokens) each the first
+ * `tokens` tokens' rows (all: page_tokens or more) of one page to another, in
+ * each of `layers` caches, which differ in `buf` alone and do not overlap: a
+ * request is forked by sharing its full pages and copying its last. A page
+ * number past the cache copies nothing. A page that one copy writes may be
+ * neither read nor written by another of the call (what it holds then is one
+ * of theirs, row by row). No counterpart in the reference. */
+int eff_kv_copy(eff_ctx *ctx, const eff_kv_cache *caches, uint32_t layers, eff_buf *copies, uint32_t count);
+
+/* After the drafts of a batch were verified: the new tokens that stay move up
+ * to the first new places of their sequence, in each of `layers` caches (as of
+ * eff_kv_copy).
+ *   kept   u32 [tokens]: of sequence s, from starts[s] on, the new tokens that
+ *          stay (counted from its first), in rising order
+ *   counts u32 [seqs]: how many stay, at most its new tokens
+ * The i-th place takes the rows that new token kept[starts[s] + i] had before
+ * the call; an entry below i, or past the new tokens, moves nothing, nor do
+ * places and tokens without a page. What lies behind the last one that stays is
+ * left as it was. new_lens (u32 [seqs], or NULL; not the batch's lens): the
+ * sequences' lengths without the drafts that do not stay. */
+int eff_kv_keep(eff_ctx *ctx, const eff_kv_cache *caches, uint32_t layers, const eff_kv_batch *batch, eff_buf *kept,
+                eff_buf *counts, eff_buf *new_lens);
 
 /* ---- rules on the logits of a batch --------------------------------------- */
 
