@@ -1681,6 +1681,12 @@ int eff_kv_append_at(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch
 
 int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
                 uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window) {
+  return eff_kv_attn_rules(ctx, cache, batch, q, q_offset, q_stride, out, q_heads, scale, window, nullptr);
+}
+
+int eff_kv_attn_rules(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
+                      uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window,
+                      const eff_kv_rules *rules) {
   if (!ctx) return EFF_E_INVALID;
   KvView kv;
   KvBatchView b;
@@ -1704,16 +1710,45 @@ int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *bat
   a.q_heads = q_heads;
   a.scale = scale;
   a.window = window;
+  KvRulesView rv{};
+  if (rules) {
+    if (rules->cap != 0.f && !(rules->cap >= 1e-6f && rules->cap <= 1e6f))
+      return fail(ctx, EFF_E_INVALID, "kv attn: cap=%g (0, or 1e-6 .. 1e6)", (double)rules->cap);
+    rv.cap = rules->cap;
+    const uint64_t range_bytes = 8ull * b.tokens, tree_bytes = 4ull * b.tokens * rules->tree_words;
+    if (rules->slopes) {
+      if ((rc = check_out(ctx, rules->slopes, 4ull * q_heads, "kv attn slopes"))) return rc;
+      rv.slopes = (const float *)rules->slopes->ptr;
+    }
+    if (rules->ranges) {
+      if (rules->tree || window) return fail(ctx, EFF_E_INVALID, "kv attn: ranges with a %s", window ? "window" : "tree");
+      if ((rc = check_out(ctx, rules->ranges, range_bytes, "kv attn ranges"))) return rc;
+      rv.ranges = (const uint32_t *)rules->ranges->ptr;
+    }
+    if (rules->tree) {
+      if (32ull * rules->tree_words < b.max_new)
+        return fail(ctx, EFF_E_BOUNDS, "kv attn: tree rows of %u words and max_new=%u", rules->tree_words, b.max_new);
+      if (window && window < b.max_new)
+        return fail(ctx, EFF_E_SHAPE, "kv attn: a window of %u below the %u new tokens of a tree", window, b.max_new);
+      if ((rc = check_out(ctx, rules->tree, tree_bytes, "kv attn tree"))) return rc;
+      rv.tree = (const uint32_t *)rules->tree->ptr;
+      rv.tree_words = rules->tree_words;
+    }
+    if (over(rows, {{rv.slopes, 4ull * q_heads}, {rv.ranges, range_bytes}, {rv.tree, tree_bytes}}))
+      return fail(ctx, EFF_E_INVALID, "kv attn: out overlaps the rules");
+  }
+  const bool ruled = rv.cap != 0.f || rv.slopes || rv.ranges || rv.tree;
   if (b.tokens == 0) return EFF_OK;
   if ((uint64_t)b.tokens * q_heads > 0x7FFFFFFFull)
     return fail(ctx, EFF_E_SHAPE, "kv attn: %u tokens of %u heads", b.tokens, q_heads);
   if ((rc = use_device(ctx))) return rc;
   // the scratch of shared tiles: its counters are zeroed when it is made
-  const size_t need = kv_attn_scratch(kv, b, a), before = ctx->attn_scratch_bytes;
+  const size_t need = ruled ? kv_attn_rules_scratch(kv, b, a, rv) : kv_attn_scratch(kv, b, a), before = ctx->attn_scratch_bytes;
   if ((rc = grow(ctx, &ctx->attn_scratch, &ctx->attn_scratch_bytes, need, "attention"))) return rc;
   if (ctx->attn_scratch_bytes != before)
     EFF_HIP(ctx, hipMemsetAsync(ctx->attn_scratch, 0, kAttnCounters * 4u, ctx->stream));
-  hipError_t e = launch_kv_attn(kv, b, a, ctx->attn_scratch, ctx->stream);
+  hipError_t e = ruled ? launch_kv_attn_rules(kv, b, a, rv, ctx->attn_scratch, ctx->stream)
+                       : launch_kv_attn(kv, b, a, ctx->attn_scratch, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "kv attn launch");
   ++ctx->stats.kv_attn;
   return EFF_OK;

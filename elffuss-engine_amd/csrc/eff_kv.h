@@ -71,6 +71,24 @@ struct KvAttnArgs {
   uint32_t window;                   // 0: none
 };
 
+// Rules on the scores of attention, and what the new tokens see.
+struct KvRulesView {
+  float cap;                         // 0: none
+  const float *slopes;               // [q_heads], null: none
+  const uint32_t *ranges;            // [tokens][2], null: none
+  const uint32_t *tree;              // [tokens][tree_words], null: none
+  uint32_t tree_words;
+};
+struct NoRules {};
+template <bool RULES>
+struct KvRulesOf {
+  typedef NoRules type;
+};
+template <>
+struct KvRulesOf<true> {
+  typedef KvRulesView type;
+};
+
 constexpr uint32_t kRopeMaxPairs = 256;
 struct RopeFreqs {
   double f[kRopeMaxPairs];
@@ -95,6 +113,9 @@ constexpr uint32_t kAttnCounters = 65536;
 size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a);
 hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch,
                           hipStream_t stream);
+size_t kv_attn_rules_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r);
+hipError_t launch_kv_attn_rules(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r, void *scratch,
+                                hipStream_t stream);
 
 struct LogitsArgs {
   const float *in;

@@ -137,6 +137,7 @@ def lib():
         "eff_rope_table": ([p, p, u32, u32, ctypes.c_float, p], i32),
         "eff_kv_append": ([p, p, p, p], i32),
         "eff_kv_append_at": ([p, p, p, p, p], i32),
+        "eff_kv_attn_rules": ([p, p, p, p, u64, u32, p, u32, ctypes.c_float, u32, p], i32),
         "eff_kv_copy": ([p, p, u32, p, u32], i32),
         "eff_kv_keep": ([p, p, u32, p, p, p, p], i32),
         "eff_kv_attn": ([p, p, p, p, u64, u32, p, u32, ctypes.c_float, u32], i32),
@@ -158,7 +159,7 @@ EXPORTED = ("eff_type_from_name eff_type_name eff_type_geometry eff_init eff_shu
             "eff_bytes_reordered eff_bytes_buffer_r eff_blocks_from_buffer eff_scales_from eff_buf_mark_r "
             "eff_buf_blocks_r eff_buf_write_r eff_repack eff_unrepack eff_quantize eff_fill_normal eff_qmatmul eff_qgemv "
             "eff_qgemm eff_qgemm_planned eff_gemm_x_layout eff_gemm_prepare_x eff_qgemm_prepared eff_qmatmul_x_layout eff_qmatmul_prepare_x eff_qmatmul_prepared eff_split_plan eff_qmatmul_cpu_path eff_qgemv_multi eff_dequant eff_gather eff_gather_norm eff_topk eff_topk_noalloc eff_qgemv_topk eff_topk_out_bytes eff_read_floor "
-            "eff_kv_page_bytes eff_rope_table eff_kv_append eff_kv_append_at eff_kv_attn eff_kv_copy eff_kv_keep eff_logits_apply").split()
+            "eff_kv_page_bytes eff_rope_table eff_kv_append eff_kv_append_at eff_kv_attn eff_kv_attn_rules eff_kv_copy eff_kv_keep eff_logits_apply").split()
 
 
 def type_code(t):
@@ -342,6 +343,11 @@ class _KvTurns(ctypes.Structure):
     _fields_ = [("at", ctypes.c_void_p), ("axes", ctypes.c_uint32), ("axis", ctypes.c_uint8 * 128)]
 
 
+class _KvRules(ctypes.Structure):
+    _fields_ = [("cap", ctypes.c_float), ("tree_words", ctypes.c_uint32), ("slopes", ctypes.c_void_p),
+                ("ranges", ctypes.c_void_p), ("tree", ctypes.c_void_p)]
+
+
 class _LogitsRules(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("history", "history_starts", "penalties", "bias_ids", "bias_values",
                                                "bias_starts", "mask", "mask_of")] + [("mask_count", ctypes.c_uint32)]
@@ -401,6 +407,13 @@ class KvTurns(_Described):
         if len(axis) > 128 or not all(0 <= a < 256 for a in axis):
             raise EffError(E_INVALID, "KvTurns: axis is up to 128 small numbers")
         self._describe(_KvTurns, at=at, axes=axes, axis=(ctypes.c_uint8 * 128)(*axis))
+
+
+class KvRules(_Described):
+    """Rules on attention's scores and on what the new tokens see (eff_kv_rules)."""
+
+    def __init__(self, *, cap=0.0, slopes=None, ranges=None, tree=None, tree_words=0):
+        self._describe(_KvRules, cap=cap, tree_words=tree_words, slopes=slopes, ranges=ranges, tree=tree)
 
 
 class LogitsRules(_Described):
@@ -636,10 +649,14 @@ class Context:
         self._check(lib().eff_kv_keep(self.h, layers.ref, len(layers), batch.ref, kept.handle, counts.handle,
                                       new_lens.handle if new_lens else None))
 
-    def kv_attn(self, cache, batch, q, out, q_heads, scale, window=0, q_offset=0, q_stride=0):
-        """Attention of the new tokens over the cache (eff_kv_attn)."""
-        self._check(lib().eff_kv_attn(self.h, cache.ref, batch.ref, q.handle, q_offset, q_stride, out.handle, q_heads,
-                                      scale, window))
+    def kv_attn(self, cache, batch, q, out, q_heads, scale, window=0, q_offset=0, q_stride=0, rules=None):
+        """Attention of the new tokens over the cache (eff_kv_attn, with rules eff_kv_attn_rules)."""
+        if rules is None:
+            self._check(lib().eff_kv_attn(self.h, cache.ref, batch.ref, q.handle, q_offset, q_stride, out.handle, q_heads,
+                                          scale, window))
+        else:
+            self._check(lib().eff_kv_attn_rules(self.h, cache.ref, batch.ref, q.handle, q_offset, q_stride, out.handle,
+                                                q_heads, scale, window, rules.ref))
 
     def logits_apply(self, logits, out, rows, vocab, rules, stride=0):
         """Penalties, biases and masks on a batch's logits (eff_logits_apply)."""

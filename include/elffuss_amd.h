@@ -598,6 +598,33 @@ int eff_kv_append_at(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch
 int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
                 uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window);
 
+/* Rules on attention's scores, and on what the new tokens see; device buffers,
+ * NULL or 0: none.
+ *   cap    a score s = scale * q . k becomes cap * tanh(s / cap) (1e-6 .. 1e6)
+ *   slopes f32 [q_heads]: a score then loses slopes[h] * |p - p_t|, p and p_t the
+ *          positions of the new token and of the cached one
+ *   ranges u32 [tokens][2], without a window: a new token sees the cached tokens
+ *          at from <= t < to of its sequence, whatever its own position is
+ *          (documents that share a prompt, a prefix that sees all of itself);
+ *          from >= to: nothing
+ *   tree   u32 [tokens][tree_words], not with ranges: the new tokens are drafts.
+ *          A new token sees the cached tokens ahead of the first new one, and the
+ *          j-th new token of its sequence if bit j % 32 of word j / 32 of its row
+ *          is set: its ancestors and itself. Its position, for the window and the
+ *          slopes, is the first new one's plus the number of bits less one.
+ *          32 * tree_words >= max_new, and a window >= max_new */
+typedef struct eff_kv_rules {
+  float cap;
+  uint32_t tree_words;
+  eff_buf *slopes, *ranges, *tree;
+} eff_kv_rules;
+
+/* eff_kv_attn under `rules` (NULL: none). A key that is not finite makes the
+ * rows that see it not finite under a cap too. out may not overlap the rules. */
+int eff_kv_attn_rules(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *batch, eff_buf *q, uint64_t q_offset,
+                      uint32_t q_stride, eff_buf *out, uint32_t q_heads, float scale, uint32_t window,
+                      const eff_kv_rules *rules);
+
 /* ---- paged key/value cache: copies, drafts that stay ----------------------- */
 
 /* Of `copies` (u32 [count][3]: from page, to page, tokens) each the first
