@@ -985,7 +985,7 @@ struct AttnPlan {
   uint32_t rows;              // rows of a tile at most
   uint32_t waves;             // of a workgroup
   uint32_t max_rows;          // of the sequences taken; those with more go to k_attn_rows:
-  uint32_t many_tiles, many_per_seq;   // its tiles (0: none go)
+  uint32_t many_tiles, many_per_seq;   // its tiles (0: none go), shared by `items` workgroups where there are no others
 };
 
 // The sums of a tile that several workgroups share: each has two slots for a head, for
@@ -1010,6 +1010,108 @@ __device__ __forceinline__ void from_lds(T &to, const T &from) {
 #pragma unroll
   for (uint32_t i = 0; i < sizeof(T) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
   __builtin_memcpy(&to, w, sizeof(T));
+}
+
+// Joins the sums of a tile that several workgroups share, `chunks` of them from workgroup
+// `first` on: the last of them to arrive adds all up, of more than kJoin values in two
+// steps, groups first. Every wave's own sums lie in its slot, stored past the XCD's L2.
+// LDS: wt as many floats as one step has workgroups times rows, half 4 T, sm and sl a
+// float a row.
+template <int D, uint32_t T, typename TILE>
+__device__ __forceinline__ void attn_join(const AttnPlan &p, rsrc_t prs, uint32_t *cnt, const KvAttnArgs &a, const TILE &t, uint32_t group,
+                                          uint32_t kvh, uint32_t item, uint32_t first, uint32_t chunks, float *wt, float *half, float *sm,
+                                          float *sl, uint32_t &arrived, uint32_t slot_floats, uint32_t ml, uint32_t tid, uint32_t lane, uint32_t wave) {
+        const auto place = [&](uint32_t z) { return 2u * (first + z) + (z == 0u ? 1u : 0u); };   // the slot of the tile's workgroup z
+        // one join, or where there is much to read, one of each group of about sqrt(chunks)
+        // workgroups, whose sums take its first one's slot, and one of the groups
+        const uint32_t side = chunks * p.rows * D <= kJoin ? chunks : __builtin_amdgcn_readfirstlane((uint32_t)ceilf(sqrtf((float)chunks)));
+        const uint32_t groups = (chunks + side - 1u) / side;
+        uint32_t z0 = (item - first) / side * side, step = 1u, count = min(side, chunks - z0);
+        for (bool last = groups == 1u;; last = true) {
+          __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          __syncthreads();
+          uint32_t *counter = cnt + (step == 1u ? 0u : kAttnCounters / 2u) + (uint64_t)kvh * p.items * 2u + place(z0);
+          if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __syncthreads();
+          if (arrived != count - 1u) break;
+          if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          // each thread a part of the workgroups' 4 columns of a row, U of them under way,
+          // the first before the weights are known
+          constexpr uint32_t U = 8;
+          const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
+          const uint32_t part_i = parts > 1u ? tid / pieces : 0u, p0 = parts > 1u ? tid % pieces : tid;
+          float4v x[U] = {};   // (else live from tile to tile)
+          const auto request = [&](uint32_t i, uint32_t z) {
+  #pragma unroll
+            for (uint32_t k = 0; k < U; ++k) {
+              const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + i / (D / 4u) * D + 4u * (i % (D / 4u));
+              x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
+            }
+          };
+          if (p0 < pieces && part_i < parts) request(p0, part_i);
+          // the workgroups' weights relative to the largest maximum, [workgroup][row],
+          // and the rows' sums: a wave per row, its lanes over the workgroups
+                  for (uint32_t r = wave; r < t.rows; r += T / 64u) {
+            const auto both = [&](uint32_t z, float &mz, float &lz) {
+              const int at = (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u);
+              mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
+              lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
+            };
+            float m0 = -INFINITY, l0 = 0.f, mz, lz;
+            if (lane < count) both(lane, m0, l0);
+            float mx = m0, l = 0.f;
+            for (uint32_t z = lane + 64u; z < count; z += 64u) both(z, mz, lz), mx = fmaxf(mx, mz);
+  #pragma unroll
+            for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+            for (uint32_t z = lane; z < count; z += 64u) {
+              if (z < 64u) mz = m0, lz = l0;
+              else both(z, mz, lz);
+              const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
+              wt[z * p.rows + r] = f;
+              l += f * lz;
+            }
+            l = wave_sum(l);
+            if (lane == 0u) sl[r] = l, sm[r] = mx;
+          }
+          __syncthreads();
+          for (uint32_t i = p0; i < (parts > 1u ? p0 + 1u : (pieces + T - 1u) / T * T); i += T) {
+            const bool here = i < pieces && part_i < parts;
+            const uint32_t r = here ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
+            float4v o = {0.f, 0.f, 0.f, 0.f};
+            if (here) {
+              for (uint32_t z = part_i; z < count; z += U * parts) {
+                if (i != p0 || z != part_i) request(i, z);
+  #pragma unroll
+                for (uint32_t k = 0; k < U; ++k)
+                  if (z + k * parts < count) o += x[k] * wt[(z + k * parts) * p.rows + r];
+              }
+            }
+            if (parts > 1u) {
+              *(float4v *)(half + 4u * tid) = o;
+              __syncthreads();
+              if (here && part_i == 0u)
+                for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * pieces));
+            }
+            if (!here || part_i != 0u) continue;
+            const float l = sl[r];
+            if (last) {
+              const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+              float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+              *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+            } else {
+              const uint32_t at = place(z0) * slot_floats;
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((at + r * D + d) * 4u), 0, kSc1);
+              if (d == 0u) {
+                // a sum that is not a number is not nothing
+                const float mx = sm[r] == -INFINITY && l != 0.f ? 0.f : sm[r];
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((at + ml + 2u * r) * 4u), 0, kSc1);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((at + ml + 2u * r + 1u) * 4u), 0, kSc1);
+              }
+            }
+          }
+          if (last) break;
+          z0 = 0u, step = side, count = groups;
+        }
 }
 
 // Few rows: NW waves take the 32-token steps of a tile in turn; their sums meet in
@@ -1135,98 +1237,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
       }
     }
     if (shared && mine && chunks > 1u) {
-      const auto place = [&](uint32_t z) { return 2u * (first + z) + (z == 0u ? 1u : 0u); };   // the slot of the tile's workgroup z
-      // one join, or where there is much to read, one of each group of about sqrt(chunks)
-      // workgroups, whose sums take its first one's slot, and one of the groups
-      const uint32_t side = chunks * p.rows * D <= kJoin ? chunks : __builtin_amdgcn_readfirstlane((uint32_t)ceilf(sqrtf((float)chunks)));
-      const uint32_t groups = (chunks + side - 1u) / side;
-      uint32_t z0 = (item - first) / side * side, step = 1u, count = min(side, chunks - z0);
-      for (bool last = groups == 1u;; last = true) {
-        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        uint32_t *counter = cnt + (step == 1u ? 0u : kAttnCounters / 2u) + (uint64_t)kvh * p.items * 2u + place(z0);
-        if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        if (arrived != count - 1u) break;
-        if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // each thread a part of the workgroups' 4 columns of a row, U of them under way,
-        // the first before the weights are known
-        constexpr uint32_t U = 8;
-        const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
-        const uint32_t part_i = parts > 1u ? tid / pieces : 0u, p0 = parts > 1u ? tid % pieces : tid;
-        float4v x[U] = {};   // (else live from tile to tile)
-        const auto request = [&](uint32_t i, uint32_t z) {
-#pragma unroll
-          for (uint32_t k = 0; k < U; ++k) {
-            const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + i / (D / 4u) * D + 4u * (i % (D / 4u));
-            x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
-          }
-        };
-        if (p0 < pieces && part_i < parts) request(p0, part_i);
-        // the workgroups' weights relative to the largest maximum, [workgroup][row],
-        // and the rows' sums: a wave per row, its lanes over the workgroups
-        float *wt = &so[0][0][0], *half = wt + NW * R * LD - 4u * T;
-        for (uint32_t r = wave; r < t.rows; r += NW) {
-          const auto both = [&](uint32_t z, float &mz, float &lz) {
-            const int at = (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u);
-            mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
-            lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
-          };
-          float m0 = -INFINITY, l0 = 0.f, mz, lz;
-          if (lane < count) both(lane, m0, l0);
-          float mx = m0, l = 0.f;
-          for (uint32_t z = lane + 64u; z < count; z += 64u) both(z, mz, lz), mx = fmaxf(mx, mz);
-#pragma unroll
-          for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-          for (uint32_t z = lane; z < count; z += 64u) {
-            if (z < 64u) mz = m0, lz = l0;
-            else both(z, mz, lz);
-            const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
-            wt[z * p.rows + r] = f;
-            l += f * lz;
-          }
-          l = wave_sum(l);
-          if (lane == 0u) sl[0][r] = l, sm[0][r] = mx;
-        }
-        __syncthreads();
-        for (uint32_t i = p0; i < (parts > 1u ? p0 + 1u : (pieces + T - 1u) / T * T); i += T) {
-          const bool here = i < pieces && part_i < parts;
-          const uint32_t r = here ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
-          float4v o = {0.f, 0.f, 0.f, 0.f};
-          if (here) {
-            for (uint32_t z = part_i; z < count; z += U * parts) {
-              if (i != p0 || z != part_i) request(i, z);
-#pragma unroll
-              for (uint32_t k = 0; k < U; ++k)
-                if (z + k * parts < count) o += x[k] * wt[(z + k * parts) * p.rows + r];
-            }
-          }
-          if (parts > 1u) {
-            *(float4v *)(half + 4u * tid) = o;
-            __syncthreads();
-            if (here && part_i == 0u)
-              for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * pieces));
-          }
-          if (!here || part_i != 0u) continue;
-          const float l = sl[0][r];
-          if (last) {
-            const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
-            float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
-            *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
-          } else {
-            const uint32_t at = place(z0) * slot_floats;
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((at + r * D + d) * 4u), 0, kSc1);
-            if (d == 0u) {
-              // a sum that is not a number is not nothing
-              const float mx = sm[0][r] == -INFINITY && l != 0.f ? 0.f : sm[0][r];
-              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((at + ml + 2u * r) * 4u), 0, kSc1);
-              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((at + ml + 2u * r + 1u) * 4u), 0, kSc1);
-            }
-          }
-        }
-        if (last) break;
-        z0 = 0u, step = side, count = groups;
-      }
+      float *wt = &so[0][0][0];
+      attn_join<D, T>(p, prs, cnt, a, t, group, kvh, item, first, chunks, wt, wt + NW * R * LD - 4u * T, sm[0], sl[0], arrived, slot_floats, ml, tid, lane, wave);
     }
     if (!on || !attn_next<R>(b, group, a.window, tree, p.max_rows, t, c)) return;
     __syncthreads();   // the next tile's sums take these ones' place
@@ -1287,9 +1299,10 @@ __device__ __forceinline__ uint2 ld_turned(const uint8_t *p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(__attribute__((address_space(3))) void *)p));
 }
 
-template <int TYPE, int D, typename RULES>
+template <int TYPE, int D, int MODE, typename RULES>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, KvBatchView b, KvAttnArgs a, uint32_t tiles,
-                                                                      uint32_t per_seq, uint32_t min_rows, RULES rules) {
+                                                                      uint32_t per_seq, uint32_t min_rows, RULES rules, AttnPlan p,
+                                                                      uint32_t *cnt, float *part) {
   constexpr bool I8 = TYPE == EFF_KV_I8, RULED = !__is_same(RULES, NoRules);
   using W = AttnWave<D, I8, false, false, D <= 128 ? kVTurned : kVLater, RULED>;
   using S = AttnStage<D>;
@@ -1301,13 +1314,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   // head to an XCD where there are 8, so that tiles which run together read the same
   // rows out of its L2 (the sequences in turn, longest tiles of all first: 199 us
   // for the above, 371 -> 453 for 4 x 500 over up to 8000)
-  const uint32_t kvh = blockIdx.x % kv.heads, tile = tiles - 1u - blockIdx.x / kv.heads;
+  constexpr bool shared = MODE == kAttnEnds;
+  const uint32_t kvh = blockIdx.x % kv.heads, item = blockIdx.x / kv.heads, tile = tiles - 1u - item;
   typename W::Tile t;
-  if (!attn_tile<R>(b, group, a.window, tile, per_seq, min_rows, ~0u, t)) return;
+  AttnShare c = {1u, 1u, 0u, 1u, 0u, 0u};
+  if constexpr (shared) {
+    uint32_t tree = 0;   // new tokens of a tree at most
+    if constexpr (RULED) tree = rules.tree ? b.max_new : 0u;
+    if (!attn_share<R, true>(b, group, a.window, tree, item, p.items, ~0u, t, c)) return;
+  } else {
+    if (!attn_tile<R>(b, group, a.window, tile, per_seq, min_rows, ~0u, t)) return;
+  }
   const int window = (int)min(a.window, 0x40000000u);
   typename W::Tile m = t;   // the wave's own rows
   attn_seen<R>(t, rules, group, window);
-  const int base = t.begin & ~31;
+  const int tile_base = t.begin & ~31;
+  int base = tile_base, hi = t.end;
+  uint32_t first = 0, chunks = 1;   // the tile's workgroups
+  if constexpr (shared) {
+    base += (int)(c.at * kUnit);
+    hi = min(tile_base + (int)(min(c.at + c.left, c.of) * kUnit), t.end);
+    if (base >= hi && base != tile_base) return;   // the tile's other workgroups have it all
+    const uint32_t units = t.end > tile_base ? ((uint32_t)(t.end - tile_base) + kUnit - 1u) / kUnit : 1u;
+    first = __builtin_amdgcn_readfirstlane(c.start / c.each);
+    chunks = __builtin_amdgcn_readfirstlane((c.start + units - 1u) / c.each) - first + 1u;
+  }
   const uint32_t row0 = 16u * wave;
   m.rows = t.rows > row0 ? min(t.rows - row0, 16u) : 0u;
   if (m.rows) {
@@ -1330,7 +1361,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   AttnWalk k;
   k.table = b.table + (uint64_t)t.seq * b.table_pages;
   k.heads = kv.base + (uint64_t)kvh * kv.block_bytes;
-  k.lo = base, k.hi = t.end, k.stride = 32;
+  k.lo = base, k.hi = hi, k.stride = 32;
   // fp16: a step's fills, K's 16 rows of each half, then V's; the wave's are NW apart.
   // int8: a step's 16-byte pieces, K's, then V's; the thread's are 256 apart
   constexpr uint32_t MINE = I8 ? (4u * D + 255u) / 256u : 4u * S::FILLS / NW;
@@ -1361,7 +1392,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
 #pragma unroll
   for (int i = 0; i < (TURN ? 1 : W::E); ++i) va[i] = S::V + vr * S::ROW + 32u * S::v_place(vr, i) + 8u * (n & 3u);
 
-  const int steps = t.end > base ? (t.end - base + 31) / 32 : 0;
+  const int steps = hi > base ? (hi - base + 31) / 32 : 0;
   u32x4 raw[I8 ? MINE : 1];
   uint32_t raw_scale = 0;
   // Requests step i: into buffer `lds`, or (int8) into registers.
@@ -1453,6 +1484,27 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     }
   }
   const float l = row_add(w.l);
+  if (shared && chunks > 1u) {
+    const uint32_t slot_floats = attn_part_floats(p, D), slot = (2u * item + (item == first ? 1u : 0u)) * slot_floats;
+    const rsrc_t prs = make_rsrc(part + (uint64_t)kvh * p.items * 2u * slot_floats, (uint64_t)p.items * 2u * slot_floats * 4u);
+    if (n < m.rows) {
+      const uint32_t r = row0 + n;
+#pragma unroll
+      for (int i = 0; i < W::E; ++i)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, I8 ? w.acc[i] * w.unit : w.acc[i]), prs,
+                                               (int)((slot + r * D + W::column(g, i, 0)) * 4u), 0, kSc1);
+      if (g == 0u) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(RULED ? w.m : w.m * w.sc), prs, (int)((slot + p.rows * D + 2u * r) * 4u), 0, kSc1);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((slot + p.rows * D + 2u * r + 1u) * 4u), 0, kSc1);
+      }
+    }
+    // the waves have passed the last step's barrier, but may still read its buffer
+    __shared__ float sm[R], sl[R];
+    __shared__ uint32_t arrived;
+    float *wt = (float *)buf;
+    attn_join<D, 256u>(p, prs, cnt, a, t, group, kvh, item, first, chunks, wt, wt + sizeof(buf) / 4u - 1024u, sm, sl, arrived, slot_floats, p.rows * D, tid, lane, wave);
+    return;
+  }
   if (n >= m.rows) return;
   // no weight: nothing seen, or the largest score past f32
   const float f = l == 0.f ? (w.m == -INFINITY ? 0.f : NAN) : (I8 ? w.unit : 1.f) / l;
@@ -1469,26 +1521,10 @@ inline void attn_tiles(uint64_t most, uint64_t rows, uint32_t seqs, uint32_t r, 
   *tiles = (uint32_t)std::min(direct, packed);
 }
 
-inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, bool tree) {
-  const uint32_t group = a.q_heads / kv.heads;
+// Tiles of 16 rows of the sequences, which have `most` rows at most and `rows` in all, and
+// see `seen` tokens at most.
+inline void attn_plan_few(AttnPlan &p, const KvView &kv, const KvBatchView &b, uint64_t most, uint64_t rows, uint64_t seen) {
   constexpr uint32_t R = 16u;
-  AttnPlan p{};
-  uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group;
-  const uint64_t rows = (uint64_t)b.tokens * group;
-  p.max_rows = ~0u;
-  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + std::max(R / group, tree ? b.max_new : 0u) + 2u) : b.max_len;
-  // Sequences with more than 64 rows go to k_attn_rows where there are enough tiles of
-  // that (1 x 32 heads of 128 on 8 over 4000 tokens: 300 new tokens 108 us, k_attn 104,
-  // 400 108 and 131; int8 pages cost a conversion more for the same tile: 600 174 and
-  // 160, 800 175 and 201). The others go with them where lengths and new tokens are
-  // alike, since a second launch waits for the first (32 of up to 24 new tokens: 71 us,
-  // two launches 97); a long one's tile there is not shared.
-  if (most > kFewRows && rows / 64u * kv.heads >= (kv.type == EFF_KV_F16 ? 176u : 400u)) {
-    attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
-    if (b.seqs == 1u || (most * b.seqs <= 3u * rows && seen <= 4096u)) return p;
-    p.max_rows = kFewRows;
-    most = kFewRows;
-  }
   attn_tiles(most, rows, b.seqs, R, &p.tiles, &p.per_seq);
   p.rows = (uint32_t)std::min<uint64_t>(most, R);
   const uint64_t span = seen + 31u, wgs = (uint64_t)p.tiles * kv.heads;
@@ -1523,11 +1559,55 @@ inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // 14.7 us, 4 waves 15.5; 128 of up to 2000 of int8, 256 wide, 32.3 and 35.6; fp16 of
   // that width 46.8 and 45.7; 1024 workgroups of up to 300 tokens 20.5 and 20.2)
   p.waves = !p.items && wgs <= 256u && span >= 512u && (kv.dim < 256u || kv.type == EFF_KV_I8) ? 8u : 4u;
+}
+
+inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a) {
+  const uint32_t group = a.q_heads / kv.heads;
+  constexpr uint32_t R = 16u;
+  AttnPlan p{};
+  uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group;
+  const uint64_t rows = (uint64_t)b.tokens * group;
+  p.max_rows = ~0u;
+  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, (uint64_t)a.window + R / group + 2u) : b.max_len;
+  // Sequences with more than 64 rows go to k_attn_rows where there are enough tiles of
+  // that (1 x 32 heads of 128 on 8 over 4000 tokens: 300 new tokens 108 us, k_attn 104,
+  // 400 108 and 131; int8 pages cost a conversion more for the same tile: 600 174 and
+  // 160, 800 175 and 201). The others go with them where lengths and new tokens are
+  // alike, since a second launch waits for the first (32 of up to 24 new tokens: 71 us,
+  // two launches 97); a long one's tile there is not shared.
+  if (most > kFewRows && rows / 64u * kv.heads >= (kv.type == EFF_KV_F16 ? 176u : 400u)) {
+    attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
+    if (b.seqs == 1u || (most * b.seqs <= 3u * rows && seen <= 4096u)) return p;
+    p.max_rows = kFewRows;
+    most = kFewRows;
+  }
+  attn_plan_few(p, kv, b, most, rows, seen);
   return p;
 }
 
-inline bool attn_tree(NoRules) { return false; }
-inline bool attn_tree(const KvRulesView &r) { return r.tree != nullptr; }
+// Under rules the sequences with more than 16 rows take all to the tiles of 64.
+inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r) {
+  const uint32_t group = a.q_heads / kv.heads;
+  AttnPlan p{};
+  const uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group, rows = (uint64_t)b.tokens * group;
+  p.max_rows = ~0u;
+  const uint64_t reach = (uint64_t)a.window + std::max(64u / group, r.tree ? b.max_new : 0u) + 2u;   // under a window
+  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, reach) : b.max_len;
+  if (most <= 16u) {
+    attn_plan_few(p, kv, b, most, rows, seen);
+    return p;
+  }
+  attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
+  p.rows = (uint32_t)std::min<uint64_t>(most, 64u);
+  const uint64_t wgs = (uint64_t)p.many_tiles * kv.heads, units = (seen + 31u + kUnit - 1u) / kUnit, each = (most + 63u) / 64u;
+  const uint32_t slots = kv.dim <= 128u ? 768u : 512u;
+  const uint64_t items = std::max<uint64_t>(slots / kv.heads, 2u * p.many_tiles);
+  if (wgs < slots && units > 2u && items <= 2048u && items * kv.heads <= kAttnCounters / 4u && each * b.seqs * units < 1u << 31)
+    p.items = (uint32_t)items;
+  return p;
+}
+
+inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, NoRules) { return attn_plan(kv, b, a); }
 
 inline size_t attn_scratch(const AttnPlan &p, const KvView &kv) {
   return p.items ? kAttnCounters * 4u + (uint64_t)p.items * kv.heads * 2u * attn_part_floats(p, kv.dim) * 4u : 0u;
@@ -1535,18 +1615,28 @@ inline size_t attn_scratch(const AttnPlan &p, const KvView &kv) {
 
 template <int TYPE, int D, typename RULES>
 hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const RULES &rules, void *scratch, hipStream_t s) {
-  const AttnPlan p = attn_plan(kv, b, a, attn_tree(rules));
-  const uint64_t many = (uint64_t)p.many_tiles * kv.heads, grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
+  const AttnPlan p = attn_plan(kv, b, a, rules);
+  constexpr bool ruled = !__is_same(RULES, NoRules);
+  const bool shared = p.items && !p.tiles;   // the tiles of 64
+  const uint64_t many = (uint64_t)(shared ? p.items : p.many_tiles) * kv.heads, grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
   if (!fits(many, 256u) || !fits(grid, 512u)) return hipErrorInvalidConfiguration;
   if (p.items && (grid > kAttnCounters / 4u || !scratch)) return hipErrorInvalidValue;
+  uint32_t *cnt = (uint32_t *)scratch;
+  float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
   if (many) {
     const uint32_t min_rows = p.tiles ? kFewRows + 1u : 1u;
-    hipLaunchKernelGGL((k_attn_rows<TYPE, D, RULES>), dim3((uint32_t)many), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows, rules);
+    const auto rows = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)many), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows, rules, p, cnt, part);
+    };
+    if constexpr (ruled) {
+      if (shared) rows(k_attn_rows<TYPE, D, kAttnEnds, RULES>);
+      else rows(k_attn_rows<TYPE, D, kAttnWhole, RULES>);
+    } else {
+      rows(k_attn_rows<TYPE, D, kAttnWhole, RULES>);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.tiles) return e;
   }
-  uint32_t *cnt = (uint32_t *)scratch;
-  float *part = (float *)((uint8_t *)scratch + kAttnCounters * 4u);
   const auto go = [&](auto kernel, uint32_t threads) {
     hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(threads), 0, s, kv, b, a, p, cnt, part, rules);
   };

@@ -4,7 +4,7 @@
 namespace eff {
 
 size_t kv_attn_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a) {
-  return attn_scratch(attn_plan(kv, b, a, false), kv);
+  return attn_scratch(attn_plan(kv, b, a), kv);
 }
 
 hipError_t launch_kv_attn(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, void *scratch, hipStream_t stream) {

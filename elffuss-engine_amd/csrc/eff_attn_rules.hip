@@ -4,7 +4,7 @@
 namespace eff {
 
 size_t kv_attn_rules_scratch(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r) {
-  return attn_scratch(attn_plan(kv, b, a, r.tree != nullptr), kv);
+  return attn_scratch(attn_plan(kv, b, a, r), kv);
 }
 
 hipError_t launch_kv_attn_rules(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r, void *scratch,
