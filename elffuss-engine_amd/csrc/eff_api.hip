@@ -1714,7 +1714,8 @@ int eff_kv_attn_rules(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batc
   if (rules) {
     if (rules->cap != 0.f && !(rules->cap >= 1e-6f && rules->cap <= 1e6f))
       return fail(ctx, EFF_E_INVALID, "kv attn: cap=%g (0, or 1e-6 .. 1e6)", (double)rules->cap);
-    rv.cap = rules->cap;
+    rv.cap = (float)(rules->cap * 1.4426950408889634);
+    rv.per_cap = rules->cap != 0.f ? (float)(1. / (rules->cap * 1.4426950408889634)) : 0.f;
     const uint64_t range_bytes = 8ull * b.tokens, tree_bytes = 4ull * b.tokens * rules->tree_words;
     if (rules->slopes) {
       if ((rc = check_out(ctx, rules->slopes, 4ull * q_heads, "kv attn slopes"))) return rc;

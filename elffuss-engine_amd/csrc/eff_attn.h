@@ -27,8 +27,7 @@
 //   cap tanh(s / cap)                 where there is a cap
 //   less slope |p - p_t|              p, p_t the positions of the row's token and of t
 // and a row sees t where its range, or for the drafts of a tree its row of the tree,
-// says so. The rows' maxima and sums are then of log2 e times the scores (else of the
-// raw sums, before `scale`).
+// says so.
 #pragma once
 
 #include <algorithm>
@@ -472,21 +471,35 @@ enum { kVRows, kVTurned, kVLater };
 constexpr float kTanhFew = 0.625f;
 constexpr float kTanh[6] = {1.f, -0.3333326f, 0.13331127f, -0.053721067f, 0.020590989f, -0.0056599886f};
 
-// What a row needs of the rules; nothing without them.
-template <bool RULES>
-struct AttnRow {};
-template <>
-struct AttnRow<true> {
-  int from, to;         // the cached tokens that it sees, but for the tree's
-  float slope;          // times log2 e
-  float to_z, most;     // a raw score times to_z is the argument of tanh, whose outcome times `most` the score
-  const uint32_t *bits; // its row of the tree
+// What a row sees and where it is, in LDS: a step reads it where it needs it, so that it
+// takes no registers from step to step.
+struct AttnRule {
+  int from, to;   // the cached tokens that it sees, but for the tree's
+  int pos;        // its position
+  float slope;    // times log2 e
 };
 
+// The rules as a wave has them; nothing without rules.
+template <bool RULES>
+struct AttnRulesOf {
+  typedef NoRules type;
+};
+struct AttnRules {
+  const KvRulesView &all;
+  AttnRule *row;   // of the wave's first row; lane n has row n
+  uint32_t group;
+};
+template <>
+struct AttnRulesOf<true> {
+  typedef AttnRules type;
+};
+__device__ __forceinline__ NoRules attn_rules(NoRules, AttnRule *, uint32_t) { return {}; }
+__device__ __forceinline__ AttnRules attn_rules(const KvRulesView &r, AttnRule *row, uint32_t group) { return {r, row, group}; }
+
 template <int D, bool SCALED, bool I8, bool QL, int VIN, bool RULES = false>
-struct AttnWave : AttnRow<RULES> {
+struct AttnWave {
   typedef typename AttnTileOf<RULES>::type Tile;
-  typedef typename KvRulesOf<RULES>::type Rules;
+  typedef typename AttnRulesOf<RULES>::type Rules;
   static constexpr int E = D / 16;                     // columns of a lane
   static constexpr int KS = D / 32;                    // matrix steps of a score
   static constexpr int KW = I8 ? 2 : 4;                // words of a lane's part of a step of K
@@ -539,84 +552,92 @@ struct AttnWave : AttnRow<RULES> {
     pos = on ? t.first + (int)(tok - t.r0 / group) : -1;
   }
 
-  // What row n sees and how it scores, once its `sc` is known.
-  __device__ __forceinline__ void init_rules(const KvAttnArgs &a, const Rules &r, const Tile &t, uint32_t group, uint32_t kvh, uint32_t n, int window) {
+  // What row n sees and how it scores, for the steps to read.
+  static __device__ __forceinline__ void put_rule(const KvAttnArgs &a, const Rules &r, const Tile &t, uint32_t kvh, uint32_t n, uint32_t g, int window) {
     if constexpr (RULES) {
       const bool on = n < t.rows;
-      const uint32_t i = t.r0 + (on ? n : 0u), tok = i / group;
+      const uint32_t i = t.r0 + (on ? n : 0u), tok = i / r.group;
       const int place = t.base + (int)tok;
-      this->from = 0, this->to = 0, this->slope = 0.f, this->bits = nullptr;
-      pos = place;
-      if (on && r.tree) {
-        this->bits = r.tree + (uint64_t)(t.token0 + tok) * r.tree_words;
-        if (window || r.slopes) pos = key_position(r, t, t.token0 + tok);
-      }
-      if (on && r.ranges) range_of(r, t.token0 + tok, max(t.len, 0), this->from, this->to);
-      else if (on) this->from = window ? max(0, pos - window + 1) : 0, this->to = r.tree ? t.len : place + 1;
-      if (place < 0) this->to = 0;   // without a position it sees nothing
+      AttnRule x = {0, 0, place, 0.f};
+      if (on && r.all.tree && (window || r.all.slopes)) x.pos = key_position(r, t, t.token0 + tok);
+      if (on && r.all.ranges) range_of(r.all, t.token0 + tok, max(t.len, 0), x.from, x.to);
+      else if (on) x.from = window ? max(0, x.pos - window + 1) : 0, x.to = r.all.tree ? t.len : place + 1;
+      if (place < 0) x.to = 0;   // without a position it sees nothing
       // far from all that it sees, a row's distances are counted from the nearest of it: the
       // same weights, and small numbers
-      if (r.ranges) pos = max(min(pos, this->to - 1), this->from);
-      if (r.slopes) this->slope = r.slopes[kvh * group + i % group] * 1.44269504088896341f;
-      if (r.cap > 0.f) {
-        this->most = r.cap * 1.44269504088896341f;
-        this->to_z = fminf(sc / this->most, 1e30f);
-      }
+      if (r.all.ranges) x.pos = max(min(x.pos, x.to - 1), x.from);
+      if (r.all.slopes) x.slope = r.all.slopes[kvh * r.group + i % r.group] * 1.44269504088896341f;
+      if (g == 0u) r.row[n] = x;
     }
+  }
+  // Row n's, read here and not kept from step to step.
+  static __device__ __forceinline__ AttnRule get_rule(const Rules &r, uint32_t n) {
+    uint32_t nothing = 0;
+    __asm__ volatile("" : "+v"(nothing));
+    return r.row[n + nothing];
   }
 
   // The position of a new token of a tree: it sees itself and its ancestors.
   static __device__ __forceinline__ int key_position(const Rules &r, const Tile &t, uint32_t token) {
     const uint32_t n = (uint32_t)(t.len - t.base);
-    const uint32_t *row = r.tree + (uint64_t)token * r.tree_words;
+    const uint32_t *row = r.all.tree + (uint64_t)token * r.all.tree_words;
     uint32_t sees = 0;
     for (uint32_t w = 0; 32u * w < n; ++w) sees += __popc(row[w] & (n - 32u * w < 32u ? (1u << (n - 32u * w)) - 1u : ~0u));
     return t.base + (int)sees - 1;
   }
 
+  // What the rows' scores and maxima are multiplied by: rules on the scores leave them in
+  // units of log2.
+  __device__ __forceinline__ float of_scores(const Rules &r) const {
+    if constexpr (RULES) return r.all.cap > 0.f || r.all.slopes ? 1.f : sc;
+    else return sc;
+  }
+
   // The scores of a step under the rules, from the raw ones.
-  __device__ __forceinline__ void rule(const Rules &r, const Tile &t, int t0, uint32_t g, float s[2][4]) const {
+  __device__ __forceinline__ void rule(const Rules &r, const Tile &t, int t0, uint32_t n, uint32_t g, float s[2][4]) const {
     if constexpr (RULES) {
-      if (r.cap > 0.f) {
+      if (r.all.cap > 0.f) {
+        const float to_z = fminf(sc * r.all.per_cap, 1e30f), most = r.all.cap;
         float top = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(s[k / 4][k % 4]));
-        if (__any(top * this->to_z >= kTanhFew)) {
+        if (__any(top * to_z >= kTanhFew)) {
           // 1 - 2 / (1 + e^2z), and the odd polynomial below kTanhFew, where that loses bits
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             float &y = s[k / 4][k % 4];
-            const float z = y * this->to_z, e = __builtin_amdgcn_exp2f(fabsf(z) * 2.88539008177792681f);
+            const float z = y * to_z, e = __builtin_amdgcn_exp2f(fabsf(z) * 2.88539008177792681f);
             const float far = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f), z);
             // a raw score that is not finite stays so
-            y = fabsf(z) < kTanhFew ? z * tanh_few(z * z) * this->most : fmaf(y, 0.f, far * this->most);
+            y = fabsf(z) < kTanhFew ? z * tanh_few(z * z) * most : fmaf(y, 0.f, far * most);
           }
         } else {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             float &y = s[k / 4][k % 4];
-            const float z = y * this->to_z;
+            const float z = y * to_z;
             y = y * sc * tanh_few(z * z);
           }
         }
-      } else {
+      } else if (r.all.slopes) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[k / 4][k % 4] *= sc;
       }
-      if (r.slopes) {
-        if (r.tree && t0 + 32 > t.base) {
+      if (r.all.slopes) {
+        const AttnRule row = get_rule(r, n);
+        if (r.all.tree && t0 + 32 > t.base) {
 #pragma unroll 1
           for (int k = 0; k < 8; ++k) {
             const int at = t0 + 16 * (k / 4) + 4 * (int)g + k % 4;
             const int key = at >= max(t.base, 0) && at < t.len ? key_position(r, t, t.token0 + (uint32_t)(at - t.base)) : at;
-            const float bias = -this->slope * fabsf((float)(pos - key));
+            const float bias = -row.slope * fabsf((float)(row.pos - key));
 #pragma unroll
             for (int i = 0; i < 8; ++i) s[i / 4][i % 4] += i == k ? bias : 0.f;
           }
         } else {
-          const float far = (float)(pos - t0 - 4 * (int)g);
+          const float far = (float)(row.pos - t0 - 4 * (int)g);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) s[k / 4][k % 4] = fmaf(-this->slope, fabsf(far - (float)(16 * (k / 4) + k % 4)), s[k / 4][k % 4]);
+          for (int k = 0; k < 8; ++k) s[k / 4][k % 4] = fmaf(-row.slope, fabsf(far - (float)(16 * (k / 4) + k % 4)), s[k / 4][k % 4]);
         }
       }
     }
@@ -629,13 +650,15 @@ struct AttnWave : AttnRow<RULES> {
   }
 
   // Of the 32 tokens of a step those that row n sees, a bit each; none without a page.
-  __device__ __forceinline__ uint32_t seen_bits(const Rules &r, const Tile &t, int t0, const bool gone[2]) const {
-    const int lo = min(max(this->from - t0, 0), 32), hi = min(max(this->to - t0, 0), 32);
+  static __device__ __forceinline__ uint32_t seen_bits(const Rules &r, const Tile &t, int t0, uint32_t n, const bool gone[2]) {
+    const AttnRule row = get_rule(r, n);
+    const int lo = min(max(row.from - t0, 0), 32), hi = min(max(row.to - t0, 0), 32);
     uint32_t m = (uint32_t)((1ull << hi) - 1ull) & ~(uint32_t)((1ull << lo) - 1ull);
-    if (r.tree && t0 + 32 > t.base && this->bits) {
+    if (r.all.tree && t0 + 32 > t.base && n < t.rows) {
       // the bits of the tree begin at token base
+      const uint32_t *bits = r.all.tree + (uint64_t)(t.token0 + (t.r0 + n) / r.group) * r.all.tree_words;
       const int j = t0 - t.base;
-      const auto word = [&](uint32_t w) { return w < r.tree_words ? this->bits[w] : 0u; };
+      const auto word = [&](uint32_t w) { return w < r.all.tree_words ? bits[w] : 0u; };
       m &= j >= 0 ? (uint32_t)(((uint64_t)word((uint32_t)j / 32u + 1u) << 32 | word((uint32_t)j / 32u)) >> (j & 31))
                   : word(0u) << -j | ((1u << -j) - 1u);
     }
@@ -729,6 +752,14 @@ struct AttnWave : AttnRow<RULES> {
     return o;
   }
 
+  // Takes out of V what is not finite.
+  __device__ __forceinline__ void clean_v() {
+#pragma unroll
+    for (int k = 0; k < VN; ++k)
+#pragma unroll
+      for (int w = 0; w < VM; ++w) vw[k][w] &= ~not_finite_halves(vw[k][w]);
+  }
+
   // Takes the tokens out of V whose halves of `keep` are 0.
   __device__ __forceinline__ void keep_v(u32x4 keep) {
     if constexpr (VIN == kVTurned) {
@@ -744,6 +775,12 @@ struct AttnWave : AttnRow<RULES> {
     }
   }
 
+  // Matrix step k's operand of the 16 tokens of half u.
+  __device__ __forceinline__ half8 k_operand(int u, int k) const {
+    if constexpr (I8) return i8_half8(kw[u][2 * k], kw[u][2 * k + 1]);
+    else return __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
+  }
+
   // The step's raw scores: s[u][j] of token 16 u + 4 g + j. The two halves in turn,
   // so that a matrix step does not wait for the one before it.
   __device__ __forceinline__ void scores(float s[2][4]) const {
@@ -755,10 +792,7 @@ struct AttnWave : AttnRow<RULES> {
     for (int k = 0; k < KS; ++k) {
       half8 a[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if constexpr (I8) a[u] = i8_half8(kw[u][2 * k], kw[u][2 * k + 1]);
-        else a[u] = __builtin_bit_cast(half8, u32x4{kw[u][4 * k], kw[u][4 * k + 1], kw[u][4 * k + 2], kw[u][4 * k + 3]});
-      }
+      for (int u = 0; u < 2; ++u) a[u] = k_operand(u, k);
       half8 h, r;
       if constexpr (QL) h = *(const half8 *)(parts + k * 2048), r = *(const half8 *)(parts + k * 2048 + 1024);
       else h = qh[k], r = ql[k];
@@ -782,15 +816,44 @@ struct AttnWave : AttnRow<RULES> {
   // -inf where the key is not finite (or the score passes f32): the row's sum becomes
   // NaN, as it does with +inf.
   template <typename V, typename S>
-  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const Tile &t, int window, const Rules &r, uint32_t g, float s[2][4], V v, S scales) {
-    rule(r, t, t0, g, s);
-    const float sc = RULES ? 1.f : this->sc;
-    uint32_t bits = 0;
+  __device__ __forceinline__ void step(int t0, bool masked, const bool gone[2], const Tile &t, int window, const Rules &r, uint32_t n, uint32_t g, float s[2][4], V v, S scales) {
     u32x4 keep = {~0u, ~0u, ~0u, ~0u};   // the halves of an operand whose token some row sees
     bool dirty = false;                  // and whether some of them are not finite
+    half8 ph, pl;
+    weights(t0, masked, gone, t, window, r, n, g, s, v, scales, keep, dirty, ph, pl);
+    if (VIN == kVLater && !SCALED && masked) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        u32x4 o = v(i) & keep;
+        if (dirty) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[x] &= ~not_finite_halves(o[x]);
+        }
+        acc[i] = mfma(__builtin_bit_cast(half8, o), ph, acc[i]);
+        acc[i] = mfma(__builtin_bit_cast(half8, o), pl, acc[i]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const half8 o = __builtin_bit_cast(half8, v(i));
+      acc[i] = mfma(o, ph, acc[i]);
+      acc[i] = mfma(o, pl, acc[i]);
+    }
+  }
+
+  // The step's weights, in their two parts; what no row sees of V is taken out (by the
+  // product itself where V is read as it is used).
+  template <typename V, typename S>
+  __device__ __forceinline__ void weights(int t0, bool masked, const bool gone[2], const Tile &t, int window, const Rules &r, uint32_t n, uint32_t g,
+                                          float s[2][4], V v, S scales, u32x4 &keep, bool &dirty, half8 &ph, half8 &pl) {
+    rule(r, t, t0, n, g, s);
+    const float sc = of_scores(r);
+    uint32_t bits = 0;
     float low = 0.f;                     // the smallest score that the row sees (a NaN hides it: no matter)
     if (masked) {
-      if constexpr (RULES) bits = seen_bits(r, t, t0, gone) >> (4u * g);
+      if constexpr (RULES) bits = seen_bits(r, t, t0, n, gone) >> (4u * g);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int at = t0 + 16 * (k / 4) + 4 * (int)g + k % 4;
@@ -805,7 +868,7 @@ struct AttnWave : AttnRow<RULES> {
       // reach the others. (int8 values are finite, and their scales go with the weights.)
       if constexpr (!SCALED) {
         keep_v(keep);
-        if (RULES || t.first != t.last) {
+        if (unlike(t, r)) {
           uint32_t most = 0;
 #pragma unroll
           for (int i = 0; i < (VIN == kVLater ? E : VN * VM / 4); ++i) {
@@ -819,7 +882,12 @@ struct AttnWave : AttnRow<RULES> {
             __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
           }
           dirty = __any(most >= 0x7C00u);
-          if (dirty) poison(t0, gone, window, g, keep, bits, v);
+          if constexpr (RULES) {
+            if (dirty) spoil(bad_tokens(keep, v), bits);
+            if (dirty && VIN != kVLater) clean_v();
+          } else {
+            if (dirty) poison(t0, gone, window, g, keep, v);
+          }
         }
       }
     } else {
@@ -873,27 +941,7 @@ struct AttnWave : AttnRow<RULES> {
     half2v hi[4], lo[4];
 #pragma unroll
     for (int k = 0; k < 8; k += 2) split2(p[k], p[k + 1], hi[k / 2], lo[k / 2]);
-    const half8 ph = join8(hi), pl = join8(lo);
-    if (VIN == kVLater && !SCALED && masked) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        u32x4 o = v(i) & keep;
-        if (dirty) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) o[x] &= ~not_finite_halves(o[x]);
-        }
-        acc[i] = mfma(__builtin_bit_cast(half8, o), ph, acc[i]);
-        acc[i] = mfma(__builtin_bit_cast(half8, o), pl, acc[i]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const half8 o = __builtin_bit_cast(half8, v(i));
-      acc[i] = mfma(o, ph, acc[i]);
-      acc[i] = mfma(o, pl, acc[i]);
-    }
+    ph = join8(hi), pl = join8(lo);
   }
 
   // fp16 1 where a half is not finite, else 0.
@@ -908,13 +956,10 @@ struct AttnWave : AttnRow<RULES> {
   // product of the two indicators says which), and such values are taken out of the
   // step (by the product itself where V is read as it is used).
   template <typename V>
-  __device__ __forceinline__ void poison(int t0, const bool gone[2], int window, uint32_t g, u32x4 keep, uint32_t bits, V v) {
+  __device__ __forceinline__ void poison(int t0, const bool gone[2], int window, uint32_t g, u32x4 keep, V v) {
     half8 seen;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool sees_it = RULES ? bits >> (16 * (k / 4) + k % 4) & 1u : !gone[k / 4] && sees(pos, window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4);
-      seen[k] = (_Float16)(sees_it ? 1.f : 0.f);
-    }
+    for (int k = 0; k < 8; ++k) seen[k] = (_Float16)(!gone[k / 4] && sees(pos, window, t0 + 16 * (k / 4) + 4 * (int)g + k % 4) ? 1.f : 0.f);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const u32x4 o = v(i) & keep;
@@ -924,14 +969,39 @@ struct AttnWave : AttnRow<RULES> {
       for (int j = 0; j < 4; ++j) acc[i][j] = c[j] > 0.f ? NAN : acc[i][j];
       __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
     }
-    if constexpr (VIN != kVLater) {
-#pragma unroll
-      for (int k = 0; k < VN; ++k)
-#pragma unroll
-        for (int w = 0; w < VM; ++w) vw[k][w] &= ~not_finite_halves(vw[k][w]);
-    }
+    if constexpr (VIN != kVLater) clean_v();
   }
 
+  // Under rules the whole row becomes NaN (its sum does: no second set of the columns'
+  // registers is needed for that). Of the lane's 8 tokens those that have a value which
+  // is not finite, a bit each:
+  template <typename V>
+  __device__ __forceinline__ uint32_t bad_tokens(u32x4 keep, V v) const {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const u32x4 o = v(i) & keep;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) bad |= (o[k / 2] >> 16 * (k & 1) & 0x7C00u) == 0x7C00u ? 1u << k : 0u;
+      __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
+    }
+    bad |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bad, 0xB1, 0xF, 0xF, false);
+    bad |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bad, 0x4E, 0xF, 0xF, false);
+    bad |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bad, 0x141, 0xF, 0xF, false);
+    bad |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)bad, 0x140, 0xF, 0xF, false);
+    return bad;
+  }
+  // bits: of the tokens 4 g .. of the two halves those that the row sees.
+  __device__ __forceinline__ void spoil(uint32_t bad, uint32_t bits) {
+    if (bad & ((bits & 0xFu) | (bits >> 12 & 0xF0u))) l = NAN;
+  }
+
+  // Whether a token that some row of the tile sees may be one that another does not: not
+  // where they are one token's, but for the drafts of a tree that it does not see.
+  static __device__ __forceinline__ bool unlike(const Tile &t, const Rules &r) {
+    if constexpr (RULES) return t.first != t.last || r.all.tree;
+    else return t.first != t.last;
+  }
   static __device__ __forceinline__ int full_of(const Tile &t) {
     if constexpr (RULES) return t.all_to - 32;
     else return t.first - 31;
@@ -967,7 +1037,7 @@ struct AttnWave : AttnRow<RULES> {
       fetch_k(k, kv, i + 1, n, g);
       __builtin_amdgcn_sched_barrier(0);
     }
-    step(t0, masked, gone, t, window, r, g, s, [&](int c) { return v_operand(c); },
+    step(t0, masked, gone, t, window, r, n, g, s, [&](int c) { return v_operand(c); },
          [&](int u) { return u32x4{vs[u][0], vs[u][1], vs[u][2], vs[u][3]}; });
   }
 
@@ -1141,6 +1211,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   static_assert(MODE == kAttnWhole || kUnit == 32u * NW, "a unit is a step of each wave");
   __shared__ float so[NW][R][LD];
   __shared__ float sm[NW][R], sl[NW][R], sv[NW][R];
+  __shared__ AttnRule rule_rows[RULED ? NW : 1u][RULED ? R : 1u];
   __shared__ uint32_t arrived;
   __shared__ typename W::Tile kept_t;
   __shared__ AttnShare kept_c;
@@ -1171,6 +1242,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
     const bool mine = lo < hi || lo == base;   // past the end the tile's other workgroups have it all
     if (mine) {
       W w;
+      const auto wr = attn_rules(rules, rule_rows[RULED ? wave : 0u], group);
       {
         AttnWalk k;
         k.table = b.table + (uint64_t)t.seq * b.table_pages;
@@ -1180,13 +1252,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
         w.load_q(q, a, t, group, kvh, n, g);
         w.fetch_k(k, kv, 0, n, g);   // of the first page, where the wave has no step
         w.init(q, a.scale, (uint8_t *)so, wave, NW);
-        w.init_rules(a, rules, t, group, kvh, n, window);
+        W::put_rule(a, wr, t, kvh, n, g, window);
         if constexpr (QL) __syncthreads();
-        w.run(k, kv, t, window, rules, n, g);
+        w.run(k, kv, t, window, wr, n, g);
         if constexpr (QL) __syncthreads();   // the sums take q's place
       }
       const float wl = row_add(w.l);
-      if (g == 0u) sm[wave][n] = RULED ? w.m : w.m * w.sc, sl[wave][n] = wl, sv[wave][n] = w.unit;
+      if (g == 0u) sm[wave][n] = w.m * w.of_scores(wr), sl[wave][n] = wl, sv[wave][n] = w.unit;
 #pragma unroll
       for (int i = 0; i < W::E; ++i)
 #pragma unroll
@@ -1355,7 +1427,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   float q[W::KS][8];
   w.load_q(q, a, m, group, kvh, n, g);
   w.init(q, a.scale, nullptr, wave, NW);
-  w.init_rules(a, rules, m, group, kvh, n, window);
+  __shared__ AttnRule rule_rows[RULED ? NW : 1u][RULED ? 16u : 1u];
+  const auto wr = attn_rules(rules, rule_rows[RULED ? wave : 0u], group);
+  W::put_rule(a, wr, m, kvh, n, g, window);
 
   const uint32_t to_v = kv.heads * kv.block_bytes;
   AttnWalk k;
@@ -1477,7 +1551,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
 #pragma unroll
           for (int c = 0; c < W::E; ++c) __builtin_memcpy(w.vw[c], &(const u32x4 &)turned(c), 16);
         }
-        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, rules, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); },
+        w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, wr, n, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); },
                [&](int u) { return *(const u32x4 *)(lds + S::SCALES + 128u + 64u * u + 16u * g); });   // late: no register waits for it
       }
       if (i + 1 < steps) convert(buf[1 - half]);
@@ -1494,7 +1568,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, I8 ? w.acc[i] * w.unit : w.acc[i]), prs,
                                                (int)((slot + r * D + W::column(g, i, 0)) * 4u), 0, kSc1);
       if (g == 0u) {
-        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(RULED ? w.m : w.m * w.sc), prs, (int)((slot + p.rows * D + 2u * r) * 4u), 0, kSc1);
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(w.m * w.of_scores(wr)), prs, (int)((slot + p.rows * D + 2u * r) * 4u), 0, kSc1);
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((slot + p.rows * D + 2u * r + 1u) * 4u), 0, kSc1);
       }
     }

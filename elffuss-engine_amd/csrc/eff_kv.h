@@ -73,22 +73,13 @@ struct KvAttnArgs {
 
 // Rules on the scores of attention, and what the new tokens see.
 struct KvRulesView {
-  float cap;                         // 0: none
+  float cap, per_cap;                // times log2 e, and 1 over that (0: none)
   const float *slopes;               // [q_heads], null: none
   const uint32_t *ranges;            // [tokens][2], null: none
   const uint32_t *tree;              // [tokens][tree_words], null: none
   uint32_t tree_words;
 };
 struct NoRules {};
-template <bool RULES>
-struct KvRulesOf {
-  typedef NoRules type;
-};
-template <>
-struct KvRulesOf<true> {
-  typedef KvRulesView type;
-};
-
 constexpr uint32_t kRopeMaxPairs = 256;
 struct RopeFreqs {
   double f[kRopeMaxPairs];
