@@ -350,6 +350,16 @@ __device__ __forceinline__ bool attn_share(const KvBatchView &b, uint32_t group,
   uint32_t each = (total + items - 1u) / items, whole = 1;
   if (ENDS && count >= items) return false;
   if (ENDS || (each < kShort && count < items)) whole = each = max((total + items - count - 1u) / (items - count), kLeast);
+  if (ENDS && __is_same(TILE, AttnTileRules) && b.seqs <= 64u) {
+    // that holds for any lengths; the smallest share that these need: one tile's last
+    // workgroup seldom has next to nothing
+    for (uint32_t least = max((total + items - 1u) / items, kLeast); least < each;) {
+      const uint32_t mid = (least + each) / 2u;
+      if ((uint32_t)wave_sum((float)(tiles * ((of + mid - 1u) / mid))) <= items) each = mid;
+      else least = mid + 1u;
+    }
+    whole = each;
+  }
   each = max(each, kLeast);
   c.each = __builtin_amdgcn_readfirstlane(each);
   whole = __builtin_amdgcn_readfirstlane(whole);
@@ -1068,6 +1078,7 @@ constexpr uint32_t kFewRows = 64;
 // trip of two (32 workgroups x 8 rows x 128: 14.7 us, in two 15.3; 64 x 8 x 128 22.3 and
 // 20.3; 128 x 8 x 128 40.9 and 26.9).
 constexpr uint32_t kJoin = 32768;
+constexpr uint32_t kJoinRows = 5;   // round trips of a join of 64 rows
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
 enum { kAttnWhole, kAttnEnds, kAttnOn };   // a workgroup has a tile; a part of one; a share that may go on into the next
@@ -1362,13 +1373,101 @@ struct AttnStage {
   }
 };
 
-// Waits for the wave's loads and LDS operations, then for the other waves.
-__device__ __forceinline__ void wait_step() { __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+// Waits for the wave's loads but the last N and for its LDS operations, then for the other waves.
+template <int N>
+__device__ __forceinline__ void wait_step() { __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "i"(N) : "memory"); }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint2 ld_turned(const uint8_t *p) {
   typedef __attribute__((address_space(3))) short4v *lds_ptr;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(__attribute__((address_space(3))) void *)p));
+}
+
+// The join of a tile of 64 rows, as attn_join: workgroup by workgroup, a thread's PIECES
+// parts of 4 columns of a row at once, since the way to the sums and back is what it
+// waits for. LDS: 128 floats for each workgroup of one step.
+template <int D, typename TILE>
+__device__ __forceinline__ void attn_join_rows(const AttnPlan &p, rsrc_t prs, uint32_t *cnt, const KvAttnArgs &a, const TILE &t, uint32_t group,
+                                               uint32_t kvh, uint32_t item, uint32_t first, uint32_t chunks, float *wt, float *sm, float *sl,
+                                               uint32_t &arrived) {
+  constexpr uint32_t T = 256u, R = 64u, PIECES = R * D / 4u / T, U = PIECES < 16u ? 16u / PIECES : 1u;   // U workgroups under way
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t slot_floats = attn_part_floats(p, D), ml = p.rows * D, pieces = t.rows * (D / 4u);
+  const auto place = [&](uint32_t z) { return 2u * (first + z) + (z == 0u ? 1u : 0u); };   // the slot of the tile's workgroup z
+  const uint32_t side = chunks <= kJoinRows * U ? chunks : __builtin_amdgcn_readfirstlane((uint32_t)ceilf(sqrtf((float)chunks)));
+  const uint32_t groups = (chunks + side - 1u) / side;
+  uint32_t z0 = (item - first) / side * side, step = 1u, count = min(side, chunks - z0);
+  for (bool last = groups == 1u;; last = true) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t *counter = cnt + (step == 1u ? 0u : kAttnCounters / 2u) + (uint64_t)kvh * p.items * 2u + place(z0);
+    if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != count - 1u) break;
+    if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    float4v x[U][PIECES], o[PIECES] = {};
+    const auto request = [&](uint32_t z) {
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t k = 0; k < PIECES; ++k) {
+          const uint32_t i = min(tid + T * k, pieces - 1u);
+          x[u][k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)((place(z0 + step * min(z + u, count - 1u)) * slot_floats + 4u * i) * 4u), 0, kSc1));
+        }
+    };
+    request(0);
+    // the rows' maxima and sums: a lane has a row, a wave every fourth workgroup; then the
+    // weights relative to the largest maximum
+    float *ls = wt + count * R;
+    if (lane < t.rows)
+      for (uint32_t z = wave; z < count; z += 4u) {
+        const int at = (int)((place(z0 + step * z) * slot_floats + ml + 2u * lane) * 4u);
+        wt[z * R + lane] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
+        ls[z * R + lane] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
+      }
+    __syncthreads();
+    if (tid < t.rows) {
+      float mx = -INFINITY, l = 0.f;
+      for (uint32_t z = 0; z < count; ++z) mx = fmaxf(mx, wt[z * R + tid]);
+      for (uint32_t z = 0; z < count; ++z) {
+        const float m = wt[z * R + tid], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+        wt[z * R + tid] = f;
+        l += f * ls[z * R + tid];
+      }
+      sl[tid] = l, sm[tid] = mx;
+    }
+    __syncthreads();
+    for (uint32_t z = 0; z < count; z += U) {
+      if (z) request(z);
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t k = 0; k < PIECES; ++k)
+          if (z + u < count) o[k] += x[u][k] * wt[(z + u) * R + min(tid + T * k, pieces - 1u) / (D / 4u)];
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < PIECES; ++k) {
+      const uint32_t i = tid + T * k, r = i / (D / 4u), d = 4u * (i % (D / 4u));
+      if (i >= pieces) break;
+      const float l = sl[r];
+      if (last) {
+        const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+        float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+        *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o[k] / l;
+      } else {
+        const uint32_t at = place(z0) * slot_floats;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[k]), prs, (int)((at + 4u * i) * 4u), 0, kSc1);
+        if (d == 0u) {
+          // a sum that is not a number is not nothing
+          const float mx = sm[r] == -INFINITY && l != 0.f ? 0.f : sm[r];
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((at + ml + 2u * r) * 4u), 0, kSc1);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((at + ml + 2u * r + 1u) * 4u), 0, kSc1);
+        }
+      }
+    }
+    if (last) break;
+    z0 = 0u, step = side, count = groups;
+  }
 }
 
 template <int TYPE, int D, int MODE, typename RULES>
@@ -1379,7 +1478,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   using W = AttnWave<D, I8, false, false, D <= 128 ? kVTurned : kVLater, RULED>;
   using S = AttnStage<D>;
   constexpr uint32_t NW = 4u, R = 16u * NW;
-  __shared__ __align__(1024) uint8_t buf[2][S::BYTES];
+  constexpr int NB = MODE == kAttnEnds && D <= 128 ? 3 : 2;   // buffers: a step's fills are requested NB - 1 steps ahead
+  __shared__ __align__(1024) uint8_t buf[NB][S::BYTES];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
   // The last tiles of a sequence see the most: first; sequence after sequence, and a
@@ -1515,19 +1615,30 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     }
   };
   const int full = W::full_of(m), from = W::from_of(m, window);   // steps from .. full need no mask
-  if (steps) {
-    issue(0, buf[0]);
-    convert(buf[0]);
+  bool gone[NB][2];   // of the steps under way
+#pragma unroll
+  for (int i = 0; i + 1 < NB; ++i) {
+    if (i >= steps) break;
+    issue(i, buf[i]);
+    gone[i][0] = k.gone[0], gone[i][1] = k.gone[1];
+    convert(buf[i]);
   }
 #pragma unroll 1
-  for (int i0 = 0; i0 < steps; i0 += 2) {
+  for (int i0 = 0; i0 < steps; i0 += NB) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < NB; ++half) {
       const int i = i0 + half;
       if (i >= steps) break;
-      const bool was[2] = {k.gone[0], k.gone[1]};
-      wait_step();
-      if (i + 1 < steps) issue(i + 1, buf[1 - half]);
+      constexpr int A = NB - 1;
+      const int next = (half + A) % NB;
+      const bool was[2] = {gone[half][0], gone[half][1]};
+      // this step's fills, and not those of the steps behind it
+      if (A > 1 && i + A - 1 < steps) wait_step<(A - 1) * MINE>();
+      else wait_step<0>();
+      if (i + A < steps) {
+        issue(i + A, buf[next]);
+        gone[next][0] = k.gone[0], gone[next][1] = k.gone[1];
+      }
       const int t0 = base + 32 * i;
       if (t0 < m.end && t0 + 32 > m.begin) {
         const uint8_t *lds = buf[half];
@@ -1554,11 +1665,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
         w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, wr, n, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); },
                [&](int u) { return *(const u32x4 *)(lds + S::SCALES + 128u + 64u * u + 16u * g); });   // late: no register waits for it
       }
-      if (i + 1 < steps) convert(buf[1 - half]);
+      if (i + A < steps) convert(buf[next]);
     }
   }
   const float l = row_add(w.l);
-  if (shared && chunks > 1u) {
+  if constexpr (shared) if (chunks > 1u) {
     const uint32_t slot_floats = attn_part_floats(p, D), slot = (2u * item + (item == first ? 1u : 0u)) * slot_floats;
     const rsrc_t prs = make_rsrc(part + (uint64_t)kvh * p.items * 2u * slot_floats, (uint64_t)p.items * 2u * slot_floats * 4u);
     if (n < m.rows) {
@@ -1575,8 +1686,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     // the waves have passed the last step's barrier, but may still read its buffer
     __shared__ float sm[R], sl[R];
     __shared__ uint32_t arrived;
-    float *wt = (float *)buf;
-    attn_join<D, 256u>(p, prs, cnt, a, t, group, kvh, item, first, chunks, wt, wt + sizeof(buf) / 4u - 1024u, sm, sl, arrived, slot_floats, p.rows * D, tid, lane, wave);
+    attn_join_rows<D>(p, prs, cnt, a, t, group, kvh, item, first, chunks, (float *)buf, sm, sl, arrived);
     return;
   }
   if (n >= m.rows) return;
@@ -1659,24 +1769,37 @@ inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   return p;
 }
 
-// Under rules the sequences with more than 16 rows take all to the tiles of 64.
+// Under rules all sequences go to one kernel.
 inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r) {
   const uint32_t group = a.q_heads / kv.heads;
   AttnPlan p{};
   const uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group, rows = (uint64_t)b.tokens * group;
   p.max_rows = ~0u;
   const uint64_t reach = (uint64_t)a.window + std::max(64u / group, r.tree ? b.max_new : 0u) + 2u;   // under a window
-  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, reach) : b.max_len;
-  if (most <= 16u) {
+  const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, reach) : b.max_len, units = (seen + 31u + kUnit - 1u) / kUnit;
+  uint32_t tiles, per_seq;
+  attn_tiles(most, rows, b.seqs, 64u, &tiles, &per_seq);
+  const uint64_t wgs = (uint64_t)tiles * kv.heads, work = (rows / 16u + b.seqs) * kv.heads * units;
+  // Tiles of 64 rows from 176 of them on, or where there is much to read (32 heads of 128 on
+  // 8: 1 x 200 new tokens 11.8 us, tiles of 16 10.0, 1 x 400 19.5 and 20.9; trees: 2 x 10
+  // over up to 3000 21.7 and 19.0, 8 x 20 over up to 8192 54 and 82). int8 pages cost
+  // them a conversion more (16 x 60 rows over up to 8000 76 and 74, 3 x 600 new tokens of 4
+  // heads 54 and 49, 2 x 900 of 8 88 and 112).
+  const bool f16 = kv.type == EFF_KV_F16;
+  if (most <= 16u || (f16 ? wgs < 176u && work < 8192u : wgs < 400u)) {
     attn_plan_few(p, kv, b, most, rows, seen);
     return p;
   }
-  attn_tiles(most, rows, b.seqs, 64u, &p.many_tiles, &p.many_per_seq);
+  p.many_tiles = tiles, p.many_per_seq = per_seq;
   p.rows = (uint32_t)std::min<uint64_t>(most, 64u);
-  const uint64_t wgs = (uint64_t)p.many_tiles * kv.heads, units = (seen + 31u + kUnit - 1u) / kUnit, each = (most + 63u) / 64u;
+  // Shared where they do not fill the card, or not evenly: few new tokens, long contexts of
+  // any length (three workgroups a CU, two 256 wide: 16 trees of up to 32 over up to 16384
+  // 174 us, two 195, four 183; a chunk of 300 tokens over 4000 70, not shared 128, of 600
+  // over 2000 87 and 73).
   const uint32_t slots = kv.dim <= 128u ? 768u : 512u;
-  const uint64_t items = std::max<uint64_t>(slots / kv.heads, 2u * p.many_tiles);
-  if (wgs < slots && units > 2u && items <= 2048u && items * kv.heads <= kAttnCounters / 4u && each * b.seqs * units < 1u << 31)
+  const uint64_t items = std::max<uint64_t>(slots / kv.heads, 2u * tiles), each = (most + 63u) / 64u;
+  if (f16 && units > 2u && (wgs < 200u || (wgs < slots && units >= 8u && seen >= 16ull * b.max_new)) && items * kv.heads <= kAttnCounters / 4u &&
+      each * b.seqs * units < 1u << 31)
     p.items = (uint32_t)items;
   return p;
 }
@@ -1690,7 +1813,6 @@ inline size_t attn_scratch(const AttnPlan &p, const KvView &kv) {
 template <int TYPE, int D, typename RULES>
 hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const RULES &rules, void *scratch, hipStream_t s) {
   const AttnPlan p = attn_plan(kv, b, a, rules);
-  constexpr bool ruled = !__is_same(RULES, NoRules);
   const bool shared = p.items && !p.tiles;   // the tiles of 64
   const uint64_t many = (uint64_t)(shared ? p.items : p.many_tiles) * kv.heads, grid = (uint64_t)(p.items ? p.items : p.tiles) * kv.heads;
   if (!fits(many, 256u) || !fits(grid, 512u)) return hipErrorInvalidConfiguration;
@@ -1702,12 +1824,9 @@ hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, 
     const auto rows = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((uint32_t)many), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows, rules, p, cnt, part);
     };
-    if constexpr (ruled) {
-      if (shared) rows(k_attn_rows<TYPE, D, kAttnEnds, RULES>);
-      else rows(k_attn_rows<TYPE, D, kAttnWhole, RULES>);
-    } else {
-      rows(k_attn_rows<TYPE, D, kAttnWhole, RULES>);
-    }
+    constexpr bool may = !__is_same(RULES, NoRules) && TYPE == EFF_KV_F16;   // tiles of 64 are shared
+    if (may && shared) rows(k_attn_rows<TYPE, D, may ? kAttnEnds : kAttnWhole, RULES>);
+    else rows(k_attn_rows<TYPE, D, kAttnWhole, RULES>);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.tiles) return e;
   }
