@@ -99,14 +99,19 @@ __device__ __forceinline__ void turn_at(const TURNS &turned, const KvAppendArgs 
 // under way (us, U = 1 / 4: 4780 tokens of 24 heads of 256 with norms 72.2 / 56.9, 3.9
 // TB/s; 4780 of 48 heads of 128 54.4 / 48.8, 4.6 TB/s; 1340 tokens 14.9 / 16.1, 270
 // 6.8 / 7.1).
+// With positions of their own (TURNED) a wave has a team's part instead of a workgroup, so
+// that few key heads do not leave the threads of whole workgroups without a row (5 prompts
+// of 1531 tokens and fewer, 16 heads of 128 on 2, q/k norm: 37 -> 20 us, 5.0 TB/s).
 template <int TYPE, int D, int U, typename TURNS>
 __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t q_wgs, uint32_t k_wgs, TURNS turned) {
 #pragma clang fp contract(off)
-  constexpr uint32_t L = D == 96 ? 32u : D / 4u, ROWS = 256u / L;
   constexpr bool TURNED = !__is_same(TURNS, ByPlace);
-  const uint32_t wgs = q_wgs + 2u * k_wgs, t = blockIdx.x / wgs, w = blockIdx.x % wgs, l = (threadIdx.x & 63u) % L;
+  constexpr uint32_t L = D == 96 ? 32u : D / 4u, TEAM = TURNED ? 64u : 256u, ROWS = TEAM / L;
+  const uint32_t id = TURNED ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6)) : blockIdx.x;
+  const uint32_t wgs = q_wgs + 2u * k_wgs, t = id / wgs, w = id % wgs, l = (threadIdx.x & 63u) % L;
+  if (TURNED && t >= b.tokens) return;
   const bool is_q = w < q_wgs, is_v = w >= q_wgs + k_wgs;
-  const uint32_t heads = is_q ? a.q_heads : kv.heads, h0 = (is_q ? w : is_v ? w - q_wgs - k_wgs : w - q_wgs) * ROWS * U + threadIdx.x / L;
+  const uint32_t heads = is_q ? a.q_heads : kv.heads, h0 = (is_q ? w : is_v ? w - q_wgs - k_wgs : w - q_wgs) * ROWS * U + threadIdx.x % TEAM / L;
   const float *src = is_q ? a.q + (uint64_t)t * a.q_stride : is_v ? a.v + (uint64_t)t * a.v_stride : a.k + (uint64_t)t * a.k_stride;
   const float *norm = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
   const uint32_t half = is_v ? 0u : a.rope_dim / 2u;
@@ -213,17 +218,22 @@ hipError_t launch_rope_table(const RopeFreqs &f, uint32_t pairs, uint32_t positi
 
 template <int TYPE, int D, int U, typename TURNS>
 static hipError_t append_launch(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const TURNS &turned, hipStream_t s) {
-  constexpr uint32_t rows = (D == 96 ? 8u : 1024u / D) * U;   // of a workgroup
+  constexpr uint32_t teams = __is_same(TURNS, ByPlace) ? 1u : 4u;         // of a workgroup
+  constexpr uint32_t rows = (D == 96 ? 8u : 1024u / D) * U / teams;   // of a team
   const uint32_t q = (a.q_heads + rows - 1u) / rows, k = (kv.heads + rows - 1u) / rows;
-  if (!fits((uint64_t)b.tokens * (q + 2u * k), 256u)) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((k_kv_append<TYPE, D, U, TURNS>), dim3(b.tokens * (q + 2u * k)), dim3(256), 0, s, kv, b, a, q, k, turned);
+  const uint64_t wgs = ((uint64_t)b.tokens * (q + 2u * k) + teams - 1u) / teams;
+  if (!fits(wgs, 256u)) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((k_kv_append<TYPE, D, U, TURNS>), dim3((uint32_t)wgs), dim3(256), 0, s, kv, b, a, q, k, turned);
   return hipGetLastError();
 }
 
 template <int TYPE, int D, typename TURNS>
 static hipError_t append_dim(const KvView &kv, const KvBatchView &b, const KvAppendArgs &a, const TURNS &turned, hipStream_t s) {
-  // 4 rows a thread where a CU still has 8 workgroups to take
-  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= 2048ull * 4096u) return append_launch<TYPE, D, 4>(kv, b, a, turned, s);
+  // 4 rows a thread where a CU still has 8 workgroups to take; of waves by themselves, from
+  // two workgroups on (32 heads of 128 on 8: 250 tokens 5.3 us, one row a thread 5.6, 500
+  // 6.9 and 8.7, 100 5.0 and 4.9)
+  const uint64_t from = __is_same(TURNS, ByPlace) ? 2048ull * 4096u : 2048ull * 512u;
+  if ((uint64_t)b.tokens * (a.q_heads + 2u * kv.heads) * D >= from) return append_launch<TYPE, D, 4>(kv, b, a, turned, s);
   return append_launch<TYPE, D, 1>(kv, b, a, turned, s);
 }
 
