@@ -99,13 +99,22 @@ __device__ __forceinline__ void turn_at(const TURNS &turned, const KvAppendArgs 
 // under way (us, U = 1 / 4: 4780 tokens of 24 heads of 256 with norms 72.2 / 56.9, 3.9
 // TB/s; 4780 of 48 heads of 128 54.4 / 48.8, 4.6 TB/s; 1340 tokens 14.9 / 16.1, 270
 // 6.8 / 7.1).
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+template <bool PAST, typename T>
+__device__ __forceinline__ void put(T *o, T v) {
+  if constexpr (PAST) __builtin_nontemporal_store(v, o);
+  else *o = v;
+}
+
 // With positions of their own (TURNED) a wave has a team's part instead of a workgroup, so
 // that few key heads do not leave the threads of whole workgroups without a row (5 prompts
-// of 1531 tokens and fewer, 16 heads of 128 on 2, q/k norm: 37 -> 20 us, 5.0 TB/s).
+// of 1531 tokens and fewer, 16 heads of 128 on 2, q/k norm, 100 MB: 37 -> 26 us; with q, which is more than
+// the L2s hold, stored past them 18.6 us, 5.4 TB/s).
 template <int TYPE, int D, int U, typename TURNS>
 __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t q_wgs, uint32_t k_wgs, TURNS turned) {
 #pragma clang fp contract(off)
-  constexpr bool TURNED = !__is_same(TURNS, ByPlace);
+  constexpr bool TURNED = !__is_same(TURNS, ByPlace), PAST = TURNED && U == 4;   // q of many tokens goes past the L2
   constexpr uint32_t L = D == 96 ? 32u : D / 4u, TEAM = TURNED ? 64u : 256u, ROWS = TEAM / L;
   const uint32_t id = TURNED ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6)) : blockIdx.x;
   const uint32_t wgs = q_wgs + 2u * k_wgs, t = id / wgs, w = id % wgs, l = (threadIdx.x & 63u) % L;
@@ -166,9 +175,9 @@ __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvA
       float *o = a.q_out + ((uint64_t)t * a.q_heads + h) * D;
       if (!placed) y[0] = y[1] = y[2] = y[3] = 0.f;
       if (apart) {
-        *(float2 *)(o + 2u * l) = make_float2(y[0], y[2]), *(float2 *)(o + half + 2u * l) = make_float2(y[1], y[3]);
+        put<PAST>((float2v *)(o + 2u * l), float2v{y[0], y[2]}), put<PAST>((float2v *)(o + half + 2u * l), float2v{y[1], y[3]});
       } else {
-        *(float4 *)(o + 4u * l) = make_float4(y[0], y[1], y[2], y[3]);
+        put<PAST>((float4v *)(o + 4u * l), float4v{y[0], y[1], y[2], y[3]});
       }
       continue;
     }
