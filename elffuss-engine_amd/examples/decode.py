@@ -68,7 +68,7 @@ class Decoder:
             at.update(mask=up(rules["mask"]), mask_of=up(np.asarray(rules["mask_of"], np.uint32)), mask_count=len(rules["mask"]))
         self.logits_rules = eff.LogitsRules(**at)
 
-    def layer(self, tokens, starts, max_new):
+    def layer(self, tokens, starts, max_new, turns=None, rules=None):
         """Buffers of a call of `tokens` new tokens, and the call up to the output projection."""
         ctx, eff, m = self.ctx, self.eff, self.m
         qkv = self.w["qkv"][2]
@@ -77,6 +77,7 @@ class Decoder:
         rows, q, o = ctx.alloc(4 * tokens * qkv), ctx.alloc(4 * tokens * m.heads * m.dim), ctx.alloc(4 * tokens * m.heads * m.dim)
         batch = eff.KvBatch(self.table, ctx.upload(np.asarray(starts, np.uint32)), self.lens, seqs=self.n, tokens=tokens,
                             table_pages=self.table_pages, max_new=max_new, max_len=self.max_len)
+        self.batch = batch
         k0, v0 = m.heads * m.dim, (m.heads + m.kv_heads) * m.dim
         kv_rows = eff.KvRows(q=(rows, 0), k=(rows, k0), v=(rows, v0), q_stride=qkv, k_stride=qkv, v_stride=qkv, q_heads=m.heads,
                              q_out=q, rope=self.rope, rope_positions=self.max_len, rope_dim=m.dim, rope_mode=eff.ROPE_HALVES,
@@ -86,8 +87,8 @@ class Decoder:
             t, w, _, _ = self.w["embedding"]
             ctx.gather_norm(t, w, ids, self.norms["norm"], m.eps, x, nrm, m.embed, tokens)
             self.product("qkv", nrm, rows, tokens)
-            ctx.kv_append(self.cache, batch, kv_rows)
-            ctx.kv_attn(self.cache, batch, q, o, m.heads, m.scale)
+            ctx.kv_append(self.cache, batch, kv_rows, turns=turns)
+            ctx.kv_attn(self.cache, batch, q, o, m.heads, m.scale, rules=rules)
             self.product("out", o, y, tokens)
         return ids, y, run
 
