@@ -277,6 +277,8 @@ napi_value Stats(napi_env env, napi_callback_info info) {
   napi_set_named_property(env, o, "cpuPath", make_int(env, (int64_t)s.cpu_path));
   napi_set_named_property(env, o, "kvAppend", make_int(env, (int64_t)s.kv_append));
   napi_set_named_property(env, o, "kvAttn", make_int(env, (int64_t)s.kv_attn));
+  napi_set_named_property(env, o, "kvCopy", make_int(env, (int64_t)s.kv_copy));
+  napi_set_named_property(env, o, "kvKeep", make_int(env, (int64_t)s.kv_keep));
   napi_set_named_property(env, o, "logits", make_int(env, (int64_t)s.logits));
   return o;
 }
@@ -772,10 +774,10 @@ napi_value RopeTable(napi_env env, napi_callback_info info) {
   return status(env, ctx, eff_rope_table(ctx, (const double *)f, (uint32_t)(len / 8), positions, scale, external<eff_buf>(env, a[4])));
 }
 
-// kvAppend(ctx, cache, batch, rows)
+// kvAppend(ctx, cache, batch, rows, turns?); turns: { at, axes, axis (Uint8Array) }
 napi_value KvAppend(napi_env env, napi_callback_info info) {
-  napi_value a[4];
-  get_args(env, info, 4, a);
+  napi_value a[5];
+  get_args(env, info, 5, a);
   eff_ctx *ctx = external<eff_ctx>(env, a[0]);
   const eff_kv_cache c = kv_cache(env, a[1]);
   const eff_kv_batch b = kv_batch(env, a[2]);
@@ -791,23 +793,92 @@ napi_value KvAppend(napi_env env, napi_callback_info info) {
   r.rope_mode = u32_prop(env, a[3], "ropeMode");
   r.q_norm = buf_prop(env, a[3], "qNorm"), r.k_norm = buf_prop(env, a[3], "kNorm");
   r.norm_eps = (float)number(env, prop(env, a[3], "normEps"), "normEps", 1e-6);
+  if (absent(env, a[4])) {
+    if (thrown(env)) return nullptr;
+    return status(env, ctx, eff_kv_append(ctx, &c, &b, &r));
+  }
+  eff_kv_turns t{};
+  t.at = buf_prop(env, a[4], "at"), t.axes = u32_prop(env, a[4], "axes");
+  napi_value axis = prop(env, a[4], "axis");
+  if (!absent(env, axis)) {
+    void *p = nullptr;
+    size_t len = 0;
+    napi_typedarray_type type;
+    if (napi_get_typedarray_info(env, axis, &type, nullptr, nullptr, nullptr, nullptr) != napi_ok || type != napi_uint8_array ||
+        !bytes_of(env, axis, &p, &len) || len > sizeof(t.axis))
+      throw_msg(env, "axis: not a Uint8Array of up to 128 axes");
+    else if (len)
+      memcpy(t.axis, p, len);
+  }
   if (thrown(env)) return nullptr;
-  return status(env, ctx, eff_kv_append(ctx, &c, &b, &r));
+  return status(env, ctx, eff_kv_append_at(ctx, &c, &b, &r, &t));
 }
 
-// kvAttn(ctx, cache, batch, q, qOffset, qStride, out, qHeads, scale, window)
+// kvAttn(ctx, cache, batch, q, qOffset, qStride, out, qHeads, scale, window, rules?);
+// rules: { cap, slopes, ranges, tree, treeWords }
 napi_value KvAttn(napi_env env, napi_callback_info info) {
-  napi_value a[10];
-  get_args(env, info, 10, a);
+  napi_value a[11];
+  get_args(env, info, 11, a);
   eff_ctx *ctx = external<eff_ctx>(env, a[0]);
   const eff_kv_cache c = kv_cache(env, a[1]);
   const eff_kv_batch b = kv_batch(env, a[2]);
   const uint64_t q_offset = offset(env, a[4], "qOffset");
   const uint32_t q_stride = u32(env, a[5], "qStride"), q_heads = u32(env, a[7], "qHeads"), window = u32(env, a[9], "window");
   const float scale = (float)number(env, a[8], "scale", 0.0);
+  if (!absent(env, a[10])) {
+    eff_kv_rules r{};
+    r.cap = (float)number(env, prop(env, a[10], "cap"), "cap", 0.0);
+    r.tree_words = u32_prop(env, a[10], "treeWords");
+    r.slopes = buf_prop(env, a[10], "slopes"), r.ranges = buf_prop(env, a[10], "ranges"), r.tree = buf_prop(env, a[10], "tree");
+    if (thrown(env)) return nullptr;
+    return status(env, ctx, eff_kv_attn_rules(ctx, &c, &b, external<eff_buf>(env, a[3]), q_offset, q_stride, external<eff_buf>(env, a[6]),
+                                              q_heads, scale, window, &r));
+  }
   if (thrown(env)) return nullptr;
   return status(env, ctx, eff_kv_attn(ctx, &c, &b, external<eff_buf>(env, a[3]), q_offset, q_stride, external<eff_buf>(env, a[6]),
                                       q_heads, scale, window));
+}
+
+// The caches of a call's layers (an array of descriptions).
+std::vector<eff_kv_cache> kv_caches(napi_env env, napi_value v) {
+  std::vector<eff_kv_cache> got;
+  bool is = false;
+  uint32_t n = 0;
+  if (napi_is_array(env, v, &is) != napi_ok || !is || napi_get_array_length(env, v, &n) != napi_ok) {
+    throw_msg(env, "caches: not an array");
+    return got;
+  }
+  for (uint32_t i = 0; i < n && !thrown(env); ++i) {
+    napi_value c = undefined(env);
+    napi_get_element(env, v, i, &c);
+    got.push_back(kv_cache(env, c));
+  }
+  return got;
+}
+
+// kvCopy(ctx, caches, copies, count)
+napi_value KvCopy(napi_env env, napi_callback_info info) {
+  napi_value a[4];
+  get_args(env, info, 4, a);
+  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
+  const std::vector<eff_kv_cache> c = kv_caches(env, a[1]);
+  const uint32_t count = thrown(env) ? 0u : u32(env, a[3], "count");
+  if (thrown(env)) return nullptr;
+  return status(env, ctx, eff_kv_copy(ctx, c.data(), (uint32_t)c.size(), external<eff_buf>(env, a[2]), count));
+}
+
+// kvKeep(ctx, caches, batch, kept, counts, newLens?)
+napi_value KvKeep(napi_env env, napi_callback_info info) {
+  napi_value a[6];
+  get_args(env, info, 6, a);
+  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
+  const std::vector<eff_kv_cache> c = kv_caches(env, a[1]);
+  if (thrown(env)) return nullptr;
+  const eff_kv_batch b = kv_batch(env, a[2]);
+  eff_buf *lens = absent(env, a[5]) ? nullptr : external<eff_buf>(env, a[5]);
+  if (!absent(env, a[5]) && !lens) throw_msg(env, "newLens: not a buffer");
+  if (thrown(env)) return nullptr;
+  return status(env, ctx, eff_kv_keep(ctx, c.data(), (uint32_t)c.size(), &b, external<eff_buf>(env, a[3]), external<eff_buf>(env, a[4]), lens));
 }
 
 // logitsApply(ctx, in, out, rows, vocab, stride, rules)
@@ -838,7 +909,7 @@ napi_value Register(napi_env env, napi_value exports) {
       {"qgemmPrepared", QGemmPrepared}, {"qmatmulXLayout", QMatmulXLayout},
       {"qmatmulPrepareX", QMatmulPrepareX}, {"qmatmulPrepared", QMatmulPrepared},
       {"qmatmulCpuPath", QMatmulCpuPath}, {"kvPageBytes", KvPageBytes}, {"ropeTable", RopeTable},
-      {"kvAppend", KvAppend}, {"kvAttn", KvAttn}, {"logitsApply", LogitsApply},
+      {"kvAppend", KvAppend}, {"kvAttn", KvAttn}, {"kvCopy", KvCopy}, {"kvKeep", KvKeep}, {"logitsApply", LogitsApply},
   };
   for (auto &f : fns) {
     napi_value v;

@@ -896,7 +896,7 @@ function createTopKGPU(device, ctx) {
 // host (README.md:101, sample.js:78-153). Here the cache is pages shared by
 // requests, and the rules on the logits of a batch run on the device; the
 // descriptions are those of include/elffuss_amd.h (eff_kv_cache, eff_kv_batch,
-// eff_kv_rows, eff_logits_rules). No counterpart in the reference's operators.
+// eff_kv_rows, eff_kv_turns, eff_kv_rules, eff_logits_rules). No counterpart in the reference's operators.
 const KV_TIPOS = { F16: 1, I8: 24 };
 const ROPE = { PARES: 0, MITADES: 1 };
 const SIN_PAGINA = 0xFFFFFFFF;
@@ -941,6 +941,20 @@ function descLote(l) {
     seqs: l.secuencias, tokens: l.tokens, tablePages: l.paginasTabla, maxNew: l.maxNuevos, maxLen: l.maxLargo };
 }
 
+// Positions to turn by: { en (u32 [ejes][tokens]), ejes, eje (the axis of each pair of channels) }.
+function descGiros(g) {
+  soloEstas(g, ['en', 'ejes', 'eje'], 'giros');
+  for (const e of g.eje || []) if (!Number.isInteger(e) || e < 0 || e > 3) throw invalido(`eje: «${e}» no es un eje`);   // a Uint8Array would wrap it
+  return { at: manejador(g.en, 'en'), axes: g.ejes === undefined ? 1 : g.ejes, axis: g.eje === undefined ? undefined : Uint8Array.from(g.eje) };
+}
+
+// Rules on attention's scores: { tope, pendientes, rangos, arbol, palabrasArbol }.
+function descReglasAtencion(r) {
+  soloEstas(r, ['tope', 'pendientes', 'rangos', 'arbol', 'palabrasArbol'], 'reglas');
+  return { cap: r.tope, slopes: manejador(r.pendientes, 'pendientes'), ranges: manejador(r.rangos, 'rangos'), tree: manejador(r.arbol, 'arbol'),
+    treeWords: r.palabrasArbol };
+}
+
 function createKvOps(device, deps) {
   const ctx = deps.ctx;
   return {
@@ -964,26 +978,40 @@ function createKvOps(device, deps) {
     },
     // New k, v rows into the cache; q rotated into a pooled buffer, which it resolves to (null without q).
     // filas: { q, k, v, desdeQ, desdeK, desdeV, pasoQ, pasoK, pasoV, cabezasQ, rope, posicionesRope, dimRope,
-    // modoRope, normaQ, normaK, eps }.
-    anade(cache, lote, filas) {
+    // modoRope, normaQ, normaK, eps }; giros (descGiros): positions of their own.
+    anade(cache, lote, filas, giros) {
       const f = soloEstas(filas, DE_FILAS, 'filas');
       const d = { q: manejador(f.q, 'q'), k: manejador(f.k, 'k'), v: manejador(f.v, 'v'), qOffset: f.desdeQ, kOffset: f.desdeK,
         vOffset: f.desdeV, qStride: f.pasoQ, kStride: f.pasoK, vStride: f.pasoV, qHeads: f.q ? f.cabezasQ : 0,
         rope: manejador(f.rope, 'rope'), ropePositions: f.posicionesRope, ropeDim: f.dimRope, ropeMode: f.modoRope,
         qNorm: manejador(f.normaQ, 'normaQ'), kNorm: manejador(f.normaK, 'normaK'), normEps: f.eps };
-      const c = descCache(cache), l = descLote(lote);
+      const c = descCache(cache), l = descLote(lote), g = giros ? descGiros(giros) : undefined;
       const q = f.q ? ctx.alloc(lote.tokens * f.cabezasQ * cache.dim * 4, 'kv.q') : null;
       d.qOut = manejador(q, 'q');
-      native.kvAppend(device._ctx, c, l, d);
+      native.kvAppend(device._ctx, c, l, d, g);
       return Promise.resolve(q);
     },
-    // Attention of the new tokens over the cache, into a pooled buffer. opts: { ventana, desdeQ, pasoQ }.
+    // Attention of the new tokens over the cache, into a pooled buffer. opts: { ventana, desdeQ, pasoQ, reglas
+    // (descReglasAtencion) }.
     atiende(cache, lote, q, cabezasQ, escala, opts) {
-      const o = soloEstas(opts || {}, ['ventana', 'desdeQ', 'pasoQ'], 'opts');
-      const c = descCache(cache), l = descLote(lote), h = manejador(q, 'q');
+      const o = soloEstas(opts || {}, ['ventana', 'desdeQ', 'pasoQ', 'reglas'], 'opts');
+      const c = descCache(cache), l = descLote(lote), h = manejador(q, 'q'), r = o.reglas ? descReglasAtencion(o.reglas) : undefined;
       const out = ctx.alloc(lote.tokens * cabezasQ * cache.dim * 4, 'kv.atencion');
-      native.kvAttn(device._ctx, c, l, h, o.desdeQ, o.pasoQ, out._h, cabezasQ, escala, o.ventana);
+      native.kvAttn(device._ctx, c, l, h, o.desdeQ, o.pasoQ, out._h, cabezasQ, escala, o.ventana, r);
       return Promise.resolve(out);
+    },
+    // Pages to others in the caches of all layers (an array): copias u32 [cuantas][3], from, to, tokens.
+    copiaPaginas(caches, copias, cuantas) {
+      if (cuantas === undefined || cuantas === null) throw invalido('copiaPaginas: ¿cuántas?');
+      native.kvCopy(device._ctx, caches.map(descCache), manejador(copias, 'copias'), cuantas);
+      return Promise.resolve();
+    },
+    // The drafts that stay move up in the caches of all layers: guardados u32 [tokens], cuantos u32 [secuencias];
+    // largosNuevos (u32 [secuencias], may be left out): the lengths after it.
+    conserva(caches, lote, guardados, cuantos, largosNuevos) {
+      native.kvKeep(device._ctx, caches.map(descCache), descLote(lote), manejador(guardados, 'guardados'), manejador(cuantos, 'cuantos'),
+        manejador(largosNuevos, 'largosNuevos'));
+      return Promise.resolve();
     },
   };
 }
