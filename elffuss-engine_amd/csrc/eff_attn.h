@@ -39,6 +39,7 @@ namespace eff {
 
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef short short2v __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -165,9 +166,9 @@ struct AttnTileOf<true> {
   typedef AttnTileRules type;
 };
 
-// Of the L lanes of a row group (16: DPP, 64: then swaps), the largest number, and the smallest.
+// Of a group of L lanes, that of lane `of` (16: DPP, 64: then swaps), the largest number, and the smallest.
 template <uint32_t L>
-__device__ __forceinline__ int lanes_max(int v) {
+__device__ __forceinline__ int lanes_max(int v, uint32_t of = 0) {
   v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
   v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
   v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
@@ -178,10 +179,10 @@ __device__ __forceinline__ int lanes_max(int v) {
     auto b = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
     v = max((int)b[0], (int)b[1]);
   }
-  return __builtin_amdgcn_readfirstlane(v);
+  return __builtin_amdgcn_readlane(v, of);
 }
 template <uint32_t L>
-__device__ __forceinline__ int lanes_min(int v) { return -lanes_max<L>(-v); }
+__device__ __forceinline__ int lanes_min(int v, uint32_t of = 0) { return -lanes_max<L>(-v, of); }
 
 constexpr int kWindowMost = 0x40000000;
 
@@ -191,12 +192,22 @@ __device__ __forceinline__ void range_of(const KvRulesView &r, uint32_t token, i
   from = (int)min(v.x, (uint32_t)len), to = (int)min(v.y, (uint32_t)len);
 }
 
-// What a tile's rows see under rules, R rows at most in the lanes of each group of R
-// (without rules it stands).
+// The range of row i of a tile; empty for a token without a position, and where there are
+// no ranges.
+__device__ __forceinline__ void attn_range(const AttnTileRules &t, const KvRulesView &r, uint32_t group, uint32_t i, int &from, int &to) {
+  from = 0, to = 0;
+  if (!r.ranges || i >= t.rows) return;
+  const uint32_t tok = (t.r0 + i) / group;
+  range_of(r, t.token0 + tok, max(t.len, 0), from, to);
+  if (t.base + (int)tok < 0) to = 0;
+}
+
+// What a tile's rows see under rules (without rules it stands): R rows at most, whose
+// ranges lie in the R lanes from lane `of` on.
 template <uint32_t R>
-__device__ __forceinline__ void attn_seen(AttnTile &, NoRules, uint32_t, int) {}
+__device__ __forceinline__ void attn_seen(AttnTile &, NoRules, int, int, int, uint32_t = 0) {}
 template <uint32_t R>
-__device__ __forceinline__ void attn_seen(AttnTileRules &t, const KvRulesView &r, uint32_t group, int window) {
+__device__ __forceinline__ void attn_seen(AttnTileRules &t, const KvRulesView &r, int window, int from, int to, uint32_t of = 0) {
   t.all_from = window ? max(0, t.last - window + 1) : 0;
   t.all_to = t.first + 1;
   if (r.tree) {
@@ -206,17 +217,12 @@ __device__ __forceinline__ void attn_seen(AttnTileRules &t, const KvRulesView &r
     t.all_from = window ? max(0, t.len - window) : 0;
     t.all_to = max(t.base, 0);
   } else if (r.ranges) {
-    const uint32_t i = (threadIdx.x & 63u) % R, tok = (t.r0 + i) / group;
-    const bool on = i < t.rows;
-    int from = 0, to = 0;
-    if (on) range_of(r, t.token0 + tok, max(t.len, 0), from, to);
-    if (t.base + (int)tok < 0) to = 0;   // a token without a position
-    const bool some = on && from < to;
-    t.begin = lanes_min<R>(some ? from : 0x7FFFFFFF);
-    t.end = lanes_max<R>(some ? to : 0);
+    const bool on = (threadIdx.x & 63u) - of < t.rows, some = on && from < to;
+    t.begin = lanes_min<R>(some ? from : 0x7FFFFFFF, of);
+    t.end = lanes_max<R>(some ? to : 0, of);
     if (t.end == 0) t.begin = 0;
-    t.all_from = lanes_max<R>(on ? from : 0);
-    t.all_to = lanes_min<R>(on ? to : 0x7FFFFFFF);
+    t.all_from = lanes_max<R>(on ? from : 0, of);
+    t.all_to = lanes_min<R>(on ? to : 0x7FFFFFFF, of);
   }
 }
 
@@ -563,14 +569,14 @@ struct AttnWave {
   }
 
   // What row n sees and how it scores, for the steps to read.
-  static __device__ __forceinline__ void put_rule(const KvAttnArgs &a, const Rules &r, const Tile &t, uint32_t kvh, uint32_t n, uint32_t g, int window) {
+  static __device__ __forceinline__ void put_rule(const Rules &r, const Tile &t, uint32_t kvh, uint32_t n, uint32_t g, int window, int from, int to) {
     if constexpr (RULES) {
       const bool on = n < t.rows;
       const uint32_t i = t.r0 + (on ? n : 0u), tok = i / r.group;
       const int place = t.base + (int)tok;
       AttnRule x = {0, 0, place, 0.f};
       if (on && r.all.tree && (window || r.all.slopes)) x.pos = key_position(r, t, t.token0 + tok);
-      if (on && r.all.ranges) range_of(r.all, t.token0 + tok, max(t.len, 0), x.from, x.to);
+      if (r.all.ranges) x.from = from, x.to = to;
       else if (on) x.from = window ? max(0, x.pos - window + 1) : 0, x.to = r.all.tree ? t.len : place + 1;
       if (place < 0) x.to = 0;   // without a position it sees nothing
       // far from all that it sees, a row's distances are counted from the nearest of it: the
@@ -880,6 +886,7 @@ struct AttnWave {
         keep_v(keep);
         if (unlike(t, r)) {
           uint32_t most = 0;
+          short2v both = {0, 0};   // under rules two at a time: no number's magnitude is negative
 #pragma unroll
           for (int i = 0; i < (VIN == kVLater ? E : VN * VM / 4); ++i) {
             u32x4 o;
@@ -888,9 +895,13 @@ struct AttnWave {
 #pragma unroll
               for (int x = 0; x < 4; ++x) o[x] = vw[(4 * i + x) / VM][(4 * i + x) % VM];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) most = max(most, max(o[x] & 0x7FFFu, o[x] >> 16 & 0x7FFFu));
+            for (int x = 0; x < 4; ++x) {
+              if constexpr (RULES) both = __builtin_elementwise_max(both, __builtin_bit_cast(short2v, o[x] & 0x7FFF7FFFu));
+              else most = max(most, max(o[x] & 0x7FFFu, o[x] >> 16 & 0x7FFFu));
+            }
             __builtin_amdgcn_sched_barrier(0);   // one column's registers at a time
           }
+          if constexpr (RULES) most = (uint32_t)max(both[0], both[1]);
           dirty = __any(most >= 0x7C00u);
           if constexpr (RULES) {
             if (dirty) spoil(bad_tokens(keep, v), bits);
@@ -1241,7 +1252,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
     if (!attn_tile<R>(b, group, a.window, item, p.per_seq, 1u, p.max_rows, t)) return;
   }
   for (;;) {
-    attn_seen<R>(t, rules, group, window);
+    int from = 0, to = 0;   // lane n: row n's range
+    if constexpr (RULED) attn_range(t, rules, group, n, from, to);
+    attn_seen<R>(t, rules, window, from, to);
     const int base = t.begin & ~31;
     int lo = base, hi = t.end;
     if (shared) {
@@ -1263,7 +1276,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
         w.load_q(q, a, t, group, kvh, n, g);
         w.fetch_k(k, kv, 0, n, g);   // of the first page, where the wave has no step
         w.init(q, a.scale, (uint8_t *)so, wave, NW);
-        W::put_rule(a, wr, t, kvh, n, g, window);
+        W::put_rule(wr, t, kvh, n, g, window, from, to);
         if constexpr (QL) __syncthreads();
         w.run(k, kv, t, window, wr, n, g);
         if constexpr (QL) __syncthreads();   // the sums take q's place
@@ -1499,7 +1512,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   }
   const int window = (int)min(a.window, 0x40000000u);
   typename W::Tile m = t;   // the wave's own rows
-  attn_seen<R>(t, rules, group, window);
+  int row_from = 0, row_to = 0;   // lane r: the range of the tile's row r
+  if constexpr (RULED) attn_range(t, rules, group, lane, row_from, row_to);
+  attn_seen<R>(t, rules, window, row_from, row_to);
   const int tile_base = t.begin & ~31;
   int base = tile_base, hi = t.end;
   uint32_t first = 0, chunks = 1;   // the tile's workgroups
@@ -1519,17 +1534,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     m.last = t.first + (int)((m.r0 + m.rows - 1u) / group - t.r0 / group);
     m.end = max(m.last + 1, 0);
     m.begin = window ? max(0, m.first - window + 1) : 0;
-    attn_seen<16>(m, rules, group, window);
+    attn_seen<16>(m, rules, window, row_from, row_to, row0);
   } else {
     m.r0 = t.r0, m.end = 0;
   }
   W w;
-  float q[W::KS][8];
-  w.load_q(q, a, m, group, kvh, n, g);
-  w.init(q, a.scale, nullptr, wave, NW);
+  const auto begin_rows = [&] {
+    float q[W::KS][8];
+    w.load_q(q, a, m, group, kvh, n, g);
+    w.init(q, a.scale, nullptr, wave, NW);
+  };
+  if constexpr (!RULED) begin_rows();
   __shared__ AttnRule rule_rows[RULED ? NW : 1u][RULED ? 16u : 1u];
   const auto wr = attn_rules(rules, rule_rows[RULED ? wave : 0u], group);
-  W::put_rule(a, wr, m, kvh, n, g, window);
+  if constexpr (RULED) W::put_rule(wr, m, kvh, n, g, window, __shfl(row_from, row0 + n), __shfl(row_to, row0 + n));
 
   const uint32_t to_v = kv.heads * kv.block_bytes;
   AttnWalk k;
@@ -1623,6 +1641,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     gone[i][0] = k.gone[0], gone[i][1] = k.gone[1];
     convert(buf[i]);
   }
+  if constexpr (RULED) begin_rows();   // on the first steps' way
 #pragma unroll 1
   for (int i0 = 0; i0 < steps; i0 += NB) {
 #pragma unroll
