@@ -1243,7 +1243,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
   const int window = (int)min(a.window, 0x40000000u);
   constexpr bool shared = MODE != kAttnWhole, on = MODE == kAttnOn;
   uint32_t tree = 0;   // new tokens of a tree at most
-  if constexpr (RULED) tree = rules.tree ? b.max_new : 0u;
+  if constexpr (RULED) tree = rules.tree ? min(b.max_new, b.tokens) : 0u;
   typename W::Tile t;
   AttnShare c = {1u, 1u, 0u, 1u, 0u, 0u};
   if constexpr (shared) {
@@ -1505,7 +1505,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   AttnShare c = {1u, 1u, 0u, 1u, 0u, 0u};
   if constexpr (shared) {
     uint32_t tree = 0;   // new tokens of a tree at most
-    if constexpr (RULED) tree = rules.tree ? b.max_new : 0u;
+    if constexpr (RULED) tree = rules.tree ? min(b.max_new, b.tokens) : 0u;
     if (!attn_share<R, true>(b, group, a.window, tree, item, p.items, ~0u, t, c)) return;
   } else {
     if (!attn_tile<R>(b, group, a.window, tile, per_seq, min_rows, ~0u, t)) return;
@@ -1792,9 +1792,10 @@ inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
 inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, const KvRulesView &r) {
   const uint32_t group = a.q_heads / kv.heads;
   AttnPlan p{};
-  const uint64_t most = std::min<uint64_t>(b.max_new, b.tokens) * group, rows = (uint64_t)b.tokens * group;
+  const uint32_t new_most = std::min(b.max_new, b.tokens);
+  const uint64_t most = (uint64_t)new_most * group, rows = (uint64_t)b.tokens * group;
   p.max_rows = ~0u;
-  const uint64_t reach = (uint64_t)a.window + std::max(64u / group, r.tree ? b.max_new : 0u) + 2u;   // under a window
+  const uint64_t reach = (uint64_t)a.window + std::max(64u / group, r.tree ? new_most : 0u) + 2u;   // under a window
   const uint64_t seen = a.window ? std::min<uint64_t>(b.max_len, reach) : b.max_len, units = (seen + 31u + kUnit - 1u) / kUnit;
   uint32_t tiles, per_seq;
   attn_tiles(most, rows, b.seqs, 64u, &tiles, &per_seq);
@@ -1817,7 +1818,7 @@ inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // over 2000 87 and 73).
   const uint32_t slots = kv.dim <= 128u ? 768u : 512u;
   const uint64_t items = std::max<uint64_t>(slots / kv.heads, 2u * tiles), each = (most + 63u) / 64u;
-  if (f16 && units > 2u && (wgs < 200u || (wgs < slots && units >= 8u && seen >= 16ull * b.max_new)) && items * kv.heads <= kAttnCounters / 4u &&
+  if (f16 && units > 2u && (wgs < 200u || (wgs < slots && units >= 8u && seen >= 16ull * new_most)) && items * kv.heads <= kAttnCounters / 4u &&
       each * b.seqs * units < 1u << 31)
     p.items = (uint32_t)items;
   return p;

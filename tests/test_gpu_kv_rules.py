@@ -156,6 +156,35 @@ def test_many_rows(ctx, eff, t, dim, name, heads, group, new, lens):
 
 
 @pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("name", ["any tree", "documents", "any range", ""])
+def test_many_rows_of_int8(ctx, eff, dim, name):
+    """Enough tiles of 64 rows for pages that are converted on the way."""
+    run(eff, ctx, dim, I8, 16, 2, dim, 32, [800, 1, 500], [850, 300, 500], **rules_of(name) or {"cap": 20.0, "slopes": True})
+
+
+@pytest.mark.parametrize("t", [F16, I8])
+@pytest.mark.parametrize("group,new,lens", [(4, [1, 3], [50, 900]), (4, [30, 9], [3000, 1200]), (1, [900, 700], [900, 700])])
+def test_rows_behind_the_last_sequence(ctx, eff, t, group, new, lens):
+    """Tokens of a padded batch that belong to no sequence: their rows stay as they were."""
+    rng = np.random.default_rng(group)
+    b = Batch(rng, new, lens, 16)
+    data, values = make(rng, t, 16, 64, b)
+    tokens = b.tokens + 5
+    q = rng.standard_normal((tokens, 16 * group, 64)).astype(np.float32)
+    out = ctx.upload(np.full(q.shape, 7, np.float32))
+    masks = trees(rng, b)
+    words = (max(new) + 31) // 32
+    tree = np.concatenate([tree_words(masks, words), np.full((5, words), 0xFFFFFFFF, np.uint32)])
+    mine = b.upload(eff, ctx)
+    batch = eff.KvBatch(*mine.buffers, seqs=2, tokens=tokens, table_pages=b.table_pages, max_new=max(new), max_len=max(lens))
+    ctx.kv_attn(eff.KvCache(t, 16, 64, 16, b.pages, ctx.upload(data)), batch, ctx.upload(q), out, 16 * group, 0.125,
+                rules=eff.KvRules(tree=ctx.upload(tree), tree_words=words))
+    got = out.read(np.float32).reshape(q.shape)
+    assert (got[b.tokens:] == 7).all()
+    check(got[:b.tokens], attend_rules(values, b, q[:b.tokens], 16 * group, 0.125, masks=masks), values)
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
 @pytest.mark.parametrize("name", ["tree", "any tree", "any range", ""])
 def test_shared_tiles(ctx, eff, dim, name):
     """Tiles of 64 rows that several workgroups share, of sequences of any length: joins of a few and of one."""

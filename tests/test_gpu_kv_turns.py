@@ -119,6 +119,30 @@ def test_more_new_tokens_than_length(ctx, eff):
     run(eff, ctx, 7, F16, 2, 1, 64, 16, [5, 2], [3, 9], 64, True, dealt(32, 3))
 
 
+@pytest.mark.parametrize("tokens", [3, 900])
+def test_rows_behind_the_last_sequence(ctx, eff, tokens):
+    """Tokens of a padded batch that belong to no sequence: their rows stay as they were, and the cache."""
+    rng = np.random.default_rng(tokens)
+    b = Batch(rng, [tokens], [tokens + 40], 64)
+    x = [rng.standard_normal((tokens + 4, n, 128)).astype(np.float32) for n in (16, 2, 2)]
+    at = rng.integers(0, 50, (1, tokens + 4)).astype(np.uint32)
+    rb, rope = rope_of(ctx, eff, 50, 128)
+    old = rng.integers(0, 256, b.pages * page_bytes(F16, 2, 128, 64), dtype=np.uint8)
+    cb, q_out = ctx.upload(old), ctx.upload(np.full(x[0].shape, 5, np.float32))
+    mine = b.upload(eff, ctx)
+    batch = eff.KvBatch(*mine.buffers, seqs=1, tokens=tokens + 4, table_pages=b.table_pages, max_new=tokens, max_len=tokens + 40)
+    ctx.kv_append(eff.KvCache(F16, 2, 128, 64, b.pages, cb), batch,
+                  eff.KvRows(q=ctx.upload(x[0]), k=ctx.upload(x[1]), v=ctx.upload(x[2]), q_heads=16, q_out=q_out, rope=rb, rope_positions=50,
+                             rope_dim=128), turns=eff.KvTurns(ctx.upload(at)))
+    got, want = q_out.read(np.float32).reshape(x[0].shape), turn_at(x[0], at, [0] * 64, rope, 128, False)
+    assert (got[tokens:] == 5).all() and (np.abs(got - want)[:tokens] <= TURN * np.abs(want[:tokens]).max(-1, keepdims=True)).all()
+    values, before = (decode(F16, d, b.pages, 2, 128, 64).view(np.uint64) for d in (cb.read(np.uint8), old))
+    written = np.zeros((b.pages, 64), bool)
+    for pos in b.positions():
+        written[b.table[0, pos // 64], pos % 64] = True
+    assert np.array_equal(values.transpose(0, 3, 1, 2, 4)[~written], before.transpose(0, 3, 1, 2, 4)[~written])
+
+
 def test_recorded(ctx, eff):
     """A recorded append takes the next step's positions."""
     rng = np.random.default_rng(8)
