@@ -357,8 +357,9 @@ __device__ __forceinline__ bool attn_share(const KvBatchView &b, uint32_t group,
   if (ENDS && count >= items) return false;
   if (ENDS || (each < kShort && count < items)) whole = each = max((total + items - count - 1u) / (items - count), kLeast);
   if (ENDS && __is_same(TILE, AttnTileRules) && b.seqs <= 64u) {
-    // that holds for any lengths; the smallest share that these need: one tile's last
-    // workgroup seldom has next to nothing
+    // that holds for any lengths; the smallest share that these need, which may be half of
+    // it (16 trees of up to 32 over up to 16384: 189 -> 174 us; 40 of up to 6 over int8
+    // pages 256 wide, 4096 of up to 9001 seen: 73 -> 64)
     for (uint32_t least = max((total + items - 1u) / items, kLeast); least < each;) {
       const uint32_t mid = (least + each) / 2u;
       if ((uint32_t)wave_sum((float)(tiles * ((of + mid - 1u) / mid))) <= items) each = mid;
@@ -483,12 +484,13 @@ struct AttnWalk {
 //           is read by the caller as it is used (for want of registers)
 enum { kVRows, kVTurned, kVLater };
 
-// tanh(z) / z in z^2 up to z = kTanhFew: within 4e-9 there (a least-maximum fit).
+// tanh(z) / z in z^2 up to z = kTanhFew: within 4e-9 there (a least-maximum fit), 5.3e-8 in
+// f32. Scores below 0.625 of the cap, the ordinary ones, cost 8 instructions each.
 constexpr float kTanhFew = 0.625f;
 constexpr float kTanh[6] = {1.f, -0.3333326f, 0.13331127f, -0.053721067f, 0.020590989f, -0.0056599886f};
 
 // What a row sees and where it is, in LDS: a step reads it where it needs it, so that it
-// takes no registers from step to step.
+// takes no registers from step to step (fp16 256 wide would not have them).
 struct AttnRule {
   int from, to;   // the cached tokens that it sees, but for the tree's
   int pos;        // its position
@@ -1089,7 +1091,9 @@ constexpr uint32_t kFewRows = 64;
 // trip of two (32 workgroups x 8 rows x 128: 14.7 us, in two 15.3; 64 x 8 x 128 22.3 and
 // 20.3; 128 x 8 x 128 40.9 and 26.9).
 constexpr uint32_t kJoin = 32768;
-constexpr uint32_t kJoinRows = 5;   // round trips of a join of 64 rows
+// Of tiles of 64 rows: round trips of one join, and workgroups of a head, of which either
+// step of two joins then has at most 32 (the LDS of 64 wide).
+constexpr uint32_t kJoinRows = 5, kItemsRows = 1024, kJoinSide = 32;
 constexpr int kSc1 = 16;   // cache policy bit 4: sc1, past the XCD's own L2
 
 enum { kAttnWhole, kAttnEnds, kAttnOn };   // a workgroup has a tile; a part of one; a share that may go on into the next
@@ -1221,7 +1225,11 @@ __device__ __forceinline__ void attn_join(const AttnPlan &p, rsrc_t prs, uint32_
 // the bytes with as many instructions, which shows where the shares are short (40 up
 // to 9001, 16 heads of 256 on 2: 43 to 46 us, 3.6 to 3.9 TB/s). A single short sequence
 // is round trips: lengths, page table, K, V, the join (517 tokens: 6.3 to 6.8 us, an
-// empty launch 3.4). Shares that go on keep 26 to 47 scalar registers in vector ones
+// empty launch 3.4). Under rules: 48 up to 8192, 16 heads of 256 on 8, capped, 319 us, 5.7
+// TB/s; one of 20001, 32 heads of 128 with slopes, 60 us, 5.5 TB/s; int8 trees of up to 6
+// drafts (48 rows, three tiles) over 4096 of up to 9001, 16 heads of 256 on 2, 64 us, 2.2
+// TB/s of the cache: each tile converts the keys and values for itself, the VALU is busy
+// 53 % of the time with 1.6 waves a SIMD. Shares that go on keep 26 to 47 scalar registers in vector ones
 // (3 of those in scratch for fp16 256 wide), outside the steps.
 template <int TYPE, int D, int NW, int MODE, typename RULES>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part, RULES rules) {
@@ -1354,6 +1362,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
 // operand comes out of LDS turned (ds_read_b64_tr_b16: of 16 lanes, lane 4 j + q reads 4
 // values of row j, and lane c gets column c of the 4 rows).
 //
+// Under rules a tile may be shared by workgroups (kAttnEnds), each with its tokens, whose
+// sums attn_join_rows adds up; q is read and split while the first step's tokens are on
+// their way. Trees: 16 of up to 32 drafts over up to 16384, 32 heads of 128 on 8, 173 us,
+// 300 TFLOP/s of the product itself (600 with the second parts), where the cache's bytes
+// alone take 109: the VALU is busy 49 % and the matrix unit 36 % of the time, with 2.45
+// waves a SIMD. Prompts into which documents were packed, 2 x 2500 tokens: 63 us; a tile
+// sees some ten steps there, a third of them masked, and the rest is its beginning (ranges,
+// table, first tokens, q) and end. Three buffers were no faster with shared tiles either
+// (105 us of 32 x 8 drafts over up to 8000: 118).
+//
 // Instruction issue bounds it: per step of 32 tokens x 16 rows x 128 a wave has 32
 // matrix instructions of 16 cycles and 106 of the softmax, the operands and the walk of
 // 4 and more, and three waves a SIMD overlap them to 44 and 37 % of the busy time (3 x
@@ -1386,9 +1404,8 @@ struct AttnStage {
   }
 };
 
-// Waits for the wave's loads but the last N and for its LDS operations, then for the other waves.
-template <int N>
-__device__ __forceinline__ void wait_step() { __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "i"(N) : "memory"); }
+// Waits for the wave's loads and LDS operations, then for the other waves.
+__device__ __forceinline__ void wait_step() { __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint2 ld_turned(const uint8_t *p) {
@@ -1397,8 +1414,11 @@ __device__ __forceinline__ uint2 ld_turned(const uint8_t *p) {
 }
 
 // The join of a tile of 64 rows, as attn_join: workgroup by workgroup, a thread's PIECES
-// parts of 4 columns of a row at once, since the way to the sums and back is what it
-// waits for. LDS: 128 floats for each workgroup of one step.
+// parts of 4 columns of a row at once, U workgroups under way, and a lane a row for the
+// maxima and sums, since the way to what the others stored is all that it waits for (8
+// trees of 20 drafts over up to 8192 tokens, 32 heads of 128 on 8: 82 -> 56 us against
+// attn_join's rows and columns one after the other). LDS: 128 floats for each workgroup
+// of one step.
 template <int D, typename TILE>
 __device__ __forceinline__ void attn_join_rows(const AttnPlan &p, rsrc_t prs, uint32_t *cnt, const KvAttnArgs &a, const TILE &t, uint32_t group,
                                                uint32_t kvh, uint32_t item, uint32_t first, uint32_t chunks, float *wt, float *sm, float *sl,
@@ -1491,8 +1511,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
   using W = AttnWave<D, I8, false, false, D <= 128 ? kVTurned : kVLater, RULED>;
   using S = AttnStage<D>;
   constexpr uint32_t NW = 4u, R = 16u * NW;
-  constexpr int NB = MODE == kAttnEnds && D <= 128 ? 3 : 2;   // buffers: a step's fills are requested NB - 1 steps ahead
-  __shared__ __align__(1024) uint8_t buf[NB][S::BYTES];
+  __shared__ __align__(1024) uint8_t buf[2][S::BYTES];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15u, g = lane >> 4;
   const uint32_t group = a.q_heads / kv.heads;
   // The last tiles of a sequence see the most: first; sequence after sequence, and a
@@ -1633,31 +1652,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
     }
   };
   const int full = W::full_of(m), from = W::from_of(m, window);   // steps from .. full need no mask
-  bool gone[NB][2];   // of the steps under way
-#pragma unroll
-  for (int i = 0; i + 1 < NB; ++i) {
-    if (i >= steps) break;
-    issue(i, buf[i]);
-    gone[i][0] = k.gone[0], gone[i][1] = k.gone[1];
-    convert(buf[i]);
+  if (steps) {
+    issue(0, buf[0]);
+    convert(buf[0]);
   }
   if constexpr (RULED) begin_rows();   // on the first steps' way
 #pragma unroll 1
-  for (int i0 = 0; i0 < steps; i0 += NB) {
+  for (int i0 = 0; i0 < steps; i0 += 2) {
 #pragma unroll
-    for (int half = 0; half < NB; ++half) {
+    for (int half = 0; half < 2; ++half) {
       const int i = i0 + half;
       if (i >= steps) break;
-      constexpr int A = NB - 1;
-      const int next = (half + A) % NB;
-      const bool was[2] = {gone[half][0], gone[half][1]};
-      // this step's fills, and not those of the steps behind it
-      if (A > 1 && i + A - 1 < steps) wait_step<(A - 1) * MINE>();
-      else wait_step<0>();
-      if (i + A < steps) {
-        issue(i + A, buf[next]);
-        gone[next][0] = k.gone[0], gone[next][1] = k.gone[1];
-      }
+      const bool was[2] = {k.gone[0], k.gone[1]};
+      wait_step();
+      if (i + 1 < steps) issue(i + 1, buf[1 - half]);
       const int t0 = base + 32 * i;
       if (t0 < m.end && t0 + 32 > m.begin) {
         const uint8_t *lds = buf[half];
@@ -1684,7 +1692,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
         w.step(t0, was[0] || was[1] || t0 > full || t0 < from, was, m, window, wr, n, g, s, [&](int c) { return D <= 128 ? w.v_operand(c) : turned(c); },
                [&](int u) { return *(const u32x4 *)(lds + S::SCALES + 128u + 64u * u + 16u * g); });   // late: no register waits for it
       }
-      if (i + A < steps) convert(buf[next]);
+      if (i + 1 < steps) convert(buf[1 - half]);
     }
   }
   const float l = row_add(w.l);
@@ -1703,6 +1711,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void k_attn_rows(KvView kv, 
       }
     }
     // the waves have passed the last step's barrier, but may still read its buffer
+    static_assert(kJoinSide * kJoinSide >= kItemsRows && sizeof(buf) >= 2u * kJoinSide * R * 4u && 4u * kJoinRows <= kJoinSide, "a join's LDS");
     __shared__ float sm[R], sl[R];
     __shared__ uint32_t arrived;
     attn_join_rows<D>(p, prs, cnt, a, t, group, kvh, item, first, chunks, (float *)buf, sm, sl, arrived);
@@ -1818,7 +1827,7 @@ inline AttnPlan attn_plan(const KvView &kv, const KvBatchView &b, const KvAttnAr
   // over 2000 87 and 73).
   const uint32_t slots = kv.dim <= 128u ? 768u : 512u;
   const uint64_t items = std::max<uint64_t>(slots / kv.heads, 2u * tiles), each = (most + 63u) / 64u;
-  if (f16 && units > 2u && (wgs < 200u || (wgs < slots && units >= 8u && seen >= 16ull * new_most)) && items * kv.heads <= kAttnCounters / 4u &&
+  if (f16 && units > 2u && (wgs < 200u || (wgs < slots && units >= 8u && seen >= 16ull * new_most)) && items <= kItemsRows && items * kv.heads <= kAttnCounters / 4u &&
       each * b.seqs * units < 1u << 31)
     p.items = (uint32_t)items;
   return p;

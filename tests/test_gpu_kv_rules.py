@@ -509,3 +509,11 @@ def test_refusals(ctx, eff):
     tree.free()
     with pytest.raises(eff.EffError):
         ctx.kv_attn(cache, batch, q, out, 4, 0.1, rules=rules)
+
+
+def test_one_long_tile_among_many_empty_ones(ctx, eff):
+    """The bound of the tiles far above those that there are: one sequence has new tokens and a long context."""
+    n = 400
+    new, lens = [0] * n, [1] * n
+    new[77], lens[77] = 40, 70001
+    run(eff, ctx, 5, F16, 1, 2, 64, 256, new, lens, masks=trees)
