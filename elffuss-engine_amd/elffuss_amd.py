@@ -406,6 +406,8 @@ class KvTurns(_Described):
         axis = [int(a) for a in axis]
         if len(axis) > 128 or not all(0 <= a < 256 for a in axis):
             raise EffError(E_INVALID, "KvTurns: axis is up to 128 small numbers")
+        if axes > 1 and not axis:
+            raise EffError(E_INVALID, "KvTurns: several axes, and not said which pairs turn by which")
         self._describe(_KvTurns, at=at, axes=axes, axis=(ctypes.c_uint8 * 128)(*axis))
 
 

@@ -945,6 +945,7 @@ function descLote(l) {
 function descGiros(g) {
   soloEstas(g, ['en', 'ejes', 'eje'], 'giros');
   for (const e of g.eje || []) if (!Number.isInteger(e) || e < 0 || e > 3) throw invalido(`eje: «${e}» no es un eje`);   // a Uint8Array would wrap it
+  if (g.ejes > 1 && !g.eje) throw invalido('giros: varios ejes, y sin decir de cuál es cada par');
   return { at: manejador(g.en, 'en'), axes: g.ejes === undefined ? 1 : g.ejes, axis: g.eje === undefined ? undefined : Uint8Array.from(g.eje) };
 }
 

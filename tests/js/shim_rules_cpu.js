@@ -28,6 +28,7 @@ for (const mal of [5, 'x', {}, muerto, true]) {
 }
 for (const mal of [[4], [-1], [0.5], [300], ['1']]) invalido(() => kv.anade(cache, lote, filas, { en: b(), eje: mal }), /^eje:/);
 invalido(() => kv.anade(cache, lote, filas, { en: b(), axis: [0] }), /«axis»/);
+invalido(() => kv.anade(cache, lote, filas, { en: b(), ejes: 2 }), /varios ejes/);
 invalido(() => kv.atiende(cache, lote, b(), 1, 1, { reglas: { cap: 5 } }), /«cap»/);
 invalido(() => kv.copiaPaginas([cache], b()), /¿cuántas\?/);
 assert.strictEqual(prestados.length, 0);

@@ -185,7 +185,9 @@ def test_refusals(ctx, eff):
     call(eff.E_BOUNDS, good, rope_positions=0)
     call(eff.E_BOUNDS, good, rope_positions=41)
     for axes in (0, 5):
-        call(eff.E_SHAPE, eff.KvTurns(pos, axes=axes))
+        call(eff.E_SHAPE, eff.KvTurns(pos, [0] * 32, axes=axes))
+    with pytest.raises(eff.EffError):
+        eff.KvTurns(pos, axes=2)
     call(eff.E_INVALID, eff.KvTurns(pos, dealt(32, 3), axes=2))
     call(eff.E_INVALID, eff.KvTurns(pos, [0] * 31 + [1], axes=1))
     call(eff.E_INVALID, eff.KvTurns(None, axes=1))
