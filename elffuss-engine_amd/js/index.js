@@ -941,6 +941,19 @@ function descLote(l) {
     seqs: l.secuencias, tokens: l.tokens, tablePages: l.paginasTabla, maxNew: l.maxNuevos, maxLen: l.maxLargo };
 }
 
+// Switched off: giros, attention's rules, copiaPaginas and conserva end in an error once their descriptions are
+// checked. A process that ran them one after the other, eagerly and from a graph, ended in a segmentation fault of the
+// host in one run of several, and the cause is not known. On the CPU, over a runtime whose kernels do nothing, the same
+// calls ran 8000 times without a fault, 390 of them with every access of the addon and of the library's host code
+// checked. The library's own calls and the Python binding's are on.
+const KV_REGLAS_ENCENDIDO = false;
+function exigeEncendido(que) {
+  if (KV_REGLAS_ENCENDIDO) return;
+  const e = new Error(`${que}: apagado en este anfitrión (un proceso que lo usaba acabó en un fallo de segmentación sin causa conocida)`);
+  e.code = STATUS.E_DEVICE;
+  throw e;
+}
+
 // Positions to turn by: { en (u32 [ejes][tokens]), ejes, eje (the axis of each pair of channels) }.
 function descGiros(g) {
   soloEstas(g, ['en', 'ejes', 'eje'], 'giros');
@@ -987,6 +1000,7 @@ function createKvOps(device, deps) {
         rope: manejador(f.rope, 'rope'), ropePositions: f.posicionesRope, ropeDim: f.dimRope, ropeMode: f.modoRope,
         qNorm: manejador(f.normaQ, 'normaQ'), kNorm: manejador(f.normaK, 'normaK'), normEps: f.eps };
       const c = descCache(cache), l = descLote(lote), g = giros ? descGiros(giros) : undefined;
+      if (g) exigeEncendido('anade con giros');
       const q = f.q ? ctx.alloc(lote.tokens * f.cabezasQ * cache.dim * 4, 'kv.q') : null;
       d.qOut = manejador(q, 'q');
       native.kvAppend(device._ctx, c, l, d, g);
@@ -997,6 +1011,7 @@ function createKvOps(device, deps) {
     atiende(cache, lote, q, cabezasQ, escala, opts) {
       const o = soloEstas(opts || {}, ['ventana', 'desdeQ', 'pasoQ', 'reglas'], 'opts');
       const c = descCache(cache), l = descLote(lote), h = manejador(q, 'q'), r = o.reglas ? descReglasAtencion(o.reglas) : undefined;
+      if (r) exigeEncendido('atiende con reglas');
       const out = ctx.alloc(lote.tokens * cabezasQ * cache.dim * 4, 'kv.atencion');
       native.kvAttn(device._ctx, c, l, h, o.desdeQ, o.pasoQ, out._h, cabezasQ, escala, o.ventana, r);
       return Promise.resolve(out);
@@ -1004,14 +1019,18 @@ function createKvOps(device, deps) {
     // Pages to others in the caches of all layers (an array): copias u32 [cuantas][3], from, to, tokens.
     copiaPaginas(caches, copias, cuantas) {
       if (cuantas === undefined || cuantas === null) throw invalido('copiaPaginas: ¿cuántas?');
-      native.kvCopy(device._ctx, caches.map(descCache), manejador(copias, 'copias'), cuantas);
+      const c = caches.map(descCache), h = manejador(copias, 'copias');
+      exigeEncendido('copiaPaginas');
+      native.kvCopy(device._ctx, c, h, cuantas);
       return Promise.resolve();
     },
     // The drafts that stay move up in the caches of all layers: guardados u32 [tokens], cuantos u32 [secuencias];
     // largosNuevos (u32 [secuencias], may be left out): the lengths after it.
     conserva(caches, lote, guardados, cuantos, largosNuevos) {
-      native.kvKeep(device._ctx, caches.map(descCache), descLote(lote), manejador(guardados, 'guardados'), manejador(cuantos, 'cuantos'),
-        manejador(largosNuevos, 'largosNuevos'));
+      const c = caches.map(descCache), l = descLote(lote), g = manejador(guardados, 'guardados'), n = manejador(cuantos, 'cuantos');
+      const nuevos = manejador(largosNuevos, 'largosNuevos');
+      exigeEncendido('conserva');
+      native.kvKeep(device._ctx, c, l, g, n, nuevos);
       return Promise.resolve();
     },
   };

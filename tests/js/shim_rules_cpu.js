@@ -31,6 +31,12 @@ invalido(() => kv.anade(cache, lote, filas, { en: b(), axis: [0] }), /«axis»/)
 invalido(() => kv.anade(cache, lote, filas, { en: b(), ejes: 2 }), /varios ejes/);
 invalido(() => kv.atiende(cache, lote, b(), 1, 1, { reglas: { cap: 5 } }), /«cap»/);
 invalido(() => kv.copiaPaginas([cache], b()), /¿cuántas\?/);
+// what is described rightly ends where these calls are switched off, with nothing lent
+const apagado = (f) => assert.throws(f, (e) => e.code === eff.STATUS.E_DEVICE && /apagado/.test(e.message));
+apagado(() => kv.anade(cache, lote, filas, { en: b(), ejes: 2, eje: [0, 1] }));
+apagado(() => kv.atiende(cache, lote, b(), 1, 1, { reglas: { tope: 5, arbol: b(), palabrasArbol: 1 } }));
+apagado(() => kv.copiaPaginas([cache], b(), 1));
+apagado(() => kv.conserva([cache], lote, b(), b(), b()));
 assert.strictEqual(prestados.length, 0);
 
 for (const mal of [5, 'x', {}, true]) {
