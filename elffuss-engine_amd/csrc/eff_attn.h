@@ -626,8 +626,9 @@ struct AttnWave {
             float &y = s[k / 4][k % 4];
             const float z = y * to_z, e = __builtin_amdgcn_exp2f(fabsf(z) * 2.88539008177792681f);
             const float far = copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + e), 1.f), z);
-            // a raw score that is not finite stays so
-            y = fabsf(z) < kTanhFew ? z * tanh_few(z * z) * most : fmaf(y, 0.f, far * most);
+            // a raw score that is not finite stays so; a small one has the same bits whatever the
+            // others are, which its row may not see
+            y = fabsf(z) < kTanhFew ? y * sc * tanh_few(z * z) : fmaf(y, 0.f, far * most);
           }
         } else {
 #pragma unroll
