@@ -400,7 +400,8 @@ class KvRows(_Described):
 
 
 class KvTurns(_Described):
-    """Positions to turn by (eff_kv_turns): `at` u32 [axes][tokens], `axis` the axis of each pair of rotated channels."""
+    """Positions to turn by (eff_kv_turns): `at` u32 [axes][tokens], `axis` the axis of each pair of rotated channels (none:
+    one axis)."""
 
     def __init__(self, at, axis=(), *, axes=1):
         axis = [int(a) for a in axis]
@@ -409,6 +410,7 @@ class KvTurns(_Described):
         if axes > 1 and not axis:
             raise EffError(E_INVALID, "KvTurns: several axes, and not said which pairs turn by which")
         self._describe(_KvTurns, at=at, axes=axes, axis=(ctypes.c_uint8 * 128)(*axis))
+        self._pairs = len(axis)
 
 
 class KvRules(_Described):
@@ -640,6 +642,8 @@ class Context:
         if turns is None:
             self._check(lib().eff_kv_append(self.h, cache.ref, batch.ref, rows.ref))
         else:
+            if 0 < turns._pairs < rows.c.rope_dim // 2:
+                raise EffError(E_INVALID, f"KvTurns: the axes of {turns._pairs} pairs, and {rows.c.rope_dim // 2} turn")
             self._check(lib().eff_kv_append_at(self.h, cache.ref, batch.ref, rows.ref, turns.ref))
 
     def kv_copy(self, layers, copies, count):
