@@ -652,8 +652,10 @@ class Context:
 
     def kv_keep(self, layers, batch, kept, counts, new_lens=None):
         """The drafts that stay move up in the caches of all layers (KvLayers; eff_kv_keep)."""
+        if new_lens is not None and not new_lens.handle:
+            raise EffError(E_INVALID, "kv_keep: the buffer new_lens was freed")
         self._check(lib().eff_kv_keep(self.h, layers.ref, len(layers), batch.ref, kept.handle, counts.handle,
-                                      new_lens.handle if new_lens else None))
+                                      None if new_lens is None else new_lens.handle))
 
     def kv_attn(self, cache, batch, q, out, q_heads, scale, window=0, q_offset=0, q_stride=0, rules=None):
         """Attention of the new tokens over the cache (eff_kv_attn, with rules eff_kv_attn_rules)."""
