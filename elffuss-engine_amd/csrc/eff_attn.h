@@ -184,8 +184,6 @@ __device__ __forceinline__ int lanes_max(int v, uint32_t of = 0) {
 template <uint32_t L>
 __device__ __forceinline__ int lanes_min(int v, uint32_t of = 0) { return -lanes_max<L>(-v, of); }
 
-constexpr int kWindowMost = 0x40000000;
-
 // The cached tokens that a row's range names, of `len`.
 __device__ __forceinline__ void range_of(const KvRulesView &r, uint32_t token, int len, int &from, int &to) {
   const uint2 v = *(const uint2 *)(r.ranges + 2ull * token);
@@ -1118,97 +1116,97 @@ template <int D, uint32_t T, typename TILE>
 __device__ __forceinline__ void attn_join(const AttnPlan &p, rsrc_t prs, uint32_t *cnt, const KvAttnArgs &a, const TILE &t, uint32_t group,
                                           uint32_t kvh, uint32_t item, uint32_t first, uint32_t chunks, float *wt, float *half, float *sm,
                                           float *sl, uint32_t &arrived, uint32_t slot_floats, uint32_t ml, uint32_t tid, uint32_t lane, uint32_t wave) {
-        const auto place = [&](uint32_t z) { return 2u * (first + z) + (z == 0u ? 1u : 0u); };   // the slot of the tile's workgroup z
-        // one join, or where there is much to read, one of each group of about sqrt(chunks)
-        // workgroups, whose sums take its first one's slot, and one of the groups
-        const uint32_t side = chunks * p.rows * D <= kJoin ? chunks : __builtin_amdgcn_readfirstlane((uint32_t)ceilf(sqrtf((float)chunks)));
-        const uint32_t groups = (chunks + side - 1u) / side;
-        uint32_t z0 = (item - first) / side * side, step = 1u, count = min(side, chunks - z0);
-        for (bool last = groups == 1u;; last = true) {
-          __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          __syncthreads();
-          uint32_t *counter = cnt + (step == 1u ? 0u : kAttnCounters / 2u) + (uint64_t)kvh * p.items * 2u + place(z0);
-          if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          __syncthreads();
-          if (arrived != count - 1u) break;
-          if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          // each thread a part of the workgroups' 4 columns of a row, U of them under way,
-          // the first before the weights are known
-          constexpr uint32_t U = 8;
-          const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
-          const uint32_t part_i = parts > 1u ? tid / pieces : 0u, p0 = parts > 1u ? tid % pieces : tid;
-          float4v x[U] = {};   // (else live from tile to tile)
-          const auto request = [&](uint32_t i, uint32_t z) {
-  #pragma unroll
-            for (uint32_t k = 0; k < U; ++k) {
-              const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + i / (D / 4u) * D + 4u * (i % (D / 4u));
-              x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
-            }
-          };
-          if (p0 < pieces && part_i < parts) request(p0, part_i);
-          // the workgroups' weights relative to the largest maximum, [workgroup][row],
-          // and the rows' sums: a wave per row, its lanes over the workgroups
-                  for (uint32_t r = wave; r < t.rows; r += T / 64u) {
-            const auto both = [&](uint32_t z, float &mz, float &lz) {
-              const int at = (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u);
-              mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
-              lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
-            };
-            float m0 = -INFINITY, l0 = 0.f, mz, lz;
-            if (lane < count) both(lane, m0, l0);
-            float mx = m0, l = 0.f;
-            for (uint32_t z = lane + 64u; z < count; z += 64u) both(z, mz, lz), mx = fmaxf(mx, mz);
-  #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-            for (uint32_t z = lane; z < count; z += 64u) {
-              if (z < 64u) mz = m0, lz = l0;
-              else both(z, mz, lz);
-              const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
-              wt[z * p.rows + r] = f;
-              l += f * lz;
-            }
-            l = wave_sum(l);
-            if (lane == 0u) sl[r] = l, sm[r] = mx;
-          }
-          __syncthreads();
-          for (uint32_t i = p0; i < (parts > 1u ? p0 + 1u : (pieces + T - 1u) / T * T); i += T) {
-            const bool here = i < pieces && part_i < parts;
-            const uint32_t r = here ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
-            float4v o = {0.f, 0.f, 0.f, 0.f};
-            if (here) {
-              for (uint32_t z = part_i; z < count; z += U * parts) {
-                if (i != p0 || z != part_i) request(i, z);
-  #pragma unroll
-                for (uint32_t k = 0; k < U; ++k)
-                  if (z + k * parts < count) o += x[k] * wt[(z + k * parts) * p.rows + r];
-              }
-            }
-            if (parts > 1u) {
-              *(float4v *)(half + 4u * tid) = o;
-              __syncthreads();
-              if (here && part_i == 0u)
-                for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * pieces));
-            }
-            if (!here || part_i != 0u) continue;
-            const float l = sl[r];
-            if (last) {
-              const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
-              float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
-              *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
-            } else {
-              const uint32_t at = place(z0) * slot_floats;
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((at + r * D + d) * 4u), 0, kSc1);
-              if (d == 0u) {
-                // a sum that is not a number is not nothing
-                const float mx = sm[r] == -INFINITY && l != 0.f ? 0.f : sm[r];
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((at + ml + 2u * r) * 4u), 0, kSc1);
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((at + ml + 2u * r + 1u) * 4u), 0, kSc1);
-              }
-            }
-          }
-          if (last) break;
-          z0 = 0u, step = side, count = groups;
+  const auto place = [&](uint32_t z) { return 2u * (first + z) + (z == 0u ? 1u : 0u); };   // the slot of the tile's workgroup z
+  // one join, or where there is much to read, one of each group of about sqrt(chunks)
+  // workgroups, whose sums take its first one's slot, and one of the groups
+  const uint32_t side = chunks * p.rows * D <= kJoin ? chunks : __builtin_amdgcn_readfirstlane((uint32_t)ceilf(sqrtf((float)chunks)));
+  const uint32_t groups = (chunks + side - 1u) / side;
+  uint32_t z0 = (item - first) / side * side, step = 1u, count = min(side, chunks - z0);
+  for (bool last = groups == 1u;; last = true) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t *counter = cnt + (step == 1u ? 0u : kAttnCounters / 2u) + (uint64_t)kvh * p.items * 2u + place(z0);
+    if (tid == 0u) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != count - 1u) break;
+    if (tid == 0u) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // each thread a part of the workgroups' 4 columns of a row, U of them under way,
+    // the first before the weights are known
+    constexpr uint32_t U = 8;
+    const uint32_t pieces = t.rows * (D / 4u), parts = max(1u, T / pieces);
+    const uint32_t part_i = parts > 1u ? tid / pieces : 0u, p0 = parts > 1u ? tid % pieces : tid;
+    float4v x[U] = {};   // (else live from tile to tile)
+    const auto request = [&](uint32_t i, uint32_t z) {
+#pragma unroll
+      for (uint32_t k = 0; k < U; ++k) {
+        const uint32_t at = place(z0 + step * min(z + k * parts, count - 1u)) * slot_floats + i / (D / 4u) * D + 4u * (i % (D / 4u));
+        x[k] = __builtin_bit_cast(float4v, __builtin_amdgcn_raw_buffer_load_b128(prs, (int)(at * 4u), 0, kSc1));
+      }
+    };
+    if (p0 < pieces && part_i < parts) request(p0, part_i);
+    // the workgroups' weights relative to the largest maximum, [workgroup][row],
+    // and the rows' sums: a wave per row, its lanes over the workgroups
+    for (uint32_t r = wave; r < t.rows; r += T / 64u) {
+      const auto both = [&](uint32_t z, float &mz, float &lz) {
+        const int at = (int)((place(z0 + step * z) * slot_floats + ml + 2u * r) * 4u);
+        mz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at, 0, kSc1));
+        lz = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(prs, at + 4, 0, kSc1));
+      };
+      float m0 = -INFINITY, l0 = 0.f, mz, lz;
+      if (lane < count) both(lane, m0, l0);
+      float mx = m0, l = 0.f;
+      for (uint32_t z = lane + 64u; z < count; z += 64u) both(z, mz, lz), mx = fmaxf(mx, mz);
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      for (uint32_t z = lane; z < count; z += 64u) {
+        if (z < 64u) mz = m0, lz = l0;
+        else both(z, mz, lz);
+        const float f = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - mx);
+        wt[z * p.rows + r] = f;
+        l += f * lz;
+      }
+      l = wave_sum(l);
+      if (lane == 0u) sl[r] = l, sm[r] = mx;
+    }
+    __syncthreads();
+    for (uint32_t i = p0; i < (parts > 1u ? p0 + 1u : (pieces + T - 1u) / T * T); i += T) {
+      const bool here = i < pieces && part_i < parts;
+      const uint32_t r = here ? i / (D / 4u) : 0u, d = 4u * (i % (D / 4u));
+      float4v o = {0.f, 0.f, 0.f, 0.f};
+      if (here) {
+        for (uint32_t z = part_i; z < count; z += U * parts) {
+          if (i != p0 || z != part_i) request(i, z);
+#pragma unroll
+          for (uint32_t k = 0; k < U; ++k)
+            if (z + k * parts < count) o += x[k] * wt[(z + k * parts) * p.rows + r];
         }
+      }
+      if (parts > 1u) {
+        *(float4v *)(half + 4u * tid) = o;
+        __syncthreads();
+        if (here && part_i == 0u)
+          for (uint32_t k = 1; k < parts; ++k) o += *(const float4v *)(half + 4u * (tid + k * pieces));
+      }
+      if (!here || part_i != 0u) continue;
+      const float l = sl[r];
+      if (last) {
+        const uint32_t tok = (t.r0 + r) / group, h = (t.r0 + r) % group;
+        float *dst = a.out + ((uint64_t)(t.token0 + tok) * a.q_heads + kvh * group + h) * D + d;
+        *(float4v *)dst = l == 0.f ? float4v{0.f, 0.f, 0.f, 0.f} : o / l;
+      } else {
+        const uint32_t at = place(z0) * slot_floats;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), prs, (int)((at + r * D + d) * 4u), 0, kSc1);
+        if (d == 0u) {
+          // a sum that is not a number is not nothing
+          const float mx = sm[r] == -INFINITY && l != 0.f ? 0.f : sm[r];
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(mx), prs, (int)((at + ml + 2u * r) * 4u), 0, kSc1);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(l), prs, (int)((at + ml + 2u * r + 1u) * 4u), 0, kSc1);
+        }
+      }
+    }
+    if (last) break;
+    z0 = 0u, step = side, count = groups;
+  }
 }
 
 // Few rows: NW waves take the 32-token steps of a tile in turn; their sums meet in
