@@ -774,7 +774,18 @@ napi_value RopeTable(napi_env env, napi_callback_info info) {
   return status(env, ctx, eff_rope_table(ctx, (const double *)f, (uint32_t)(len / 8), positions, scale, external<eff_buf>(env, a[4])));
 }
 
-// kvAppend(ctx, cache, batch, rows, turns?); turns: { at, axes, axis (Uint8Array) }
+// Switched off in this host: positions of their own, rules on attention, copies of pages and kept
+// drafts. A process that ran them one after the other ended in a segmentation fault of the host in
+// one run of several, and the cause is not known. Their arguments are checked, so that a wrong one
+// says what it is; then the call ends here, and reaches neither the library nor the device.
+napi_value switched_off(napi_env env, eff_ctx *ctx, const char *what) {
+  if (thrown(env)) return nullptr;
+  if (!ctx) return status(env, nullptr, EFF_E_INVALID);
+  return throw_msg(env, std::string(what) + ": switched off in this host (a process that used it ended in a segmentation fault of unknown cause)",
+                   EFF_E_DEVICE);
+}
+
+// kvAppend(ctx, cache, batch, rows); with turns, { at, axes, axis (Uint8Array) }, it is switched off
 napi_value KvAppend(napi_env env, napi_callback_info info) {
   napi_value a[5];
   get_args(env, info, 5, a);
@@ -797,25 +808,18 @@ napi_value KvAppend(napi_env env, napi_callback_info info) {
     if (thrown(env)) return nullptr;
     return status(env, ctx, eff_kv_append(ctx, &c, &b, &r));
   }
-  eff_kv_turns t{};
-  t.at = buf_prop(env, a[4], "at"), t.axes = u32_prop(env, a[4], "axes");
+  buf_prop(env, a[4], "at"), u32_prop(env, a[4], "axes");
   napi_value axis = prop(env, a[4], "axis");
-  if (!absent(env, axis)) {
-    void *p = nullptr;
-    size_t len = 0;
-    napi_typedarray_type type;
-    if (napi_get_typedarray_info(env, axis, &type, nullptr, nullptr, nullptr, nullptr) != napi_ok || type != napi_uint8_array ||
-        !bytes_of(env, axis, &p, &len) || len > sizeof(t.axis))
-      throw_msg(env, "axis: not a Uint8Array of up to 128 axes");
-    else if (len)
-      memcpy(t.axis, p, len);
-  }
-  if (thrown(env)) return nullptr;
-  return status(env, ctx, eff_kv_append_at(ctx, &c, &b, &r, &t));
+  size_t len = 0;
+  napi_typedarray_type type;
+  if (!absent(env, axis) && (napi_get_typedarray_info(env, axis, &type, &len, nullptr, nullptr, nullptr) != napi_ok || type != napi_uint8_array ||
+                             len > sizeof(eff_kv_turns::axis)))
+    throw_msg(env, "axis: not a Uint8Array of up to 128 axes");
+  return switched_off(env, ctx, "kvAppend with turns");
 }
 
-// kvAttn(ctx, cache, batch, q, qOffset, qStride, out, qHeads, scale, window, rules?);
-// rules: { cap, slopes, ranges, tree, treeWords }
+// kvAttn(ctx, cache, batch, q, qOffset, qStride, out, qHeads, scale, window); with rules, { cap,
+// slopes, ranges, tree, treeWords }, it is switched off
 napi_value KvAttn(napi_env env, napi_callback_info info) {
   napi_value a[11];
   get_args(env, info, 11, a);
@@ -826,59 +830,48 @@ napi_value KvAttn(napi_env env, napi_callback_info info) {
   const uint32_t q_stride = u32(env, a[5], "qStride"), q_heads = u32(env, a[7], "qHeads"), window = u32(env, a[9], "window");
   const float scale = (float)number(env, a[8], "scale", 0.0);
   if (!absent(env, a[10])) {
-    eff_kv_rules r{};
-    r.cap = (float)number(env, prop(env, a[10], "cap"), "cap", 0.0);
-    r.tree_words = u32_prop(env, a[10], "treeWords");
-    r.slopes = buf_prop(env, a[10], "slopes"), r.ranges = buf_prop(env, a[10], "ranges"), r.tree = buf_prop(env, a[10], "tree");
-    if (thrown(env)) return nullptr;
-    return status(env, ctx, eff_kv_attn_rules(ctx, &c, &b, external<eff_buf>(env, a[3]), q_offset, q_stride, external<eff_buf>(env, a[6]),
-                                              q_heads, scale, window, &r));
+    number(env, prop(env, a[10], "cap"), "cap", 0.0), u32_prop(env, a[10], "treeWords");
+    for (const char *name : {"slopes", "ranges", "tree"}) buf_prop(env, a[10], name);
+    return switched_off(env, ctx, "kvAttn with rules");
   }
   if (thrown(env)) return nullptr;
   return status(env, ctx, eff_kv_attn(ctx, &c, &b, external<eff_buf>(env, a[3]), q_offset, q_stride, external<eff_buf>(env, a[6]),
                                       q_heads, scale, window));
 }
 
-// The caches of a call's layers (an array of descriptions).
-std::vector<eff_kv_cache> kv_caches(napi_env env, napi_value v) {
-  std::vector<eff_kv_cache> got;
+// The caches of a call's layers (an array of descriptions), checked.
+void check_caches(napi_env env, napi_value v) {
   bool is = false;
   uint32_t n = 0;
   if (napi_is_array(env, v, &is) != napi_ok || !is || napi_get_array_length(env, v, &n) != napi_ok) {
     throw_msg(env, "caches: not an array");
-    return got;
+    return;
   }
   for (uint32_t i = 0; i < n && !thrown(env); ++i) {
     napi_value c = undefined(env);
     napi_get_element(env, v, i, &c);
-    got.push_back(kv_cache(env, c));
+    kv_cache(env, c);
   }
-  return got;
 }
 
-// kvCopy(ctx, caches, copies, count)
+// kvCopy(ctx, caches, copies, count): switched off
 napi_value KvCopy(napi_env env, napi_callback_info info) {
   napi_value a[4];
   get_args(env, info, 4, a);
-  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
-  const std::vector<eff_kv_cache> c = kv_caches(env, a[1]);
-  const uint32_t count = thrown(env) ? 0u : u32(env, a[3], "count");
-  if (thrown(env)) return nullptr;
-  return status(env, ctx, eff_kv_copy(ctx, c.data(), (uint32_t)c.size(), external<eff_buf>(env, a[2]), count));
+  check_caches(env, a[1]);
+  if (!thrown(env)) u32(env, a[3], "count");
+  return switched_off(env, external<eff_ctx>(env, a[0]), "kvCopy");
 }
 
-// kvKeep(ctx, caches, batch, kept, counts, newLens?)
+// kvKeep(ctx, caches, batch, kept, counts, newLens?): switched off
 napi_value KvKeep(napi_env env, napi_callback_info info) {
   napi_value a[6];
   get_args(env, info, 6, a);
-  eff_ctx *ctx = external<eff_ctx>(env, a[0]);
-  const std::vector<eff_kv_cache> c = kv_caches(env, a[1]);
+  check_caches(env, a[1]);
   if (thrown(env)) return nullptr;
-  const eff_kv_batch b = kv_batch(env, a[2]);
-  eff_buf *lens = absent(env, a[5]) ? nullptr : external<eff_buf>(env, a[5]);
-  if (!absent(env, a[5]) && !lens) throw_msg(env, "newLens: not a buffer");
-  if (thrown(env)) return nullptr;
-  return status(env, ctx, eff_kv_keep(ctx, c.data(), (uint32_t)c.size(), &b, external<eff_buf>(env, a[3]), external<eff_buf>(env, a[4]), lens));
+  kv_batch(env, a[2]);
+  if (!absent(env, a[5]) && !external<eff_buf>(env, a[5])) throw_msg(env, "newLens: not a buffer");
+  return switched_off(env, external<eff_ctx>(env, a[0]), "kvKeep");
 }
 
 // logitsApply(ctx, in, out, rows, vocab, stride, rules)

@@ -942,31 +942,28 @@ function descLote(l) {
 }
 
 // Switched off: giros, attention's rules, copiaPaginas and conserva end in an error once their descriptions are
-// checked. A process that ran them one after the other, eagerly and from a graph, ended in a segmentation fault of the
-// host in one run of several, and the cause is not known. On the CPU, over a runtime whose kernels do nothing, the same
-// calls ran 8000 times without a fault, 390 of them with every access of the addon and of the library's host code
-// checked. The library's own calls and the Python binding's are on.
+// checked, and so do the addon's calls of them. A process that ran them one after the other, eagerly and from a graph,
+// ended in a segmentation fault of the host in one run of several, and the cause is not known; nor is it shown that the
+// calls that are on cannot end so. The library's own calls and the Python binding's are on.
 const KV_REGLAS_ENCENDIDO = false;
-function exigeEncendido(que) {
-  if (KV_REGLAS_ENCENDIDO) return;
+function apagado(que) {
   const e = new Error(`${que}: apagado en este anfitrión (un proceso que lo usaba acabó en un fallo de segmentación sin causa conocida)`);
   e.code = STATUS.E_DEVICE;
-  throw e;
+  return e;
 }
 
-// Positions to turn by: { en (u32 [ejes][tokens]), ejes, eje (the axis of each pair of channels) }.
-function descGiros(g) {
+// Positions to turn by, checked: { en (u32 [ejes][tokens]), ejes, eje (the axis of each pair of channels) }.
+function compruebaGiros(g) {
   soloEstas(g, ['en', 'ejes', 'eje'], 'giros');
   for (const e of g.eje || []) if (!Number.isInteger(e) || e < 0 || e > 3) throw invalido(`eje: «${e}» no es un eje`);   // a Uint8Array would wrap it
   if (g.ejes > 1 && !g.eje) throw invalido('giros: varios ejes, y sin decir de cuál es cada par');
-  return { at: manejador(g.en, 'en'), axes: g.ejes === undefined ? 1 : g.ejes, axis: g.eje === undefined ? undefined : Uint8Array.from(g.eje) };
+  manejador(g.en, 'en');
 }
 
-// Rules on attention's scores: { tope, pendientes, rangos, arbol, palabrasArbol }.
-function descReglasAtencion(r) {
+// Rules on attention's scores, checked: { tope, pendientes, rangos, arbol, palabrasArbol }.
+function compruebaReglasAtencion(r) {
   soloEstas(r, ['tope', 'pendientes', 'rangos', 'arbol', 'palabrasArbol'], 'reglas');
-  return { cap: r.tope, slopes: manejador(r.pendientes, 'pendientes'), ranges: manejador(r.rangos, 'rangos'), tree: manejador(r.arbol, 'arbol'),
-    treeWords: r.palabrasArbol };
+  for (const n of ['pendientes', 'rangos', 'arbol']) manejador(r[n], n);
 }
 
 function createKvOps(device, deps) {
@@ -992,46 +989,50 @@ function createKvOps(device, deps) {
     },
     // New k, v rows into the cache; q rotated into a pooled buffer, which it resolves to (null without q).
     // filas: { q, k, v, desdeQ, desdeK, desdeV, pasoQ, pasoK, pasoV, cabezasQ, rope, posicionesRope, dimRope,
-    // modoRope, normaQ, normaK, eps }; giros (descGiros): positions of their own.
+    // modoRope, normaQ, normaK, eps }; giros (compruebaGiros): switched off.
     anade(cache, lote, filas, giros) {
       const f = soloEstas(filas, DE_FILAS, 'filas');
       const d = { q: manejador(f.q, 'q'), k: manejador(f.k, 'k'), v: manejador(f.v, 'v'), qOffset: f.desdeQ, kOffset: f.desdeK,
         vOffset: f.desdeV, qStride: f.pasoQ, kStride: f.pasoK, vStride: f.pasoV, qHeads: f.q ? f.cabezasQ : 0,
         rope: manejador(f.rope, 'rope'), ropePositions: f.posicionesRope, ropeDim: f.dimRope, ropeMode: f.modoRope,
         qNorm: manejador(f.normaQ, 'normaQ'), kNorm: manejador(f.normaK, 'normaK'), normEps: f.eps };
-      const c = descCache(cache), l = descLote(lote), g = giros ? descGiros(giros) : undefined;
-      if (g) exigeEncendido('anade con giros');
+      const c = descCache(cache), l = descLote(lote);
+      if (giros) {
+        compruebaGiros(giros);
+        throw apagado('anade con giros');
+      }
       const q = f.q ? ctx.alloc(lote.tokens * f.cabezasQ * cache.dim * 4, 'kv.q') : null;
       d.qOut = manejador(q, 'q');
-      native.kvAppend(device._ctx, c, l, d, g);
+      native.kvAppend(device._ctx, c, l, d);
       return Promise.resolve(q);
     },
     // Attention of the new tokens over the cache, into a pooled buffer. opts: { ventana, desdeQ, pasoQ, reglas
-    // (descReglasAtencion) }.
+    // (compruebaReglasAtencion): switched off }.
     atiende(cache, lote, q, cabezasQ, escala, opts) {
       const o = soloEstas(opts || {}, ['ventana', 'desdeQ', 'pasoQ', 'reglas'], 'opts');
-      const c = descCache(cache), l = descLote(lote), h = manejador(q, 'q'), r = o.reglas ? descReglasAtencion(o.reglas) : undefined;
-      if (r) exigeEncendido('atiende con reglas');
+      const c = descCache(cache), l = descLote(lote), h = manejador(q, 'q');
+      if (o.reglas) {
+        compruebaReglasAtencion(o.reglas);
+        throw apagado('atiende con reglas');
+      }
       const out = ctx.alloc(lote.tokens * cabezasQ * cache.dim * 4, 'kv.atencion');
-      native.kvAttn(device._ctx, c, l, h, o.desdeQ, o.pasoQ, out._h, cabezasQ, escala, o.ventana, r);
+      native.kvAttn(device._ctx, c, l, h, o.desdeQ, o.pasoQ, out._h, cabezasQ, escala, o.ventana);
       return Promise.resolve(out);
     },
-    // Pages to others in the caches of all layers (an array): copias u32 [cuantas][3], from, to, tokens.
+    // Pages to others in the caches of all layers (an array): copias u32 [cuantas][3], from, to, tokens. Switched off.
     copiaPaginas(caches, copias, cuantas) {
       if (cuantas === undefined || cuantas === null) throw invalido('copiaPaginas: ¿cuántas?');
-      const c = caches.map(descCache), h = manejador(copias, 'copias');
-      exigeEncendido('copiaPaginas');
-      native.kvCopy(device._ctx, c, h, cuantas);
-      return Promise.resolve();
+      caches.forEach(descCache);
+      manejador(copias, 'copias');
+      throw apagado('copiaPaginas');
     },
     // The drafts that stay move up in the caches of all layers: guardados u32 [tokens], cuantos u32 [secuencias];
-    // largosNuevos (u32 [secuencias], may be left out): the lengths after it.
+    // largosNuevos (u32 [secuencias], may be left out): the lengths after it. Switched off.
     conserva(caches, lote, guardados, cuantos, largosNuevos) {
-      const c = caches.map(descCache), l = descLote(lote), g = manejador(guardados, 'guardados'), n = manejador(cuantos, 'cuantos');
-      const nuevos = manejador(largosNuevos, 'largosNuevos');
-      exigeEncendido('conserva');
-      native.kvKeep(device._ctx, c, l, g, n, nuevos);
-      return Promise.resolve();
+      caches.forEach(descCache);
+      descLote(lote);
+      manejador(guardados, 'guardados'), manejador(cuantos, 'cuantos'), manejador(largosNuevos, 'largosNuevos');
+      throw apagado('conserva');
     },
   };
 }
@@ -1058,7 +1059,7 @@ function createLogitsOps(device, deps) {
 }
 
 module.exports = {
-  native, STATUS, OPT, GEMV_MODE, TOPK, QUANT_TYPES, quantInfo, createKvOps, createLogitsOps, KV_TIPOS, ROPE, SIN_PAGINA,
+  native, STATUS, OPT, GEMV_MODE, TOPK, QUANT_TYPES, quantInfo, createKvOps, createLogitsOps, KV_REGLAS_ENCENDIDO, KV_TIPOS, ROPE, SIN_PAGINA,
   requestDevice, readback, createContext,
   createQuantOps, createGemvOps, GEMV2_TIPOS, GEMV2_MAX_TOKENS, createGemm2Ops, GEMM2_TIPOS, createFusionOps, createTopKGPU, estadisticasTopK, TIPOS_GATHER_NORMA,
   TIPOS_R, TIPO_R, TIPO_GGUF, bytesReordenado, bytesBufferR, bloquesDeBuffer, escalasDesde,
