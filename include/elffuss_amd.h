@@ -612,7 +612,8 @@ int eff_kv_attn(eff_ctx *ctx, const eff_kv_cache *cache, const eff_kv_batch *bat
  *          j-th new token of its sequence if bit j % 32 of word j / 32 of its row
  *          is set: its ancestors and itself. Its position, for the window and the
  *          slopes, is the first new one's plus the number of bits less one.
- *          32 * tree_words >= max_new, and a window >= max_new */
+ *          32 * tree_words >= max_new, and a window >= max_new: it leaves out
+ *          tokens ahead of the drafts, and no draft whose bit is set */
 typedef struct eff_kv_rules {
   float cap;
   uint32_t tree_words;
