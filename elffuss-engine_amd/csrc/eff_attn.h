@@ -1226,10 +1226,12 @@ __device__ __forceinline__ void attn_join(const AttnPlan &p, rsrc_t prs, uint32_
 // is round trips: lengths, page table, K, V, the join (517 tokens: 6.3 to 6.8 us, an
 // empty launch 3.4). Under rules: 48 up to 8192, 16 heads of 256 on 8, capped, 319 us, 5.7
 // TB/s; one of 20001, 32 heads of 128 with slopes, 60 us, 5.5 TB/s; int8 trees of up to 6
-// drafts (48 rows, three tiles) over 4096 of up to 9001, 16 heads of 256 on 2, 64 us, 2.2
-// TB/s of the cache: each tile converts the keys and values for itself, the VALU is busy
-// 53 % of the time with 1.6 waves a SIMD. Shares that go on keep 26 to 47 scalar registers in vector ones
-// (3 of those in scratch for fp16 256 wide), outside the steps.
+// drafts (48 rows, three tiles) over 4096 of up to 9001, 16 heads of 256 on 2, 65 us: each
+// tile reads and converts the keys and values for itself, and what another has read is
+// seldom left in its L2, so that 297 MB come where the caches have 142, at 4.6 TB/s, 88 % of
+// a large copy's rate; the VALU is busy 53 % of the time with 1.6 waves a SIMD. Shares that
+// go on keep 32 to 52 scalar registers in vector ones (under rules 71 to 85; fp16 256 wide
+// has 3 vector ones in scratch for that, under rules 5), outside the steps.
 template <int TYPE, int D, int NW, int MODE, typename RULES>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, KvBatchView b, KvAttnArgs a, AttnPlan p, uint32_t *cnt, float *part, RULES rules) {
   constexpr bool I8 = TYPE == EFF_KV_I8, QL = D == 256;   // 256 wide, q's parts would take a quarter of the registers
@@ -1363,10 +1365,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
 //
 // Under rules a tile may be shared by workgroups (kAttnEnds), each with its tokens, whose
 // sums attn_join_rows adds up; q is read and split while the first step's tokens are on
-// their way. Trees: 16 of up to 32 drafts over up to 16384, 32 heads of 128 on 8, 173 us,
-// 300 TFLOP/s of the product itself (600 with the second parts), where the cache's bytes
-// alone take 109: the VALU is busy 49 % and the matrix unit 36 % of the time, with 2.45
-// waves a SIMD. Prompts into which documents were packed, 2 x 2500 tokens: 63 us; a tile
+// their way. Trees: 16 of up to 32 drafts over up to 16384, 32 heads of 128 on 8, 167 to 173
+// us, 300 TFLOP/s of the product itself (600 with the second parts), where the cache's bytes
+// alone take 109: the second tile of a long sequence reads a quarter again (702 MB of 557, 4.1
+// TB/s), the VALU is busy 49 % and the matrix unit 37 % of the time with 2.45 waves a SIMD,
+// and a wave does its matrix steps and its softmax in turn; none of these is a limit by
+// itself. Prompts into which documents were packed, 2 x 2500 tokens: 63 us; a tile
 // sees some ten steps there, a third of them masked, and the rest is its beginning (ranges,
 // table, first tokens, q) and end. Three buffers were no faster with shared tiles either
 // (105 us of 32 x 8 drafts over up to 8000: 118).
@@ -1377,8 +1381,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void k_attn(KvView kv, Kv
 // 1000 new tokens at lengths up to 3001, 32 heads of 128 on 8: 181 to 190 us, 440
 // TFLOP/s of the product itself, 880 with q's and p's second parts, where a large fp16
 // product reaches 1090; of int8 239, where the conversions are VALU work too). Three
-// buffers, two steps ahead, were no faster (185 us): the loads are not waited for. At
-// 256 wide 2 (fp16) and 9 (int8) registers are in scratch.
+// buffers, two steps ahead, were no faster (185 us): the loads are not waited for. Vector
+// registers in scratch: 9 of int8 256 wide, fp16 none; under rules 10 and, shared, 13 of
+// fp16 256 wide, 20 of int8, 2 of fp16 128 wide shared, 4 of int8.
 template <int D>
 struct AttnStage {
   static constexpr uint32_t ROW = 2 * D, PIECES = ROW / 16u;
@@ -1852,7 +1857,10 @@ hipError_t attn_go(const KvView &kv, const KvBatchView &b, const KvAttnArgs &a, 
     const auto rows = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((uint32_t)many), dim3(256), 0, s, kv, b, a, p.many_tiles, p.many_per_seq, min_rows, rules, p, cnt, part);
     };
-    constexpr bool may = !__is_same(RULES, NoRules) && TYPE == EFF_KV_F16;   // tiles of 64 are shared
+    // Tiles of 64 are shared under rules only: the plain plan has not been measured with it (a
+    // chunk of 300 tokens over 4000, 32 heads of 128 on 8: capped 71 us, plain, in shared tiles
+    // of 16, 103; 400 tokens over 400 and 1000 over 1000, not shared: 19 and 40, plain 17 and 35).
+    constexpr bool may = !__is_same(RULES, NoRules) && TYPE == EFF_KV_F16;
     if (may && shared) rows(k_attn_rows<TYPE, D, may ? kAttnEnds : kAttnWhole, RULES>);
     else rows(k_attn_rows<TYPE, D, kAttnWhole, RULES>);
     const hipError_t e = hipGetLastError();

@@ -109,12 +109,18 @@ __device__ __forceinline__ void put(T *o, T v) {
 
 // With positions of their own (TURNED) a wave has a team's part instead of a workgroup, so
 // that few key heads do not leave the threads of whole workgroups without a row (5 prompts
-// of 1531 tokens and fewer, 16 heads of 128 on 2, q/k norm, 100 MB: 37 -> 26 us; with q, which is more than
-// the L2s hold, stored past them 18.6 us, 5.4 TB/s).
+// of 1531 tokens and fewer, 16 heads of 128 on 2, q/k norm, 100 MB: 37 -> 26 us; with q stored
+// past the L2 18.7 us, 5.4 TB/s). Where there are 4 rows a thread q goes past it whatever its
+// size: the attention that reads it next gives a part of that back or, from 20 MB of q on, a
+// little more. Append and attention of 32 heads of 128 on 8, q past the L2 and through it: 8 x
+// 24 drafts over 1000 (3 MB of q) 29.5 and 29.7 us, a prompt of 1000 (16 MB) 48.8 and 49.3, 48
+// x 25 drafts over 2000 (20 MB) 134 and 134, over 500 53.6 and 52.4, a prompt of 4000 (66 MB)
+// 331 and 328; the append alone 4.9 and 5.6, 8.6 and 9.8, 10.4 and 11.4, 10.0 and 11.1, 27.7
+// and 36.8.
 template <int TYPE, int D, int U, typename TURNS>
 __global__ __launch_bounds__(256) void k_kv_append(KvView kv, KvBatchView b, KvAppendArgs a, uint32_t q_wgs, uint32_t k_wgs, TURNS turned) {
 #pragma clang fp contract(off)
-  constexpr bool TURNED = !__is_same(TURNS, ByPlace), PAST = TURNED && U == 4;   // q of many tokens goes past the L2
+  constexpr bool TURNED = !__is_same(TURNS, ByPlace), PAST = TURNED && U == 4;   // q goes past the L2
   constexpr uint32_t L = D == 96 ? 32u : D / 4u, TEAM = TURNED ? 64u : 256u, ROWS = TEAM / L;
   const uint32_t id = TURNED ? __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6)) : blockIdx.x;
   const uint32_t wgs = q_wgs + 2u * k_wgs, t = id / wgs, w = id % wgs, l = (threadIdx.x & 63u) % L;
