@@ -613,7 +613,9 @@ struct AttnWave {
   __device__ __forceinline__ void rule(const Rules &r, const Tile &t, int t0, uint32_t n, uint32_t g, float s[2][4]) const {
     if constexpr (RULES) {
       if (r.all.cap > 0.f) {
-        const float to_z = fminf(sc * r.all.per_cap, 1e30f), most = r.all.cap;
+        // finite, so that a raw score of 0 stays 0, and not less than that: int8 keys may have raw
+        // scores of 1e-32 that are far past the cap
+        const float to_z = fminf(sc * r.all.per_cap, 0x1.fffffep127f), most = r.all.cap;
         float top = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(s[k / 4][k % 4]));
